@@ -295,7 +295,8 @@ int obs_set_decode_path(obs_ctx* ctx, int path);
 /* Waits for the stream, then reports (OBS_E_HIP + message) and clears a
  * device-side failure: a bounded wait that timed out in the fused decode
  * path, the fused attention half or the grouped prefill's one-launch expert
- * FFN; OBS_OK otherwise. The reference never checks GPU status. */
+ * FFN, or (OBS_E_INVALID) a page id, length or slot out of range that a call
+ * on a paged cache met; OBS_OK otherwise. The reference never checks GPU status. */
 int obs_device_status(obs_ctx* ctx);
 
 /* Dispatch facts and the one-launch paths they allow (no reference
@@ -471,6 +472,115 @@ int obs_attn_prep_rows(obs_ctx* ctx, uint16_t* q, const uint16_t* k, const uint1
 int obs_sdpa_prefill(obs_ctx* ctx, const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache_t,
                      uint16_t* out, uint32_t n_heads, uint32_t n_kv, uint32_t head_dim, uint32_t max_len,
                      uint32_t pos0, uint32_t n_tokens, uint32_t q_ld);
+
+/* ------------------------------------------------------------------ */
+/* Paged key/value cache of several sequences (no reference counterpart: */
+/* the reference's KvCache holds one sequence, kv_cache.rs:5-24)         */
+/* ------------------------------------------------------------------ */
+/* The pool of one layer: n_pages pages of `page` entries (a power of two from
+ * 16 to 256), head_dim 64 or 128. Keys [n_pages, n_kv, page, head_dim], values
+ * transposed [n_pages, n_kv, head_dim, page], both 16-byte aligned, in bf16 or
+ * in e4m3 (OCP, magnitudes up to 448) with one fp32 scale per kv head: an entry
+ * is the stored value times the scale. */
+enum { OBS_KV_BF16 = 0, OBS_KV_E4M3 = 1 };
+typedef struct obs_paged_kv {
+  void* k_pages; void* v_pages;
+  const float* k_scale; const float* v_scale; /* [n_kv] under OBS_KV_E4M3, else unused */
+  uint32_t n_pages, page, n_kv, head_dim;
+  int32_t dtype; /* OBS_KV_BF16 or OBS_KV_E4M3 */
+} obs_paged_kv;
+
+/* The sequences of a call, read on the device (a captured call follows their
+ * present contents). Entry j of sequence b lies in page
+ * pages[b * max_pages + j / page] at j % page. len[b]: its entries, the call's
+ * new tokens included; 0 or less: none (a padded batch); more than max_pages *
+ * page: as many as that, and obs_device_status reports it. Token rows row[b] to
+ * row[b + 1] - 1 (row[0] <= row[1] <= ... <= n_rows) are its last entries, in
+ * order; rows outside every sequence are left alone. row NULL: one token a
+ * sequence, row b of sequence b, n_rows == n_seqs. Page ids of entries that a
+ * call does not touch may be anything; an id outside [0, n_pages) that it needs
+ * hides the page's entries, appends nothing there, and is reported by
+ * obs_device_status (OBS_E_INVALID). At most 4,096 sequences, 2^30 entries each. */
+typedef struct obs_paged_seqs {
+  const int32_t* pages; const int32_t* len; const int32_t* row;
+  uint32_t n_seqs, max_pages, n_rows;
+} obs_paged_seqs;
+
+/* Attention weight gathered by entries: w fp32 [n_slots, n_kv, ld], sequence b
+ * of a call in slot[b] (NULL: slot b), ld >= max_pages * page of the call. The
+ * slots of a call's sequences are distinct; a slot outside [0, n_slots) gathers
+ * nothing and is reported like a page id. */
+typedef struct obs_kv_weight {
+  float* w; const int32_t* slot;
+  uint32_t n_slots, ld;
+} obs_kv_weight;
+
+/* obs_attn_prep_rows for the token rows of a paged batch: per-head q/k RMSNorm
+ * (eps), NeoX RoPE at pos[row] (NULL: at the row's entry index; entries that an
+ * eviction moved keep the rotation they were stored with, so such a sequence
+ * needs pos), q to q_out, k and v to their entries, weight (nullable) of those
+ * entries set to 0. bf16 results are obs_attn_prep_rows' bit for bit; e4m3 ones
+ * are rounded once from the fp32 value over the scale (to nearest even, beyond
+ * 448 to 448). q, k, v: bf16 rows of q_ld, kv_ld elements (multiples of 8; 0 =
+ * dense), 16-byte aligned, so they may be column ranges of one projection's
+ * output; q_out rows of q_out_ld (q_out may be q if q_out_ld == q_ld).
+ * rope_len: positions lie in [0, rope_len); a row at another one writes nothing.
+ * The context's RoPE table is built on the first call of a theta and length (run
+ * one before a capture). n_heads a multiple of n_kv, at most 16 per kv head.
+ * Two rows of a call must not name the same entry of a page. */
+int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,
+                        const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm,
+                        const uint16_t* k_norm, uint16_t* q_out, uint32_t n_heads, float eps, float theta,
+                        const int32_t* pos, uint32_t rope_len, uint32_t q_ld, uint32_t kv_ld, uint32_t q_out_ld);
+
+/* Bytes of device workspace that obs_sdpa_paged_decode (seqs->row NULL, weight as
+ * there) or obs_sdpa_paged_prefill (seqs->row set, weight NULL) needs for such a
+ * call, by sizes alone (pointers in kv and seqs are not read; no device work). */
+int obs_sdpa_paged_workspace(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs,
+                             const obs_kv_weight* weight, uint32_t n_heads, uint32_t window, uint32_t sinks,
+                             size_t* bytes);
+
+/* obs_sdpa_decode for one new token of every sequence (its last entry): GQA
+ * attention, scale 1/sqrt(head_dim), of entries j < len[b] with window == 0, or
+ * j > len[b] - 1 - window (the last `window` ones), or j < sinks (the first
+ * ones). What lies in hidden entries has no effect, NaN included. Nothing
+ * visible, or no finite score: zeros. q bf16 rows of q_ld elements (a multiple
+ * of 8; 0 = dense); out bf16 [n_seqs, n_heads, head_dim]; q, out and ws 16-byte
+ * aligned; row NULL. weight (nullable): every visible entry's softmax weights,
+ * summed over the kv head's query heads, are added to w[slot][kv head][j].
+ * Long sequences are split over workgroups by all lengths of the call and
+ * joined in order: the same call gives the same bits, another batch may round
+ * differently. ws: workspace of obs_sdpa_paged_workspace bytes, for one call at
+ * a time (calls or graphs that overlap in time need their own). */
+int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs,
+                          const obs_kv_weight* weight, const uint16_t* q, uint16_t* out, uint32_t n_heads,
+                          uint32_t window, uint32_t sinks, uint32_t q_ld, void* ws, size_t ws_bytes);
+
+/* The same for all token rows of a batch of prompts (obs_sdpa_prefill; row set):
+ * the row at entry i attends to j <= i with window == 0, or j > i - window, or
+ * j < sinks; a row whose i is negative (len shorter than its tokens) gets zeros.
+ * The rows' own keys and values are in the pages already (obs_attn_prep_paged).
+ * out bf16 [n_rows, n_heads, head_dim]; workspace as above. */
+int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const uint16_t* q,
+                           uint16_t* out, uint32_t n_heads, uint32_t window, uint32_t sinks, uint32_t q_ld, void* ws,
+                           size_t ws_bytes);
+
+/* Eviction by gathered weight. For each sequence with len[b] > budget and each kv
+ * head: entries [0, sinks), the last `recent` ones, and of the others the
+ * budget - sinks - recent with the largest weight (ties: the lowest entry; NaN
+ * counts as the least) are copied, in order, to entries 0 .. budget - 1 of the
+ * pages dst_pages[b * dst_max_pages + ...]; a sequence with no more than budget
+ * entries is copied whole. sinks + recent <= budget <= dst_max_pages * page.
+ * new_len [n_seqs] receives the entries kept, kept int32 [n_seqs, n_kv, budget]
+ * their old indices (-1 behind the last), dst_weight their weights; weights
+ * and entries behind the last one are left alone. seqs->row is not read. The
+ * destination pages and weight rows must not be among the call's source pages
+ * and rows (a shared prefix stays whole for its other users). A source page id
+ * that is out of range copies zeros, a destination one nothing; both are
+ * reported by obs_device_status. */
+int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,
+                 const int32_t* dst_pages, uint32_t dst_max_pages, const obs_kv_weight* dst_weight, uint32_t sinks,
+                 uint32_t recent, uint32_t budget, int32_t* kept, int32_t* new_len);
 
 /* ------------------------------------------------------------------ */
 /* Checkpoint loading: safetensors -> HBM-resident expert table        */

@@ -14,6 +14,7 @@
 // (exact algebra; it removes one multiply-add per weight). h stays fp32,
 // the combine accumulates sum_r w_r*y_r in fp32 (forward.rs:440) and rounds
 // once to bf16.
+#include "obs_paged.hpp"
 #include "obs_q4_dequant.hpp"
 
 namespace obs {
@@ -488,7 +489,8 @@ int obs_device_status(obs_ctx* ctx) {
   const int c = ctx->scratch_used ? obs::fused_decode_status_ws(ctx, ctx->scratch) : OBS_OK;
   const int f = obs::ffn_status(ctx);
   const int l = obs::layer_fused_status(ctx);
-  return a != OBS_OK ? a : b != OBS_OK ? b : c != OBS_OK ? c : f != OBS_OK ? f : l;
+  const int p = obs::paged_status(ctx);
+  return a != OBS_OK ? a : b != OBS_OK ? b : c != OBS_OK ? c : f != OBS_OK ? f : l != OBS_OK ? l : p;
 }
 
 }  // extern "C"

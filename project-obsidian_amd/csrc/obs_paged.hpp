@@ -1,0 +1,149 @@
+// obs_paged.hpp — what the operators on a paged key/value cache share: the
+// checks of their arguments, the sequences as a kernel sees them, and the
+// plan that splits their work over workgroups.
+#pragma once
+
+#include "obs_internal.hpp"
+
+namespace obs {
+
+// Word of obs_ctx::status_dev (behind the one-launch FFN's): a page id, length
+// or slot out of range that a kernel met.
+constexpr uint32_t CTX_ST_PAGED = 2;
+static_assert(CTX_ST_PAGED > CTX_ST_FFN_SCHED && CTX_ST_PAGED < CTX_ST_WORDS, "a word of its own");
+int paged_status(obs_ctx* ctx);  // reads and clears it (obs_device_status)
+
+constexpr uint32_t PAGED_MAX_SEQS = 4096;
+constexpr uint64_t PAGED_MAX_ENTRIES = 1ull << 30;
+
+// Makes the context's device current for a call's launches (a caller may work
+// on another one).
+struct DeviceGuard {
+  int before = -1;
+  explicit DeviceGuard(const obs_ctx* ctx) {
+    int d = -1;
+    if (hipGetDevice(&d) == hipSuccess && d != ctx->device && hipSetDevice(ctx->device) == hipSuccess) before = d;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// Shapes and pointers of kv and seqs; `pointers` false: sizes only.
+int check_paged(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs_paged_seqs* seqs, bool pointers);
+int check_heads(obs_ctx* ctx, const char* who, uint32_t n_heads, uint32_t n_kv);
+int check_weight(obs_ctx* ctx, const char* who, const obs_kv_weight* w, uint64_t entries, bool pointers);
+
+// The pool and the sequences as kernels take them.
+struct Paged {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* table;
+  const int32_t* len;
+  const int32_t* row;
+  uint32_t* status;
+  uint32_t n_pages, lp, n_kv, n_seqs, max_pages, n_rows;  // page = 1 << lp
+};
+inline Paged paged_args(const obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* s) {
+  return Paged{static_cast<const uint8_t*>(kv->k_pages), static_cast<const uint8_t*>(kv->v_pages),
+               kv->k_scale, kv->v_scale, s->pages, s->len, s->row, ctx->status_dev + CTX_ST_PAGED,
+               kv->n_pages, static_cast<uint32_t>(__builtin_ctz(kv->page)), kv->n_kv, s->n_seqs, s->max_pages, s->n_rows};
+}
+struct Weight {
+  float* w;
+  const int32_t* slot;
+  uint32_t n_slots, ld;
+};
+inline Weight weight_args(const obs_kv_weight* w) {
+  return w ? Weight{w->w, w->slot, w->n_slots, w->ld} : Weight{nullptr, nullptr, 0u, 0u};
+}
+
+}  // namespace obs
+
+namespace obsd {
+
+typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_v;
+typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_v __attribute__((ext_vector_type(2)));
+
+// Reports an argument in device memory that is out of range. The word is only
+// ever set to 1, so the order of several stores does not matter.
+__device__ __forceinline__ void paged_flag(uint32_t* status) {
+  __hip_atomic_store(status, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The functions below that decide what is read are host functions too, so they
+// can be tested without a GPU.
+__host__ __device__ __forceinline__ uint32_t umin(uint32_t x, uint32_t y) { return x < y ? x : y; }
+
+// Entries of sequence b, within [0, max_pages * page].
+__host__ __device__ __forceinline__ uint32_t paged_len(const obs::Paged& a, uint32_t b) {
+  const int32_t n = a.len[b];
+  const uint32_t cap = a.max_pages << a.lp;
+  return n <= 0 ? 0u : umin(static_cast<uint32_t>(n), cap);
+}
+__host__ __device__ __forceinline__ bool paged_len_bad(const obs::Paged& a, uint32_t b) {
+  const int32_t n = a.len[b];
+  return n > 0 && static_cast<uint32_t>(n) > (a.max_pages << a.lp);
+}
+// Token rows [r0, r1) of sequence b, within [0, n_rows].
+struct RowSpan {
+  uint32_t r0, r1;
+};
+__host__ __device__ __forceinline__ RowSpan paged_rows(const obs::Paged& a, uint32_t b) {
+  if (!a.row) return {b, b + 1u};
+  const int32_t lo = a.row[b], hi = a.row[b + 1u];
+  const uint32_t r0 = umin(lo > 0 ? static_cast<uint32_t>(lo) : 0u, a.n_rows);
+  const uint32_t r1 = umin(hi > 0 ? static_cast<uint32_t>(hi) : 0u, a.n_rows);
+  return {r0, r1 > r0 ? r1 : r0};
+}
+
+// Page id of entry j; `ok` is false for an id out of range, which then reads as page 0.
+__host__ __device__ __forceinline__ uint32_t paged_id(const obs::Paged& a, uint32_t b, uint32_t j, bool& ok) {
+  const uint32_t id = static_cast<uint32_t>(a.table[static_cast<size_t>(b) * a.max_pages + umin(j >> a.lp, a.max_pages - 1u)]);
+  ok = id < a.n_pages;
+  return ok ? id : 0u;
+}
+
+// What a query sees, in blocks of 32 entries.
+// Entry j of the queries at entries i0 <= i <= i1: the blocks that hold the
+// first `sinks` entries and those from the window of i0 to i1. Block x of the
+// nblk listed ones starts at entry 32 * (x < sb ? x : x - sb + wb).
+struct Span {
+  uint32_t hi, lo, sb, wb, nblk;
+  __host__ __device__ __forceinline__ uint32_t start(uint32_t x) const { return 32u * (x < sb ? x : x - sb + wb); }
+};
+__host__ __device__ __forceinline__ Span span_of(uint32_t i0, uint32_t hi, uint32_t window, uint32_t sinks) {
+  Span s;
+  s.hi = hi;
+  s.lo = window && i0 + 1u > window ? i0 + 1u - window : 0u;
+  s.wb = s.lo / 32u;
+  s.sb = umin((umin(sinks, hi) + 31u) / 32u, s.wb);
+  s.nblk = hi ? s.sb + (hi + 31u) / 32u - s.wb : 0u;
+  return s;
+}
+
+// Slot of sequence b's gathered weight, or -1.
+__device__ __forceinline__ int64_t weight_slot(const obs::Weight& w, uint32_t b) {
+  const int32_t s = w.slot ? w.slot[b] : static_cast<int32_t>(b);
+  return s >= 0 && static_cast<uint32_t>(s) < w.n_slots ? static_cast<int64_t>(s) : -1;
+}
+
+// fp32 pair -> two e4m3 bytes (OCP, round to nearest even; beyond 448 -> 448, NaN stays NaN).
+__device__ __forceinline__ float e4m3_clamp(float v) {
+  return v != v ? v : __builtin_fminf(__builtin_fmaxf(v, -448.0f), 448.0f);
+}
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(a), e4m3_clamp(b), 0, false);
+  r = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_clamp(c), e4m3_clamp(d), r, true);
+  return static_cast<uint32_t>(r);
+}
+// Two e4m3 bytes (the low or the high half of w) -> two bf16, exact (3 mantissa bits).
+template <bool HIGH>
+__device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+}
+
+}  // namespace obsd

@@ -1,0 +1,449 @@
+// obs_paged_cache.hip — a paged key/value cache of several sequences: the
+// checks of its arguments, q/k norm + RoPE + append (obs_attn_prep_paged) and
+// the eviction by gathered attention weight (obs_kv_evict).
+#include "obs_paged.hpp"
+
+namespace {
+using namespace obsd;
+using obs::Paged;
+using obs::Weight;
+
+// ---------------------------------------------------------------------------
+// q/k RMSNorm + NeoX RoPE + append
+// ---------------------------------------------------------------------------
+// The sequence that token row t belongs to: the number of ends row[1..n_seqs]
+// at or below t, counted by a wave (64 ends at once, or 64 ends of 64 each and
+// then one such block). n_seqs and above: behind the last sequence.
+__device__ __forceinline__ uint32_t seq_of_row(const Paged& a, uint32_t t, uint32_t lane) {
+  if (!a.row) return t;
+  uint32_t base = 0u;
+  if (a.n_seqs > 64u) {
+    const uint32_t blocks = (a.n_seqs + 63u) / 64u;  // <= 64
+    const int32_t end = a.row[min(64u * (min(lane, blocks - 1u) + 1u), a.n_seqs)];
+    base = 64u * static_cast<uint32_t>(__popcll(__ballot(lane < blocks && end <= static_cast<int32_t>(t))));
+    if (base >= a.n_seqs) return a.n_seqs;
+  }
+  const uint32_t b = base + lane;
+  const int32_t end = a.row[min(b, a.n_seqs - 1u) + 1u];
+  return base + static_cast<uint32_t>(__popcll(__ballot(b < a.n_seqs && end <= static_cast<int32_t>(t))));
+}
+
+struct PrepArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const uint16_t* q_norm;
+  const uint16_t* k_norm;
+  uint16_t* q_out;
+  const int32_t* pos;
+  const float* rope;
+  uint32_t nh, rope_len, q_ld, kv_ld, q_out_ld;
+  float eps;
+};
+
+// One workgroup per token row; HD / 8 lanes per head with 8 dims each, so a
+// wave norms and rotates 512 / HD heads at once. The sums and the rotation are
+// attn_prep_rows_kernel's, in its order.
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(256) prep_paged_kernel(Paged a, PrepArgs p, Weight w) {
+  constexpr uint32_t LPH = HD / 8u, HPW = 64u / LPH;  // lanes per head, heads per wave
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, m = lane % LPH, c0 = 8u * m;
+  const uint32_t t = blockIdx.x;
+  const uint32_t b = __builtin_amdgcn_readfirstlane(seq_of_row(a, t, lane));
+  if (b >= a.n_seqs) return;  // uniform
+  const RowSpan rs = paged_rows(a, b);
+  if (t < rs.r0 || t >= rs.r1) return;
+  const uint32_t n = paged_len(a, b);
+  if (t == rs.r0 && threadIdx.x == 0u && paged_len_bad(a, b)) paged_flag(a.status);
+  const int32_t entry = static_cast<int32_t>(n) - static_cast<int32_t>(rs.r1 - t);
+  const int32_t pos = p.pos ? p.pos[t] : entry;
+  if (pos < 0 || static_cast<uint32_t>(pos) >= p.rope_len) return;  // uniform
+  bool there = entry >= 0;
+  const uint32_t e = there ? static_cast<uint32_t>(entry) : 0u;
+  bool ok;
+  const uint32_t page = paged_id(a, b, e, ok);
+  if (there && !ok && threadIdx.x == 0u) paged_flag(a.status);
+  there = there && ok;
+  const uint32_t off = e & ((1u << a.lp) - 1u);
+  if (w.w && entry >= 0 && threadIdx.x < a.n_kv) {
+    const int64_t s = weight_slot(w, b);
+    if (s >= 0)
+      for (uint32_t h = threadIdx.x; h < a.n_kv; h += 256u) w.w[(static_cast<size_t>(s) * a.n_kv + h) * w.ld + e] = 0.0f;
+    else if (threadIdx.x == 0u)
+      paged_flag(a.status);
+  }
+  const uint16_t* q = p.q + static_cast<size_t>(t) * p.q_ld;
+  const uint16_t* k = p.k + static_cast<size_t>(t) * p.kv_ld;
+  const uint16_t* v = p.v + static_cast<size_t>(t) * p.kv_ld;
+  uint16_t* q_out = p.q_out + static_cast<size_t>(t) * p.q_out_ld;
+  const size_t page0 = static_cast<size_t>(page) * a.n_kv;
+  const uint32_t heads = p.nh + a.n_kv, pg = 1u << a.lp;
+  const bool first = m < LPH / 2u;
+  float cs[8], sn[8];  // of the lane's pairs: columns c0 .. c0 + 7 modulo HD / 2
+  {
+    const float* tab = p.rope + static_cast<size_t>(pos) * 128u + (HD == 128u ? 16u : 32u) * (m % (LPH / 2u));
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      // the table's pair i has theta^(-2i/128); a head of 64 takes every second one
+      const float2 t2 = *reinterpret_cast<const float2*>(tab + (HD == 128u ? 2u : 4u) * i);
+      cs[i] = t2.x;
+      sn[i] = t2.y;
+    }
+  }
+  for (uint32_t hb = HPW * wave; hb < heads; hb += 4u * HPW) {  // uniform per wave
+    const uint32_t head = hb + lane / LPH, hc = min(head, heads - 1u);
+    const bool is_q = hc < p.nh;
+    const uint4 xv = *reinterpret_cast<const uint4*>((is_q ? q + hc * HD : k + (hc - p.nh) * HD) + c0);
+    const uint4 wv = *reinterpret_cast<const uint4*>((is_q ? p.q_norm : p.k_norm) + c0);
+    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, ww[4] = {wv.x, wv.y, wv.z, wv.w};
+    float ps[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const float x0 = bf16lo(xw[i]), x1 = bf16hi(xw[i]);
+      ps[i] = __builtin_fmaf(x0, x0, 0.0f);
+      ps[i] = __builtin_fmaf(x1, x1, ps[i]);
+    }
+    float ss = (ps[0] + ps[1]) + (ps[2] + ps[3]);
+    ss = ss + dpp_f32<DPP_XOR1>(ss);
+    ss = ss + dpp_f32<DPP_XOR2>(ss);
+    ss = ss + dpp_f32<DPP_HALF_MIRROR>(ss);
+    if constexpr (HD == 128u) ss = ss + dpp_f32<DPP_MIRROR>(ss);
+    const float inv = 1.0f / __builtin_sqrtf(ss / static_cast<float>(HD) + p.eps);
+    float r[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const float x = i & 1u ? bf16hi(xw[i / 2u]) : bf16lo(xw[i / 2u]);
+      const float wn = i & 1u ? bf16hi(ww[i / 2u]) : bf16lo(ww[i / 2u]);
+      const float nv = bf16_to_f32(f32_to_bf16((x * inv) * wn));  // as the stored q / k would be
+      float other;  // columns +- HD / 2
+      if constexpr (HD == 128u)
+        other = dpp_f32<DPP_ROW_ROR8>(nv);
+      else
+        other = dpp_xor4_f32(nv);
+      const float x0 = nv * cs[i], x1 = other * sn[i];
+      r[i] = first ? x0 - x1 : x0 + x1;
+    }
+    if (head >= heads) continue;
+    if (is_q) {
+      *reinterpret_cast<uint4*>(q_out + head * HD + c0) =
+          make_uint4(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]), pack_bf16x2(r[4], r[5]), pack_bf16x2(r[6], r[7]));
+    } else if (there) {
+      const uint32_t h = head - p.nh;
+      const size_t at = ((page0 + h) * pg + off) * HD + c0;
+      if constexpr (F8) {
+        const float s = a.k_scale[h];
+        uint2 o;
+        o.x = pack_e4m3x4(r[0] / s, r[1] / s, r[2] / s, r[3] / s);
+        o.y = pack_e4m3x4(r[4] / s, r[5] / s, r[6] / s, r[7] / s);
+        *reinterpret_cast<uint2*>(const_cast<uint8_t*>(a.k) + at) = o;
+      } else {
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(a.k)) + at) = make_uint4(
+            pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]), pack_bf16x2(r[4], r[5]), pack_bf16x2(r[6], r[7]));
+      }
+    }
+  }
+  if (!there) return;
+  for (uint32_t i = threadIdx.x; i < a.n_kv * HD; i += 256u) {  // values: one transposed column
+    const uint32_t h = i / HD, d = i % HD;
+    const size_t at = ((page0 + h) * HD + d) * pg + off;
+    if constexpr (F8)
+      const_cast<uint8_t*>(a.v)[at] =
+          static_cast<uint8_t>(pack_e4m3x4(bf16_to_f32(v[i]) / a.v_scale[h], 0.0f, 0.0f, 0.0f));
+    else
+      reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(a.v))[at] = v[i];
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Eviction
+// ---------------------------------------------------------------------------
+// Order-preserving image of a weight: larger weight, larger key; -0 as +0; NaN below everything.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return w != w ? 0u : ((u >> 31) ? ~u : (u | 0x80000000u));
+}
+
+constexpr uint32_t EV_THREADS = 1024;
+
+// One workgroup per (sequence, kv head): the K-th largest key of the entries
+// between the first and the last ones, digit by digit (8 bits a pass, counts
+// in LDS), then one pass in order that ranks what is kept.
+__global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weight w, Weight wd, uint32_t sinks,
+                                                                 uint32_t recent, uint32_t budget,
+                                                                 int32_t* __restrict__ kept,
+                                                                 int32_t* __restrict__ new_len) {
+  __shared__ uint32_t s_hist[256];
+  __shared__ uint32_t s_wave[2][EV_THREADS / 64u];
+  __shared__ uint32_t s_pick[2];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t b = blockIdx.x / a.n_kv, h = blockIdx.x % a.n_kv;
+  const uint32_t n = paged_len(a, b), now = min(n, budget);
+  const int64_t slot = weight_slot(w, b), dslot = weight_slot(wd, b);
+  if (tid == 0u) {
+    if (paged_len_bad(a, b) || slot < 0 || dslot < 0) paged_flag(a.status);
+    if (h == 0u) new_len[b] = static_cast<int32_t>(now);
+  }
+  const float* src = w.w + (static_cast<size_t>(max(slot, int64_t(0))) * a.n_kv + h) * w.ld;
+  float* dst = wd.w + (static_cast<size_t>(max(dslot, int64_t(0))) * a.n_kv + h) * wd.ld;
+  int32_t* kp = kept + (static_cast<size_t>(b) * a.n_kv + h) * budget;
+  auto weight_of = [&](uint32_t j) { return slot >= 0 ? src[j] : 0.0f; };
+  for (uint32_t e = now + tid; e < budget; e += EV_THREADS) kp[e] = -1;
+  const uint32_t lo = n > budget ? sinks : n, hi = n > budget ? n - recent : n;  // the candidates [lo, hi)
+  uint32_t want = n > budget ? budget - sinks - recent : 0u;                     // < hi - lo
+  uint32_t thr = 0xffffffffu, ties = 0u;  // kept: key > thr, and the first `ties` with key == thr
+  if (want > 0u) {
+    uint32_t prefix = 0u;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (tid < 256u) s_hist[tid] = 0u;
+      __syncthreads();
+      for (uint32_t j = lo + tid; j < hi; j += EV_THREADS) {
+        const uint32_t key = weight_key(weight_of(j));
+        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
+      }
+      __syncthreads();
+      if (tid == 0u) {
+        uint32_t left = want, d = 255u;
+        while (d > 0u && s_hist[d] < left) left -= s_hist[d--];
+        s_pick[0] = d;
+        s_pick[1] = left;
+      }
+      __syncthreads();
+      prefix |= s_pick[0] << shift;
+      want = s_pick[1];
+      __syncthreads();
+    }
+    thr = prefix;
+    ties = want;
+  }
+  uint32_t at = 0u, tie_at = 0u;
+  for (uint32_t j0 = 0; j0 < n; j0 += EV_THREADS) {
+    const uint32_t j = j0 + tid;
+    const float wt = j < n ? weight_of(j) : 0.0f;
+    const uint32_t key = weight_key(wt);
+    const bool mid = j >= lo && j < hi;
+    const bool tie = mid && key == thr && ties > 0u;
+    const unsigned long long below = (1ull << lane) - 1ull;
+    const unsigned long long mt = __ballot(tie);
+    if (lane == 0u) s_wave[0][wave] = static_cast<uint32_t>(__popcll(mt));
+    __syncthreads();
+    uint32_t tb = tie_at, tsum = 0u;
+    for (uint32_t i = 0; i < EV_THREADS / 64u; ++i) {
+      tb += i < wave ? s_wave[0][i] : 0u;
+      tsum += s_wave[0][i];
+    }
+    const uint32_t trank = tb + static_cast<uint32_t>(__popcll(mt & below));
+    const bool keep = j < n && (!mid || key > thr || (tie && trank < ties));
+    const unsigned long long mk = __ballot(keep);
+    if (lane == 0u) s_wave[1][wave] = static_cast<uint32_t>(__popcll(mk));
+    __syncthreads();
+    uint32_t kb = at, ksum = 0u;
+    for (uint32_t i = 0; i < EV_THREADS / 64u; ++i) {
+      kb += i < wave ? s_wave[1][i] : 0u;
+      ksum += s_wave[1][i];
+    }
+    const uint32_t e = kb + static_cast<uint32_t>(__popcll(mk & below));
+    if (keep && e < budget) {
+      kp[e] = static_cast<int32_t>(j);
+      if (dslot >= 0) dst[e] = wt;
+    }
+    at += ksum;
+    tie_at += tsum;
+  }
+}
+
+// 64 kept entries of one (sequence, kv head) a workgroup: key rows by 16 bytes,
+// then the transposed values, 64 entries of one dim at a time.
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t* __restrict__ dst_pages,
+                                                         uint32_t dst_max_pages, uint32_t budget,
+                                                         const int32_t* __restrict__ kept) {
+  typedef typename std::conditional<F8, uint8_t, uint16_t>::type T;
+  constexpr uint32_t CH = HD * sizeof(T) / 16u;  // 16-byte chunks of a key row
+  __shared__ int32_t s_src[64], s_dst[64];       // (page * n_kv + head) of both sides, -1: none
+  __shared__ uint32_t s_so[64], s_do[64];        // entries in the pages
+  const uint32_t tid = threadIdx.x, groups = (budget + 63u) / 64u;
+  const uint32_t gi = blockIdx.x % groups, bh = blockIdx.x / groups, b = bh / a.n_kv, h = bh % a.n_kv;
+  const uint32_t mask = (1u << a.lp) - 1u;
+  if (tid < 64u) {
+    const uint32_t e = 64u * gi + tid;
+    const int32_t j = e < budget ? kept[static_cast<size_t>(bh) * budget + e] : -1;
+    int32_t s = -1, d = -1;
+    if (j >= 0) {
+      bool ok;
+      const uint32_t sp = paged_id(a, b, static_cast<uint32_t>(j), ok);
+      if (ok) s = static_cast<int32_t>(sp);
+      const uint32_t dp = static_cast<uint32_t>(dst_pages[static_cast<size_t>(b) * dst_max_pages + (e >> a.lp)]);
+      if (dp < a.n_pages) d = static_cast<int32_t>(dp);
+      if (s < 0 || d < 0) paged_flag(a.status);
+      s_so[tid] = static_cast<uint32_t>(j) & mask;
+      s_do[tid] = e & mask;
+    }
+    s_src[tid] = s;
+    s_dst[tid] = d;
+  }
+  __syncthreads();
+  for (uint32_t i = tid; i < 64u * CH; i += 256u) {
+    const uint32_t e = i / CH, c = i % CH;
+    if (s_dst[e] < 0) continue;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (s_src[e] >= 0)
+      x = *reinterpret_cast<const uint4*>(
+          a.k + (((static_cast<size_t>(s_src[e]) * a.n_kv + h) << a.lp) + s_so[e]) * (HD * sizeof(T)) + 16u * c);
+    *reinterpret_cast<uint4*>(const_cast<uint8_t*>(a.k) +
+                              (((static_cast<size_t>(s_dst[e]) * a.n_kv + h) << a.lp) + s_do[e]) * (HD * sizeof(T)) +
+                              16u * c) = x;
+  }
+  const T* vs = reinterpret_cast<const T*>(a.v);
+  T* vd = reinterpret_cast<T*>(const_cast<uint8_t*>(a.v));
+  const uint32_t e = tid & 63u;
+  if (s_dst[e] < 0) return;
+  for (uint32_t d = tid >> 6; d < HD; d += 4u) {
+    T x = 0;
+    if (s_src[e] >= 0) x = vs[((((static_cast<size_t>(s_src[e]) * a.n_kv + h) * HD) + d) << a.lp) + s_so[e]];
+    vd[((((static_cast<size_t>(s_dst[e]) * a.n_kv + h) * HD) + d) << a.lp) + s_do[e]] = x;
+  }
+}
+
+}  // namespace
+
+namespace obs {
+
+int paged_status(obs_ctx* ctx) {
+  uint32_t st = 0;
+  OBS_HIP_TRY(ctx, hipStreamSynchronize(ctx->stream));
+  OBS_HIP_TRY(ctx, hipMemcpy(&st, ctx->status_dev + CTX_ST_PAGED, sizeof st, hipMemcpyDeviceToHost));
+  if (!st) return OBS_OK;
+  OBS_HIP_TRY(ctx, hipMemset(ctx->status_dev + CTX_ST_PAGED, 0, sizeof st));
+  OBS_HIP_TRY(ctx, hipDeviceSynchronize());
+  return set_error(ctx, OBS_E_INVALID, "paged cache: a page id, length or slot in device memory was out of range");
+}
+
+int check_paged(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs_paged_seqs* s, bool pointers) {
+  if (!kv || !s) return set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+  if (kv->dtype != OBS_KV_BF16 && kv->dtype != OBS_KV_E4M3)
+    return set_error(ctx, OBS_E_INVALID, "%s: dtype must be OBS_KV_BF16 or OBS_KV_E4M3 (got %d)", who, kv->dtype);
+  if (pointers) {
+    if (!kv->k_pages || !kv->v_pages || !s->pages || !s->len || (kv->dtype == OBS_KV_E4M3 && (!kv->k_scale || !kv->v_scale)))
+      return set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+    if (!aligned(kv->k_pages, 16) || !aligned(kv->v_pages, 16))
+      return set_error(ctx, OBS_E_ALIGN, "%s: the pages must be 16-byte aligned", who);
+  }
+  if ((kv->head_dim != 64u && kv->head_dim != 128u) || kv->page < 16u || kv->page > 256u || (kv->page & (kv->page - 1u)) ||
+      kv->n_kv == 0 || kv->n_kv > 1024u || kv->n_pages == 0 || kv->n_pages > 0x7fffffffu)
+    return set_error(ctx, OBS_E_SHAPE,
+                     "%s: head_dim must be 64 or 128, page a power of two in [16, 256], n_kv in [1, 1024], n_pages in "
+                     "[1, 2^31) (got %u, %u, %u, %u)", who, kv->head_dim, kv->page, kv->n_kv, kv->n_pages);
+  if (s->n_seqs > PAGED_MAX_SEQS || s->max_pages == 0 ||
+      static_cast<uint64_t>(s->max_pages) * kv->page > PAGED_MAX_ENTRIES || s->n_rows > (1u << 24))
+    return set_error(ctx, OBS_E_SHAPE,
+                     "%s: at most %u sequences, 1 to 2^30 / page pages each and 2^24 token rows (got %u, %u, %u)", who,
+                     PAGED_MAX_SEQS, s->n_seqs, s->max_pages, s->n_rows);
+  return OBS_OK;
+}
+
+int check_heads(obs_ctx* ctx, const char* who, uint32_t n_heads, uint32_t n_kv) {
+  if (n_heads == 0 || n_heads % n_kv != 0 || n_heads / n_kv > 16u)
+    return set_error(ctx, OBS_E_SHAPE, "%s: n_heads must be a multiple of n_kv with at most 16 per kv head (got %u, %u)",
+                     who, n_heads, n_kv);
+  return OBS_OK;
+}
+
+int check_weight(obs_ctx* ctx, const char* who, const obs_kv_weight* w, uint64_t entries, bool pointers) {
+  if (pointers && !w->w) return set_error(ctx, OBS_E_INVALID, "%s: null weight", who);
+  if (pointers && !aligned(w->w, 4)) return set_error(ctx, OBS_E_ALIGN, "%s: weight must be 4-byte aligned", who);
+  if (w->n_slots == 0 || w->n_slots > 0x7fffffffu || w->ld < entries)
+    return set_error(ctx, OBS_E_SHAPE, "%s: weight needs slots and rows of at least %llu entries (got %u, %u)", who,
+                     static_cast<unsigned long long>(entries), w->n_slots, w->ld);
+  return OBS_OK;
+}
+
+}  // namespace obs
+
+extern "C" {
+
+int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,
+                        const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm,
+                        const uint16_t* k_norm, uint16_t* q_out, uint32_t n_heads, float eps, float theta,
+                        const int32_t* pos, uint32_t rope_len, uint32_t q_ld, uint32_t kv_ld, uint32_t q_out_ld) {
+  if (!ctx) return OBS_E_INVALID;
+  const char* who = "obs_attn_prep_paged";
+  int rc = obs::check_paged(ctx, who, kv, seqs, true);
+  if (rc == OBS_OK) rc = obs::check_heads(ctx, who, n_heads, kv->n_kv);
+  if (rc == OBS_OK && weight) rc = obs::check_weight(ctx, who, weight, static_cast<uint64_t>(seqs->max_pages) * kv->page, true);
+  if (rc != OBS_OK) return rc;
+  if (!q || !k || !v || !q_norm || !k_norm || !q_out) return obs::set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+  if (!seqs->row && seqs->n_rows != seqs->n_seqs)
+    return obs::set_error(ctx, OBS_E_SHAPE, "%s: without row, n_rows must be n_seqs (got %u, %u)", who, seqs->n_rows, seqs->n_seqs);
+  const uint32_t hd = kv->head_dim;
+  q_ld = q_ld ? q_ld : n_heads * hd;
+  kv_ld = kv_ld ? kv_ld : kv->n_kv * hd;
+  q_out_ld = q_out_ld ? q_out_ld : n_heads * hd;
+  if (q_ld < n_heads * hd || kv_ld < kv->n_kv * hd || q_out_ld < n_heads * hd || q_ld % 8u || kv_ld % 8u || q_out_ld % 8u)
+    return obs::set_error(ctx, OBS_E_SHAPE, "%s: row strides %u, %u, %u must be multiples of 8 and hold a row", who, q_ld, kv_ld, q_out_ld);
+  if (q_out == q && q_out_ld != q_ld)
+    return obs::set_error(ctx, OBS_E_INVALID, "%s: q_out may be q only with the same row stride", who);
+  if (!obs::aligned(q, 16) || !obs::aligned(k, 16) || !obs::aligned(v, 16) || !obs::aligned(q_norm, 16) ||
+      !obs::aligned(k_norm, 16) || !obs::aligned(q_out, 16))
+    return obs::set_error(ctx, OBS_E_ALIGN, "%s: q, k, v, the norm weights and q_out must be 16-byte aligned", who);
+  if (rope_len == 0 || rope_len > (1u << 24))
+    return obs::set_error(ctx, OBS_E_SHAPE, "%s: rope_len must be in [1, 2^24] (got %u)", who, rope_len);
+  if (seqs->n_rows == 0 || seqs->n_seqs == 0) return OBS_OK;
+  obs::DeviceGuard guard(ctx);
+  PrepArgs p{q, k, v, q_norm, k_norm, q_out, pos, nullptr, n_heads, rope_len, q_ld, kv_ld, q_out_ld, eps};
+  rc = obs::ensure_rope_table(ctx, theta, rope_len, &p.rope);
+  if (rc != OBS_OK) return rc;
+  const Paged a = obs::paged_args(ctx, kv, seqs);
+  const Weight w = obs::weight_args(weight);
+  const uint32_t grid = seqs->n_rows;
+  const bool f8 = kv->dtype == OBS_KV_E4M3;
+  if (hd == 128u && !f8)
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, false><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+  else if (hd == 128u)
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, true><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+  else if (!f8)
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, false><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+  else
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, true><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+  return OBS_OK;
+}
+
+int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,
+                 const int32_t* dst_pages, uint32_t dst_max_pages, const obs_kv_weight* dst_weight, uint32_t sinks,
+                 uint32_t recent, uint32_t budget, int32_t* kept, int32_t* new_len) {
+  if (!ctx) return OBS_E_INVALID;
+  const char* who = "obs_kv_evict";
+  int rc = obs::check_paged(ctx, who, kv, seqs, true);
+  if (rc != OBS_OK) return rc;
+  if (!weight || !dst_weight || !dst_pages || !kept || !new_len)
+    return obs::set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+  rc = obs::check_weight(ctx, who, weight, static_cast<uint64_t>(seqs->max_pages) * kv->page, true);
+  if (rc == OBS_OK) rc = obs::check_weight(ctx, who, dst_weight, budget, true);
+  if (rc != OBS_OK) return rc;
+  if (budget == 0 || static_cast<uint64_t>(sinks) + recent > budget || dst_max_pages == 0 ||
+      static_cast<uint64_t>(dst_max_pages) * kv->page > obs::PAGED_MAX_ENTRIES ||
+      budget > static_cast<uint64_t>(dst_max_pages) * kv->page)
+    return obs::set_error(ctx, OBS_E_SHAPE,
+                          "%s: sinks + recent <= budget <= dst_max_pages * page, at most 2^30 entries (got %u + %u, %u, %u pages)",
+                          who, sinks, recent, budget, dst_max_pages);
+  if (seqs->n_seqs == 0) return OBS_OK;
+  const uint64_t copies = static_cast<uint64_t>(seqs->n_seqs) * kv->n_kv * ((budget + 63u) / 64u);
+  if (copies > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many entries to copy", who);
+  obs::DeviceGuard guard(ctx);
+  const Paged a = obs::paged_args(ctx, kv, seqs);
+  OBS_LAUNCH(ctx, "kv_evict_select", evict_select_kernel<<<seqs->n_seqs * kv->n_kv, EV_THREADS, 0, ctx->stream>>>(
+                                         a, obs::weight_args(weight), obs::weight_args(dst_weight), sinks, recent, budget,
+                                         kept, new_len));
+  const uint32_t grid = static_cast<uint32_t>(copies);
+  const bool f8 = kv->dtype == OBS_KV_E4M3;
+  if (kv->head_dim == 128u && !f8)
+    OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<128, false><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+  else if (kv->head_dim == 128u)
+    OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<128, true><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+  else if (!f8)
+    OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<64, false><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+  else
+    OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<64, true><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+  return OBS_OK;
+}
+
+}  // extern "C"

@@ -35,6 +35,7 @@ OBS_E_UNSUPPORTED = -6
 
 OBS_DECODE_AUTO, OBS_DECODE_MULTI, OBS_DECODE_FUSED = 0, 1, 2
 OBS_PATH_FUSED_DECODE, OBS_PATH_FUSED_ATTN, OBS_PATH_FFN_ONE_LAUNCH = 1, 2, 4  # obs_dispatch_gate bits
+KV_BF16, KV_E4M3 = 0, 1  # OBS_KV_*: what a paged cache holds (PagedKv.dtype)
 # routing rules (obs_route_topk, MoeConfig.route_rule)
 ROUTE_REF, ROUTE_F32 = 0, 1
 
@@ -63,6 +64,7 @@ EXPORTS = (
     "obs_argmax_workspace", "obs_argmax", "obs_embed_q4_rows", "obs_attn_prep_rows", "obs_sdpa_prefill",
     "obs_attn_decode", "obs_layer_decode", "obs_dispatch_gate", "obs_dispatch_info", "obs_set_dispatch_facts", "obs_debug_ffn_wait",
     "obs_measure_read", "obs_measure_mfma",
+    "obs_attn_prep_paged", "obs_sdpa_paged_workspace", "obs_sdpa_paged_decode", "obs_sdpa_paged_prefill", "obs_kv_evict",
 )
 
 
@@ -93,6 +95,21 @@ class ObsAttnLayer(C.Structure):
     KEYS = ("q_w", "q_s", "q_b", "k_w", "k_s", "k_b", "v_w", "v_s", "v_b", "o_w", "o_s", "o_b",
             "in_norm", "q_norm", "k_norm")
     _fields_ = [(k, C.c_void_p) for k in KEYS]
+
+
+class ObsPagedKv(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_uint32), ("page", C.c_uint32), ("n_kv", C.c_uint32), ("head_dim", C.c_uint32),
+                ("dtype", C.c_int32)]
+
+
+class ObsPagedSeqs(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("len", C.c_void_p), ("row", C.c_void_p), ("n_seqs", C.c_uint32),
+                ("max_pages", C.c_uint32), ("n_rows", C.c_uint32)]
+
+
+class ObsKvWeight(C.Structure):
+    _fields_ = [("w", C.c_void_p), ("slot", C.c_void_p), ("n_slots", C.c_uint32), ("ld", C.c_uint32)]
 
 
 class ObsTensorInfo(C.Structure):
@@ -193,6 +210,16 @@ def lib() -> C.CDLL:
         "obs_attn_decode": (i32, [vp, C.POINTER(ObsAttnLayer), vp, vp, vp, u32, f32, f32, vp, vp]),
         "obs_layer_decode": (i32, [vp, C.POINTER(ObsAttnLayer), C.POINTER(ObsMoeConfig), C.POINTER(ObsMoeLayer), vp,
                                    vp, vp, u32, f32, f32, vp, vp, vp, vp, vp]),
+        "obs_attn_prep_paged": (i32, [vp, C.POINTER(ObsPagedKv), C.POINTER(ObsPagedSeqs), C.POINTER(ObsKvWeight), vp,
+                                      vp, vp, vp, vp, vp, u32, f32, f32, vp, u32, u32, u32, u32]),
+        "obs_sdpa_paged_workspace": (i32, [vp, C.POINTER(ObsPagedKv), C.POINTER(ObsPagedSeqs), C.POINTER(ObsKvWeight),
+                                           u32, u32, u32, C.POINTER(sz)]),
+        "obs_sdpa_paged_decode": (i32, [vp, C.POINTER(ObsPagedKv), C.POINTER(ObsPagedSeqs), C.POINTER(ObsKvWeight),
+                                        vp, vp, u32, u32, u32, u32, vp, sz]),
+        "obs_sdpa_paged_prefill": (i32, [vp, C.POINTER(ObsPagedKv), C.POINTER(ObsPagedSeqs), vp, vp, u32, u32, u32,
+                                         u32, vp, sz]),
+        "obs_kv_evict": (i32, [vp, C.POINTER(ObsPagedKv), C.POINTER(ObsPagedSeqs), C.POINTER(ObsKvWeight), vp, u32,
+                               C.POINTER(ObsKvWeight), u32, u32, u32, vp, vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -517,6 +544,46 @@ class ObsidianExecutor:
         self._check(lib().obs_sdpa_prefill(self.ctx, _ptr(q), _ptr(k_cache), _ptr(v_cache_t), _ptr(out), n_heads,
                                            n_kv, head_dim, max_len, pos0, n_tokens, q_ld))
 
+    # -- a paged cache of several sequences (no reference counterpart) ----
+    def attn_prep_paged(self, kv: "PagedKv", seqs: "PagedSeqs", q, k, v, q_norm, k_norm, q_out, n_heads: int,
+                        eps: float, theta: float, rope_len: int, pos=None, weight: "Optional[KvWeight]" = None,
+                        q_ld: int = 0, kv_ld: int = 0, q_out_ld: int = 0) -> None:
+        """q/k norm + RoPE of the batch's token rows, q to q_out, k and v into their pages; the
+        gathered weight of the new entries, if given, starts at 0."""
+        self._check(lib().obs_attn_prep_paged(self.ctx, kv.ref, seqs.ref, weight.ref if weight else None, _ptr(q),
+                                              _ptr(k), _ptr(v), _ptr(q_norm), _ptr(k_norm), _ptr(q_out), n_heads, eps,
+                                              theta, _ptr(pos), rope_len, q_ld, kv_ld, q_out_ld))
+
+    def sdpa_paged_workspace(self, kv: "PagedKv", seqs: "PagedSeqs", n_heads: int,
+                             weight: "Optional[KvWeight]" = None, window: int = 0, sinks: int = 0) -> int:
+        n = C.c_size_t()
+        self._check(lib().obs_sdpa_paged_workspace(self.ctx, kv.ref, seqs.ref, weight.ref if weight else None, n_heads,
+                                                   window, sinks, C.byref(n)))
+        return n.value
+
+    def sdpa_paged_decode(self, kv: "PagedKv", seqs: "PagedSeqs", q, out, n_heads: int, ws,
+                          ws_bytes: Optional[int] = None, window: int = 0, sinks: int = 0,
+                          weight: "Optional[KvWeight]" = None, q_ld: int = 0) -> None:
+        """Attention of one new token a sequence; window 0: of all entries; weight: gathers the
+        softmax weights."""
+        ws_bytes = ws.nbytes if ws_bytes is None else ws_bytes
+        self._check(lib().obs_sdpa_paged_decode(self.ctx, kv.ref, seqs.ref, weight.ref if weight else None, _ptr(q),
+                                                _ptr(out), n_heads, window, sinks, q_ld, _ptr(ws), ws_bytes))
+
+    def sdpa_paged_prefill(self, kv: "PagedKv", seqs: "PagedSeqs", q, out, n_heads: int, ws,
+                           ws_bytes: Optional[int] = None, window: int = 0, sinks: int = 0, q_ld: int = 0) -> None:
+        """Causal attention of a ragged batch of token rows (seqs.row set)."""
+        ws_bytes = ws.nbytes if ws_bytes is None else ws_bytes
+        self._check(lib().obs_sdpa_paged_prefill(self.ctx, kv.ref, seqs.ref, _ptr(q), _ptr(out), n_heads, window,
+                                                 sinks, q_ld, _ptr(ws), ws_bytes))
+
+    def kv_evict(self, kv: "PagedKv", seqs: "PagedSeqs", weight: "KvWeight", dst_pages, dst_max_pages: int,
+                 dst_weight: "KvWeight", sinks: int, recent: int, budget: int, kept, new_len) -> None:
+        """Keeps at most `budget` entries a kv head (the first, the last, and those with the largest
+        gathered weight) and copies them to other pages."""
+        self._check(lib().obs_kv_evict(self.ctx, kv.ref, seqs.ref, weight.ref, _ptr(dst_pages), dst_max_pages,
+                                       dst_weight.ref, sinks, recent, budget, _ptr(kept), _ptr(new_len)))
+
     def download_raw(self, ptr: int, shape, dtype) -> np.ndarray:
         """Copies device bytes at `ptr` into a new host array (Buffer::contents after a drain)."""
         out = np.empty(shape, dtype=dtype)
@@ -545,6 +612,39 @@ class ObsidianExecutor:
             ws_bytes = ws.nbytes if isinstance(ws, DeviceBuffer) else 0
         self._check(lib().obs_moe_prefill(self.ctx, C.byref(c), C.byref(l), _ptr(X), _ptr(residual), _ptr(Y), T,
                                           _ptr(ids), _ptr(weights), _ptr(ws), ws_bytes))
+
+
+class PagedKv:
+    """One layer's pool of key/value pages (obs_paged_kv): keys [n_pages, n_kv, page, head_dim],
+    values [n_pages, n_kv, head_dim, page], bf16 or e4m3 bytes with fp32 scales [n_kv]."""
+
+    def __init__(self, k_pages, v_pages, n_pages: int, page: int, n_kv: int, head_dim: int, dtype: int = KV_BF16,
+                 k_scale=None, v_scale=None):
+        self.held = (k_pages, v_pages, k_scale, v_scale)
+        self.c = ObsPagedKv(_ptr(k_pages), _ptr(v_pages), _ptr(k_scale), _ptr(v_scale), n_pages, page, n_kv, head_dim,
+                            dtype)
+        self.ref = C.byref(self.c)
+
+
+class PagedSeqs:
+    """The sequences of a call (obs_paged_seqs): device arrays pages [n_seqs, max_pages], len [n_seqs]
+    and, for more than one token a sequence, row [n_seqs + 1]."""
+
+    def __init__(self, pages, len_, n_seqs: int, max_pages: int, n_rows: Optional[int] = None, row=None):
+        self.held = (pages, len_, row)
+        self.c = ObsPagedSeqs(_ptr(pages), _ptr(len_), _ptr(row), n_seqs, max_pages,
+                              n_seqs if n_rows is None else n_rows)
+        self.ref = C.byref(self.c)
+
+
+class KvWeight:
+    """Gathered attention weight (obs_kv_weight): fp32 [n_slots, n_kv, ld]; slot: device int32 [n_seqs]
+    or None for slot b of sequence b."""
+
+    def __init__(self, w, n_slots: int, ld: int, slot=None):
+        self.held = (w, slot)
+        self.c = ObsKvWeight(_ptr(w), _ptr(slot), n_slots, ld)
+        self.ref = C.byref(self.c)
 
 
 @dataclass
