@@ -480,8 +480,8 @@ int obs_sdpa_prefill(obs_ctx* ctx, const uint16_t* q, const uint16_t* k_cache, c
 /* The pool of one layer: n_pages pages of `page` entries (a power of two from
  * 16 to 256), head_dim 64 or 128. Keys [n_pages, n_kv, page, head_dim], values
  * transposed [n_pages, n_kv, head_dim, page], both 16-byte aligned, in bf16 or
- * in e4m3 (OCP, magnitudes up to 448) with one fp32 scale per kv head: an entry
- * is the stored value times the scale. */
+ * in e4m3 (OCP, magnitudes up to 448) with one positive fp32 scale per kv head: an
+ * entry is the stored value times the scale. */
 enum { OBS_KV_BF16 = 0, OBS_KV_E4M3 = 1 };
 typedef struct obs_paged_kv {
   void* k_pages; void* v_pages;
@@ -559,6 +559,7 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
 /* The same for all token rows of a batch of prompts (obs_sdpa_prefill; row set):
  * the row at entry i attends to j <= i with window == 0, or j > i - window, or
  * j < sinks; a row whose i is negative (len shorter than its tokens) gets zeros.
+ * A row is not touched by what other rows see, NaN and infinities included.
  * The rows' own keys and values are in the pages already (obs_attn_prep_paged).
  * out bf16 [n_rows, n_heads, head_dim]; workspace as above. */
 int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const uint16_t* q,

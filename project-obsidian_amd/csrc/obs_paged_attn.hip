@@ -427,77 +427,414 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, AttnArgs p, We
 // ---------------------------------------------------------------------------
 // Token rows of prompts
 // ---------------------------------------------------------------------------
-// One wave takes TPG = 16 / G consecutive rows of one sequence and the G heads
-// of one kv head: 16 columns over the entries that any of them sees.
-template <uint32_t HD, bool F8>
-__global__ void __launch_bounds__(64) paged_prefill_kernel(Paged a, AttnArgs p) {
-  constexpr uint32_t NT = HD / 16u;
-  const uint32_t lane = threadIdx.x, col = lane & 15u, g = lane >> 4;
-  const uint32_t TPG = 16u / p.G, kv = blockIdx.x % a.n_kv, item = blockIdx.x / a.n_kv;
-  uint32_t b = a.n_seqs, tile = 0, acc = 0;
-  for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-    const uint32_t o = base + lane;
-    uint32_t own = 0;
-    if (o < a.n_seqs) {
-      const RowSpan r = paged_rows(a, o);
-      own = (r.r1 - r.r0 + TPG - 1u) / TPG;
+// A workgroup takes 256 / G consecutive rows of one sequence and the G heads of
+// one kv head: 256 columns, 64 a wave (two groups of 32), over the blocks of 32
+// entries that any of them sees (or a part of those, where there are few rows).
+// Keys and values go through LDS, read there once per 64 columns: a block is
+// 16 + 16 v_mfma_f32_32x32x16_bf16 (1,024 cycles of a SIMD) against 16 KB of LDS
+// reads a wave (512 of the CU's cycles for the four).
+//   S^T [32 entries x 32 columns] = K . Q^T, O^T [dims x 32 columns] += V^T . P: a
+// lane (column lane % 32, half lane / 32) keeps its column throughout. Row r of
+// the score tile is the block's entry with bits 2 and 3 of r exchanged, so a
+// lane's sixteen scores are entries 8 half .. + 7 and 16 + 8 half .. + 7: the
+// values of one 16-byte read of a transposed value row, in the order of the
+// second product's operand.
+// One wave has a SIMD to itself (512 registers), so products and softmax only
+// overlap inside it: an iteration computes block x's softmax and value product
+// together with block x + 1's scores, which do not depend on them. The running
+// maximum follows the scores only when they pass it by 2^8 (the sums and O are
+// in fp32 and P in bf16, which has fp32's range), so O is hardly ever rescaled.
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
+
+constexpr uint32_t PF_COLS = 256, PF_TARGET = 512, PF_MIN_CHUNK = 8;
+constexpr float PF_SLACK = 8.0f;
+
+// Tiles and blocks of the sequences, as the parts are planned by.
+struct PrefillSeq {
+  uint32_t tiles, nblk;
+};
+__device__ __forceinline__ Span tile_span(const AttnArgs& p, const RowSpan& r, uint32_t n, uint32_t t0, uint32_t t1) {
+  // entry of row t is n - (r1 - t); negative: nothing to see
+  const uint32_t hi0 = n + t0 + 1u > r.r1 ? n + t0 + 1u - r.r1 : 0u, hi1 = n + t1 > r.r1 ? n + t1 - r.r1 : 0u;
+  return span_of(hi0 ? hi0 - 1u : 0u, hi1, p.window, p.sinks);
+}
+__device__ __forceinline__ PrefillSeq prefill_seq(const Paged& a, const AttnArgs& p, uint32_t b) {
+  const RowSpan r = paged_rows(a, b);
+  const uint32_t tq = PF_COLS / p.G, tiles = (r.r1 - r.r0 + tq - 1u) / tq;
+  return {tiles, tiles ? tile_span(p, r, paged_len(a, b), r.r0 + (tiles - 1u) * tq, r.r1).nblk : 0u};
+}
+struct PrefillItem {
+  uint32_t b, tile, split, splits, chunk, first;  // first: the part of the tile's split 0
+};
+// Part `item` of a kv head: sequences in order, in each the last tile (the
+// longest) first, a tile's parts together.
+__device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const AttnArgs& p, uint32_t item, uint32_t lane) {
+  uint32_t chunk = 0xffffffffu;
+  if (p.target) {  // few rows: parts of equal length
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
+      PrefillSeq s{0u, 0u};
+      if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
+      total += wave_sum_u32(s.tiles * s.nblk);
     }
-    const uint32_t incl = wave_scan_u32(own, lane), all = __builtin_amdgcn_readlane(incl, 63);
+    chunk = max(PF_MIN_CHUNK, static_cast<uint32_t>((total * a.n_kv + p.target - 1u) / p.target));
+  }
+  uint32_t acc = 0;
+  for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
+    PrefillSeq s{0u, 0u};
+    if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
+    const uint32_t splits = p.target ? plan_splits(s.nblk, chunk) : 1u;
+    const uint32_t incl = wave_scan_u32(s.tiles * splits, lane), all = __builtin_amdgcn_readlane(incl, 63);
     if (item < acc + all) {
-      const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
-      b = base + before;
-      tile = item - acc - (before ? static_cast<uint32_t>(__builtin_amdgcn_readlane(incl, before - 1u)) : 0u);
-      break;
+      const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
+      const uint32_t before = acc + (l ? static_cast<uint32_t>(__builtin_amdgcn_readlane(incl, l - 1u)) : 0u);
+      const uint32_t tl = __builtin_amdgcn_readlane(s.tiles, l), sp = __builtin_amdgcn_readlane(splits, l);
+      const uint32_t x = (item - before) / sp, split = (item - before) % sp;
+      return {base + l, tl - 1u - x, split, sp, chunk, item - split};
     }
     acc += all;
   }
-  b = __builtin_amdgcn_readfirstlane(b);
-  tile = __builtin_amdgcn_readfirstlane(tile);
+  return {a.n_seqs, 0u, 0u, 1u, chunk, 0u};
+}
+
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(256, 1) paged_prefill_kernel(Paged a, AttnArgs p) {
+  constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = F8 ? 1u : 2u;
+  constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
+  constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
+  constexpr uint32_t NK = (32u * KC + 255u) / 256u, NV = (HD * VC + 255u) / 256u;  // a thread's chunks
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][32u * KROW];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[2][HD * VROW];
+  __shared__ uint32_t s_bad[4];  // entries of a block whose values are not finite, hidden from some rows
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const uint32_t col = lane & 31u, half = lane >> 5;
+  const uint32_t kv = blockIdx.x % a.n_kv;
+  const PrefillItem it = prefill_find(a, p, blockIdx.x / a.n_kv, lane);
+  const uint32_t b = __builtin_amdgcn_readfirstlane(it.b);
   if (b >= a.n_seqs) return;  // uniform
   const RowSpan r = paged_rows(a, b);
-  const uint32_t n = paged_len(a, b);
-  if (lane == 0u && tile == 0u && kv == 0u && paged_len_bad(a, b)) paged_flag(a.status);
-  const uint32_t t0r = r.r0 + tile * TPG, t1r = min(r.r1, t0r + TPG);  // the wave's rows
-  const uint32_t cj = col / p.G, t = t0r + cj, h = kv * p.G + col % p.G;
-  const bool have = cj < TPG && t < t1r;
-  // entry of row t is n - (r1 - t); negative: nothing to see
-  const uint32_t hi = have && n + t + 1u > r.r1 ? n + t + 1u - r.r1 : 0u;
-  const uint32_t lo = p.window && hi > p.window ? hi - p.window : 0u;
-  const uint32_t vhi = n + t1r > r.r1 ? n + t1r - r.r1 : 0u, ihi0 = n + t0r + 1u > r.r1 ? n + t0r + 1u - r.r1 : 0u;
-  const Span s = span_of(ihi0 ? ihi0 - 1u : 0u, vhi, p.window, p.sinks);
+  const uint32_t n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
+  const uint32_t tq = PF_COLS / p.G, t0r = r.r0 + it.tile * tq, t1r = min(r.r1, t0r + tq);
+  if (tid == 0u && it.tile == 0u && it.split == 0u && kv == 0u && paged_len_bad(a, b)) paged_flag(a.status);
+  const Span s = tile_span(p, r, n, t0r, t1r);
+  const uint32_t hi_first = n + t0r + 1u > r.r1 ? n + t0r + 1u - r.r1 : 0u;
+  const uint32_t lo_last = p.window && s.hi > p.window ? s.hi - p.window : 0u;
+  const uint32_t x0 = it.split * (it.splits > 1u ? it.chunk : 0u);
+  const uint32_t x1 = it.splits > 1u ? min(s.nblk, x0 + it.chunk) : s.nblk;
   const float scale = F8 ? p.scale_log2 * a.k_scale[kv] : p.scale_log2;
-  bf16x8_v qb[HD / 32u];
+  if (tid < 4u) s_bad[tid] = 0u;
+
+  // the wave's columns: query slices, limits, state
+  bf16x8_v qb[2][KS];
+  uint32_t hi[2], lo[2];
+  float m[2] = {NEG_INF, NEG_INF}, l[2] = {0.0f, 0.0f};
+  f32x16_v o[2][DT];
 #pragma unroll
-  for (uint32_t ks = 0; ks < HD / 32u; ++ks) {
-    u32x4_v v = {0u, 0u, 0u, 0u};
-    if (have) v = *reinterpret_cast<const u32x4_v*>(p.q + static_cast<size_t>(t) * p.q_ld + h * HD + Block<HD, F8>::q_dim(ks, g));
-    qb[ks] = __builtin_bit_cast(bf16x8_v, v);
-  }
-  Column<HD> c;
-  c.clear();
-  for (uint32_t x = 0; x < s.nblk; ++x) {
-    const uint32_t t0 = s.start(x);
-    bool ok0, ok1;
-    const uint32_t p0 = paged_id(a, b, t0, ok0), p1 = paged_id(a, b, t0 + 16u, ok1);
-    auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
-    if (lane == 0u && ((!ok0 && counts(t0)) || (!ok1 && counts(t0 + 16u)))) paged_flag(a.status);
-    Block<HD, F8> blk;
-    blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
-    __builtin_amdgcn_sched_barrier(0);
-    float sv[8];
-    block_step<HD, F8>(blk, qb, c, t0 + 8u * g, hi, lo, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, true, scale, sv, lane);
-  }
-  c.l += lane_xor16_f32(c.l, lane);
-  c.l += lane_xor32_f32(c.l, lane);
-  if (!have) return;
-  const float inv = c.l == 0.0f ? 0.0f : (F8 ? a.v_scale[kv] : 1.0f) / c.l;
+  for (uint32_t cg = 0; cg < 2; ++cg) {
+    const uint32_t c = 64u * wave + 32u * cg + col, t = t0r + c / p.G;
+    const bool have = c / p.G < tq && t < t1r;
+    hi[cg] = have && n + t + 1u > r.r1 ? n + t + 1u - r.r1 : 0u;
+    lo[cg] = p.window && hi[cg] > p.window ? hi[cg] - p.window : 0u;
+    const uint16_t* qr = p.q + static_cast<size_t>(have ? t : t0r) * p.q_ld + (kv * p.G + c % p.G) * HD + 8u * half;
 #pragma unroll
-  for (uint32_t nt = 0; nt < NT; ++nt) {
-    const float r0 = c.l == 0.0f ? 0.0f : c.o[nt][0] * inv, r1 = c.l == 0.0f ? 0.0f : c.o[nt][1] * inv;
-    const float r2 = c.l == 0.0f ? 0.0f : c.o[nt][2] * inv, r3 = c.l == 0.0f ? 0.0f : c.o[nt][3] * inv;
-    *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t) * p.nh + h) * HD + 16u * nt + 4u * g) =
-        make_uint2(pack_bf16x2(r0, r1), pack_bf16x2(r2, r3));
+    for (uint32_t ks = 0; ks < KS; ++ks) {
+      u32x4_v v = *reinterpret_cast<const u32x4_v*>(qr + 16u * ks);
+      if (!have) v = u32x4_v{0u, 0u, 0u, 0u};
+      qb[cg][ks] = __builtin_bit_cast(bf16x8_v, v);
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d) o[cg][d] = f32x16_v{};
   }
+
+  // page ids of block x's two halves
+  struct Ids {
+    uint32_t p0, p1;
+  };
+  const int32_t* table = a.table + static_cast<size_t>(b) * a.max_pages;
+  auto ids_of = [&](uint32_t x) __attribute__((always_inline)) {
+    const uint32_t t = s.start(min(x, s.nblk - 1u));
+    return Ids{static_cast<uint32_t>(table[min(t >> a.lp, a.max_pages - 1u)]),
+               static_cast<uint32_t>(table[min((t + 16u) >> a.lp, a.max_pages - 1u)])};
+  };
+  const uint32_t pmask = (1u << a.lp) - 1u;
+  u32x4_v kr[NK], vr[NV];
+  auto load_k = [&](uint32_t x, const Ids& id) __attribute__((always_inline)) {
+    const uint32_t t = s.start(min(x, s.nblk - 1u));
+#pragma unroll
+    for (uint32_t i = 0; i < NK; ++i) {
+      const uint32_t c = tid + 256u * i, row = c / KC, e = t + row;
+      if (32u * KC % 256u != 0u && c >= 32u * KC) break;
+      uint32_t pg = row < 16u ? id.p0 : id.p1;
+      pg = pg < a.n_pages ? pg : 0u;
+      kr[i] = *reinterpret_cast<const u32x4_v*>(
+          a.k + (((static_cast<size_t>(pg) * a.n_kv + kv) << a.lp) + (e & pmask)) * (HD * SZ) + 16u * (c % KC));
+    }
+  };
+  auto load_v = [&](uint32_t x, const Ids& id) __attribute__((always_inline)) {
+    const uint32_t t = s.start(min(x, s.nblk - 1u));
+#pragma unroll
+    for (uint32_t i = 0; i < NV; ++i) {
+      const uint32_t c = tid + 256u * i, d = c / VC, e = (16u / SZ) * (c % VC);
+      if (HD * VC % 256u != 0u && c >= HD * VC) break;
+      uint32_t pg = e < 16u ? id.p0 : id.p1;
+      pg = pg < a.n_pages ? pg : 0u;
+      vr[i] = *reinterpret_cast<const u32x4_v*>(
+          a.v + ((((static_cast<size_t>(pg) * a.n_kv + kv) * HD + d) << a.lp) + ((t + e) & pmask)) * SZ);
+    }
+  };
+  // 16 stored bytes as bf16: one or two 16-byte words
+  auto widen = [](const u32x4_v& w, uint32_t j) __attribute__((always_inline)) {
+    if constexpr (F8) {
+      const uint32_t w0 = j ? w.z : w.x, w1 = j ? w.w : w.y;
+      return u32x4_v{e4m3x2_bf16<false>(w0), e4m3x2_bf16<true>(w0), e4m3x2_bf16<false>(w1), e4m3x2_bf16<true>(w1)};
+    } else {
+      return w;
+    }
+  };
+  auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < NK; ++i) {
+      const uint32_t c = tid + 256u * i;
+      if (32u * KC % 256u != 0u && c >= 32u * KC) break;
+      uint16_t* to = &s_k[buf][(c / KC) * KROW + (16u / SZ) * (c % KC)];
+#pragma unroll
+      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(to + 8u * j) = widen(kr[i], j);
+    }
+  };
+  // A block that every row sees whole; the others mask scores and values.
+  auto inner = [&](uint32_t x, const Ids& id) __attribute__((always_inline)) {
+    const uint32_t t = s.start(x);
+    return id.p0 < a.n_pages && id.p1 < a.n_pages && t + 32u <= hi_first && (t >= lo_last || t + 32u <= p.sinks);
+  };
+  // At the edge, values hidden from every row are stored as zero (the pool may
+  // hold anything there), and those that are not finite too: they are added to
+  // the rows that see them apart (add_bad), and no other row meets them.
+  auto store_v = [&](uint32_t buf, uint32_t x, const Ids& id) __attribute__((always_inline)) {
+    const bool edge = !inner(min(x, s.nblk - 1u), id);  // uniform
+    const uint32_t t = s.start(min(x, s.nblk - 1u));
+#pragma unroll
+    for (uint32_t i = 0; i < NV; ++i) {
+      const uint32_t c = tid + 256u * i, d = c / VC;
+      if (HD * VC % 256u != 0u && c >= HD * VC) break;
+#pragma unroll
+      for (uint32_t j = 0; j < 2u / SZ; ++j) {
+        const uint32_t e = (16u / SZ) * (c % VC) + 8u * j;
+        u32x4_v w = widen(vr[i], j);
+        if (edge) {
+          const bool ok = (e < 16u ? id.p0 : id.p1) < a.n_pages;
+          w &= entry_masks(t + e, s.hi, s.lo, p.sinks, ok);
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            const bool blo = (w[q] & 0x7f80u) == 0x7f80u, bhi = (w[q] & 0x7f800000u) == 0x7f800000u;
+            if (blo || bhi) {
+              atomicOr(&s_bad[x & 3u], (blo ? 1u << (e + 2u * q) : 0u) | (bhi ? 2u << (e + 2u * q) : 0u));
+              w[q] &= (blo ? 0u : 0xffffu) | (bhi ? 0u : 0xffff0000u);
+            }
+          }
+        }
+        *reinterpret_cast<u32x4_v*>(&s_v[buf][d * VROW + e]) = w;
+      }
+    }
+  };
+  auto sees = [&](uint32_t e, uint32_t cg) __attribute__((always_inline)) {
+    return e < hi[cg] && (e >= lo[cg] || e < p.sinks);
+  };
+  auto add_bad = [&](uint32_t x, uint32_t bad, const Ids& id) {
+    const uint32_t t = s.start(x);
+    for (; bad; bad &= bad - 1u) {
+      const uint32_t e = t + static_cast<uint32_t>(__builtin_ctz(bad));
+      const uint32_t pg = (e - t) < 16u ? id.p0 : id.p1;  // in range: a bad id's values were masked
+      const size_t base = (static_cast<size_t>(pg) * a.n_kv + kv) * HD;
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+          const size_t at = ((base + 32u * d + 8u * (i / 4u) + 4u * half + i % 4u) << a.lp) + (e & pmask);
+          const uint32_t w = F8 ? e4m3x2_bf16<false>(a.v[at]) << 16
+                                : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(a.v)[at]) << 16;
+          const bool wild = (w & 0x7f800000u) == 0x7f800000u;
+#pragma unroll
+          for (uint32_t cg = 0; cg < 2; ++cg)
+            if (wild && sees(e, cg)) o[cg][d][i] += __uint_as_float(w);
+        }
+    }
+  };
+
+  f32x16_v sc[2];
+  float mx[2];
+  const uint32_t krow = (col & 0x13u) | ((col & 4u) << 1) | ((col & 8u) >> 1);  // bits 2 and 3 exchanged
+  auto scores = [&](uint32_t buf, f32x16_v (&to)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t cg = 0; cg < 2; ++cg) to[cg] = f32x16_v{};
+#pragma unroll
+    for (uint32_t ks = 0; ks < KS; ++ks) {
+      const bf16x8_v kf = *reinterpret_cast<const bf16x8_v*>(&s_k[buf][krow * KROW + 16u * ks + 8u * half]);
+#pragma unroll
+      for (uint32_t cg = 0; cg < 2; ++cg) to[cg] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[cg][ks], to[cg], 0, 0, 0);
+    }
+  };
+  auto maxima = [&](const f32x16_v (&v)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t cg = 0; cg < 2; ++cg) {
+      float t = fmaxf(v[cg][0], v[cg][1]);
+#pragma unroll
+      for (uint32_t i = 2; i < 16; i += 2) t = fmaxf(fmaxf(t, v[cg][i]), v[cg][i + 1]);
+      mx[cg] = fmaxf(t, lane_xor32_f32(t, lane));
+    }
+  };
+
+  if (x0 < x1) {  // uniform
+    Ids id_a = ids_of(x0), id_b = ids_of(x0 + 1u), id_c = ids_of(x0 + 2u);
+    load_k(x0, id_a);
+    load_v(x0, id_a);
+    __syncthreads();  // s_bad is zero
+    store_k(x0 & 1u);
+    store_v(x0 & 1u, x0, id_a);
+    load_k(x0 + 1u, id_b);
+    store_k((x0 + 1u) & 1u);
+    __syncthreads();
+    scores(x0 & 1u, sc);
+    maxima(sc);
+    for (uint32_t x = x0;; ++x) {
+      const Ids id_d = ids_of(x + 3u);
+      const bool edge = !inner(x, id_a);  // uniform
+      if (edge) {
+        const uint32_t t = s.start(x);
+        const bool ok0 = id_a.p0 < a.n_pages, ok1 = id_a.p1 < a.n_pages;
+        auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
+        if (tid == 0u && ((!ok0 && counts(t)) || (!ok1 && counts(t + 16u)))) paged_flag(a.status);
+#pragma unroll
+        for (uint32_t cg = 0; cg < 2; ++cg)
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) {
+            const uint32_t e = t + 16u * (i / 8u) + 8u * half + i % 8u;
+            sc[cg][i] = (i < 8u ? ok0 : ok1) && sees(e, cg) ? sc[cg][i] : NEG_INF;
+          }
+        maxima(sc);
+        const uint32_t bad = __builtin_amdgcn_readfirstlane(s_bad[x & 3u]);
+        if (bad) add_bad(x, bad, id_a);
+      }
+      const bool up0 = mx[0] * scale > m[0] + PF_SLACK, up1 = mx[1] * scale > m[1] + PF_SLACK;
+      if (__any(up0 || up1)) {
+#pragma unroll
+        for (uint32_t cg = 0; cg < 2; ++cg) {
+          const float mn = (cg ? up1 : up0) ? mx[cg] * scale : m[cg];
+          const float f = mn == m[cg] ? 1.0f : __builtin_amdgcn_exp2f(m[cg] - mn);
+          l[cg] *= f;
+          m[cg] = mn;
+#pragma unroll
+          for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) o[cg][d][i] *= f;
+        }
+      }
+      load_k(x + 2u, id_c);
+      load_v(x + 1u, id_b);
+      f32x16_v next[2];
+      scores((x + 1u) & 1u, next);
+      bf16x8_v pb[2][2];
+#pragma unroll
+      for (uint32_t cg = 0; cg < 2; ++cg) {
+        const float mu = m[cg] == NEG_INF ? 0.0f : m[cg];
+        typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+        const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
+#pragma unroll
+        for (uint32_t k2 = 0; k2 < 2; ++k2) {
+          uint32_t pk[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            pk[i] = pack_bf16_pair_rne(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[cg][8 * k2 + 2 * i], scale, -mu)),
+                                       __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cg][8 * k2 + 2 * i + 1], scale, -mu)));
+            l[cg] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pk[i]), ones, l[cg], false);
+          }
+          pb[cg][k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
+        }
+      }
+#pragma unroll
+      for (uint32_t k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d) {
+          const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]);
+#pragma unroll
+          for (uint32_t cg = 0; cg < 2; ++cg) o[cg][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[cg][k2], o[cg][d], 0, 0, 0);
+        }
+      maxima(next);
+      sc[0] = next[0];
+      sc[1] = next[1];
+      if (x + 1u >= x1) break;  // uniform
+      // K of x was read an iteration ago, V of x - 1 too: their buffers take K of x + 2 and V of x + 1
+      store_k(x & 1u);
+      store_v((x + 1u) & 1u, x + 1u, id_b);
+      if (tid == 0u) s_bad[(x + 2u) & 3u] = 0u;
+      __syncthreads();
+      id_a = id_b;
+      id_b = id_c;
+      id_c = id_d;
+    }
+  }
+#pragma unroll
+  for (uint32_t cg = 0; cg < 2; ++cg) {
+    const uint32_t c = 64u * wave + 32u * cg + col, t = t0r + c / p.G, h = kv * p.G + c % p.G;
+    const float L = l[cg] + lane_xor32_f32(l[cg], lane);
+    if (c / p.G >= tq || t >= t1r) continue;
+    if (it.splits == 1u) {
+      const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i += 4) {
+          float v[4];
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[cg][d][i + j] * inv;
+          *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t) * p.nh + h) * HD + 32u * d + 2u * i + 4u * half) =
+              make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+        }
+    } else {
+      if (half == 0u) {
+        p.ml[(static_cast<size_t>(blockIdx.x) * PF_COLS + c) * 2u] = m[cg];
+        p.ml[(static_cast<size_t>(blockIdx.x) * PF_COLS + c) * 2u + 1u] = L;
+      }
+#pragma unroll
+      for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(p.part + (static_cast<size_t>(blockIdx.x) * PF_COLS + c) * HD + 32u * d + 2u * i + 4u * half) =
+              make_float4(o[cg][d][i], o[cg][d][i + 1], o[cg][d][i + 2], o[cg][d][i + 3]);
+    }
+  }
+}
+
+// A tile's parts joined in order: a workgroup per 256 / HD * 4 columns.
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, AttnArgs p, uint32_t items) {
+  constexpr uint32_t CW = 1024u / HD;  // columns of a workgroup, 4 dims a thread
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t part = blockIdx.x / (PF_COLS / CW), c = blockIdx.x % (PF_COLS / CW) * CW + tid / (HD / 4u), d = 4u * (tid % (HD / 4u));
+  const uint32_t kv = part % a.n_kv;
+  const PrefillItem it = prefill_find(a, p, part / a.n_kv, lane);
+  if (it.b >= a.n_seqs || it.splits == 1u || it.split != 0u) return;  // uniform
+  const RowSpan r = paged_rows(a, it.b);
+  const uint32_t tq = PF_COLS / p.G, t = r.r0 + it.tile * tq + c / p.G, h = kv * p.G + c % p.G;
+  if (c / p.G >= tq || t >= r.r1) return;
+  float M = NEG_INF;
+  for (uint32_t i = 0; i < it.splits; ++i)
+    M = fmaxf(M, p.ml[((static_cast<size_t>(it.first + i) * a.n_kv + kv) * PF_COLS + c) * 2u]);
+  float L = 0.0f;
+  f32x4_v o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t i = 0; i < it.splits; ++i) {
+    const size_t at = (static_cast<size_t>(it.first + i) * a.n_kv + kv) * PF_COLS + c;
+    const float m = p.ml[at * 2u], f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+    const f32x4_v x = *reinterpret_cast<const f32x4_v*>(p.part + at * HD + d);
+    L = __builtin_fmaf(p.ml[at * 2u + 1u], f, L);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) o[j] = __builtin_fmaf(x[j], f, o[j]);
+  }
+  const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
+  float v[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[j] * inv;
+  *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t) * p.nh + h) * HD + d) =
+      make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
 // ---------------------------------------------------------------------------
@@ -506,10 +843,10 @@ __global__ void __launch_bounds__(64) paged_prefill_kernel(Paged a, AttnArgs p) 
 constexpr uint32_t DECODE_TARGET = 1024, DECODE_MIN_CHUNK = 8;
 
 // Blocks of 32 that a token can see of a sequence of `entries`.
-uint64_t most_blocks(uint64_t entries, uint32_t window, uint32_t sinks) {
+uint64_t most_blocks(uint64_t entries, uint64_t window, uint32_t sinks) {
   const uint64_t all = (entries + 31u) / 32u;
   if (!window) return all;
-  const uint64_t w = (static_cast<uint64_t>(window) + 31u) / 32u + 1u + (std::min<uint64_t>(sinks, entries) + 31u) / 32u;
+  const uint64_t w = (window + 31u) / 32u + 1u + (std::min<uint64_t>(sinks, entries) + 31u) / 32u;
   return std::min(all, w);
 }
 struct DecodePlan {
@@ -528,6 +865,28 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
   d.ml = up256(d.items * 32u * sizeof(float));
   d.part = up256(d.items * (n_heads / kv->n_kv) * kv->head_dim * sizeof(float));
   d.scores = weight ? up256(static_cast<size_t>(s->n_seqs) * n_heads * d.vis * sizeof(float)) : 0u;
+  return d;
+}
+
+// Prefill: with few rows for the chip (tiles of both kinds of sequence ends
+// counted by the rows alone) a tile's blocks are cut into parts.
+struct PrefillPlan {
+  uint64_t items;  // workgroups at most
+  bool split;
+  size_t ml, part;
+};
+PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32_t n_heads, uint32_t window, uint32_t sinks) {
+  PrefillPlan d{};
+  const uint32_t tq = PF_COLS / (n_heads / kv->n_kv);
+  const uint64_t full = static_cast<uint64_t>(kv->n_kv) * ((s->n_rows + tq - 1u) / tq);
+  // tiles: at most one that is not full a sequence, and none of a sequence without rows
+  const uint64_t tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
+  d.split = 2u * full <= PF_TARGET && most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks) > PF_MIN_CHUNK;
+  d.items = d.split ? PF_TARGET + tiles : tiles;
+  if (d.split) {
+    d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
+    d.part = up256(d.items * PF_COLS * kv->head_dim * sizeof(float));
+  }
   return d;
 }
 
@@ -563,6 +922,16 @@ int launch_decode(obs_ctx* ctx, const Paged& a, const AttnArgs& p, const Weight&
   return OBS_OK;
 }
 
+template <uint32_t HD, bool F8>
+int launch_prefill(obs_ctx* ctx, const Paged& a, const AttnArgs& p, const PrefillPlan& d) {
+  const uint32_t grid = static_cast<uint32_t>(d.items);
+  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, 256, 0, ctx->stream>>>(a, p));
+  if (d.split)
+    OBS_LAUNCH(ctx, "paged_prefill_join",
+               paged_prefill_join_kernel<HD, F8><<<grid * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
+  return OBS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -576,8 +945,13 @@ int obs_sdpa_paged_workspace(obs_ctx* ctx, const obs_paged_kv* kv, const obs_pag
   int rc = obs::check_paged(ctx, who, kv, seqs, false);
   if (rc == OBS_OK) rc = obs::check_heads(ctx, who, n_heads, kv->n_kv);
   if (rc != OBS_OK) return rc;
-  const DecodePlan d = decode_plan(kv, seqs, weight != nullptr, n_heads, window, sinks);
-  *bytes = seqs->row ? 256u : d.ml + d.part + d.scores;
+  if (seqs->row) {
+    const PrefillPlan f = prefill_plan(kv, seqs, n_heads, window, sinks);
+    *bytes = f.ml + f.part + 256u;
+  } else {
+    const DecodePlan d = decode_plan(kv, seqs, weight != nullptr, n_heads, window, sinks);
+    *bytes = d.ml + d.part + d.scores;
+  }
   return OBS_OK;
 }
 
@@ -620,27 +994,20 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
   if (rc == OBS_OK) rc = obs::check_heads(ctx, who, n_heads, kv->n_kv);
   if (rc != OBS_OK) return rc;
   if (!seqs->row) return obs::set_error(ctx, OBS_E_INVALID, "%s: null row (obs_sdpa_paged_decode takes one token a sequence)", who);
-  rc = check_attn(ctx, who, kv, seqs, nullptr, q, out, n_heads, &q_ld, ws, ws_bytes, 256u);
+  const PrefillPlan d = prefill_plan(kv, seqs, n_heads, window, sinks);
+  rc = check_attn(ctx, who, kv, seqs, nullptr, q, out, n_heads, &q_ld, ws, ws_bytes, d.ml + d.part + 256u);
   if (rc != OBS_OK) return rc;
   if (seqs->n_seqs == 0 || seqs->n_rows == 0) return OBS_OK;
-  const uint32_t G = n_heads / kv->n_kv, tpg = 16u / G;
-  const uint64_t grid = (static_cast<uint64_t>(seqs->n_rows + tpg - 1u) / tpg + seqs->n_seqs) * kv->n_kv;
-  if (grid > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many rows and heads", who);
+  if (d.items * 32u > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many rows and heads", who);
   obs::DeviceGuard guard(ctx);
   const Paged a = obs::paged_args(ctx, kv, seqs);
-  const AttnArgs p{q, out, nullptr, nullptr, nullptr, n_heads, G, window, sinks, q_ld, 0u, 0u, 1u,
+  uint8_t* wb = static_cast<uint8_t*>(ws);
+  const AttnArgs p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr, n_heads,
+                   n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u,
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
-  const uint32_t gr = static_cast<uint32_t>(grid);
   const bool f8 = kv->dtype == OBS_KV_E4M3;
-  if (kv->head_dim == 128u && !f8)
-    OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<128, false><<<gr, 64, 0, ctx->stream>>>(a, p));
-  else if (kv->head_dim == 128u)
-    OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<128, true><<<gr, 64, 0, ctx->stream>>>(a, p));
-  else if (!f8)
-    OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<64, false><<<gr, 64, 0, ctx->stream>>>(a, p));
-  else
-    OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<64, true><<<gr, 64, 0, ctx->stream>>>(a, p));
-  return OBS_OK;
+  if (kv->head_dim == 128u) return f8 ? launch_prefill<128, true>(ctx, a, p, d) : launch_prefill<128, false>(ctx, a, p, d);
+  return f8 ? launch_prefill<64, true>(ctx, a, p, d) : launch_prefill<64, false>(ctx, a, p, d);
 }
 
 }  // extern "C"

@@ -337,6 +337,47 @@ def test_prefill_peaked_scores(exe):
     _prefill_case(exe, (32, 4, 128, 32, False), [300, 65], [129, 65], 0, 0, 37, k_std=30.0)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (24, 2), (90, 40)])
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16, False), (16, 16, 64, 32, True), (12, 2, 128, 32, False)], ids=str)
+def test_prefill_rows_do_not_meet_hidden_nan(exe, shape, window, sinks):
+    """NaN keys and NaN (in bf16 also infinite) values in some entries: rows that do
+    not see them are as if they were not there, rows that do are not finite."""
+    nh, nkv, hd, page, f8 = shape
+    lens, new = [150, 40], [120, 40]
+    rows = [0, 120, 160]
+    nan_k, nan_v, inf_v = [35, 100], [3, 77, 110], [] if f8 else [60]
+    for what in ("k", "v"):
+        rng = np.random.default_rng(83)
+        pool = Pool(exe, rng, lens, nkv, hd, page, f8)
+        clean = {b: (pool.entries(b, "k"), pool.entries(b, "v")) for b in range(2)}
+        bad = nan_k if what == "k" else nan_v + inf_v
+        for j in bad:
+            p, o = pool.table[0, j // page], j % page
+            if what == "k":
+                pool.k[p, :, o, 5] = 0x7F if f8 else NAN16
+            else:
+                pool.v[p, :, :, o] = 0x7F if f8 else (0x7F80 if j in inf_v else NAN16)
+        pool.up()
+        q = synth.bf16_normal(rng, (160, nh, hd), 2.0)
+        out = exe.upload(np.full((160, nh, hd), FILL16, np.uint16))
+        seqs = pool.seqs(rows)
+        ws = exe.alloc(exe.sdpa_paged_workspace(pool.kv, seqs, nh, None, window, sinks), np.uint8)
+        exe.sdpa_paged_prefill(pool.kv, seqs, exe.upload(q), out, nh, ws, window=window, sinks=sinks)
+        exe.device_status()
+        got = _f64(out.download())
+        for b in range(2):
+            k, v = clean[b]
+            for r in range(new[b]):
+                n, i = lens[b], lens[b] - new[b] + r
+                vis = _visible(i, n, window, sinks)
+                g = got[rows[b] + r]
+                if b == 0 and any(vis[j] for j in bad):
+                    assert not np.any(np.isfinite(g)), (what, r)
+                    continue
+                ref, bound, _, _ = _attend(_f64(q[rows[b] + r]), k, v, vis)
+                assert np.all(np.abs(g - ref) <= bound), (what, b, r)
+
+
 # ---- append -------------------------------------------------------------------
 
 def _prep_case(exe, shape, lens, new, seed, pos=None, rope_len=9000, pad_rows=0, weight=True, one=False):
