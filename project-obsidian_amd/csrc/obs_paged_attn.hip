@@ -445,6 +445,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, AttnArgs p, We
 // maximum follows the scores only when they pass it by 2^8 (the sums and O are
 // in fp32 and P in bf16, which has fp32's range), so O is hardly ever rescaled.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
 
 constexpr uint32_t PF_COLS = 256, PF_TARGET = 512, PF_MIN_CHUNK = 8;
 constexpr float PF_SLACK = 8.0f;
@@ -477,7 +478,7 @@ __device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const AttnAr
       if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
       total += wave_sum_u32(s.tiles * s.nblk);
     }
-    chunk = max(PF_MIN_CHUNK, static_cast<uint32_t>((total * a.n_kv + p.target - 1u) / p.target));
+    chunk = uniform(max(PF_MIN_CHUNK, static_cast<uint32_t>((total * a.n_kv + p.target - 1u) / p.target)));
   }
   uint32_t acc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
@@ -490,7 +491,7 @@ __device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const AttnAr
       const uint32_t before = acc + (l ? static_cast<uint32_t>(__builtin_amdgcn_readlane(incl, l - 1u)) : 0u);
       const uint32_t tl = __builtin_amdgcn_readlane(s.tiles, l), sp = __builtin_amdgcn_readlane(splits, l);
       const uint32_t x = (item - before) / sp, split = (item - before) % sp;
-      return {base + l, tl - 1u - x, split, sp, chunk, item - split};
+      return {uniform(base + l), uniform(tl - 1u - x), uniform(split), uniform(sp), uniform(chunk), uniform(item - split)};
     }
     acc += all;
   }
@@ -498,89 +499,94 @@ __device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const AttnAr
 }
 
 template <uint32_t HD, bool F8>
-__global__ void __launch_bounds__(256, 1) paged_prefill_kernel(Paged a, AttnArgs p) {
+__global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p) {
   constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = F8 ? 1u : 2u;
   constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
   constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
-  constexpr uint32_t NK = (32u * KC + 255u) / 256u, NV = (HD * VC + 255u) / 256u;  // a thread's chunks
+  constexpr uint32_t KN = 32u * KC, VN = HD * VC;       // chunks of a block: 512, 256 or 128, at most one a thread
   __shared__ __attribute__((aligned(16))) uint16_t s_k[2][32u * KROW];
   __shared__ __attribute__((aligned(16))) uint16_t s_v[2][HD * VROW];
-  __shared__ uint32_t s_bad[4];  // entries of a block whose values are not finite, hidden from some rows
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ uint32_t s_bad;  // an edge block holds values that are not finite
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
   const uint32_t col = lane & 31u, half = lane >> 5;
   const uint32_t kv = blockIdx.x % a.n_kv;
   const PrefillItem it = prefill_find(a, p, blockIdx.x / a.n_kv, lane);
-  const uint32_t b = __builtin_amdgcn_readfirstlane(it.b);
+  const uint32_t b = it.b;
   if (b >= a.n_seqs) return;  // uniform
-  const RowSpan r = paged_rows(a, b);
-  const uint32_t n = __builtin_amdgcn_readfirstlane(paged_len(a, b));
-  const uint32_t tq = PF_COLS / p.G, t0r = r.r0 + it.tile * tq, t1r = min(r.r1, t0r + tq);
+  // everything of the tile in scalar registers: no address or branch below takes the vector unit
+  RowSpan r = paged_rows(a, b);
+  r = {uniform(r.r0), uniform(r.r1)};
+  const uint32_t n = uniform(paged_len(a, b));
+  const uint32_t tq = PF_COLS / p.G, t0r = r.r0 + it.tile * tq, t1r = umin(r.r1, t0r + tq);
   if (tid == 0u && it.tile == 0u && it.split == 0u && kv == 0u && paged_len_bad(a, b)) paged_flag(a.status);
   const Span s = tile_span(p, r, n, t0r, t1r);
   const uint32_t hi_first = n + t0r + 1u > r.r1 ? n + t0r + 1u - r.r1 : 0u;
   const uint32_t lo_last = p.window && s.hi > p.window ? s.hi - p.window : 0u;
   const uint32_t x0 = it.split * (it.splits > 1u ? it.chunk : 0u);
-  const uint32_t x1 = it.splits > 1u ? min(s.nblk, x0 + it.chunk) : s.nblk;
-  const float scale = F8 ? p.scale_log2 * a.k_scale[kv] : p.scale_log2;
-  if (tid < 4u) s_bad[tid] = 0u;
+  const uint32_t x1 = it.splits > 1u ? umin(s.nblk, x0 + it.chunk) : s.nblk;
+  const float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
+  if (tid == 0u) s_bad = 0u;
 
   // the wave's columns: query slices, limits, state
-  bf16x8_v qb[2][KS];
-  uint32_t hi[2], lo[2];
-  float m[2] = {NEG_INF, NEG_INF}, l[2] = {0.0f, 0.0f};
-  f32x16_v o[2][DT];
-#pragma unroll
-  for (uint32_t cg = 0; cg < 2; ++cg) {
-    const uint32_t c = 64u * wave + 32u * cg + col, t = t0r + c / p.G;
-    const bool have = c / p.G < tq && t < t1r;
-    hi[cg] = have && n + t + 1u > r.r1 ? n + t + 1u - r.r1 : 0u;
-    lo[cg] = p.window && hi[cg] > p.window ? hi[cg] - p.window : 0u;
-    const uint16_t* qr = p.q + static_cast<size_t>(have ? t : t0r) * p.q_ld + (kv * p.G + c % p.G) * HD + 8u * half;
+  const uint32_t c = 32u * wave + col, t_row = t0r + c / p.G;
+  const bool have = c / p.G < tq && t_row < t1r;
+  const uint32_t hi = have && n + t_row + 1u > r.r1 ? n + t_row + 1u - r.r1 : 0u;
+  const uint32_t lo = p.window && hi > p.window ? hi - p.window : 0u;
+  bf16x8_v qb[KS];
+  {
+    const uint16_t* qr = p.q + static_cast<size_t>(have ? t_row : t0r) * p.q_ld + (kv * p.G + c % p.G) * HD + 8u * half;
 #pragma unroll
     for (uint32_t ks = 0; ks < KS; ++ks) {
       u32x4_v v = *reinterpret_cast<const u32x4_v*>(qr + 16u * ks);
       if (!have) v = u32x4_v{0u, 0u, 0u, 0u};
-      qb[cg][ks] = __builtin_bit_cast(bf16x8_v, v);
+      qb[ks] = __builtin_bit_cast(bf16x8_v, v);
     }
-#pragma unroll
-    for (uint32_t d = 0; d < DT; ++d) o[cg][d] = f32x16_v{};
   }
+  float m = NEG_INF, l = 0.0f;
+  f32x16_v o[DT];
+#pragma unroll
+  for (uint32_t d = 0; d < DT; ++d) o[d] = f32x16_v{};
 
-  // page ids of block x's two halves
-  struct Ids {
-    uint32_t p0, p1;
+  // A listed block: its first entry, the page ids of its halves, and whether any
+  // row hides any of it. Behind the last block the last one again (unused).
+  struct Blk {
+    uint32_t t, p0, p1;
+    bool edge;
   };
   const int32_t* table = a.table + static_cast<size_t>(b) * a.max_pages;
-  auto ids_of = [&](uint32_t x) __attribute__((always_inline)) {
-    const uint32_t t = s.start(min(x, s.nblk - 1u));
-    return Ids{static_cast<uint32_t>(table[min(t >> a.lp, a.max_pages - 1u)]),
-               static_cast<uint32_t>(table[min((t + 16u) >> a.lp, a.max_pages - 1u)])};
-  };
   const uint32_t pmask = (1u << a.lp) - 1u;
-  u32x4_v kr[NK], vr[NV];
-  auto load_k = [&](uint32_t x, const Ids& id) __attribute__((always_inline)) {
-    const uint32_t t = s.start(min(x, s.nblk - 1u));
-#pragma unroll
-    for (uint32_t i = 0; i < NK; ++i) {
-      const uint32_t c = tid + 256u * i, row = c / KC, e = t + row;
-      if (32u * KC % 256u != 0u && c >= 32u * KC) break;
-      uint32_t pg = row < 16u ? id.p0 : id.p1;
-      pg = pg < a.n_pages ? pg : 0u;
-      kr[i] = *reinterpret_cast<const u32x4_v*>(
-          a.k + (((static_cast<size_t>(pg) * a.n_kv + kv) << a.lp) + (e & pmask)) * (HD * SZ) + 16u * (c % KC));
-    }
+  auto block_ids = [&](uint32_t x) __attribute__((always_inline)) {
+    const uint32_t t = s.start(umin(x, s.nblk - 1u));
+    return Blk{t, static_cast<uint32_t>(table[umin(t >> a.lp, a.max_pages - 1u)]),
+               static_cast<uint32_t>(table[umin((t + 16u) >> a.lp, a.max_pages - 1u)]), false};
   };
-  auto load_v = [&](uint32_t x, const Ids& id) __attribute__((always_inline)) {
-    const uint32_t t = s.start(min(x, s.nblk - 1u));
-#pragma unroll
-    for (uint32_t i = 0; i < NV; ++i) {
-      const uint32_t c = tid + 256u * i, d = c / VC, e = (16u / SZ) * (c % VC);
-      if (HD * VC % 256u != 0u && c >= HD * VC) break;
-      uint32_t pg = e < 16u ? id.p0 : id.p1;
-      pg = pg < a.n_pages ? pg : 0u;
-      vr[i] = *reinterpret_cast<const u32x4_v*>(
-          a.v + ((((static_cast<size_t>(pg) * a.n_kv + kv) * HD + d) << a.lp) + ((t + e) & pmask)) * SZ);
-    }
+  auto block_of = [&](Blk k) __attribute__((always_inline)) {  // waits for the ids
+    k.p0 = uniform(k.p0);
+    k.p1 = uniform(k.p1);
+    k.edge = !(k.p0 < a.n_pages && k.p1 < a.n_pages && k.t + 32u <= hi_first && (k.t >= lo_last || k.t + 32u <= p.sinks));
+    return k;
+  };
+  // A wave's chunks lie in one half of the block, so in one page: a scalar base
+  // and a constant offset a lane. Where a block has fewer chunks than threads,
+  // the first waves bring keys and the last ones values.
+  const uint32_t kc = tid, vc = VN == 512u ? tid : tid ^ 256u;
+  const bool has_k = kc < KN, has_v = vc < VN;  // wave-uniform
+  const uint32_t kh = uniform(kc / (KN / 2u)), vh = uniform(vc / (VN / 2u));
+  const uint32_t v_dim = vc % (VN / 2u) / (VC / 2u), v_ent = 16u * vh + (16u / SZ) * (vc % (VC / 2u));
+  const uint32_t koff = ((kc / KC) & pmask) * (HD * SZ) + 16u * (kc % KC);
+  const uint32_t voff = ((v_dim << a.lp) + (v_ent & pmask)) * SZ;
+  u32x4_v kr, vr;
+  auto page_of = [&](const Blk& k, uint32_t h) __attribute__((always_inline)) {
+    const uint32_t pg = h ? k.p1 : k.p0;
+    return static_cast<size_t>(pg < a.n_pages ? pg : 0u) * a.n_kv + kv;
+  };
+  auto load_k = [&](const Blk& k) __attribute__((always_inline)) {
+    const uint8_t* base = a.k + ((page_of(k, kh) << a.lp) + (k.t & pmask)) * (HD * SZ);
+    if (KN == 512u || has_k) kr = *reinterpret_cast<const u32x4_v*>(base + koff);
+  };
+  auto load_v = [&](const Blk& k) __attribute__((always_inline)) {
+    const uint8_t* base = a.v + ((page_of(k, vh) * HD << a.lp) + (k.t & pmask)) * SZ;
+    if (VN == 512u || has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
   };
   // 16 stored bytes as bf16: one or two 16-byte words
   auto widen = [](const u32x4_v& w, uint32_t j) __attribute__((always_inline)) {
@@ -592,215 +598,180 @@ __global__ void __launch_bounds__(256, 1) paged_prefill_kernel(Paged a, AttnArgs
     }
   };
   auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
+    if (KN == 512u || has_k) {
+      uint16_t* to = &s_k[buf][(kc / KC) * KROW + (16u / SZ) * (kc % KC)];
 #pragma unroll
-    for (uint32_t i = 0; i < NK; ++i) {
-      const uint32_t c = tid + 256u * i;
-      if (32u * KC % 256u != 0u && c >= 32u * KC) break;
-      uint16_t* to = &s_k[buf][(c / KC) * KROW + (16u / SZ) * (c % KC)];
-#pragma unroll
-      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(to + 8u * j) = widen(kr[i], j);
+      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(to + 8u * j) = widen(kr, j);
     }
-  };
-  // A block that every row sees whole; the others mask scores and values.
-  auto inner = [&](uint32_t x, const Ids& id) __attribute__((always_inline)) {
-    const uint32_t t = s.start(x);
-    return id.p0 < a.n_pages && id.p1 < a.n_pages && t + 32u <= hi_first && (t >= lo_last || t + 32u <= p.sinks);
   };
   // At the edge, values hidden from every row are stored as zero (the pool may
-  // hold anything there), and those that are not finite too: they are added to
-  // the rows that see them apart (add_bad), and no other row meets them.
-  auto store_v = [&](uint32_t buf, uint32_t x, const Ids& id) __attribute__((always_inline)) {
-    const bool edge = !inner(min(x, s.nblk - 1u), id);  // uniform
-    const uint32_t t = s.start(min(x, s.nblk - 1u));
+  // hold anything there), and those that are not finite too: the rows that see
+  // them get them at the end, and no other row meets them.
+  auto store_v = [&](uint32_t buf, const Blk& k) __attribute__((always_inline)) {
+    if (VN == 512u || has_v) {
+      u32x4_v w[2u / SZ];
 #pragma unroll
-    for (uint32_t i = 0; i < NV; ++i) {
-      const uint32_t c = tid + 256u * i, d = c / VC;
-      if (HD * VC % 256u != 0u && c >= HD * VC) break;
+      for (uint32_t j = 0; j < 2u / SZ; ++j) w[j] = widen(vr, j);
+      if (k.edge) {  // uniform
+        const bool ok = (vh ? k.p1 : k.p0) < a.n_pages;
+        bool bad = false;
 #pragma unroll
-      for (uint32_t j = 0; j < 2u / SZ; ++j) {
-        const uint32_t e = (16u / SZ) * (c % VC) + 8u * j;
-        u32x4_v w = widen(vr[i], j);
-        if (edge) {
-          const bool ok = (e < 16u ? id.p0 : id.p1) < a.n_pages;
-          w &= entry_masks(t + e, s.hi, s.lo, p.sinks, ok);
+        for (uint32_t j = 0; j < 2u / SZ; ++j) {
+          w[j] &= entry_masks(k.t + v_ent + 8u * j, s.hi, s.lo, p.sinks, ok);
 #pragma unroll
           for (uint32_t q = 0; q < 4; ++q) {
-            const bool blo = (w[q] & 0x7f80u) == 0x7f80u, bhi = (w[q] & 0x7f800000u) == 0x7f800000u;
-            if (blo || bhi) {
-              atomicOr(&s_bad[x & 3u], (blo ? 1u << (e + 2u * q) : 0u) | (bhi ? 2u << (e + 2u * q) : 0u));
-              w[q] &= (blo ? 0u : 0xffffu) | (bhi ? 0u : 0xffff0000u);
-            }
+            const bool blo = (w[j][q] & 0x7f80u) == 0x7f80u, bhi = (w[j][q] & 0x7f800000u) == 0x7f800000u;
+            bad = bad || blo || bhi;
+            w[j][q] &= (blo ? 0u : 0xffffu) | (bhi ? 0u : 0xffff0000u);
           }
         }
-        *reinterpret_cast<u32x4_v*>(&s_v[buf][d * VROW + e]) = w;
+        if (bad) s_bad = 1u;
       }
+#pragma unroll
+      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(&s_v[buf][v_dim * VROW + v_ent + 8u * j]) = w[j];
     }
   };
-  auto sees = [&](uint32_t e, uint32_t cg) __attribute__((always_inline)) {
-    return e < hi[cg] && (e >= lo[cg] || e < p.sinks);
-  };
-  auto add_bad = [&](uint32_t x, uint32_t bad, const Ids& id) {
-    const uint32_t t = s.start(x);
-    for (; bad; bad &= bad - 1u) {
-      const uint32_t e = t + static_cast<uint32_t>(__builtin_ctz(bad));
-      const uint32_t pg = (e - t) < 16u ? id.p0 : id.p1;  // in range: a bad id's values were masked
-      const size_t base = (static_cast<size_t>(pg) * a.n_kv + kv) * HD;
-#pragma unroll
-      for (uint32_t d = 0; d < DT; ++d)
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-          const size_t at = ((base + 32u * d + 8u * (i / 4u) + 4u * half + i % 4u) << a.lp) + (e & pmask);
-          const uint32_t w = F8 ? e4m3x2_bf16<false>(a.v[at]) << 16
-                                : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(a.v)[at]) << 16;
-          const bool wild = (w & 0x7f800000u) == 0x7f800000u;
-#pragma unroll
-          for (uint32_t cg = 0; cg < 2; ++cg)
-            if (wild && sees(e, cg)) o[cg][d][i] += __uint_as_float(w);
-        }
-    }
-  };
+  auto sees = [&](uint32_t e) __attribute__((always_inline)) { return e < hi && (e >= lo || e < p.sinks); };
 
-  f32x16_v sc[2];
-  float mx[2];
+  f32x16_v sa, sb;  // scores of this block and of the next, in turn
+  float mx;
   const uint32_t krow = (col & 0x13u) | ((col & 4u) << 1) | ((col & 8u) >> 1);  // bits 2 and 3 exchanged
-  auto scores = [&](uint32_t buf, f32x16_v (&to)[2]) __attribute__((always_inline)) {
+  auto scores = [&](uint32_t buf, f32x16_v& to) __attribute__((always_inline)) {
+    to = f32x16_v{};
 #pragma unroll
-    for (uint32_t cg = 0; cg < 2; ++cg) to[cg] = f32x16_v{};
-#pragma unroll
-    for (uint32_t ks = 0; ks < KS; ++ks) {
-      const bf16x8_v kf = *reinterpret_cast<const bf16x8_v*>(&s_k[buf][krow * KROW + 16u * ks + 8u * half]);
-#pragma unroll
-      for (uint32_t cg = 0; cg < 2; ++cg) to[cg] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qb[cg][ks], to[cg], 0, 0, 0);
-    }
+    for (uint32_t ks = 0; ks < KS; ++ks)
+      to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          *reinterpret_cast<const bf16x8_v*>(&s_k[buf][krow * KROW + 16u * ks + 8u * half]), qb[ks], to, 0, 0, 0);
   };
-  auto maxima = [&](const f32x16_v (&v)[2]) __attribute__((always_inline)) {
+  auto maximum = [&](const f32x16_v& v) __attribute__((always_inline)) {
+    float t = fmaxf(v[0], v[1]);
 #pragma unroll
-    for (uint32_t cg = 0; cg < 2; ++cg) {
-      float t = fmaxf(v[cg][0], v[cg][1]);
-#pragma unroll
-      for (uint32_t i = 2; i < 16; i += 2) t = fmaxf(fmaxf(t, v[cg][i]), v[cg][i + 1]);
-      mx[cg] = fmaxf(t, lane_xor32_f32(t, lane));
-    }
+    for (uint32_t i = 2; i < 16; i += 2) t = fmaxf(fmaxf(t, v[i]), v[i + 1]);
+    mx = fmaxf(t, lane_xor32_f32(t, lane));
   };
 
   if (x0 < x1) {  // uniform
-    Ids id_a = ids_of(x0), id_b = ids_of(x0 + 1u), id_c = ids_of(x0 + 2u);
-    load_k(x0, id_a);
-    load_v(x0, id_a);
+    Blk ka = block_of(block_ids(x0)), kb = block_of(block_ids(x0 + 1u)), kcb = block_of(block_ids(x0 + 2u));
+    load_k(ka);
+    load_v(ka);
     __syncthreads();  // s_bad is zero
     store_k(x0 & 1u);
-    store_v(x0 & 1u, x0, id_a);
-    load_k(x0 + 1u, id_b);
+    store_v(x0 & 1u, ka);
+    load_k(kb);
     store_k((x0 + 1u) & 1u);
     __syncthreads();
-    scores(x0 & 1u, sc);
-    maxima(sc);
-    for (uint32_t x = x0;; ++x) {
-      const Ids id_d = ids_of(x + 3u);
-      const bool edge = !inner(x, id_a);  // uniform
-      if (edge) {
-        const uint32_t t = s.start(x);
-        const bool ok0 = id_a.p0 < a.n_pages, ok1 = id_a.p1 < a.n_pages;
+    scores(x0 & 1u, sa);
+    maximum(sa);
+    auto iteration = [&](uint32_t x, f32x16_v& sc, f32x16_v& next) __attribute__((always_inline)) {
+      const Blk kd = block_ids(x + 3u);
+      if (ka.edge) {  // uniform
+        const bool ok0 = ka.p0 < a.n_pages, ok1 = ka.p1 < a.n_pages;
         auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
-        if (tid == 0u && ((!ok0 && counts(t)) || (!ok1 && counts(t + 16u)))) paged_flag(a.status);
+        if (tid == 0u && ((!ok0 && counts(ka.t)) || (!ok1 && counts(ka.t + 16u)))) paged_flag(a.status);
 #pragma unroll
-        for (uint32_t cg = 0; cg < 2; ++cg)
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
-            const uint32_t e = t + 16u * (i / 8u) + 8u * half + i % 8u;
-            sc[cg][i] = (i < 8u ? ok0 : ok1) && sees(e, cg) ? sc[cg][i] : NEG_INF;
-          }
-        maxima(sc);
-        const uint32_t bad = __builtin_amdgcn_readfirstlane(s_bad[x & 3u]);
-        if (bad) add_bad(x, bad, id_a);
+        for (uint32_t i = 0; i < 16; ++i)
+          sc[i] = (i < 8u ? ok0 : ok1) && sees(ka.t + 16u * (i / 8u) + 8u * half + i % 8u) ? sc[i] : NEG_INF;
+        maximum(sc);
       }
-      const bool up0 = mx[0] * scale > m[0] + PF_SLACK, up1 = mx[1] * scale > m[1] + PF_SLACK;
-      if (__any(up0 || up1)) {
+      const bool up = mx * scale > m + PF_SLACK;
+      if (__any(up)) {
+        const float mn = up ? mx * scale : m;
+        const float f = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        m = mn;
 #pragma unroll
-        for (uint32_t cg = 0; cg < 2; ++cg) {
-          const float mn = (cg ? up1 : up0) ? mx[cg] * scale : m[cg];
-          const float f = mn == m[cg] ? 1.0f : __builtin_amdgcn_exp2f(m[cg] - mn);
-          l[cg] *= f;
-          m[cg] = mn;
+        for (uint32_t d = 0; d < DT; ++d)
 #pragma unroll
-          for (uint32_t d = 0; d < DT; ++d)
-#pragma unroll
-            for (uint32_t i = 0; i < 16; ++i) o[cg][d][i] *= f;
-        }
+          for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
       }
-      load_k(x + 2u, id_c);
-      load_v(x + 1u, id_b);
-      f32x16_v next[2];
+      load_k(kcb);
+      load_v(kb);
+      __builtin_amdgcn_sched_barrier(0);  // in flight from here to the end of the iteration
       scores((x + 1u) & 1u, next);
-      bf16x8_v pb[2][2];
+      const float mu = m == NEG_INF ? 0.0f : m;
+      typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+      const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
+      bf16x8_v pb[2];
 #pragma unroll
-      for (uint32_t cg = 0; cg < 2; ++cg) {
-        const float mu = m[cg] == NEG_INF ? 0.0f : m[cg];
-        typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
-        const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
+      for (uint32_t k2 = 0; k2 < 2; ++k2) {
+        uint32_t pk[4];
 #pragma unroll
-        for (uint32_t k2 = 0; k2 < 2; ++k2) {
-          uint32_t pk[4];
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            pk[i] = pack_bf16_pair_rne(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[cg][8 * k2 + 2 * i], scale, -mu)),
-                                       __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cg][8 * k2 + 2 * i + 1], scale, -mu)));
-            l[cg] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pk[i]), ones, l[cg], false);
-          }
-          pb[cg][k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
+        for (uint32_t i = 0; i < 4; ++i) {
+          pk[i] = pack_bf16_pair_rne(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i], scale, -mu)),
+                                     __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i + 1], scale, -mu)));
+          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pk[i]), ones, l, false);
         }
+        pb[k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
       }
 #pragma unroll
       for (uint32_t k2 = 0; k2 < 2; ++k2)
 #pragma unroll
-        for (uint32_t d = 0; d < DT; ++d) {
-          const bf16x8_v vf = *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]);
-#pragma unroll
-          for (uint32_t cg = 0; cg < 2; ++cg) o[cg][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pb[cg][k2], o[cg][d], 0, 0, 0);
-        }
-      maxima(next);
-      sc[0] = next[0];
-      sc[1] = next[1];
-      if (x + 1u >= x1) break;  // uniform
+        for (uint32_t d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]), pb[k2], o[d], 0, 0, 0);
+      maximum(next);
       // K of x was read an iteration ago, V of x - 1 too: their buffers take K of x + 2 and V of x + 1
       store_k(x & 1u);
-      store_v((x + 1u) & 1u, x + 1u, id_b);
-      if (tid == 0u) s_bad[(x + 2u) & 3u] = 0u;
+      store_v((x + 1u) & 1u, kb);
       __syncthreads();
-      id_a = id_b;
-      id_b = id_c;
-      id_c = id_d;
+      ka = kb;
+      kb = kcb;
+      kcb = block_of(kd);
+    };
+    for (uint32_t x = x0; x < x1; x += 2u) {
+      iteration(x, sa, sb);
+      if (x + 1u < x1) iteration(x + 1u, sb, sa);  // uniform
+    }
+    if (uniform(s_bad)) {  // after the last barrier; rare
+      for (uint32_t x = x0; x < x1; ++x) {
+        const Blk k = block_of(block_ids(x));
+        if (!k.edge) continue;
+        for (uint32_t i = 0; i < 32u; ++i) {
+          const uint32_t e = k.t + i;
+          if ((i < 16u ? k.p0 : k.p1) >= a.n_pages || e >= s.hi) continue;
+          const size_t base = page_of(k, i / 16u) * HD;
+          const bool seen = sees(e);
+#pragma unroll
+          for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) {
+              const size_t at = ((base + 32u * d + 8u * (j / 4u) + 4u * half + j % 4u) << a.lp) + (e & pmask);
+              const uint32_t w = F8 ? e4m3x2_bf16<false>(a.v[at]) << 16
+                                    : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(a.v)[at]) << 16;
+              const float v = (w & 0x7f800000u) == 0x7f800000u ? __uint_as_float(w) : 0.0f;
+              o[d][j] += seen ? v : 0.0f;
+            }
+        }
+      }
     }
   }
+  const uint32_t h = kv * p.G + c % p.G;
+  const float L = l + lane_xor32_f32(l, lane);
+  if (!have) return;
+  if (it.splits == 1u) {
+    const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
 #pragma unroll
-  for (uint32_t cg = 0; cg < 2; ++cg) {
-    const uint32_t c = 64u * wave + 32u * cg + col, t = t0r + c / p.G, h = kv * p.G + c % p.G;
-    const float L = l[cg] + lane_xor32_f32(l[cg], lane);
-    if (c / p.G >= tq || t >= t1r) continue;
-    if (it.splits == 1u) {
-      const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
+    for (uint32_t d = 0; d < DT; ++d)
 #pragma unroll
-      for (uint32_t d = 0; d < DT; ++d)
+      for (uint32_t i = 0; i < 16; i += 4) {
+        float v[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 16; i += 4) {
-          float v[4];
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[cg][d][i + j] * inv;
-          *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t) * p.nh + h) * HD + 32u * d + 2u * i + 4u * half) =
-              make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
-        }
-    } else {
-      if (half == 0u) {
-        p.ml[(static_cast<size_t>(blockIdx.x) * PF_COLS + c) * 2u] = m[cg];
-        p.ml[(static_cast<size_t>(blockIdx.x) * PF_COLS + c) * 2u + 1u] = L;
+        for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[d][i + j] * inv;
+        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t_row) * p.nh + h) * HD + 32u * d + 2u * i + 4u * half) =
+            make_uint2(pack_bf16_pair_rne(v[0], v[1]), pack_bf16_pair_rne(v[2], v[3]));
       }
-#pragma unroll
-      for (uint32_t d = 0; d < DT; ++d)
-#pragma unroll
-        for (uint32_t i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4*>(p.part + (static_cast<size_t>(blockIdx.x) * PF_COLS + c) * HD + 32u * d + 2u * i + 4u * half) =
-              make_float4(o[cg][d][i], o[cg][d][i + 1], o[cg][d][i + 2], o[cg][d][i + 3]);
+  } else {
+    const size_t at = static_cast<size_t>(blockIdx.x) * PF_COLS + c;
+    if (half == 0u) {
+      p.ml[at * 2u] = m;
+      p.ml[at * 2u + 1u] = L;
     }
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(p.part + at * HD + 32u * d + 2u * i + 4u * half) =
+            make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
   }
 }
 
@@ -925,7 +896,7 @@ int launch_decode(obs_ctx* ctx, const Paged& a, const AttnArgs& p, const Weight&
 template <uint32_t HD, bool F8>
 int launch_prefill(obs_ctx* ctx, const Paged& a, const AttnArgs& p, const PrefillPlan& d) {
   const uint32_t grid = static_cast<uint32_t>(d.items);
-  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, 256, 0, ctx->stream>>>(a, p));
+  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, 512, 0, ctx->stream>>>(a, p));
   if (d.split)
     OBS_LAUNCH(ctx, "paged_prefill_join",
                paged_prefill_join_kernel<HD, F8><<<grid * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
