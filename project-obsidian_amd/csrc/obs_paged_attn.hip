@@ -547,45 +547,49 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
 #pragma unroll
   for (uint32_t d = 0; d < DT; ++d) o[d] = f32x16_v{};
 
-  // A listed block: its first entry, the page ids of its halves, and whether any
-  // row hides any of it. Behind the last block the last one again (unused).
+  // A wave's chunks lie in one half of a block, so in one page: a scalar offset
+  // and a constant one a lane. Where a block has fewer chunks than threads, the
+  // first waves bring keys and the last ones values.
+  const uint32_t kc = tid, vc = VN == 512u ? tid : tid ^ 256u;
+  const bool has_k = kc < KN, has_v = vc < VN;  // wave-uniform
+  const uint32_t kh = uniform(kc / (KN / 2u)) & 1u, vh = uniform(vc / (VN / 2u)) & 1u;
+  // A listed block: its first entry, whether its halves' page ids are good, the
+  // (page, kv head) of the wave's keys and of its values, and whether any row
+  // hides any of it. Behind the last block the last one again (unused).
   struct Blk {
-    uint32_t t, p0, p1;
-    bool edge;
+    uint32_t t, ik, iv;
+    bool ok0, ok1, edge;
   };
   const int32_t* table = a.table + static_cast<size_t>(b) * a.max_pages;
   const uint32_t pmask = (1u << a.lp) - 1u;
-  auto block_ids = [&](uint32_t x) __attribute__((always_inline)) {
-    const uint32_t t = s.start(umin(x, s.nblk - 1u));
-    return Blk{t, static_cast<uint32_t>(table[umin(t >> a.lp, a.max_pages - 1u)]),
-               static_cast<uint32_t>(table[umin((t + 16u) >> a.lp, a.max_pages - 1u)]), false};
+  uint32_t id0 = 0, id1 = 0;  // page ids of 64 blocks' halves, a block a lane
+  auto fetch_ids = [&](uint32_t x) __attribute__((always_inline)) {
+    const uint32_t t = s.start(umin(x + lane, s.nblk - 1u));
+    id0 = static_cast<uint32_t>(table[umin(t >> a.lp, a.max_pages - 1u)]);
+    id1 = static_cast<uint32_t>(table[umin((t + 16u) >> a.lp, a.max_pages - 1u)]);
   };
-  auto block_of = [&](Blk k) __attribute__((always_inline)) {  // waits for the ids
-    k.p0 = uniform(k.p0);
-    k.p1 = uniform(k.p1);
-    k.edge = !(k.p0 < a.n_pages && k.p1 < a.n_pages && k.t + 32u <= hi_first && (k.t >= lo_last || k.t + 32u <= p.sinks));
+  auto block_of = [&](uint32_t x) __attribute__((always_inline)) {  // x within the 64 fetched last
+    Blk k;
+    k.t = s.start(umin(x, s.nblk - 1u));
+    const uint32_t p0 = __builtin_amdgcn_readlane(id0, (x - x0) & 63u), p1 = __builtin_amdgcn_readlane(id1, (x - x0) & 63u);
+    k.ok0 = p0 < a.n_pages;
+    k.ok1 = p1 < a.n_pages;
+    const uint32_t pk = kh ? p1 : p0, pv = vh ? p1 : p0;
+    k.ik = (pk < a.n_pages ? pk : 0u) * a.n_kv + kv;
+    k.iv = (pv < a.n_pages ? pv : 0u) * a.n_kv + kv;
+    k.edge = !(k.ok0 && k.ok1 && k.t + 32u <= hi_first && (k.t >= lo_last || k.t + 32u <= p.sinks));
     return k;
   };
-  // A wave's chunks lie in one half of the block, so in one page: a scalar base
-  // and a constant offset a lane. Where a block has fewer chunks than threads,
-  // the first waves bring keys and the last ones values.
-  const uint32_t kc = tid, vc = VN == 512u ? tid : tid ^ 256u;
-  const bool has_k = kc < KN, has_v = vc < VN;  // wave-uniform
-  const uint32_t kh = uniform(kc / (KN / 2u)), vh = uniform(vc / (VN / 2u));
   const uint32_t v_dim = vc % (VN / 2u) / (VC / 2u), v_ent = 16u * vh + (16u / SZ) * (vc % (VC / 2u));
   const uint32_t koff = ((kc / KC) & pmask) * (HD * SZ) + 16u * (kc % KC);
   const uint32_t voff = ((v_dim << a.lp) + (v_ent & pmask)) * SZ;
   u32x4_v kr, vr;
-  auto page_of = [&](const Blk& k, uint32_t h) __attribute__((always_inline)) {
-    const uint32_t pg = h ? k.p1 : k.p0;
-    return static_cast<size_t>(pg < a.n_pages ? pg : 0u) * a.n_kv + kv;
-  };
   auto load_k = [&](const Blk& k) __attribute__((always_inline)) {
-    const uint8_t* base = a.k + ((page_of(k, kh) << a.lp) + (k.t & pmask)) * (HD * SZ);
+    const uint8_t* base = a.k + ((static_cast<size_t>(k.ik) << a.lp) + (k.t & pmask)) * (HD * SZ);
     if (KN == 512u || has_k) kr = *reinterpret_cast<const u32x4_v*>(base + koff);
   };
   auto load_v = [&](const Blk& k) __attribute__((always_inline)) {
-    const uint8_t* base = a.v + ((page_of(k, vh) * HD << a.lp) + (k.t & pmask)) * SZ;
+    const uint8_t* base = a.v + ((static_cast<size_t>(k.iv) * HD << a.lp) + (k.t & pmask)) * SZ;
     if (VN == 512u || has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
   };
   // 16 stored bytes as bf16: one or two 16-byte words
@@ -613,7 +617,7 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
 #pragma unroll
       for (uint32_t j = 0; j < 2u / SZ; ++j) w[j] = widen(vr, j);
       if (k.edge) {  // uniform
-        const bool ok = (vh ? k.p1 : k.p0) < a.n_pages;
+        const bool ok = vh ? k.ok1 : k.ok0;
         bool bad = false;
 #pragma unroll
         for (uint32_t j = 0; j < 2u / SZ; ++j) {
@@ -651,7 +655,8 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
   };
 
   if (x0 < x1) {  // uniform
-    Blk ka = block_of(block_ids(x0)), kb = block_of(block_ids(x0 + 1u)), kcb = block_of(block_ids(x0 + 2u));
+    fetch_ids(x0);
+    Blk ka = block_of(x0), kb = block_of(x0 + 1u), kcb = block_of(x0 + 2u);
     load_k(ka);
     load_v(ka);
     __syncthreads();  // s_bad is zero
@@ -662,18 +667,18 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
     __syncthreads();
     scores(x0 & 1u, sa);
     maximum(sa);
+    bool up = mx * scale > m + PF_SLACK;
     auto iteration = [&](uint32_t x, f32x16_v& sc, f32x16_v& next) __attribute__((always_inline)) {
-      const Blk kd = block_ids(x + 3u);
+      if (((x - x0) & 63u) == 61u) fetch_ids(x + 3u);  // uniform
       if (ka.edge) {  // uniform
-        const bool ok0 = ka.p0 < a.n_pages, ok1 = ka.p1 < a.n_pages;
         auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
-        if (tid == 0u && ((!ok0 && counts(ka.t)) || (!ok1 && counts(ka.t + 16u)))) paged_flag(a.status);
+        if (tid == 0u && ((!ka.ok0 && counts(ka.t)) || (!ka.ok1 && counts(ka.t + 16u)))) paged_flag(a.status);
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i)
-          sc[i] = (i < 8u ? ok0 : ok1) && sees(ka.t + 16u * (i / 8u) + 8u * half + i % 8u) ? sc[i] : NEG_INF;
+          sc[i] = (i < 8u ? ka.ok0 : ka.ok1) && sees(ka.t + 16u * (i / 8u) + 8u * half + i % 8u) ? sc[i] : NEG_INF;
         maximum(sc);
+        up = mx * scale > m + PF_SLACK;
       }
-      const bool up = mx * scale > m + PF_SLACK;
       if (__any(up)) {
         const float mn = up ? mx * scale : m;
         const float f = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -684,9 +689,6 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
       }
-      load_k(kcb);
-      load_v(kb);
-      __builtin_amdgcn_sched_barrier(0);  // in flight from here to the end of the iteration
       scores((x + 1u) & 1u, next);
       const float mu = m == NEG_INF ? 0.0f : m;
       typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
@@ -703,6 +705,9 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
         }
         pb[k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
       }
+      load_k(kcb);
+      load_v(kb);
+      __builtin_amdgcn_sched_barrier(0);  // the loads go out beside the scores' products, not behind the rest
 #pragma unroll
       for (uint32_t k2 = 0; k2 < 2; ++k2)
 #pragma unroll
@@ -710,13 +715,15 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]), pb[k2], o[d], 0, 0, 0);
       maximum(next);
+      up = mx * scale > m + PF_SLACK;
+      const Blk kd = block_of(x + 3u);
       // K of x was read an iteration ago, V of x - 1 too: their buffers take K of x + 2 and V of x + 1
       store_k(x & 1u);
       store_v((x + 1u) & 1u, kb);
       __syncthreads();
       ka = kb;
       kb = kcb;
-      kcb = block_of(kd);
+      kcb = kd;
     };
     for (uint32_t x = x0; x < x1; x += 2u) {
       iteration(x, sa, sb);
@@ -724,12 +731,14 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, AttnArgs p)
     }
     if (uniform(s_bad)) {  // after the last barrier; rare
       for (uint32_t x = x0; x < x1; ++x) {
-        const Blk k = block_of(block_ids(x));
+        if (((x - x0) & 63u) == 0u) fetch_ids(x);
+        const Blk k = block_of(x);
         if (!k.edge) continue;
+        const uint32_t p0 = __builtin_amdgcn_readlane(id0, (x - x0) & 63u), p1 = __builtin_amdgcn_readlane(id1, (x - x0) & 63u);
         for (uint32_t i = 0; i < 32u; ++i) {
           const uint32_t e = k.t + i;
-          if ((i < 16u ? k.p0 : k.p1) >= a.n_pages || e >= s.hi) continue;
-          const size_t base = page_of(k, i / 16u) * HD;
+          if (!(i < 16u ? k.ok0 : k.ok1) || e >= s.hi) continue;
+          const size_t base = (static_cast<size_t>(i < 16u ? p0 : p1) * a.n_kv + kv) * HD;
           const bool seen = sees(e);
 #pragma unroll
           for (uint32_t d = 0; d < DT; ++d)

@@ -329,10 +329,11 @@ int check_paged(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs
       return set_error(ctx, OBS_E_ALIGN, "%s: the pages must be 16-byte aligned", who);
   }
   if ((kv->head_dim != 64u && kv->head_dim != 128u) || kv->page < 16u || kv->page > 256u || (kv->page & (kv->page - 1u)) ||
-      kv->n_kv == 0 || kv->n_kv > 1024u || kv->n_pages == 0 || kv->n_pages > 0x7fffffffu)
+      kv->n_kv == 0 || kv->n_kv > 1024u || kv->n_pages == 0 || kv->n_pages > 0x7fffffffu ||
+      static_cast<uint64_t>(kv->n_pages) * kv->n_kv > 0xffffffffull)
     return set_error(ctx, OBS_E_SHAPE,
                      "%s: head_dim must be 64 or 128, page a power of two in [16, 256], n_kv in [1, 1024], n_pages in "
-                     "[1, 2^31) (got %u, %u, %u, %u)", who, kv->head_dim, kv->page, kv->n_kv, kv->n_pages);
+                     "[1, 2^31) with n_pages * n_kv below 2^32 (got %u, %u, %u, %u)", who, kv->head_dim, kv->page, kv->n_kv, kv->n_pages);
   if (s->n_seqs > PAGED_MAX_SEQS || s->max_pages == 0 ||
       static_cast<uint64_t>(s->max_pages) * kv->page > PAGED_MAX_ENTRIES || s->n_rows > (1u << 24))
     return set_error(ctx, OBS_E_SHAPE,
