@@ -3,6 +3,8 @@
 // plan that splits their work over workgroups.
 #pragma once
 
+#include <algorithm>
+
 #include "obs_internal.hpp"
 
 namespace obs {
@@ -60,12 +62,41 @@ inline Weight weight_args(const obs_kv_weight* w) {
   return w ? Weight{w->w, w->slot, w->n_slots, w->ld} : Weight{nullptr, nullptr, 0u, 0u};
 }
 
+// Arguments of the attention kernels.
+struct PagedAttn {
+  const uint16_t* q;
+  uint16_t* out;
+  float* ml;      // of each part and column: maximum and sum
+  float* part;    // of each part and column: its unnormalised output
+  float* scores;  // [sequence][head][vis]: scores in base 2, where the weights are gathered
+  uint2* plan;    // of each sequence: its first part and its parts a kv head
+  uint32_t nh, G, window, sinks, q_ld, vis, min_chunk, target;
+  float scale_log2;
+};
+// Blocks of 32 that a token can see of a sequence of `entries`.
+inline uint64_t most_blocks(uint64_t entries, uint64_t window, uint32_t sinks) {
+  const uint64_t all = (entries + 31u) / 32u;
+  if (!window) return all;
+  const uint64_t w = (window + 31u) / 32u + 1u + (std::min<uint64_t>(sinks, entries) + 31u) / 32u;
+  return std::min(all, w);
+}
+inline size_t up256(size_t n) { return (n + 255u) & ~size_t(255); }
+// q, out, weight and the workspace of an attention call; q_ld 0 becomes the dense stride.
+int check_attn(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs_paged_seqs* seqs,
+               const obs_kv_weight* weight, const uint16_t* q, const uint16_t* out, uint32_t n_heads, uint32_t* q_ld,
+               const void* ws, size_t ws_bytes, size_t need);
+// Workspace of obs_sdpa_paged_prefill.
+size_t prefill_paged_ws(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32_t n_heads, uint32_t window, uint32_t sinks);
+
 }  // namespace obs
 
 namespace obsd {
 
+constexpr float NEG_INF = -__builtin_huge_valf();
+
 typedef __attribute__((__vector_size__(8 * sizeof(__bf16)))) __bf16 bf16x8_v;
 typedef uint32_t u32x4_v __attribute__((ext_vector_type(4)));
+typedef __attribute__((__vector_size__(4 * sizeof(float)))) float f32x4_v;
 typedef uint32_t u32x2_v __attribute__((ext_vector_type(2)));
 
 // Reports an argument in device memory that is out of range. The word is only
@@ -145,5 +176,46 @@ template <bool HIGH>
 __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
 }
+
+// Word masks of eight consecutive bf16 from entry t: those below hi, and at or
+// above lo or below sinks, are kept.
+__device__ __forceinline__ u32x4_v entry_masks(uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok) {
+  u32x4_v m;
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    const uint32_t a = t + 2u * i, b = a + 1u;
+    const bool sa = ok && a < hi && (a >= lo || a < sinks), sb = ok && b < hi && (b >= lo || b < sinks);
+    m[i] = (sa ? 0xffffu : 0u) | (sb ? 0xffff0000u : 0u);
+  }
+  return m;
+}
+
+// Sum and inclusive scan over a wave by DPP (rows of 16 lanes, then the row
+// broadcasts): a few VALU steps instead of six trips through the LDS crossbar.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {  // inclusive
+  v = dpp_add<0x111, 0xF>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<DPP_ROW_BCAST15, 0xA>(v);
+  return dpp_add<DPP_ROW_BCAST31, 0xC>(v);
+}
+__device__ __forceinline__ uint32_t wave_sum_u32(uint32_t v) {  // uniform
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan_u32(v)), 63));
+}
+__device__ __forceinline__ float wave_max_f32(float v) {  // uniform
+  v = fmaxf(v, dpp_f32<DPP_XOR1>(v));
+  v = fmaxf(v, dpp_f32<DPP_XOR2>(v));
+  v = fmaxf(v, dpp_f32<DPP_HALF_MIRROR>(v));
+  v = fmaxf(v, dpp_f32<DPP_MIRROR>(v));
+  return fmaxf(fmaxf(readlane_f32(v, 0), readlane_f32(v, 16)), fmaxf(readlane_f32(v, 32), readlane_f32(v, 48)));
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
+// Parts of a sequence's nblk blocks.
+__device__ __forceinline__ uint32_t plan_splits(uint32_t nblk, uint32_t chunk) { return max(1u, (nblk + chunk - 1u) / chunk); }
 
 }  // namespace obsd

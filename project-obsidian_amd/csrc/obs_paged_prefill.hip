@@ -1,0 +1,473 @@
+// obs_paged_prefill.hip — attention of the token rows of a batch of prompts over
+// a paged key/value cache (obs_sdpa_paged_prefill), with a sliding window that
+// keeps the first tokens visible.
+#include "obs_paged.hpp"
+
+namespace {
+using namespace obsd;
+using obs::most_blocks;
+using obs::Paged;
+using obs::PagedAttn;
+using obs::up256;
+
+// ---------------------------------------------------------------------------
+// Token rows of prompts
+// ---------------------------------------------------------------------------
+// A workgroup takes 256 / G consecutive rows of one sequence and the G heads of
+// one kv head: 256 columns, 64 a wave (two groups of 32), over the blocks of 32
+// entries that any of them sees (or a part of those, where there are few rows).
+// Keys and values go through LDS, read there once per 64 columns: a block is
+// 16 + 16 v_mfma_f32_32x32x16_bf16 (1,024 cycles of a SIMD) against 16 KB of LDS
+// reads a wave (512 of the CU's cycles for the four).
+//   S^T [32 entries x 32 columns] = K . Q^T, O^T [dims x 32 columns] += V^T . P: a
+// lane (column lane % 32, half lane / 32) keeps its column throughout. Row r of
+// the score tile is the block's entry with bits 2 and 3 of r exchanged, so a
+// lane's sixteen scores are entries 8 half .. + 7 and 16 + 8 half .. + 7: the
+// values of one 16-byte read of a transposed value row, in the order of the
+// second product's operand.
+// One wave has a SIMD to itself (512 registers), so products and softmax only
+// overlap inside it: an iteration computes block x's softmax and value product
+// together with block x + 1's scores, which do not depend on them. The running
+// maximum follows the scores only when they pass it by 2^8 (the sums and O are
+// in fp32 and P in bf16, which has fp32's range), so O is hardly ever rescaled.
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
+
+constexpr uint32_t PF_COLS = 256, PF_TARGET = 512, PF_MIN_CHUNK = 8;
+constexpr float PF_SLACK = 8.0f;
+
+// Tiles and blocks of the sequences, as the parts are planned by.
+struct PrefillSeq {
+  uint32_t tiles, nblk;
+};
+__device__ __forceinline__ Span tile_span(const PagedAttn& p, const RowSpan& r, uint32_t n, uint32_t t0, uint32_t t1) {
+  // entry of row t is n - (r1 - t); negative: nothing to see
+  const uint32_t hi0 = n + t0 + 1u > r.r1 ? n + t0 + 1u - r.r1 : 0u, hi1 = n + t1 > r.r1 ? n + t1 - r.r1 : 0u;
+  return span_of(hi0 ? hi0 - 1u : 0u, hi1, p.window, p.sinks);
+}
+__device__ __forceinline__ PrefillSeq prefill_seq(const Paged& a, const PagedAttn& p, uint32_t b) {
+  const RowSpan r = paged_rows(a, b);
+  const uint32_t tq = PF_COLS / p.G, tiles = (r.r1 - r.r0 + tq - 1u) / tq;
+  return {tiles, tiles ? tile_span(p, r, paged_len(a, b), r.r0 + (tiles - 1u) * tq, r.r1).nblk : 0u};
+}
+struct PrefillItem {
+  uint32_t b, tile, split, splits, chunk, first;  // first: the part of the tile's split 0
+};
+// Part `item` of a kv head: sequences in order, in each the last tile (the
+// longest) first, a tile's parts together.
+__device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane) {
+  uint32_t chunk = 0xffffffffu;
+  if (p.target) {  // few rows: parts of equal length
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
+      PrefillSeq s{0u, 0u};
+      if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
+      total += wave_sum_u32(s.tiles * s.nblk);
+    }
+    chunk = uniform(max(PF_MIN_CHUNK, static_cast<uint32_t>((total * a.n_kv + p.target - 1u) / p.target)));
+  }
+  uint32_t acc = 0;
+  for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
+    PrefillSeq s{0u, 0u};
+    if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
+    const uint32_t splits = p.target ? plan_splits(s.nblk, chunk) : 1u;
+    const uint32_t incl = wave_scan_u32(s.tiles * splits), all = __builtin_amdgcn_readlane(incl, 63);
+    if (item < acc + all) {
+      const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
+      const uint32_t before = acc + (l ? static_cast<uint32_t>(__builtin_amdgcn_readlane(incl, l - 1u)) : 0u);
+      const uint32_t tl = __builtin_amdgcn_readlane(s.tiles, l), sp = __builtin_amdgcn_readlane(splits, l);
+      const uint32_t x = (item - before) / sp, split = (item - before) % sp;
+      return {uniform(base + l), uniform(tl - 1u - x), uniform(split), uniform(sp), uniform(chunk), uniform(item - split)};
+    }
+    acc += all;
+  }
+  return {a.n_seqs, 0u, 0u, 1u, chunk, 0u};
+}
+
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p) {
+  constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = F8 ? 1u : 2u;
+  constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
+  constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
+  constexpr uint32_t KN = 32u * KC, VN = HD * VC;       // chunks of a block: 512, 256 or 128, at most one a thread
+  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][32u * KROW];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v[2][HD * VROW];
+  __shared__ uint32_t s_bad;  // an edge block holds values that are not finite
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
+  const uint32_t col = lane & 31u, half = lane >> 5;
+  const uint32_t kv = blockIdx.x % a.n_kv;
+  const PrefillItem it = prefill_find(a, p, blockIdx.x / a.n_kv, lane);
+  const uint32_t b = it.b;
+  if (b >= a.n_seqs) return;  // uniform
+  // everything of the tile in scalar registers: no address or branch below takes the vector unit
+  RowSpan r = paged_rows(a, b);
+  r = {uniform(r.r0), uniform(r.r1)};
+  const uint32_t n = uniform(paged_len(a, b));
+  const uint32_t tq = PF_COLS / p.G, t0r = r.r0 + it.tile * tq, t1r = umin(r.r1, t0r + tq);
+  if (tid == 0u && it.tile == 0u && it.split == 0u && kv == 0u && paged_len_bad(a, b)) paged_flag(a.status);
+  const Span s = tile_span(p, r, n, t0r, t1r);
+  const uint32_t hi_first = n + t0r + 1u > r.r1 ? n + t0r + 1u - r.r1 : 0u;
+  const uint32_t lo_last = p.window && s.hi > p.window ? s.hi - p.window : 0u;
+  const uint32_t x0 = it.split * (it.splits > 1u ? it.chunk : 0u);
+  const uint32_t x1 = it.splits > 1u ? umin(s.nblk, x0 + it.chunk) : s.nblk;
+  const float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
+  if (tid == 0u) s_bad = 0u;
+
+  // the wave's columns: query slices, limits, state
+  const uint32_t c = 32u * wave + col, t_row = t0r + c / p.G;
+  const bool have = c / p.G < tq && t_row < t1r;
+  const uint32_t hi = have && n + t_row + 1u > r.r1 ? n + t_row + 1u - r.r1 : 0u;
+  const uint32_t lo = p.window && hi > p.window ? hi - p.window : 0u;
+  bf16x8_v qb[KS];
+  {
+    const uint16_t* qr = p.q + static_cast<size_t>(have ? t_row : t0r) * p.q_ld + (kv * p.G + c % p.G) * HD + 8u * half;
+#pragma unroll
+    for (uint32_t ks = 0; ks < KS; ++ks) {
+      u32x4_v v = *reinterpret_cast<const u32x4_v*>(qr + 16u * ks);
+      if (!have) v = u32x4_v{0u, 0u, 0u, 0u};
+      qb[ks] = __builtin_bit_cast(bf16x8_v, v);
+    }
+  }
+  float m = NEG_INF, l = 0.0f;
+  f32x16_v o[DT];
+#pragma unroll
+  for (uint32_t d = 0; d < DT; ++d) o[d] = f32x16_v{};
+
+  // A wave's chunks lie in one half of a block, so in one page: a scalar offset
+  // and a constant one a lane. Where a block has fewer chunks than threads, the
+  // first waves bring keys and the last ones values.
+  const uint32_t kc = tid, vc = VN == 512u ? tid : tid ^ 256u;
+  const bool has_k = kc < KN, has_v = vc < VN;  // wave-uniform
+  const uint32_t kh = uniform(kc / (KN / 2u)) & 1u, vh = uniform(vc / (VN / 2u)) & 1u;
+  // A listed block: its first entry, whether its halves' page ids are good, the
+  // (page, kv head) of the wave's keys and of its values, and whether any row
+  // hides any of it. Behind the last block the last one again (unused).
+  struct Blk {
+    uint32_t t, ik, iv;
+    bool ok0, ok1, edge;
+  };
+  const int32_t* table = a.table + static_cast<size_t>(b) * a.max_pages;
+  const uint32_t pmask = (1u << a.lp) - 1u;
+  uint32_t id0 = 0, id1 = 0;  // page ids of 64 blocks' halves, a block a lane
+  auto fetch_ids = [&](uint32_t x) __attribute__((always_inline)) {
+    const uint32_t t = s.start(umin(x + lane, s.nblk - 1u));
+    id0 = static_cast<uint32_t>(table[umin(t >> a.lp, a.max_pages - 1u)]);
+    id1 = static_cast<uint32_t>(table[umin((t + 16u) >> a.lp, a.max_pages - 1u)]);
+  };
+  auto block_of = [&](uint32_t x) __attribute__((always_inline)) {  // x within the 64 fetched last
+    Blk k;
+    k.t = s.start(umin(x, s.nblk - 1u));
+    const uint32_t p0 = __builtin_amdgcn_readlane(id0, (x - x0) & 63u), p1 = __builtin_amdgcn_readlane(id1, (x - x0) & 63u);
+    k.ok0 = p0 < a.n_pages;
+    k.ok1 = p1 < a.n_pages;
+    const uint32_t pk = kh ? p1 : p0, pv = vh ? p1 : p0;
+    k.ik = (pk < a.n_pages ? pk : 0u) * a.n_kv + kv;
+    k.iv = (pv < a.n_pages ? pv : 0u) * a.n_kv + kv;
+    k.edge = !(k.ok0 && k.ok1 && k.t + 32u <= hi_first && (k.t >= lo_last || k.t + 32u <= p.sinks));
+    return k;
+  };
+  const uint32_t v_dim = vc % (VN / 2u) / (VC / 2u), v_ent = 16u * vh + (16u / SZ) * (vc % (VC / 2u));
+  const uint32_t koff = ((kc / KC) & pmask) * (HD * SZ) + 16u * (kc % KC);
+  const uint32_t voff = ((v_dim << a.lp) + (v_ent & pmask)) * SZ;
+  u32x4_v kr, vr;
+  auto load_k = [&](const Blk& k) __attribute__((always_inline)) {
+    const uint8_t* base = a.k + ((static_cast<size_t>(k.ik) << a.lp) + (k.t & pmask)) * (HD * SZ);
+    if (KN == 512u || has_k) kr = *reinterpret_cast<const u32x4_v*>(base + koff);
+  };
+  auto load_v = [&](const Blk& k) __attribute__((always_inline)) {
+    const uint8_t* base = a.v + ((static_cast<size_t>(k.iv) * HD << a.lp) + (k.t & pmask)) * SZ;
+    if (VN == 512u || has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
+  };
+  // 16 stored bytes as bf16: one or two 16-byte words
+  auto widen = [](const u32x4_v& w, uint32_t j) __attribute__((always_inline)) {
+    if constexpr (F8) {
+      const uint32_t w0 = j ? w.z : w.x, w1 = j ? w.w : w.y;
+      return u32x4_v{e4m3x2_bf16<false>(w0), e4m3x2_bf16<true>(w0), e4m3x2_bf16<false>(w1), e4m3x2_bf16<true>(w1)};
+    } else {
+      return w;
+    }
+  };
+  auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
+    if (KN == 512u || has_k) {
+      uint16_t* to = &s_k[buf][(kc / KC) * KROW + (16u / SZ) * (kc % KC)];
+#pragma unroll
+      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(to + 8u * j) = widen(kr, j);
+    }
+  };
+  // At the edge, values hidden from every row are stored as zero (the pool may
+  // hold anything there), and those that are not finite too: the rows that see
+  // them get them at the end, and no other row meets them.
+  auto store_v = [&](uint32_t buf, const Blk& k) __attribute__((always_inline)) {
+    if (VN == 512u || has_v) {
+      u32x4_v w[2u / SZ];
+#pragma unroll
+      for (uint32_t j = 0; j < 2u / SZ; ++j) w[j] = widen(vr, j);
+      if (k.edge) {  // uniform
+        const bool ok = vh ? k.ok1 : k.ok0;
+        bool bad = false;
+#pragma unroll
+        for (uint32_t j = 0; j < 2u / SZ; ++j) {
+          w[j] &= entry_masks(k.t + v_ent + 8u * j, s.hi, s.lo, p.sinks, ok);
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            const bool blo = (w[j][q] & 0x7f80u) == 0x7f80u, bhi = (w[j][q] & 0x7f800000u) == 0x7f800000u;
+            bad = bad || blo || bhi;
+            w[j][q] &= (blo ? 0u : 0xffffu) | (bhi ? 0u : 0xffff0000u);
+          }
+        }
+        if (bad) s_bad = 1u;
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(&s_v[buf][v_dim * VROW + v_ent + 8u * j]) = w[j];
+    }
+  };
+  auto sees = [&](uint32_t e) __attribute__((always_inline)) { return e < hi && (e >= lo || e < p.sinks); };
+
+  f32x16_v sa, sb;  // scores of this block and of the next, in turn
+  float mx;
+  const uint32_t krow = (col & 0x13u) | ((col & 4u) << 1) | ((col & 8u) >> 1);  // bits 2 and 3 exchanged
+  auto scores = [&](uint32_t buf, f32x16_v& to) __attribute__((always_inline)) {
+    to = f32x16_v{};
+#pragma unroll
+    for (uint32_t ks = 0; ks < KS; ++ks)
+      to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+          *reinterpret_cast<const bf16x8_v*>(&s_k[buf][krow * KROW + 16u * ks + 8u * half]), qb[ks], to, 0, 0, 0);
+  };
+  auto maximum = [&](const f32x16_v& v) __attribute__((always_inline)) {
+    float t = fmaxf(v[0], v[1]);
+#pragma unroll
+    for (uint32_t i = 2; i < 16; i += 2) t = fmaxf(fmaxf(t, v[i]), v[i + 1]);
+    mx = fmaxf(t, lane_xor32_f32(t, lane));
+  };
+
+  if (x0 < x1) {  // uniform
+    fetch_ids(x0);
+    Blk ka = block_of(x0), kb = block_of(x0 + 1u), kcb = block_of(x0 + 2u);
+    load_k(ka);
+    load_v(ka);
+    __syncthreads();  // s_bad is zero
+    store_k(x0 & 1u);
+    store_v(x0 & 1u, ka);
+    load_k(kb);
+    store_k((x0 + 1u) & 1u);
+    __syncthreads();
+    scores(x0 & 1u, sa);
+    maximum(sa);
+    bool up = mx * scale > m + PF_SLACK;
+    auto iteration = [&](uint32_t x, f32x16_v& sc, f32x16_v& next) __attribute__((always_inline)) {
+      if (((x - x0) & 63u) == 61u) fetch_ids(x + 3u);  // uniform
+      if (ka.edge) {  // uniform
+        auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
+        if (tid == 0u && ((!ka.ok0 && counts(ka.t)) || (!ka.ok1 && counts(ka.t + 16u)))) paged_flag(a.status);
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+          sc[i] = (i < 8u ? ka.ok0 : ka.ok1) && sees(ka.t + 16u * (i / 8u) + 8u * half + i % 8u) ? sc[i] : NEG_INF;
+        maximum(sc);
+        up = mx * scale > m + PF_SLACK;
+      }
+      if (__any(up)) {
+        const float mn = up ? mx * scale : m;
+        const float f = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+        m = mn;
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
+      }
+      scores((x + 1u) & 1u, next);
+      const float mu = m == NEG_INF ? 0.0f : m;
+      typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+      const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
+      bf16x8_v pb[2];
+#pragma unroll
+      for (uint32_t k2 = 0; k2 < 2; ++k2) {
+        uint32_t pk[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          pk[i] = pack_bf16_pair_rne(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i], scale, -mu)),
+                                     __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i + 1], scale, -mu)));
+          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pk[i]), ones, l, false);
+        }
+        pb[k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
+      }
+      load_k(kcb);
+      load_v(kb);
+      __builtin_amdgcn_sched_barrier(0);  // the loads go out beside the scores' products, not behind the rest
+#pragma unroll
+      for (uint32_t k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]), pb[k2], o[d], 0, 0, 0);
+      maximum(next);
+      up = mx * scale > m + PF_SLACK;
+      const Blk kd = block_of(x + 3u);
+      // K of x was read an iteration ago, V of x - 1 too: their buffers take K of x + 2 and V of x + 1
+      store_k(x & 1u);
+      store_v((x + 1u) & 1u, kb);
+      __syncthreads();
+      ka = kb;
+      kb = kcb;
+      kcb = kd;
+    };
+    for (uint32_t x = x0; x < x1; x += 2u) {
+      iteration(x, sa, sb);
+      if (x + 1u < x1) iteration(x + 1u, sb, sa);  // uniform
+    }
+    if (uniform(s_bad)) {  // after the last barrier; rare
+      for (uint32_t x = x0; x < x1; ++x) {
+        if (((x - x0) & 63u) == 0u) fetch_ids(x);
+        const Blk k = block_of(x);
+        if (!k.edge) continue;
+        const uint32_t p0 = __builtin_amdgcn_readlane(id0, (x - x0) & 63u), p1 = __builtin_amdgcn_readlane(id1, (x - x0) & 63u);
+        for (uint32_t i = 0; i < 32u; ++i) {
+          const uint32_t e = k.t + i;
+          if (!(i < 16u ? k.ok0 : k.ok1) || e >= s.hi) continue;
+          const size_t base = (static_cast<size_t>(i < 16u ? p0 : p1) * a.n_kv + kv) * HD;
+          const bool seen = sees(e);
+#pragma unroll
+          for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+            for (uint32_t j = 0; j < 16; ++j) {
+              const size_t at = ((base + 32u * d + 8u * (j / 4u) + 4u * half + j % 4u) << a.lp) + (e & pmask);
+              const uint32_t w = F8 ? e4m3x2_bf16<false>(a.v[at]) << 16
+                                    : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(a.v)[at]) << 16;
+              const float v = (w & 0x7f800000u) == 0x7f800000u ? __uint_as_float(w) : 0.0f;
+              o[d][j] += seen ? v : 0.0f;
+            }
+        }
+      }
+    }
+  }
+  const uint32_t h = kv * p.G + c % p.G;
+  const float L = l + lane_xor32_f32(l, lane);
+  if (!have) return;
+  if (it.splits == 1u) {
+    const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; i += 4) {
+        float v[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[d][i + j] * inv;
+        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t_row) * p.nh + h) * HD + 32u * d + 2u * i + 4u * half) =
+            make_uint2(pack_bf16_pair_rne(v[0], v[1]), pack_bf16_pair_rne(v[2], v[3]));
+      }
+  } else {
+    const size_t at = static_cast<size_t>(blockIdx.x) * PF_COLS + c;
+    if (half == 0u) {
+      p.ml[at * 2u] = m;
+      p.ml[at * 2u + 1u] = L;
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; i += 4)
+        *reinterpret_cast<float4*>(p.part + at * HD + 32u * d + 2u * i + 4u * half) =
+            make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+  }
+}
+
+// A tile's parts joined in order: a workgroup per 256 / HD * 4 columns.
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedAttn p, uint32_t items) {
+  constexpr uint32_t CW = 1024u / HD;  // columns of a workgroup, 4 dims a thread
+  const uint32_t tid = threadIdx.x, lane = tid & 63u;
+  const uint32_t part = blockIdx.x / (PF_COLS / CW), c = blockIdx.x % (PF_COLS / CW) * CW + tid / (HD / 4u), d = 4u * (tid % (HD / 4u));
+  const uint32_t kv = part % a.n_kv;
+  const PrefillItem it = prefill_find(a, p, part / a.n_kv, lane);
+  if (it.b >= a.n_seqs || it.splits == 1u || it.split != 0u) return;  // uniform
+  const RowSpan r = paged_rows(a, it.b);
+  const uint32_t tq = PF_COLS / p.G, t = r.r0 + it.tile * tq + c / p.G, h = kv * p.G + c % p.G;
+  if (c / p.G >= tq || t >= r.r1) return;
+  float M = NEG_INF;
+  for (uint32_t i = 0; i < it.splits; ++i)
+    M = fmaxf(M, p.ml[((static_cast<size_t>(it.first + i) * a.n_kv + kv) * PF_COLS + c) * 2u]);
+  float L = 0.0f;
+  f32x4_v o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t i = 0; i < it.splits; ++i) {
+    const size_t at = (static_cast<size_t>(it.first + i) * a.n_kv + kv) * PF_COLS + c;
+    const float m = p.ml[at * 2u], f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+    const f32x4_v x = *reinterpret_cast<const f32x4_v*>(p.part + at * HD + d);
+    L = __builtin_fmaf(p.ml[at * 2u + 1u], f, L);
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) o[j] = __builtin_fmaf(x[j], f, o[j]);
+  }
+  const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
+  float v[4];
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[j] * inv;
+  *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t) * p.nh + h) * HD + d) =
+      make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
+// Prefill: with few rows for the chip (tiles of both kinds of sequence ends
+// counted by the rows alone) a tile's blocks are cut into parts.
+struct PrefillPlan {
+  uint64_t items;  // workgroups at most
+  bool split;
+  size_t ml, part;
+};
+PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32_t n_heads, uint32_t window, uint32_t sinks) {
+  PrefillPlan d{};
+  const uint32_t tq = PF_COLS / (n_heads / kv->n_kv);
+  const uint64_t full = static_cast<uint64_t>(kv->n_kv) * ((s->n_rows + tq - 1u) / tq);
+  // tiles: at most one that is not full a sequence, and none of a sequence without rows
+  const uint64_t tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
+  d.split = 2u * full <= PF_TARGET && most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks) > PF_MIN_CHUNK;
+  d.items = d.split ? PF_TARGET + tiles : tiles;
+  if (d.split) {
+    d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
+    d.part = up256(d.items * PF_COLS * kv->head_dim * sizeof(float));
+  }
+  return d;
+}
+
+template <uint32_t HD, bool F8>
+int launch_prefill(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const PrefillPlan& d) {
+  const uint32_t grid = static_cast<uint32_t>(d.items);
+  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, 512, 0, ctx->stream>>>(a, p));
+  if (d.split)
+    OBS_LAUNCH(ctx, "paged_prefill_join",
+               paged_prefill_join_kernel<HD, F8><<<grid * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
+  return OBS_OK;
+}
+
+}  // namespace
+
+namespace obs {
+size_t prefill_paged_ws(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32_t n_heads, uint32_t window, uint32_t sinks) {
+  const PrefillPlan d = prefill_plan(kv, s, n_heads, window, sinks);
+  return d.ml + d.part + 256u;
+}
+}  // namespace obs
+
+extern "C" {
+
+int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const uint16_t* q,
+                           uint16_t* out, uint32_t n_heads, uint32_t window, uint32_t sinks, uint32_t q_ld, void* ws,
+                           size_t ws_bytes) {
+  if (!ctx) return OBS_E_INVALID;
+  const char* who = "obs_sdpa_paged_prefill";
+  int rc = obs::check_paged(ctx, who, kv, seqs, true);
+  if (rc == OBS_OK) rc = obs::check_heads(ctx, who, n_heads, kv->n_kv);
+  if (rc != OBS_OK) return rc;
+  if (!seqs->row) return obs::set_error(ctx, OBS_E_INVALID, "%s: null row (obs_sdpa_paged_decode takes one token a sequence)", who);
+  const PrefillPlan d = prefill_plan(kv, seqs, n_heads, window, sinks);
+  rc = obs::check_attn(ctx, who, kv, seqs, nullptr, q, out, n_heads, &q_ld, ws, ws_bytes, d.ml + d.part + 256u);
+  if (rc != OBS_OK) return rc;
+  if (seqs->n_seqs == 0 || seqs->n_rows == 0) return OBS_OK;
+  if (d.items * 32u > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many rows and heads", who);
+  obs::DeviceGuard guard(ctx);
+  const Paged a = obs::paged_args(ctx, kv, seqs);
+  uint8_t* wb = static_cast<uint8_t*>(ws);
+  const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr, nullptr, n_heads,
+                   n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u,
+                   1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
+  const bool f8 = kv->dtype == OBS_KV_E4M3;
+  if (kv->head_dim == 128u) return f8 ? launch_prefill<128, true>(ctx, a, p, d) : launch_prefill<128, false>(ctx, a, p, d);
+  return f8 ? launch_prefill<64, true>(ctx, a, p, d) : launch_prefill<64, false>(ctx, a, p, d);
+}
+
+}  // extern "C"
