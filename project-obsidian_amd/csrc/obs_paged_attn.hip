@@ -144,40 +144,53 @@ __device__ __forceinline__ Span decode_span(const Paged& a, const PagedAttn& p, 
   const uint32_t n = paged_len(a, b);
   return span_of(n ? n - 1u : 0u, n, p.window, p.sinks);
 }
-// Parts a block: `target` over all blocks of the call.
-__device__ __forceinline__ float plan_rate(const Paged& a, const PagedAttn& p, uint32_t lane) {
-  uint64_t total = 0;
-  for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-    const uint32_t b = base + lane;
-    total += wave_sum_u32(b < a.n_seqs ? decode_span(a, p, b).nblk : 0u);
-  }
-  return static_cast<float>(p.target) / static_cast<float>(max(total * a.n_kv, static_cast<uint64_t>(1)));
-}
 // Parts of a sequence: its share of the target, rounded up but for the rounding
 // of the fp32 product, each of min_chunk blocks at least.
 __device__ __forceinline__ uint32_t plan_parts(uint32_t nblk, float rate, uint32_t min_chunk) {
   const uint32_t share = static_cast<uint32_t>(__builtin_ceilf(static_cast<float>(nblk) * rate - 0.001f));
   return max(1u, umin(share, (nblk + min_chunk - 1u) / min_chunk));
 }
-// The sequence of part `item` and its first part; n_seqs behind the last.
+// The sequence of part `item`, its entries, parts and first part; b is n_seqs
+// behind the last. Up to 64 sequences the lengths are read once, a sequence a lane.
 struct Found {
-  uint32_t b, first;
+  uint32_t b, n, splits, first;
 };
-__device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, float rate, uint32_t item, uint32_t lane) {
+__device__ __forceinline__ uint32_t span_blocks(const PagedAttn& p, uint32_t n) {
+  return span_of(n ? n - 1u : 0u, n, p.window, p.sinks).nblk;
+}
+__device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane) {
+  float rate = 0.0f;
+  uint32_t n = 0, nblk = 0;
+  if (a.n_seqs <= 64u) {  // uniform
+    n = lane < a.n_seqs ? paged_len(a, lane) : 0u;
+    nblk = span_blocks(p, n);
+    rate = static_cast<float>(p.target) / fmaxf(static_cast<float>(wave_sum_u32(nblk)) * static_cast<float>(a.n_kv), 1.0f);
+  } else {
+    float total = 0.0f;
+    for (uint32_t base = 0; base < a.n_seqs; base += 64u)
+      total += static_cast<float>(wave_sum_u32(base + lane < a.n_seqs ? span_blocks(p, paged_len(a, base + lane)) : 0u));
+    rate = static_cast<float>(p.target) / fmaxf(total * static_cast<float>(a.n_kv), 1.0f);
+  }
   uint32_t acc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
     const uint32_t b = base + lane;
-    const uint32_t own = b < a.n_seqs ? a.n_kv * plan_parts(decode_span(a, p, b).nblk, rate, p.min_chunk) : 0u;
-    const uint32_t incl = wave_scan_u32(own);
-    const uint32_t all = __builtin_amdgcn_readlane(incl, 63);
+    if (a.n_seqs > 64u) {
+      n = b < a.n_seqs ? paged_len(a, b) : 0u;
+      nblk = span_blocks(p, n);
+    }
+    const uint32_t parts = plan_parts(nblk, rate, p.min_chunk);
+    const uint32_t incl = wave_scan_u32(b < a.n_seqs ? a.n_kv * parts : 0u);
+    const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(incl), 63));
     if (item < acc + all) {
-      const uint32_t before = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
-      const uint32_t first = acc + (before ? static_cast<uint32_t>(__builtin_amdgcn_readlane(incl, before - 1u)) : 0u);
-      return {base + before, first};
+      const int l = static_cast<int>(__popcll(__ballot(acc + incl <= item)));
+      const uint32_t end = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(incl), l));
+      const uint32_t sp = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(parts), l));
+      return {base + static_cast<uint32_t>(l), static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(n), l)), sp,
+              acc + end - a.n_kv * sp};
     }
     acc += all;
   }
-  return {a.n_seqs, 0u};
+  return {a.n_seqs, 0u, 1u, 0u};
 }
 
 // ---------------------------------------------------------------------------
@@ -193,12 +206,10 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
   __shared__ float s_ml[4][16][2];
   __shared__ float s_o[4][16][HD + 4u];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, col = lane & 15u, g = lane >> 4;
-  const float rate = plan_rate(a, p, lane);
-  const Found f = plan_find(a, p, rate, blockIdx.x, lane);
-  const uint32_t b = uniform(f.b);
+  const Found f = plan_find(a, p, blockIdx.x, lane);
+  const uint32_t b = f.b, splits = f.splits, at = blockIdx.x - f.first;
   if (b >= a.n_seqs) return;  // uniform
-  const Span s = decode_span(a, p, b);
-  const uint32_t splits = uniform(plan_parts(s.nblk, rate, p.min_chunk)), at = blockIdx.x - uniform(f.first);
+  const Span s = span_of(f.n ? f.n - 1u : 0u, f.n, p.window, p.sinks);
   if (at == 0u && tid == 0u) p.plan[b] = make_uint2(blockIdx.x, splits);
   const uint32_t kv = at / splits, sp = at % splits;
   const uint32_t q0 = s.nblk / splits, q1 = s.nblk % splits;  // parts of q0 or q0 + 1 blocks
@@ -418,7 +429,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, W
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-constexpr uint32_t DECODE_TARGET = 1152, DECODE_MIN_CHUNK = 8;
+constexpr uint32_t DECODE_MIN_CHUNK = 4;
+// Parts of a call: three workgroups a CU are resident (768). Few rows give
+// nearly equal parts, which fill the chip once (one sequence of 100,003 entries
+// 48.2 us against 55.2 with 1,152); the parts of many sequences differ, and
+// finer ones even out (48 sequences of up to 16,000: 69.5 us against 74.0).
+uint32_t decode_target(const obs_paged_kv* kv, const obs_paged_seqs* s) { return s->n_seqs * kv->n_kv <= 32u ? 768u : 1152u; }
 
 struct DecodePlan {
   uint64_t items, vis, blocks;
@@ -435,7 +451,7 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
   d.vis = 32u * d.blocks;
   const uint64_t rows = static_cast<uint64_t>(s->n_seqs) * kv->n_kv;
   // sum of the rows' rounded shares: at most target + rows (and what fp32 rounds), and at most each row's own most
-  d.items = std::min<uint64_t>(DECODE_TARGET + rows + 64u, rows * ((d.blocks + DECODE_MIN_CHUNK - 1u) / DECODE_MIN_CHUNK));
+  d.items = std::min<uint64_t>(decode_target(kv, s) + rows + 64u, rows * ((d.blocks + DECODE_MIN_CHUNK - 1u) / DECODE_MIN_CHUNK));
   d.ml = up256(d.items * 32u * sizeof(float));
   d.part = up256(d.items * (n_heads / kv->n_kv) * kv->head_dim * sizeof(float));
   d.scores = weight ? up256(static_cast<size_t>(s->n_seqs) * n_heads * d.vis * sizeof(float)) : 0u;
@@ -523,7 +539,7 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
   uint8_t* wb = static_cast<uint8_t*>(ws);
   const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml),
                    reinterpret_cast<float*>(wb + d.ml + d.part), reinterpret_cast<uint2*>(wb + d.ml + d.part + d.scores), n_heads, n_heads / kv->n_kv, window, sinks, q_ld,
-                   static_cast<uint32_t>(d.vis), DECODE_MIN_CHUNK, DECODE_TARGET,
+                   static_cast<uint32_t>(d.vis), DECODE_MIN_CHUNK, decode_target(kv, seqs),
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const Weight w = obs::weight_args(weight);
   const bool f8 = kv->dtype == OBS_KV_E4M3;

@@ -163,21 +163,38 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return w != w ? 0u : ((u >> 31) ? ~u : (u | 0x80000000u));
 }
 
-constexpr uint32_t EV_THREADS = 1024;
+constexpr uint32_t EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64u, EV_KEYS = 16, EV_BINS = 2048;
 
-// One workgroup per (sequence, kv head): the K-th largest key of the entries
-// between the first and the last ones, digit by digit (8 bits a pass, counts
-// in LDS), then one pass in order that ranks what is kept.
+// Exclusive scan over the workgroup, in thread order; s_w: EV_WAVES words.
+__device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_w, uint32_t lane, uint32_t wave, uint32_t& total) {
+  const uint32_t incl = wave_scan_u32(v);
+  __syncthreads();  // what s_w held before was read
+  if (lane == 63u) s_w[wave] = incl;
+  __syncthreads();
+  const uint32_t w = lane < EV_WAVES ? s_w[lane] : 0u, ws = wave_scan_u32(w);
+  total = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ws), EV_WAVES - 1u));
+  const uint32_t before = wave ? static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ws), static_cast<int>(wave) - 1)) : 0u;
+  return before + incl - v;
+}
+
+// One workgroup per (sequence, kv head). The entries' weights lie in registers,
+// up to 16 consecutive ones a thread (16,384 entries at once; longer sequences
+// pass through in segments, again for each step). Three steps of 11, 11 and 10
+// bits find the K-th largest key of the entries between the first and the last
+// ones: counts by digit in LDS, then a scan from the top. Attention weights
+// spread over many powers of two, so the top digit (sign, exponent, two mantissa
+// bits) has few lanes at one counter. The kept entries' places are two scans
+// over the threads (ties, then all).
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weight w, Weight wd, uint32_t sinks,
                                                                  uint32_t recent, uint32_t budget,
                                                                  int32_t* __restrict__ kept,
                                                                  int32_t* __restrict__ new_len) {
-  __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_wave[2][EV_THREADS / 64u];
+  __shared__ uint32_t s_hist[EV_BINS];
+  __shared__ uint32_t s_w[EV_WAVES];
   __shared__ uint32_t s_pick[2];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
   const uint32_t b = blockIdx.x / a.n_kv, h = blockIdx.x % a.n_kv;
-  const uint32_t n = paged_len(a, b), now = min(n, budget);
+  const uint32_t n = uniform(paged_len(a, b)), now = umin(n, budget);
   const int64_t slot = weight_slot(w, b), dslot = weight_slot(wd, b);
   if (tid == 0u) {
     if (paged_len_bad(a, b) || slot < 0 || dslot < 0) paged_flag(a.status);
@@ -186,26 +203,62 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
   const float* src = w.w + (static_cast<size_t>(max(slot, int64_t(0))) * a.n_kv + h) * w.ld;
   float* dst = wd.w + (static_cast<size_t>(max(dslot, int64_t(0))) * a.n_kv + h) * wd.ld;
   int32_t* kp = kept + (static_cast<size_t>(b) * a.n_kv + h) * budget;
-  auto weight_of = [&](uint32_t j) { return slot >= 0 ? src[j] : 0.0f; };
   for (uint32_t e = now + tid; e < budget; e += EV_THREADS) kp[e] = -1;
+  // entries a thread holds of a segment: a multiple of 4, so its loads can be 16 bytes
+  const uint32_t per = umin(EV_KEYS, ((n + EV_THREADS - 1u) / EV_THREADS + 3u) & ~3u), seg = per * EV_THREADS;
+  const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0u;
+  float wt[EV_KEYS];
+  uint32_t held = 0xffffffffu;
+  auto load = [&](uint32_t s0) __attribute__((always_inline)) {  // the segment from entry s0
+    if (held == s0) return;  // uniform
+    held = s0;
+    const uint32_t j0 = s0 + per * tid;
+#pragma unroll
+    for (uint32_t i = 0; i < EV_KEYS; i += 4u) {
+      if (i >= per) break;  // uniform
+      if (slot < 0) {
+        wt[i] = wt[i + 1] = wt[i + 2] = wt[i + 3] = 0.0f;
+      } else if (vec && j0 + i + 4u <= n) {
+        const float4 v = *reinterpret_cast<const float4*>(src + j0 + i);
+        wt[i] = v.x;
+        wt[i + 1] = v.y;
+        wt[i + 2] = v.z;
+        wt[i + 3] = v.w;
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) wt[i + j] = j0 + i + j < n ? src[j0 + i + j] : 0.0f;
+      }
+    }
+  };
   const uint32_t lo = n > budget ? sinks : n, hi = n > budget ? n - recent : n;  // the candidates [lo, hi)
   uint32_t want = n > budget ? budget - sinks - recent : 0u;                     // < hi - lo
   uint32_t thr = 0xffffffffu, ties = 0u;  // kept: key > thr, and the first `ties` with key == thr
-  if (want > 0u) {
+  if (want > 0u) {  // uniform
     uint32_t prefix = 0u;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256u) s_hist[tid] = 0u;
+#pragma unroll
+    for (uint32_t step = 0; step < 3; ++step) {
+      const uint32_t shift = step == 0u ? 21u : step == 1u ? 10u : 0u, bits = step == 2u ? 10u : 11u;
+      for (uint32_t i = tid; i < EV_BINS; i += EV_THREADS) s_hist[i] = 0u;
       __syncthreads();
-      for (uint32_t j = lo + tid; j < hi; j += EV_THREADS) {
-        const uint32_t key = weight_key(weight_of(j));
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
+      for (uint32_t s0 = 0; s0 < n; s0 += seg) {
+        load(s0);
+#pragma unroll
+        for (uint32_t i = 0; i < EV_KEYS; ++i) {
+          if (i >= per) break;  // uniform
+          const uint32_t j = s0 + per * tid + i, key = weight_key(wt[i]);
+          if (j >= lo && j < hi && (step == 0u || (key >> (shift + bits)) == (prefix >> (shift + bits))))
+            atomicAdd(&s_hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+        }
       }
       __syncthreads();
-      if (tid == 0u) {
-        uint32_t left = want, d = 255u;
-        while (d > 0u && s_hist[d] < left) left -= s_hist[d--];
-        s_pick[0] = d;
-        s_pick[1] = left;
+      // thread t looks at bins top - 2 t and top - 2 t - 1: the one where the count from the top reaches `want`
+      const uint32_t top = EV_BINS - 1u - 2u * tid, c1 = s_hist[top], c0 = s_hist[top - 1u];
+      uint32_t total;
+      const uint32_t above = group_scan(c0 + c1, s_w, lane, wave, total);
+      if (above < want && above + c0 + c1 >= want) {  // one thread
+        const bool first = above + c1 >= want;
+        s_pick[0] = first ? top : top - 1u;
+        s_pick[1] = want - above - (first ? 0u : c1);
       }
       __syncthreads();
       prefix |= s_pick[0] << shift;
@@ -216,56 +269,59 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
     ties = want;
   }
   uint32_t at = 0u, tie_at = 0u;
-  for (uint32_t j0 = 0; j0 < n; j0 += EV_THREADS) {
-    const uint32_t j = j0 + tid;
-    const float wt = j < n ? weight_of(j) : 0.0f;
-    const uint32_t key = weight_key(wt);
-    const bool mid = j >= lo && j < hi;
-    const bool tie = mid && key == thr && ties > 0u;
-    const unsigned long long below = (1ull << lane) - 1ull;
-    const unsigned long long mt = __ballot(tie);
-    if (lane == 0u) s_wave[0][wave] = static_cast<uint32_t>(__popcll(mt));
-    __syncthreads();
-    uint32_t tb = tie_at, tsum = 0u;
-    for (uint32_t i = 0; i < EV_THREADS / 64u; ++i) {
-      tb += i < wave ? s_wave[0][i] : 0u;
-      tsum += s_wave[0][i];
+  for (uint32_t s0 = 0; s0 < n; s0 += seg) {
+    load(s0);
+    const uint32_t j0 = s0 + per * tid;
+    uint32_t tie = 0u, keep = 0u;  // bits of the thread's entries
+#pragma unroll
+    for (uint32_t i = 0; i < EV_KEYS; ++i) {
+      if (i >= per) break;  // uniform
+      const uint32_t j = j0 + i, key = weight_key(wt[i]);
+      const bool mid = j >= lo && j < hi;
+      tie |= mid && key == thr && ties > 0u ? 1u << i : 0u;
+      keep |= j < n && (!mid || key > thr) ? 1u << i : 0u;
     }
-    const uint32_t trank = tb + static_cast<uint32_t>(__popcll(mt & below));
-    const bool keep = j < n && (!mid || key > thr || (tie && trank < ties));
-    const unsigned long long mk = __ballot(keep);
-    if (lane == 0u) s_wave[1][wave] = static_cast<uint32_t>(__popcll(mk));
-    __syncthreads();
-    uint32_t kb = at, ksum = 0u;
-    for (uint32_t i = 0; i < EV_THREADS / 64u; ++i) {
-      kb += i < wave ? s_wave[1][i] : 0u;
-      ksum += s_wave[1][i];
+    uint32_t tsum = 0u, ksum;
+    if (ties > 0u) {  // uniform
+      uint32_t rank = tie_at + group_scan(static_cast<uint32_t>(__popc(tie)), s_w, lane, wave, tsum);
+#pragma unroll
+      for (uint32_t i = 0; i < EV_KEYS; ++i)
+        if (tie >> i & 1u) keep |= rank++ < ties ? 1u << i : 0u;
     }
-    const uint32_t e = kb + static_cast<uint32_t>(__popcll(mk & below));
-    if (keep && e < budget) {
-      kp[e] = static_cast<int32_t>(j);
-      if (dslot >= 0) dst[e] = wt;
-    }
+    uint32_t e = at + group_scan(static_cast<uint32_t>(__popc(keep)), s_w, lane, wave, ksum);
+#pragma unroll
+    for (uint32_t i = 0; i < EV_KEYS; ++i)
+      if (keep >> i & 1u) {
+        if (e < budget) {
+          kp[e] = static_cast<int32_t>(j0 + i);
+          if (dslot >= 0) dst[e] = wt[i];
+        }
+        ++e;
+      }
     at += ksum;
     tie_at += tsum;
   }
 }
 
-// 64 kept entries of one (sequence, kv head) a workgroup: key rows by 16 bytes,
-// then the transposed values, 64 entries of one dim at a time.
+// 64 kept entries of one (sequence, kv head) a workgroup. Keys: rows of 16-byte
+// chunks. Values: a wave takes 64 dims (32 where a head has 64), a dim a lane,
+// of 16 entries: the entries are the wave's, so their pages are scalar bases,
+// sixteen loads are in flight, and a lane writes 16 consecutive entries of its
+// row. A transposed value page is read whole as soon as one of its entries is
+// kept (an entry's dims lie a row apart), which is what bounds this kernel.
 template <uint32_t HD, bool F8>
 __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t* __restrict__ dst_pages,
                                                          uint32_t dst_max_pages, uint32_t budget,
                                                          const int32_t* __restrict__ kept) {
   typedef typename std::conditional<F8, uint8_t, uint16_t>::type T;
-  constexpr uint32_t CH = HD * sizeof(T) / 16u;  // 16-byte chunks of a key row
-  __shared__ int32_t s_src[64], s_dst[64];       // (page * n_kv + head) of both sides, -1: none
-  __shared__ uint32_t s_so[64], s_do[64];        // entries in the pages
-  const uint32_t tid = threadIdx.x, groups = (budget + 63u) / 64u;
+  constexpr uint32_t SZ = sizeof(T), CH = HD * SZ / 16u;  // 16-byte chunks of a key row
+  __shared__ int32_t s_src[64], s_dst[64];                // pages of both sides, -1: none
+  __shared__ uint32_t s_so[64];                           // entries in the source pages
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), groups = (budget + 63u) / 64u;
   const uint32_t gi = blockIdx.x % groups, bh = blockIdx.x / groups, b = bh / a.n_kv, h = bh % a.n_kv;
-  const uint32_t mask = (1u << a.lp) - 1u;
+  const uint32_t mask = (1u << a.lp) - 1u, e0 = 64u * gi;
   if (tid < 64u) {
-    const uint32_t e = 64u * gi + tid;
+    const uint32_t e = e0 + tid;
     const int32_t j = e < budget ? kept[static_cast<size_t>(bh) * budget + e] : -1;
     int32_t s = -1, d = -1;
     if (j >= 0) {
@@ -275,32 +331,64 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
       const uint32_t dp = static_cast<uint32_t>(dst_pages[static_cast<size_t>(b) * dst_max_pages + (e >> a.lp)]);
       if (dp < a.n_pages) d = static_cast<int32_t>(dp);
       if (s < 0 || d < 0) paged_flag(a.status);
-      s_so[tid] = static_cast<uint32_t>(j) & mask;
-      s_do[tid] = e & mask;
     }
+    s_so[tid] = static_cast<uint32_t>(j) & mask;
     s_src[tid] = s;
     s_dst[tid] = d;
   }
   __syncthreads();
-  for (uint32_t i = tid; i < 64u * CH; i += 256u) {
-    const uint32_t e = i / CH, c = i % CH;
-    if (s_dst[e] < 0) continue;
-    uint4 x = make_uint4(0u, 0u, 0u, 0u);
-    if (s_src[e] >= 0)
-      x = *reinterpret_cast<const uint4*>(
-          a.k + (((static_cast<size_t>(s_src[e]) * a.n_kv + h) << a.lp) + s_so[e]) * (HD * sizeof(T)) + 16u * c);
-    *reinterpret_cast<uint4*>(const_cast<uint8_t*>(a.k) +
-                              (((static_cast<size_t>(s_dst[e]) * a.n_kv + h) << a.lp) + s_do[e]) * (HD * sizeof(T)) +
-                              16u * c) = x;
+  uint8_t* const kb = const_cast<uint8_t*>(a.k);
+  constexpr uint32_t KN = (64u * CH + 255u) / 256u;  // a thread's chunks: all read before the first is written
+  uint4 kx[KN];
+#pragma unroll
+  for (uint32_t i = 0; i < KN; ++i) {
+    const uint32_t t = tid + 256u * i, e = t / CH % 64u, c = t % CH;
+    kx[i] = *reinterpret_cast<const uint4*>(kb + (((static_cast<size_t>(max(s_src[e], 0)) * a.n_kv + h) << a.lp) + s_so[e]) * (HD * SZ) + 16u * c);
+    if (s_src[e] < 0) kx[i] = make_uint4(0u, 0u, 0u, 0u);
   }
+#pragma unroll
+  for (uint32_t i = 0; i < KN; ++i) {
+    const uint32_t t = tid + 256u * i, e = t / CH % 64u, c = t % CH;
+    if ((64u * CH % 256u == 0u || t < 64u * CH) && s_dst[e] >= 0)
+      *reinterpret_cast<uint4*>(kb + (((static_cast<size_t>(s_dst[e]) * a.n_kv + h) << a.lp) + ((e0 + e) & mask)) * (HD * SZ) + 16u * c) = kx[i];
+  }
+  constexpr uint32_t DW = HD / 64u;  // waves across the dims
   const T* vs = reinterpret_cast<const T*>(a.v);
   T* vd = reinterpret_cast<T*>(const_cast<uint8_t*>(a.v));
-  const uint32_t e = tid & 63u;
-  if (s_dst[e] < 0) return;
-  for (uint32_t d = tid >> 6; d < HD; d += 4u) {
-    T x = 0;
-    if (s_src[e] >= 0) x = vs[((((static_cast<size_t>(s_src[e]) * a.n_kv + h) * HD) + d) << a.lp) + s_so[e]];
-    vd[((((static_cast<size_t>(s_dst[e]) * a.n_kv + h) * HD) + d) << a.lp) + s_do[e]] = x;
+  const uint32_t d = 64u * (wave % DW) + lane;
+  for (uint32_t q = wave / DW; q < 4u; q += 4u / DW) {  // 16 entries, of one destination page
+    const int32_t dp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_dst[16u * q])));
+    if (dp < 0) continue;  // uniform: no page, or behind the last entry
+    T x[16];
+    uint32_t cnt = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      const uint32_t e = 16u * q + i;
+      const int32_t sp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_src[e])));
+      const uint32_t so = uniform(s_so[e]);
+      cnt += uniform(static_cast<uint32_t>(s_dst[e])) == static_cast<uint32_t>(dp) ? 1u : 0u;
+      // (an entry that is not copied reads page 0)
+      const T* row = vs + ((static_cast<size_t>(max(sp, 0)) * a.n_kv + h) * HD << a.lp) + so;
+      x[i] = row[d << a.lp];
+      if (sp < 0) x[i] = 0;  // uniform
+    }
+    T* to = vd + ((static_cast<size_t>(dp) * a.n_kv + h) * HD << a.lp) + (static_cast<size_t>(d) << a.lp) + ((e0 + 16u * q) & mask);
+    if (cnt == 16u) {  // uniform
+      uint32_t o[4 * SZ];
+#pragma unroll
+      for (uint32_t i = 0; i < 4 * SZ; ++i) {
+        if constexpr (F8)
+          o[i] = x[4 * i] | x[4 * i + 1] << 8 | x[4 * i + 2] << 16 | static_cast<uint32_t>(x[4 * i + 3]) << 24;
+        else
+          o[i] = x[2 * i] | static_cast<uint32_t>(x[2 * i + 1]) << 16;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < SZ; ++i) reinterpret_cast<uint4*>(to)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    } else {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i)
+        if (i < cnt) to[i] = x[i];
+    }
   }
 }
 
