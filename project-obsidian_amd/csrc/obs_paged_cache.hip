@@ -41,44 +41,106 @@ struct PrepArgs {
   float eps;
 };
 
-// One workgroup per token row; HD / 8 lanes per head with 8 dims each, so a
-// wave norms and rotates 512 / HD heads at once. The sums and the rotation are
-// attn_prep_rows_kernel's, in its order.
+// The sequence of row t for a lane of its own: a search over the ends from
+// sequence lo on (the first one that ends behind t).
+__device__ __forceinline__ uint32_t seq_of_row_lane(const Paged& a, uint32_t t, uint32_t lo) {
+  uint32_t hi = a.n_seqs;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2u;
+    if (a.row[mid + 1u] <= static_cast<int32_t>(t))
+      lo = mid + 1u;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Values of 64 consecutive token rows of one kv head, transposed through LDS:
+// a lane owns a row, so a store of one dim writes the runs of consecutive
+// entries that the rows are. (From each row's own workgroup, one entry of a
+// cache row at a time, the stores cost more than everything else: 43 against
+// 28 us for 5,475 rows into an e4m3 cache.)
+constexpr uint32_t PREP_TILE = 64;
 template <uint32_t HD, bool F8>
-__global__ void __launch_bounds__(256) prep_paged_kernel(Paged a, PrepArgs p, Weight w) {
+__device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs& p, uint32_t vi) {
+  __shared__ uint32_t s_v[PREP_TILE][HD / 2u + 1u];  // rows of dim pairs (+1 word: bank spread)
+  const uint32_t h = vi % a.n_kv, t0 = vi / a.n_kv * PREP_TILE, nt = umin(PREP_TILE, a.n_rows - t0);
+#pragma unroll
+  for (uint32_t i = 0; i < PREP_TILE * HD / 2048u; ++i) {  // 16-byte chunks
+    const uint32_t c = threadIdx.x + 256u * i, r = c / (HD / 8u), d = 8u * (c % (HD / 8u));
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (r < nt) x = *reinterpret_cast<const uint4*>(p.v + static_cast<size_t>(t0 + r) * p.kv_ld + h * HD + d);
+    uint32_t* to = &s_v[r][d / 2u];
+    to[0] = x.x;
+    to[1] = x.y;
+    to[2] = x.z;
+    to[3] = x.w;
+  }
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, t = t0 + lane;
+  const uint32_t b0 = seq_of_row(a, t0, lane);
+  bool there = false;
+  size_t at = 0;
+  if (lane < nt && b0 < a.n_seqs) {
+    const uint32_t b = seq_of_row_lane(a, t, b0);
+    if (b < a.n_seqs) {
+      const RowSpan r = paged_rows(a, b);
+      const int32_t entry = static_cast<int32_t>(paged_len(a, b)) - static_cast<int32_t>(r.r1 - t);
+      const int32_t pos = p.pos ? p.pos[t] : entry;
+      if (t >= r.r0 && t < r.r1 && entry >= 0 && pos >= 0 && static_cast<uint32_t>(pos) < p.rope_len) {
+        const uint32_t page = paged_id(a, b, static_cast<uint32_t>(entry), there);  // reported by the row's workgroup
+        at = ((static_cast<size_t>(page) * a.n_kv + h) * HD << a.lp) + (static_cast<uint32_t>(entry) & ((1u << a.lp) - 1u));
+      }
+    }
+  }
+  const float s = F8 ? a.v_scale[h] : 1.0f;
+  __syncthreads();
+  if (!there) return;
+  for (uint32_t d = wave * (HD / 4u); d < (wave + 1u) * (HD / 4u); d += 2u) {
+    const uint32_t w = s_v[lane][d / 2u];
+    if constexpr (F8) {
+      const uint32_t b2 = pack_e4m3x4(bf16lo(w) / s, bf16hi(w) / s, 0.0f, 0.0f);
+      uint8_t* to = const_cast<uint8_t*>(a.v) + at + (static_cast<size_t>(d) << a.lp);
+      to[0] = static_cast<uint8_t>(b2);
+      to[1u << a.lp] = static_cast<uint8_t>(b2 >> 8);
+    } else {
+      uint16_t* to = reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(a.v)) + at + (static_cast<size_t>(d) << a.lp);
+      to[0] = static_cast<uint16_t>(w);
+      to[1u << a.lp] = static_cast<uint16_t>(w >> 16);
+    }
+  }
+}
+
+// Workgroups 0 .. n_vt - 1 bring the values of prompts (none with one token a
+// sequence). The others: a token row each; HD / 8 lanes per head with 8 dims
+// each, so a wave norms and rotates 512 / HD heads at once. The sums and the
+// rotation are attn_prep_rows_kernel's, in its order. The first heads are
+// requested before the row's sequence, entry and position are known.
+template <uint32_t HD, bool F8>
+__global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p, Weight w, uint32_t n_vt) {
   constexpr uint32_t LPH = HD / 8u, HPW = 64u / LPH;  // lanes per head, heads per wave
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, m = lane % LPH, c0 = 8u * m;
-  const uint32_t t = blockIdx.x;
-  const uint32_t b = __builtin_amdgcn_readfirstlane(seq_of_row(a, t, lane));
+  if (blockIdx.x < n_vt) {  // uniform
+    prep_paged_values<HD, F8>(a, p, blockIdx.x);
+    return;
+  }
+  const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), m = lane % LPH, c0 = 8u * m;
+  const uint32_t t = blockIdx.x - n_vt, heads = p.nh + a.n_kv;
+  const uint16_t* q = p.q + static_cast<size_t>(t) * p.q_ld;
+  const uint16_t* k = p.k + static_cast<size_t>(t) * p.kv_ld;
+  auto load_head = [&](uint32_t head) __attribute__((always_inline)) {  // clamped: past the last head, unused
+    const uint32_t hc = umin(head, heads - 1u);
+    return *reinterpret_cast<const uint4*>((hc < p.nh ? q + hc * HD : k + (hc - p.nh) * HD) + c0);
+  };
+  uint4 xv = load_head(HPW * wave + lane / LPH);
+  const uint4 wq = *reinterpret_cast<const uint4*>(p.q_norm + c0), wk = *reinterpret_cast<const uint4*>(p.k_norm + c0);
+  const uint32_t b = uniform(seq_of_row(a, t, lane));
   if (b >= a.n_seqs) return;  // uniform
   const RowSpan rs = paged_rows(a, b);
   if (t < rs.r0 || t >= rs.r1) return;
-  const uint32_t n = paged_len(a, b);
+  const uint32_t n = uniform(paged_len(a, b));
   if (t == rs.r0 && threadIdx.x == 0u && paged_len_bad(a, b)) paged_flag(a.status);
-  const int32_t entry = static_cast<int32_t>(n) - static_cast<int32_t>(rs.r1 - t);
-  const int32_t pos = p.pos ? p.pos[t] : entry;
+  const int32_t entry = static_cast<int32_t>(n) - static_cast<int32_t>(uniform(rs.r1) - t);
+  const int32_t pos = p.pos ? static_cast<int32_t>(uniform(static_cast<uint32_t>(p.pos[t]))) : entry;
   if (pos < 0 || static_cast<uint32_t>(pos) >= p.rope_len) return;  // uniform
-  bool there = entry >= 0;
-  const uint32_t e = there ? static_cast<uint32_t>(entry) : 0u;
-  bool ok;
-  const uint32_t page = paged_id(a, b, e, ok);
-  if (there && !ok && threadIdx.x == 0u) paged_flag(a.status);
-  there = there && ok;
-  const uint32_t off = e & ((1u << a.lp) - 1u);
-  if (w.w && entry >= 0 && threadIdx.x < a.n_kv) {
-    const int64_t s = weight_slot(w, b);
-    if (s >= 0)
-      for (uint32_t h = threadIdx.x; h < a.n_kv; h += 256u) w.w[(static_cast<size_t>(s) * a.n_kv + h) * w.ld + e] = 0.0f;
-    else if (threadIdx.x == 0u)
-      paged_flag(a.status);
-  }
-  const uint16_t* q = p.q + static_cast<size_t>(t) * p.q_ld;
-  const uint16_t* k = p.k + static_cast<size_t>(t) * p.kv_ld;
-  const uint16_t* v = p.v + static_cast<size_t>(t) * p.kv_ld;
-  uint16_t* q_out = p.q_out + static_cast<size_t>(t) * p.q_out_ld;
-  const size_t page0 = static_cast<size_t>(page) * a.n_kv;
-  const uint32_t heads = p.nh + a.n_kv, pg = 1u << a.lp;
-  const bool first = m < LPH / 2u;
   float cs[8], sn[8];  // of the lane's pairs: columns c0 .. c0 + 7 modulo HD / 2
   {
     const float* tab = p.rope + static_cast<size_t>(pos) * 128u + (HD == 128u ? 16u : 32u) * (m % (LPH / 2u));
@@ -90,12 +152,31 @@ __global__ void __launch_bounds__(256) prep_paged_kernel(Paged a, PrepArgs p, We
       sn[i] = t2.y;
     }
   }
+  bool there = entry >= 0;
+  const uint32_t e = there ? static_cast<uint32_t>(entry) : 0u;
+  bool ok;
+  const uint32_t page = uniform(paged_id(a, b, e, ok));
+  if (there && !ok && threadIdx.x == 0u) paged_flag(a.status);
+  there = there && ok;
+  const uint32_t off = e & ((1u << a.lp) - 1u);
+  if (w.w && entry >= 0 && threadIdx.x < a.n_kv) {
+    const int64_t s = weight_slot(w, b);
+    if (s >= 0)
+      for (uint32_t h = threadIdx.x; h < a.n_kv; h += 256u) w.w[(static_cast<size_t>(s) * a.n_kv + h) * w.ld + e] = 0.0f;
+    else if (threadIdx.x == 0u)
+      paged_flag(a.status);
+  }
+  uint16_t* q_out = p.q_out + static_cast<size_t>(t) * p.q_out_ld;
+  const size_t page0 = static_cast<size_t>(page) * a.n_kv;
+  const uint32_t pg = 1u << a.lp;
+  const bool first = m < LPH / 2u;
   for (uint32_t hb = HPW * wave; hb < heads; hb += 4u * HPW) {  // uniform per wave
-    const uint32_t head = hb + lane / LPH, hc = min(head, heads - 1u);
-    const bool is_q = hc < p.nh;
-    const uint4 xv = *reinterpret_cast<const uint4*>((is_q ? q + hc * HD : k + (hc - p.nh) * HD) + c0);
-    const uint4 wv = *reinterpret_cast<const uint4*>((is_q ? p.q_norm : p.k_norm) + c0);
-    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w}, ww[4] = {wv.x, wv.y, wv.z, wv.w};
+    const uint32_t head = hb + lane / LPH;
+    const bool is_q = head < p.nh;
+    const uint4 xnext = load_head(head + 4u * HPW);
+    const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+    const uint32_t ww[4] = {is_q ? wq.x : wk.x, is_q ? wq.y : wk.y, is_q ? wq.z : wk.z, is_q ? wq.w : wk.w};
+    xv = xnext;
     float ps[4];
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
@@ -109,12 +190,16 @@ __global__ void __launch_bounds__(256) prep_paged_kernel(Paged a, PrepArgs p, We
     ss = ss + dpp_f32<DPP_HALF_MIRROR>(ss);
     if constexpr (HD == 128u) ss = ss + dpp_f32<DPP_MIRROR>(ss);
     const float inv = 1.0f / __builtin_sqrtf(ss / static_cast<float>(HD) + p.eps);
-    float r[8];
+    float nvs[8], r[8];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {  // rounded as the stored q / k would be
+      const uint32_t pr = pack_bf16_pair_rne((bf16lo(xw[i]) * inv) * bf16lo(ww[i]), (bf16hi(xw[i]) * inv) * bf16hi(ww[i]));
+      nvs[2 * i] = bf16lo(pr);
+      nvs[2 * i + 1] = bf16hi(pr);
+    }
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      const float x = i & 1u ? bf16hi(xw[i / 2u]) : bf16lo(xw[i / 2u]);
-      const float wn = i & 1u ? bf16hi(ww[i / 2u]) : bf16lo(ww[i / 2u]);
-      const float nv = bf16_to_f32(f32_to_bf16((x * inv) * wn));  // as the stored q / k would be
+      const float nv = nvs[i];
       float other;  // columns +- HD / 2
       if constexpr (HD == 128u)
         other = dpp_f32<DPP_ROW_ROR8>(nv);
@@ -126,7 +211,8 @@ __global__ void __launch_bounds__(256) prep_paged_kernel(Paged a, PrepArgs p, We
     if (head >= heads) continue;
     if (is_q) {
       *reinterpret_cast<uint4*>(q_out + head * HD + c0) =
-          make_uint4(pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]), pack_bf16x2(r[4], r[5]), pack_bf16x2(r[6], r[7]));
+          make_uint4(pack_bf16_pair_rne(r[0], r[1]), pack_bf16_pair_rne(r[2], r[3]), pack_bf16_pair_rne(r[4], r[5]),
+                     pack_bf16_pair_rne(r[6], r[7]));
     } else if (there) {
       const uint32_t h = head - p.nh;
       const size_t at = ((page0 + h) * pg + off) * HD + c0;
@@ -138,12 +224,14 @@ __global__ void __launch_bounds__(256) prep_paged_kernel(Paged a, PrepArgs p, We
         *reinterpret_cast<uint2*>(const_cast<uint8_t*>(a.k) + at) = o;
       } else {
         *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(a.k)) + at) = make_uint4(
-            pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]), pack_bf16x2(r[4], r[5]), pack_bf16x2(r[6], r[7]));
+            pack_bf16_pair_rne(r[0], r[1]), pack_bf16_pair_rne(r[2], r[3]), pack_bf16_pair_rne(r[4], r[5]),
+            pack_bf16_pair_rne(r[6], r[7]));
       }
     }
   }
-  if (!there) return;
-  for (uint32_t i = threadIdx.x; i < a.n_kv * HD; i += 256u) {  // values: one transposed column
+  if (!there || n_vt) return;
+  const uint16_t* v = p.v + static_cast<size_t>(t) * p.kv_ld;
+  for (uint32_t i = threadIdx.x; i < a.n_kv * HD; i += 256u) {  // one token: one transposed column
     const uint32_t h = i / HD, d = i % HD;
     const size_t at = ((page0 + h) * HD + d) * pg + off;
     if constexpr (F8)
@@ -483,16 +571,17 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
   if (rc != OBS_OK) return rc;
   const Paged a = obs::paged_args(ctx, kv, seqs);
   const Weight w = obs::weight_args(weight);
-  const uint32_t grid = seqs->n_rows;
+  const uint32_t n_vt = seqs->row ? kv->n_kv * ((seqs->n_rows + PREP_TILE - 1u) / PREP_TILE) : 0u;
+  const uint32_t grid = n_vt + seqs->n_rows;
   const bool f8 = kv->dtype == OBS_KV_E4M3;
   if (hd == 128u && !f8)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, false><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, false><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
   else if (hd == 128u)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, true><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, true><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
   else if (!f8)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, false><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, false><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
   else
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, true><<<grid, 256, 0, ctx->stream>>>(a, p, w));
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, true><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
   return OBS_OK;
 }
 
