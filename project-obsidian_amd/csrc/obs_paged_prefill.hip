@@ -32,7 +32,7 @@ using obs::up256;
 // in fp32 and P in bf16, which has fp32's range), so O is hardly ever rescaled.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
 
-constexpr uint32_t PF_COLS = 256, PF_TARGET = 512, PF_MIN_CHUNK = 8;
+constexpr uint32_t PF_COLS = 256, PF_TARGET = 256, PF_MIN_CHUNK = 4;
 constexpr float PF_SLACK = 8.0f;
 
 // Tiles and blocks of the sequences, as the parts are planned by.
@@ -50,37 +50,42 @@ __device__ __forceinline__ PrefillSeq prefill_seq(const Paged& a, const PagedAtt
   return {tiles, tiles ? tile_span(p, r, paged_len(a, b), r.r0 + (tiles - 1u) * tq, r.r1).nblk : 0u};
 }
 struct PrefillItem {
-  uint32_t b, tile, split, splits, chunk, first;  // first: the part of the tile's split 0
+  uint32_t b, tile, split, splits, first, place;  // first: the part of the tile's split 0; place: the tile among all
 };
 // Part `item` of a kv head: sequences in order, in each the last tile (the
-// longest) first, a tile's parts together.
+// longest) first, a tile's parts together. With few rows (target > 0) a
+// sequence's tiles are cut into equal parts, its share of the target rounded
+// down: the parts then fill the chip once (a workgroup fills a CU).
 __device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane) {
-  uint32_t chunk = 0xffffffffu;
-  if (p.target) {  // few rows: parts of equal length
-    uint64_t total = 0;
+  float rate = 0.0f;
+  if (p.target) {
+    float total = 0.0f;
     for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
       PrefillSeq s{0u, 0u};
       if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
-      total += wave_sum_u32(s.tiles * s.nblk);
+      total += wave_sum_asc(static_cast<float>(s.tiles) * static_cast<float>(s.nblk));
     }
-    chunk = uniform(max(PF_MIN_CHUNK, static_cast<uint32_t>((total * a.n_kv + p.target - 1u) / p.target)));
+    rate = static_cast<float>(p.target) / fmaxf(total * static_cast<float>(a.n_kv), 1.0f);
   }
-  uint32_t acc = 0;
+  uint32_t acc = 0, tacc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
     PrefillSeq s{0u, 0u};
     if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
-    const uint32_t splits = p.target ? plan_splits(s.nblk, chunk) : 1u;
+    const uint32_t share = static_cast<uint32_t>(static_cast<float>(s.nblk) * rate);
+    const uint32_t splits = max(1u, umin(share, s.nblk / PF_MIN_CHUNK));
     const uint32_t incl = wave_scan_u32(s.tiles * splits), all = __builtin_amdgcn_readlane(incl, 63);
+    const uint32_t tincl = wave_scan_u32(s.tiles);
     if (item < acc + all) {
       const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
-      const uint32_t before = acc + (l ? static_cast<uint32_t>(__builtin_amdgcn_readlane(incl, l - 1u)) : 0u);
       const uint32_t tl = __builtin_amdgcn_readlane(s.tiles, l), sp = __builtin_amdgcn_readlane(splits, l);
-      const uint32_t x = (item - before) / sp, split = (item - before) % sp;
-      return {uniform(base + l), uniform(tl - 1u - x), uniform(split), uniform(sp), uniform(chunk), uniform(item - split)};
+      const uint32_t end = acc + __builtin_amdgcn_readlane(incl, l), tend = tacc + __builtin_amdgcn_readlane(tincl, l);
+      const uint32_t at = item - (end - tl * sp), x = at / sp, split = at % sp;
+      return {uniform(base + l), uniform(tl - 1u - x), uniform(split), uniform(sp), uniform(item - split), uniform(tend - tl + x)};
     }
     acc += all;
+    tacc += __builtin_amdgcn_readlane(tincl, 63);
   }
-  return {a.n_seqs, 0u, 0u, 1u, chunk, 0u};
+  return {a.n_seqs, 0u, 0u, 1u, 0u, 0u};
 }
 
 template <uint32_t HD, bool F8>
@@ -107,8 +112,10 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
   const Span s = tile_span(p, r, n, t0r, t1r);
   const uint32_t hi_first = n + t0r + 1u > r.r1 ? n + t0r + 1u - r.r1 : 0u;
   const uint32_t lo_last = p.window && s.hi > p.window ? s.hi - p.window : 0u;
-  const uint32_t x0 = it.split * (it.splits > 1u ? it.chunk : 0u);
-  const uint32_t x1 = it.splits > 1u ? umin(s.nblk, x0 + it.chunk) : s.nblk;
+  const uint32_t q0 = s.nblk / it.splits, q1 = s.nblk % it.splits;  // parts of q0 or q0 + 1 blocks
+  const uint32_t x0 = it.split * q0 + umin(it.split, q1), x1 = x0 + q0 + (it.split < q1 ? 1u : 0u);
+  if (p.target && it.split == 0u && tid == 0u)  // for the join
+    reinterpret_cast<uint4*>(p.plan)[static_cast<size_t>(it.place) * a.n_kv + kv] = make_uint4(it.first, it.splits, t0r, t1r);
   const float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
   if (tid == 0u) s_bad = 0u;
 
@@ -369,30 +376,48 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
   }
 }
 
-// A tile's parts joined in order: a workgroup per 256 / HD * 4 columns.
+// A tile's parts joined in order: 1024 / HD columns a workgroup, four dims a
+// thread, eight parts in flight at once.
 template <uint32_t HD, bool F8>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedAttn p, uint32_t items) {
-  constexpr uint32_t CW = 1024u / HD;  // columns of a workgroup, 4 dims a thread
-  const uint32_t tid = threadIdx.x, lane = tid & 63u;
-  const uint32_t part = blockIdx.x / (PF_COLS / CW), c = blockIdx.x % (PF_COLS / CW) * CW + tid / (HD / 4u), d = 4u * (tid % (HD / 4u));
-  const uint32_t kv = part % a.n_kv;
-  const PrefillItem it = prefill_find(a, p, part / a.n_kv, lane);
-  if (it.b >= a.n_seqs || it.splits == 1u || it.split != 0u) return;  // uniform
-  const RowSpan r = paged_rows(a, it.b);
-  const uint32_t tq = PF_COLS / p.G, t = r.r0 + it.tile * tq + c / p.G, h = kv * p.G + c % p.G;
-  if (c / p.G >= tq || t >= r.r1) return;
-  float M = NEG_INF;
-  for (uint32_t i = 0; i < it.splits; ++i)
-    M = fmaxf(M, p.ml[((static_cast<size_t>(it.first + i) * a.n_kv + kv) * PF_COLS + c) * 2u]);
-  float L = 0.0f;
+  constexpr uint32_t CW = 1024u / HD, WG = PF_COLS / CW;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, place = blockIdx.x / (WG * a.n_kv), kv = blockIdx.x / WG % a.n_kv;
+  const uint32_t c = blockIdx.x % WG * CW + tid / (HD / 4u), d = 4u * (tid % (HD / 4u));
+  uint32_t tiles = 0;
+  for (uint32_t base = 0; base < a.n_seqs; base += 64u)
+    tiles += wave_sum_u32(base + lane < a.n_seqs ? prefill_seq(a, p, base + lane).tiles : 0u);
+  if (place >= tiles) return;  // uniform
+  const uint4 plan = reinterpret_cast<const uint4*>(p.plan)[static_cast<size_t>(place) * a.n_kv + kv];
+  const uint32_t splits = uniform(plan.y), first = uniform(plan.x), t = plan.z + c / p.G, h = kv * p.G + c % p.G;
+  if (splits == 1u || c / p.G >= PF_COLS / p.G || t >= plan.w) return;
+  float M = NEG_INF, L = 0.0f;
   f32x4_v o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t i = 0; i < it.splits; ++i) {
-    const size_t at = (static_cast<size_t>(it.first + i) * a.n_kv + kv) * PF_COLS + c;
-    const float m = p.ml[at * 2u], f = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-    const f32x4_v x = *reinterpret_cast<const f32x4_v*>(p.part + at * HD + d);
-    L = __builtin_fmaf(p.ml[at * 2u + 1u], f, L);
+  for (uint32_t i0 = 0; i0 < splits; i0 += 8u) {
+    float2 ml[8];
+    f32x4_v x[8];
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) o[j] = __builtin_fmaf(x[j], f, o[j]);
+    for (uint32_t i = 0; i < 8; ++i) {
+      // behind the last part it again, without weight (and within the launch's parts whatever the rows)
+      const size_t part = umin((first + umin(i0 + i, splits - 1u)) * a.n_kv + kv, items - 1u);
+      ml[i] = *reinterpret_cast<const float2*>(p.ml + (part * PF_COLS + c) * 2u);
+      x[i] = *reinterpret_cast<const f32x4_v*>(p.part + (part * PF_COLS + c) * HD + d);
+    }
+    float mn = M;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+    const float back = M == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(M - mn);
+    M = mn;
+    L *= back;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) o[j] *= back;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      if (i0 + i >= splits) break;  // uniform
+      const float f = ml[i].x == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(ml[i].x - mn);
+      L = __builtin_fmaf(ml[i].y, f, L);
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) o[j] = __builtin_fmaf(x[i][j], f, o[j]);
+    }
   }
   const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
   float v[4];
@@ -405,21 +430,23 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedA
 // Prefill: with few rows for the chip (tiles of both kinds of sequence ends
 // counted by the rows alone) a tile's blocks are cut into parts.
 struct PrefillPlan {
-  uint64_t items;  // workgroups at most
+  uint64_t items, tiles;  // workgroups and tiles (of all kv heads) at most
   bool split;
-  size_t ml, part;
+  size_t ml, part, plan;
+  size_t all() const { return ml + part + plan + 256u; }
 };
 PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32_t n_heads, uint32_t window, uint32_t sinks) {
   PrefillPlan d{};
   const uint32_t tq = PF_COLS / (n_heads / kv->n_kv);
   const uint64_t full = static_cast<uint64_t>(kv->n_kv) * ((s->n_rows + tq - 1u) / tq);
   // tiles: at most one that is not full a sequence, and none of a sequence without rows
-  const uint64_t tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
-  d.split = 2u * full <= PF_TARGET && most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks) > PF_MIN_CHUNK;
-  d.items = d.split ? PF_TARGET + tiles : tiles;
+  d.tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
+  d.split = 2u * full <= PF_TARGET + 128u && most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks) > PF_MIN_CHUNK;
+  d.items = d.split ? PF_TARGET + d.tiles + 64u : d.tiles;  // (64: what fp32 rounds)
   if (d.split) {
     d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
     d.part = up256(d.items * PF_COLS * kv->head_dim * sizeof(float));
+    d.plan = up256(d.tiles * sizeof(uint4));
   }
   return d;
 }
@@ -430,7 +457,7 @@ int launch_prefill(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Prefi
   OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, 512, 0, ctx->stream>>>(a, p));
   if (d.split)
     OBS_LAUNCH(ctx, "paged_prefill_join",
-               paged_prefill_join_kernel<HD, F8><<<grid * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
+               paged_prefill_join_kernel<HD, F8><<<static_cast<uint32_t>(d.tiles) * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
   return OBS_OK;
 }
 
@@ -439,7 +466,7 @@ int launch_prefill(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Prefi
 namespace obs {
 size_t prefill_paged_ws(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32_t n_heads, uint32_t window, uint32_t sinks) {
   const PrefillPlan d = prefill_plan(kv, s, n_heads, window, sinks);
-  return d.ml + d.part + 256u;
+  return d.all();
 }
 }  // namespace obs
 
@@ -455,14 +482,14 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
   if (rc != OBS_OK) return rc;
   if (!seqs->row) return obs::set_error(ctx, OBS_E_INVALID, "%s: null row (obs_sdpa_paged_decode takes one token a sequence)", who);
   const PrefillPlan d = prefill_plan(kv, seqs, n_heads, window, sinks);
-  rc = obs::check_attn(ctx, who, kv, seqs, nullptr, q, out, n_heads, &q_ld, ws, ws_bytes, d.ml + d.part + 256u);
+  rc = obs::check_attn(ctx, who, kv, seqs, nullptr, q, out, n_heads, &q_ld, ws, ws_bytes, d.all());
   if (rc != OBS_OK) return rc;
   if (seqs->n_seqs == 0 || seqs->n_rows == 0) return OBS_OK;
   if (d.items * 32u > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many rows and heads", who);
   obs::DeviceGuard guard(ctx);
   const Paged a = obs::paged_args(ctx, kv, seqs);
   uint8_t* wb = static_cast<uint8_t*>(ws);
-  const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr, nullptr, n_heads,
+  const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr, reinterpret_cast<uint2*>(wb + d.ml + d.part), n_heads,
                    n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u,
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const bool f8 = kv->dtype == OBS_KV_E4M3;
