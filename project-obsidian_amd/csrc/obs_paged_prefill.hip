@@ -53,26 +53,38 @@ struct PrefillItem {
   uint32_t b, tile, split, splits, first, place;  // first: the part of the tile's split 0; place: the tile among all
 };
 // Part `item` of a kv head: sequences in order, in each the last tile (the
-// longest) first, a tile's parts together. With few rows (target > 0) a
-// sequence's tiles are cut into equal parts, its share of the target rounded
-// down: the parts then fill the chip once (a workgroup fills a CU).
+// longest) first, a tile's parts together. With few rows (target > 0) the tiles
+// are cut into parts that fill the chip once (a workgroup fills a CU).
 __device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane) {
-  float rate = 0.0f;
+  // The shortest parts, in steps of an eighth, of which there are no more than
+  // the target: the longest one sets the time.
+  uint32_t chunk = 0xffffffffu;
   if (p.target) {
+    PrefillSeq own{0u, 0u};
+    if (lane < a.n_seqs) own = prefill_seq(a, p, lane);
     float total = 0.0f;
     for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-      PrefillSeq s{0u, 0u};
-      if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
+      PrefillSeq s = own;
+      if (base) s = base + lane < a.n_seqs ? prefill_seq(a, p, base + lane) : PrefillSeq{0u, 0u};
       total += wave_sum_asc(static_cast<float>(s.tiles) * static_cast<float>(s.nblk));
     }
-    rate = static_cast<float>(p.target) / fmaxf(total * static_cast<float>(a.n_kv), 1.0f);
+    const float even = total * static_cast<float>(a.n_kv) / static_cast<float>(p.target);
+    for (uint32_t k = 8; k <= 16u; ++k) {
+      chunk = max(PF_MIN_CHUNK, static_cast<uint32_t>(__builtin_ceilf(even * static_cast<float>(k) * 0.125f)));
+      uint32_t parts = 0;
+      for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
+        PrefillSeq s = own;
+        if (base) s = base + lane < a.n_seqs ? prefill_seq(a, p, base + lane) : PrefillSeq{0u, 0u};
+        parts += wave_sum_u32(s.tiles * plan_splits(s.nblk, chunk));
+      }
+      if (parts * a.n_kv <= p.target) break;  // uniform
+    }
   }
   uint32_t acc = 0, tacc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
     PrefillSeq s{0u, 0u};
     if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
-    const uint32_t share = static_cast<uint32_t>(static_cast<float>(s.nblk) * rate);
-    const uint32_t splits = max(1u, umin(share, s.nblk / PF_MIN_CHUNK));
+    const uint32_t splits = p.target ? plan_splits(s.nblk, chunk) : 1u;
     const uint32_t incl = wave_scan_u32(s.tiles * splits), all = __builtin_amdgcn_readlane(incl, 63);
     const uint32_t tincl = wave_scan_u32(s.tiles);
     if (item < acc + all) {
@@ -442,7 +454,7 @@ PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32
   // tiles: at most one that is not full a sequence, and none of a sequence without rows
   d.tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
   d.split = 2u * full <= PF_TARGET + 128u && most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks) > PF_MIN_CHUNK;
-  d.items = d.split ? PF_TARGET + d.tiles + 64u : d.tiles;  // (64: what fp32 rounds)
+  d.items = d.split ? PF_TARGET + d.tiles + 64u : d.tiles;  // parts of 1 / target of all blocks at least, and one a tile
   if (d.split) {
     d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
     d.part = up256(d.items * PF_COLS * kv->head_dim * sizeof(float));
