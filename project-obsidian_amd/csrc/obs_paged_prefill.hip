@@ -13,26 +13,29 @@ using obs::up256;
 // ---------------------------------------------------------------------------
 // Token rows of prompts
 // ---------------------------------------------------------------------------
-// A workgroup takes 256 / G consecutive rows of one sequence and the G heads of
-// one kv head: 256 columns, 64 a wave (two groups of 32), over the blocks of 32
-// entries that any of them sees (or a part of those, where there are few rows).
-// Keys and values go through LDS, read there once per 64 columns: a block is
-// 16 + 16 v_mfma_f32_32x32x16_bf16 (1,024 cycles of a SIMD) against 16 KB of LDS
-// reads a wave (512 of the CU's cycles for the four).
+// A workgroup takes 384 / G consecutive rows of one sequence and the G heads of
+// one kv head: 384 columns, 32 a wave, over the blocks of 32 entries that any of
+// them sees (or a part of those, where there are few rows). Keys and values go
+// through LDS: a block is 8 + 8 v_mfma_f32_32x32x16_bf16 a wave.
 //   S^T [32 entries x 32 columns] = K . Q^T, O^T [dims x 32 columns] += V^T . P: a
 // lane (column lane % 32, half lane / 32) keeps its column throughout. Row r of
 // the score tile is the block's entry with bits 2 and 3 of r exchanged, so a
 // lane's sixteen scores are entries 8 half .. + 7 and 16 + 8 half .. + 7: the
 // values of one 16-byte read of a transposed value row, in the order of the
 // second product's operand.
-// One wave has a SIMD to itself (512 registers), so products and softmax only
-// overlap inside it: an iteration computes block x's softmax and value product
-// together with block x + 1's scores, which do not depend on them. The running
-// maximum follows the scores only when they pass it by 2^8 (the sums and O are
-// in fp32 and P in bf16, which has fp32's range), so O is hardly ever rescaled.
+// Three waves a SIMD (168 registers) overlap each other's products and softmax.
+// Measured against it, at 8,192 rows under a window of 4,096 and at a prompt of
+// 5,001: one wave of 64 columns a SIMD 936 and 332 us (a wave issues an
+// instruction every four cycles), two of 32 columns with the next block's scores
+// beside this one's softmax 602 and 245, this one 594 and 223. More loads in
+// flight, LDS reads earlier, two blocks a barrier, wave priorities and the other
+// machine schedulers gained nothing.
+// The running maximum follows the scores only when they pass it by 2^8 (the sums
+// and O are in fp32 and P in bf16, which has fp32's range), so O is hardly ever
+// rescaled.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
 
-constexpr uint32_t PF_COLS = 256, PF_TARGET = 256, PF_MIN_CHUNK = 4;
+constexpr uint32_t PF_COLS = 384, PF_THREADS = 2u * PF_COLS, PF_TARGET = 256, PF_MIN_CHUNK = 4;
 constexpr float PF_SLACK = 8.0f;
 
 // Tiles and blocks of the sequences, as the parts are planned by.
@@ -101,7 +104,7 @@ __device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const PagedA
 }
 
 template <uint32_t HD, bool F8>
-__global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p) {
+__global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, PagedAttn p) {
   constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = F8 ? 1u : 2u;
   constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
   constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
@@ -152,9 +155,8 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
   for (uint32_t d = 0; d < DT; ++d) o[d] = f32x16_v{};
 
   // A wave's chunks lie in one half of a block, so in one page: a scalar offset
-  // and a constant one a lane. Where a block has fewer chunks than threads, the
-  // first waves bring keys and the last ones values.
-  const uint32_t kc = tid, vc = VN == 512u ? tid : tid ^ 256u;
+  // and a constant one a lane. The first waves bring keys, others values.
+  const uint32_t kc = tid, vc = tid >= 256u ? tid - 256u : tid + 512u;
   const bool has_k = kc < KN, has_v = vc < VN;  // wave-uniform
   const uint32_t kh = uniform(kc / (KN / 2u)) & 1u, vh = uniform(vc / (VN / 2u)) & 1u;
   // A listed block: its first entry, whether its halves' page ids are good, the
@@ -190,11 +192,11 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
   u32x4_v kr, vr;
   auto load_k = [&](const Blk& k) __attribute__((always_inline)) {
     const uint8_t* base = a.k + ((static_cast<size_t>(k.ik) << a.lp) + (k.t & pmask)) * (HD * SZ);
-    if (KN == 512u || has_k) kr = *reinterpret_cast<const u32x4_v*>(base + koff);
+    if (has_k) kr = *reinterpret_cast<const u32x4_v*>(base + koff);
   };
   auto load_v = [&](const Blk& k) __attribute__((always_inline)) {
     const uint8_t* base = a.v + ((static_cast<size_t>(k.iv) * HD << a.lp) + (k.t & pmask)) * SZ;
-    if (VN == 512u || has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
+    if (has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
   };
   // 16 stored bytes as bf16: one or two 16-byte words
   auto widen = [](const u32x4_v& w, uint32_t j) __attribute__((always_inline)) {
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
     }
   };
   auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
-    if (KN == 512u || has_k) {
+    if (has_k) {
       uint16_t* to = &s_k[buf][(kc / KC) * KROW + (16u / SZ) * (kc % KC)];
 #pragma unroll
       for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(to + 8u * j) = widen(kr, j);
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
   // hold anything there), and those that are not finite too: the rows that see
   // them get them at the end, and no other row meets them.
   auto store_v = [&](uint32_t buf, const Blk& k) __attribute__((always_inline)) {
-    if (VN == 512u || has_v) {
+    if (has_v) {
       u32x4_v w[2u / SZ];
 #pragma unroll
       for (uint32_t j = 0; j < 2u / SZ; ++j) w[j] = widen(vr, j);
@@ -241,7 +243,6 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
   };
   auto sees = [&](uint32_t e) __attribute__((always_inline)) { return e < hi && (e >= lo || e < p.sinks); };
 
-  f32x16_v sa, sb;  // scores of this block and of the next, in turn
   float mx;
   const uint32_t krow = (col & 0x13u) | ((col & 4u) << 1) | ((col & 8u) >> 1);  // bits 2 and 3 exchanged
   auto scores = [&](uint32_t buf, f32x16_v& to) __attribute__((always_inline)) {
@@ -260,29 +261,29 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
 
   if (x0 < x1) {  // uniform
     fetch_ids(x0);
-    Blk ka = block_of(x0), kb = block_of(x0 + 1u), kcb = block_of(x0 + 2u);
+    Blk ka = block_of(x0), kb = block_of(x0 + 1u);
     load_k(ka);
     load_v(ka);
     __syncthreads();  // s_bad is zero
     store_k(x0 & 1u);
     store_v(x0 & 1u, ka);
-    load_k(kb);
-    store_k((x0 + 1u) & 1u);
     __syncthreads();
-    scores(x0 & 1u, sa);
-    maximum(sa);
-    bool up = mx * scale > m + PF_SLACK;
-    auto iteration = [&](uint32_t x, f32x16_v& sc, f32x16_v& next) __attribute__((always_inline)) {
-      if (((x - x0) & 63u) == 61u) fetch_ids(x + 3u);  // uniform
+    for (uint32_t x = x0; x < x1; ++x) {
+      if (((x - x0) & 63u) == 62u) fetch_ids(x + 2u);  // uniform
+      load_k(kb);  // in flight until the end of the iteration
+      load_v(kb);
+      __builtin_amdgcn_sched_barrier(0);
+      f32x16_v sc;
+      scores(x & 1u, sc);
       if (ka.edge) {  // uniform
         auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
         if (tid == 0u && ((!ka.ok0 && counts(ka.t)) || (!ka.ok1 && counts(ka.t + 16u)))) paged_flag(a.status);
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i)
           sc[i] = (i < 8u ? ka.ok0 : ka.ok1) && sees(ka.t + 16u * (i / 8u) + 8u * half + i % 8u) ? sc[i] : NEG_INF;
-        maximum(sc);
-        up = mx * scale > m + PF_SLACK;
       }
+      maximum(sc);
+      const bool up = mx * scale > m + PF_SLACK;
       if (__any(up)) {
         const float mn = up ? mx * scale : m;
         const float f = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -293,7 +294,6 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
       }
-      scores((x + 1u) & 1u, next);
       const float mu = m == NEG_INF ? 0.0f : m;
       typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
       const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
@@ -309,29 +309,19 @@ __global__ void __launch_bounds__(512) paged_prefill_kernel(Paged a, PagedAttn p
         }
         pb[k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
       }
-      load_k(kcb);
-      load_v(kb);
-      __builtin_amdgcn_sched_barrier(0);  // the loads go out beside the scores' products, not behind the rest
 #pragma unroll
       for (uint32_t k2 = 0; k2 < 2; ++k2)
 #pragma unroll
         for (uint32_t d = 0; d < DT; ++d)
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]), pb[k2], o[d], 0, 0, 0);
-      maximum(next);
-      up = mx * scale > m + PF_SLACK;
-      const Blk kd = block_of(x + 3u);
-      // K of x was read an iteration ago, V of x - 1 too: their buffers take K of x + 2 and V of x + 1
-      store_k(x & 1u);
+      const Blk kn = block_of(x + 2u);
+      // the slots of block x - 1, last read before the barrier that began this iteration
+      store_k((x + 1u) & 1u);
       store_v((x + 1u) & 1u, kb);
       __syncthreads();
       ka = kb;
-      kb = kcb;
-      kcb = kd;
-    };
-    for (uint32_t x = x0; x < x1; x += 2u) {
-      iteration(x, sa, sb);
-      if (x + 1u < x1) iteration(x + 1u, sb, sa);  // uniform
+      kb = kn;
     }
     if (uniform(s_bad)) {  // after the last barrier; rare
       for (uint32_t x = x0; x < x1; ++x) {
@@ -466,7 +456,7 @@ PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32
 template <uint32_t HD, bool F8>
 int launch_prefill(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const PrefillPlan& d) {
   const uint32_t grid = static_cast<uint32_t>(d.items);
-  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, 512, 0, ctx->stream>>>(a, p));
+  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, PF_THREADS, 0, ctx->stream>>>(a, p));
   if (d.split)
     OBS_LAUNCH(ctx, "paged_prefill_join",
                paged_prefill_join_kernel<HD, F8><<<static_cast<uint32_t>(d.tiles) * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
