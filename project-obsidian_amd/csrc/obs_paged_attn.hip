@@ -391,6 +391,20 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, W
       if (tid == 0u && kv == 0u && c0 == 0u) paged_flag(a.status);
       return;
     }
+    // the first heads' scores and the entries' weights are requested before the totals
+    const uint32_t i0 = c0 + 4u * tid, ic = umin(i0, 32u * s.nblk - 4u), e0 = s.start(ic / 32u) + ic % 32u;
+    const float* sc0 = p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G) * p.vis + ic;
+    float* to = w.w + (static_cast<size_t>(slot) * a.n_kv + kv) * w.ld;
+    auto sees = [&](uint32_t e) { return i0 < 32u * s.nblk && e < s.hi && (e >= s.lo || e < p.sinks); };
+    float4 sc[8];
+    float old[4];
+    auto scores_from = [&](uint32_t h0) __attribute__((always_inline)) {
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) sc[i] = *reinterpret_cast<const float4*>(sc0 + static_cast<size_t>(umin(h0 + i, p.G - 1u)) * p.vis);
+    };
+    scores_from(0u);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) old[i] = sees(e0 + i) ? to[e0 + i] : 0.0f;
     for (uint32_t hh = wave; hh < p.G; hh += 4u) {
       const Total t = join_total(p.ml + (first * 16u + hh) * 2u, splits, lane);
       if (lane == 0u) {
@@ -399,14 +413,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, W
       }
     }
     __syncthreads();
-    const uint32_t i0 = c0 + 4u * tid;
-    if (i0 >= 32u * s.nblk) return;
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const float* sc0 = p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G) * p.vis + i0;
     for (uint32_t h0 = 0; h0 < p.G; h0 += 8u) {
-      float4 sc[8];
-#pragma unroll
-      for (uint32_t i = 0; i < 8; ++i) sc[i] = *reinterpret_cast<const float4*>(sc0 + static_cast<size_t>(umin(h0 + i, p.G - 1u)) * p.vis);
+      if (h0) scores_from(h0);
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
         const float m = s_tot[umin(h0 + i, p.G - 1u)][0], r = h0 + i < p.G ? s_tot[h0 + i][1] : 0.0f;
@@ -416,13 +425,9 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, W
         sum[3] = __builtin_fmaf(__builtin_amdgcn_exp2f(sc[i].w - m), r, sum[3]);
       }
     }
-    const uint32_t e0 = s.start(i0 / 32u) + i0 % 32u;
-    float* to = w.w + (static_cast<size_t>(slot) * a.n_kv + kv) * w.ld;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      const uint32_t e = e0 + i;
-      if (e < s.hi && (e >= s.lo || e < p.sinks)) to[e] += sum[i];
-    }
+    for (uint32_t i = 0; i < 4; ++i)
+      if (sees(e0 + i)) to[e0 + i] = old[i] + sum[i];
   }
 }
 
