@@ -394,9 +394,10 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
 // head) a workgroup. Keys: rows of 16-byte
 // chunks. Values: a wave takes 64 dims (32 where a head has 64), a dim a lane,
 // of 16 entries: the entries are the wave's, so their pages are scalar bases,
-// sixteen loads are in flight, and a lane writes 16 consecutive entries of its
-// row. A transposed value page is read whole as soon as one of its entries is
-// kept (an entry's dims lie a row apart), which is what bounds this kernel.
+// neighbours in one 16-byte chunk share a load, all loads are in flight before
+// the first is taken apart, and a lane writes 16 consecutive entries of its row.
+// A transposed value page is read whole as soon as one of its entries is kept
+// (an entry's dims lie a row apart).
 template <uint32_t HD, bool F8, uint32_t GE>
 __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t* __restrict__ dst_pages,
                                                          uint32_t dst_max_pages, uint32_t budget,
@@ -448,17 +449,47 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
     const int32_t dp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_dst[16u * q])));
     if (dp < 0) continue;  // uniform: no page, or behind the last entry
     T x[16];
-    uint32_t cnt = 0;
+    uint32_t cnt = 0;  // entries of the destination page
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) {
-      const uint32_t e = 16u * q + i;
-      const int32_t sp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_src[e])));
-      const uint32_t so = uniform(s_so[e]);
-      cnt += uniform(static_cast<uint32_t>(s_dst[e])) == static_cast<uint32_t>(dp) ? 1u : 0u;
-      // (an entry that is not copied reads page 0)
-      const T* row = vs + ((static_cast<size_t>(max(sp, 0)) * a.n_kv + h) * HD << a.lp) + so;
-      x[i] = row[d << a.lp];
-      if (sp < 0) x[i] = 0;  // uniform
+    for (uint32_t i = 0; i < 16; ++i)
+      cnt += uniform(static_cast<uint32_t>(s_dst[16u * q + i])) == static_cast<uint32_t>(dp) ? 1u : 0u;
+    if constexpr (GE == 16u) {  // few entries: a load each, the shortest way (6.2 us against 8.0; of many 125 against 103)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        const int32_t sp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_src[16u * q + i])));
+        // (a page that is not there reads page 0)
+        const T* row = vs + ((static_cast<size_t>(max(sp, 0)) * a.n_kv + h) * HD << a.lp) + uniform(s_so[16u * q + i]);
+        x[i] = row[d << a.lp];
+        if (sp < 0) x[i] = 0;  // uniform
+      }
+    } else {
+      // one load for the entries of one 16-byte chunk (CE neighbours of a row)
+      constexpr uint32_t CE = 16u / SZ;
+      u32x4_v ch[16];
+      uint32_t fresh = 0;  // entries that begin another chunk
+      uint32_t ps = 0xffffffffu, pc = 0u;
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        const uint32_t e = 16u * q + i, sp = uniform(static_cast<uint32_t>(s_src[e])), c = uniform(s_so[e]) / CE;
+        if (i == 0u || sp != ps || c != pc) {  // uniform
+          fresh |= 1u << i;
+          // (a page that is not there reads page 0)
+          const T* row = vs + ((static_cast<size_t>(static_cast<int32_t>(sp) < 0 ? 0u : sp) * a.n_kv + h) * HD << a.lp) + CE * c;
+          ch[i] = *reinterpret_cast<const u32x4_v*>(row + (d << a.lp));
+          if (static_cast<int32_t>(sp) < 0) ch[i] = u32x4_v{0u, 0u, 0u, 0u};
+        }
+        ps = sp;
+        pc = c;
+      }
+      u32x4_v cur = ch[0];
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        if (i && (fresh >> i & 1u)) cur = ch[i];  // uniform
+        const uint32_t k = uniform(s_so[16u * q + i]) % CE, byte = k * SZ % 8u;  // its bytes in the chunk's half
+        const uint32_t pick = SZ == 2u ? (0x0c0c0000u | (byte + 1u) << 8 | byte) : (0x0c0c0c00u | byte);
+        const uint32_t lo = __builtin_amdgcn_perm(cur.y, cur.x, pick), hi = __builtin_amdgcn_perm(cur.w, cur.z, pick);
+        x[i] = static_cast<T>(k * SZ < 8u ? lo : hi);
+      }
     }
     T* to = vd + ((static_cast<size_t>(dp) * a.n_kv + h) * HD << a.lp) + (static_cast<size_t>(d) << a.lp) + ((e0 + 16u * q) & mask);
     if (cnt == 16u) {  // uniform
