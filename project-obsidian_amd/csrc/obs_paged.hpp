@@ -177,15 +177,23 @@ __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
 }
 
-// Word masks of eight consecutive bf16 from entry t: those below hi, and at or
-// above lo or below sinks, are kept.
-__device__ __forceinline__ u32x4_v entry_masks(uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok) {
+// The entries of the block of 32 from entry t that are below hi, and at or above
+// lo or below sinks: a bit each. Arithmetic on whole words, no branch an entry.
+__host__ __device__ __forceinline__ uint32_t below_bits(uint32_t t, uint32_t end) {  // entries below `end`
+  const uint32_t n = end > t ? umin(end - t, 32u) : 0u;
+  return n == 32u ? ~0u : (1u << n) - 1u;
+}
+__host__ __device__ __forceinline__ uint32_t seen_bits(uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks) {
+  return below_bits(t, hi) & (~below_bits(t, lo) | below_bits(t, sinks));
+}
+// Word masks of eight bf16 from their bits 0 .. 7.
+__device__ __forceinline__ u32x4_v word_masks(uint32_t bits) {
   u32x4_v m;
 #pragma unroll
   for (uint32_t i = 0; i < 4; ++i) {
-    const uint32_t a = t + 2u * i, b = a + 1u;
-    const bool sa = ok && a < hi && (a >= lo || a < sinks), sb = ok && b < hi && (b >= lo || b < sinks);
-    m[i] = (sa ? 0xffffu : 0u) | (sb ? 0xffff0000u : 0u);
+    const uint32_t a = static_cast<uint32_t>(static_cast<int32_t>(bits << (31u - 2u * i)) >> 31);
+    const uint32_t b = static_cast<uint32_t>(static_cast<int32_t>(bits << (30u - 2u * i)) >> 31);
+    m[i] = (a & 0xffffu) | (b & 0xffff0000u);
   }
   return m;
 }

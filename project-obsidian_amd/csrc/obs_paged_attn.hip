@@ -81,13 +81,13 @@ struct Column {
   }
 };
 
-// One block into the lane's column. hi, lo: the column's own limits; vhi, vlo:
-// the limits of what any column of the wave sees (values outside read as zero:
-// the pool may hold anything there). masked: whether the block needs any of it.
+// One block into the lane's column; t: the lane's first entry; hi, lo: what the
+// token sees (values it does not see read as zero: the pool may hold anything
+// there); ok: whether the lane's page is there; masked: whether the block needs
+// any of it.
 template <uint32_t HD, bool F8>
 __device__ __forceinline__ void block_step(const Block<HD, F8>& blk, const bf16x8_v (&qb)[HD / 32u], Column<HD>& c,
-                                           uint32_t t, uint32_t hi, uint32_t lo, uint32_t vhi, uint32_t vlo,
-                                           uint32_t sinks, bool ok, bool masked, float scale_log2, float (&sv)[8],
+                                           uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok, bool masked, float scale_log2, float (&sv)[8],
                                            uint32_t lane) {
   constexpr uint32_t KS = HD / 32u, NT = HD / 16u;
 #pragma unroll
@@ -98,12 +98,11 @@ __device__ __forceinline__ void block_step(const Block<HD, F8>& blk, const bf16x
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) sv[4 * tt + i] = acc[i] * scale_log2;
   }
-  if (masked) {
+  uint32_t bits = 0u;
+  if (masked) {  // uniform
+    bits = ok ? seen_bits(t, hi, lo, sinks) : 0u;
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      const uint32_t e = t + j;
-      sv[j] = ok && e < hi && (e >= lo || e < sinks) ? sv[j] : NEG_INF;
-    }
+    for (uint32_t j = 0; j < 8; ++j) sv[j] = bits >> j & 1u ? sv[j] : NEG_INF;
   }
   float bm = sv[0];
 #pragma unroll
@@ -123,7 +122,7 @@ __device__ __forceinline__ void block_step(const Block<HD, F8>& blk, const bf16x
   const bf16x8_v pb = __builtin_bit_cast(bf16x8_v, u32x4_v{pack_bf16_pair_rne(p[0], p[1]), pack_bf16_pair_rne(p[2], p[3]),
                                                            pack_bf16_pair_rne(p[4], p[5]), pack_bf16_pair_rne(p[6], p[7])});
   u32x4_v vm = {~0u, ~0u, ~0u, ~0u};
-  if (masked) vm = entry_masks(t, vhi, vlo, sinks, ok);
+  if (masked) vm = word_masks(bits);
 #pragma unroll
   for (uint32_t nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -249,7 +248,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
     blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
     __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
     float sv[8];
-    block_step<HD, F8>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
+    block_step<HD, F8>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
                        !(whole && ok0 && ok1), scale, sv, lane);
     if constexpr (WEIGHT) {
       if (col < p.G) {

@@ -198,6 +198,9 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     const uint8_t* base = a.v + ((static_cast<size_t>(k.iv) * HD << a.lp) + (k.t & pmask)) * SZ;
     if (has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
   };
+  auto page_bits = [](const Blk& k) __attribute__((always_inline)) {
+    return (k.ok0 ? 0xffffu : 0u) | (k.ok1 ? 0xffff0000u : 0u);
+  };
   // 16 stored bytes as bf16: one or two 16-byte words
   auto widen = [](const u32x4_v& w, uint32_t j) __attribute__((always_inline)) {
     if constexpr (F8) {
@@ -223,16 +226,18 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
 #pragma unroll
       for (uint32_t j = 0; j < 2u / SZ; ++j) w[j] = widen(vr, j);
       if (k.edge) {  // uniform
-        const bool ok = vh ? k.ok1 : k.ok0;
-        bool bad = false;
+        const uint32_t bits = seen_bits(k.t, s.hi, s.lo, p.sinks) & page_bits(k);
+        uint32_t bad = 0u;
 #pragma unroll
         for (uint32_t j = 0; j < 2u / SZ; ++j) {
-          w[j] &= entry_masks(k.t + v_ent + 8u * j, s.hi, s.lo, p.sinks, ok);
+          w[j] &= word_masks(bits >> (v_ent + 8u * j));
 #pragma unroll
           for (uint32_t q = 0; q < 4; ++q) {
-            const bool blo = (w[j][q] & 0x7f80u) == 0x7f80u, bhi = (w[j][q] & 0x7f800000u) == 0x7f800000u;
-            bad = bad || blo || bhi;
-            w[j][q] &= (blo ? 0u : 0xffffu) | (bhi ? 0u : 0xffff0000u);
+            // all ones in the exponent: adding one in its last place carries into the sign's
+            const uint32_t e = (w[j][q] & 0x7f807f80u) + 0x00800080u;
+            const uint32_t wild = (e & 0x80008000u) >> 15;  // bit 0, bit 16
+            bad |= wild;
+            w[j][q] &= ~(wild * 0xffffu);
           }
         }
         if (bad) s_bad = 1u;
@@ -278,9 +283,9 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       if (ka.edge) {  // uniform
         auto counts = [&](uint32_t e) { return e < s.hi && (e + 16u > s.lo || e < p.sinks); };
         if (tid == 0u && ((!ka.ok0 && counts(ka.t)) || (!ka.ok1 && counts(ka.t + 16u)))) paged_flag(a.status);
+        const uint32_t bits = (seen_bits(ka.t, hi, lo, p.sinks) & page_bits(ka)) >> (8u * half);
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-          sc[i] = (i < 8u ? ka.ok0 : ka.ok1) && sees(ka.t + 16u * (i / 8u) + 8u * half + i % 8u) ? sc[i] : NEG_INF;
+        for (uint32_t i = 0; i < 16; ++i) sc[i] = bits >> (16u * (i / 8u) + i % 8u) & 1u ? sc[i] : NEG_INF;
       }
       maximum(sc);
       const bool up = mx * scale > m + PF_SLACK;
