@@ -27,7 +27,7 @@ using obs::up256;
 // Measured against it, at 8,192 rows under a window of 4,096 and at a prompt of
 // 5,001: one wave of 64 columns a SIMD 936 and 332 us (a wave issues an
 // instruction every four cycles), two of 32 columns with the next block's scores
-// beside this one's softmax 602 and 245, this one 594 and 223. More loads in
+// beside this one's softmax 602 and 245, this one 577 and 220. More loads in
 // flight, LDS reads earlier, two blocks a barrier, wave priorities and the other
 // machine schedulers gained nothing.
 // The running maximum follows the scores only when they pass it by 2^8 (the sums
@@ -109,8 +109,13 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
   constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
   constexpr uint32_t KN = 32u * KC, VN = HD * VC;       // chunks of a block: 512, 256 or 128, at most one a thread
-  __shared__ __attribute__((aligned(16))) uint16_t s_k[2][32u * KROW];
-  __shared__ __attribute__((aligned(16))) uint16_t s_v[2][HD * VROW];
+  // Keys and values of two blocks; before and after them a slab a wave, through
+  // which queries come in and outputs go out by whole 64-byte runs.
+  constexpr uint32_t SLAB = 32u * 80u;  // 32 columns of 64 bytes (+16: bank spread)
+  constexpr uint32_t K_BYTES = 2u * 32u * KROW * 2u, V_BYTES = 2u * HD * VROW * 2u, SLABS = PF_THREADS / 64u * SLAB;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[K_BYTES + V_BYTES > SLABS ? K_BYTES + V_BYTES : SLABS];
+  uint16_t(*const s_k)[32u * KROW] = reinterpret_cast<uint16_t(*)[32u * KROW]>(s_mem);
+  uint16_t(*const s_v)[HD * VROW] = reinterpret_cast<uint16_t(*)[HD * VROW]>(s_mem + K_BYTES);
   __shared__ uint32_t s_bad;  // an edge block holds values that are not finite
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
   const uint32_t col = lane & 31u, half = lane >> 5;
@@ -134,21 +139,47 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   const float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
   if (tid == 0u) s_bad = 0u;
 
-  // the wave's columns: query slices, limits, state
-  const uint32_t c = 32u * wave + col, t_row = t0r + c / p.G;
-  const bool have = c / p.G < tq && t_row < t1r;
+  // the wave's columns: limits, state
+  const uint32_t per_g = (65536u + p.G - 1u) / p.G;  // c / G as c * per_g >> 16: exact below 384 columns and up to 16 heads
+  auto row_of = [&](uint32_t c) __attribute__((always_inline)) { return c * per_g >> 16; };
+  auto is_col = [&](uint32_t c) __attribute__((always_inline)) { return row_of(c) < tq && t0r + row_of(c) < t1r; };
+  const uint32_t c = 32u * wave + col, t_row = t0r + row_of(c);
+  const bool have = is_col(c);
   const uint32_t hi = have && n + t_row + 1u > r.r1 ? n + t_row + 1u - r.r1 : 0u;
   const uint32_t lo = p.window && hi > p.window ? hi - p.window : 0u;
-  bf16x8_v qb[KS];
-  {
-    const uint16_t* qr = p.q + static_cast<size_t>(have ? t_row : t0r) * p.q_ld + (kv * p.G + c % p.G) * HD + 8u * half;
+  // the columns' queries by whole rows (a lane's own column, 16 bytes of a row at a
+  // time, would fetch every line four times)
+  constexpr uint32_t QC = HD / 8u, QR = 64u / QC;  // 16-byte chunks of a row, rows a load
+  u32x4_v qt[HD / 16u];
 #pragma unroll
-    for (uint32_t ks = 0; ks < KS; ++ks) {
-      u32x4_v v = *reinterpret_cast<const u32x4_v*>(qr + 16u * ks);
-      if (!have) v = u32x4_v{0u, 0u, 0u, 0u};
-      qb[ks] = __builtin_bit_cast(bf16x8_v, v);
-    }
+  for (uint32_t i = 0; i < HD / 16u; ++i) {
+    const uint32_t qc = 32u * wave + QR * i + lane / QC, qr = row_of(qc);
+    const bool ok = is_col(qc);
+    qt[i] = *reinterpret_cast<const u32x4_v*>(p.q + static_cast<size_t>(ok ? t0r + qr : t0r) * p.q_ld +
+                                              (kv * p.G + (ok ? qc - qr * p.G : 0u)) * HD + 8u * (lane % QC));
+    if (!ok) qt[i] = u32x4_v{0u, 0u, 0u, 0u};
   }
+  uint8_t* const slab = s_mem + wave * SLAB;
+  auto wave_sync = [] __attribute__((always_inline))() {  // a wave's LDS traffic is in order; the compiler keeps it so
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  };
+  bf16x8_v qb[KS];
+  auto take_queries = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t k4 = 0; k4 < HD / 32u; ++k4) {  // 32 dims at a time
+      if (lane % QC / 4u == k4) {
+#pragma unroll
+        for (uint32_t i = 0; i < HD / 16u; ++i)
+          *reinterpret_cast<u32x4_v*>(slab + (QR * i + lane / QC) * 80u + 16u * (lane % 4u)) = qt[i];
+      }
+      wave_sync();
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        qb[2u * k4 + j] = *reinterpret_cast<const bf16x8_v*>(slab + col * 80u + 32u * j + 16u * half);
+      wave_sync();
+    }
+  };
   float m = NEG_INF, l = 0.0f;
   f32x16_v o[DT];
 #pragma unroll
@@ -269,7 +300,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     Blk ka = block_of(x0), kb = block_of(x0 + 1u);
     load_k(ka);
     load_v(ka);
-    __syncthreads();  // s_bad is zero
+    take_queries();
+    __syncthreads();  // s_bad is zero, the slabs are free
     store_k(x0 & 1u);
     store_v(x0 & 1u, ka);
     __syncthreads();
@@ -353,33 +385,57 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       }
     }
   }
-  const uint32_t h = kv * p.G + c % p.G;
   const float L = l + lane_xor32_f32(l, lane);
-  if (!have) return;
+  __syncthreads();  // the last block's keys and values were read
+  // column and 16-byte chunk that a lane stores of a slab
+  const uint32_t ocol = lane / 4u, och = lane % 4u;
   if (it.splits == 1u) {
     const float inv = (F8 ? a.v_scale[kv] : 1.0f) / L;
+    uint16_t* to[2];
 #pragma unroll
-    for (uint32_t d = 0; d < DT; ++d)
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint32_t oc = 32u * wave + ocol + 16u * j, orow = row_of(oc);
+      to[j] = is_col(oc) ? p.out + (static_cast<size_t>(t0r + orow) * p.nh + kv * p.G + oc - orow * p.G) * HD + 8u * och : nullptr;
+    }
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d) {
 #pragma unroll
       for (uint32_t i = 0; i < 16; i += 4) {
         float v[4];
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) v[j] = L == 0.0f ? 0.0f : o[d][i + j] * inv;
-        *reinterpret_cast<uint2*>(p.out + (static_cast<size_t>(t_row) * p.nh + h) * HD + 32u * d + 2u * i + 4u * half) =
+        *reinterpret_cast<uint2*>(slab + col * 80u + 4u * i + 8u * half) =
             make_uint2(pack_bf16_pair_rne(v[0], v[1]), pack_bf16_pair_rne(v[2], v[3]));
       }
+      wave_sync();
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j)
+        if (to[j]) *reinterpret_cast<u32x4_v*>(to[j] + 32u * d) = *reinterpret_cast<const u32x4_v*>(slab + (ocol + 16u * j) * 80u + 16u * och);
+      wave_sync();
+    }
   } else {
-    const size_t at = static_cast<size_t>(blockIdx.x) * PF_COLS + c;
-    if (half == 0u) {
-      p.ml[at * 2u] = m;
-      p.ml[at * 2u + 1u] = L;
+    const size_t at = static_cast<size_t>(blockIdx.x) * PF_COLS;
+    if (have && half == 0u) {
+      p.ml[(at + c) * 2u] = m;
+      p.ml[(at + c) * 2u + 1u] = L;
     }
 #pragma unroll
-    for (uint32_t d = 0; d < DT; ++d)
+    for (uint32_t d = 0; d < 2u * DT; ++d) {  // 16 dims in fp32
 #pragma unroll
-      for (uint32_t i = 0; i < 16; i += 4)
-        *reinterpret_cast<float4*>(p.part + at * HD + 32u * d + 2u * i + 4u * half) =
-            make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+      for (uint32_t i = 0; i < 8; i += 4) {
+        const uint32_t e = 8u * (d & 1u) + i;
+        *reinterpret_cast<f32x4_v*>(slab + col * 80u + 8u * i + 16u * half) =
+            f32x4_v{o[d / 2u][e], o[d / 2u][e + 1], o[d / 2u][e + 2], o[d / 2u][e + 3]};
+      }
+      wave_sync();
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        const uint32_t oc = 32u * wave + ocol + 16u * j;
+        if (is_col(oc))
+          *reinterpret_cast<u32x4_v*>(p.part + (at + oc) * HD + 16u * d + 4u * och) = *reinterpret_cast<const u32x4_v*>(slab + (ocol + 16u * j) * 80u + 16u * och);
+      }
+      wave_sync();
+    }
   }
 }
 
