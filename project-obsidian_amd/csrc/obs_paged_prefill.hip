@@ -35,7 +35,7 @@ using obs::up256;
 // rescaled.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
 
-constexpr uint32_t PF_COLS = 384, PF_THREADS = 2u * PF_COLS, PF_TARGET = 256, PF_MIN_CHUNK = 4;
+constexpr uint32_t PF_COLS = 384, PF_THREADS = 2u * PF_COLS, PF_TARGET = 256, PF_MIN_CHUNK = 4, PF_WHOLE = 12;
 constexpr float PF_SLACK = 8.0f;
 
 // Tiles and blocks of the sequences, as the parts are planned by.
@@ -491,7 +491,10 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedA
 }
 
 // Prefill: with few rows for the chip (tiles of both kinds of sequence ends
-// counted by the rows alone) a tile's blocks are cut into parts.
+// counted by the rows alone) a tile's blocks are cut into parts, unless the table
+// and the window leave a tile at most twelve: up to there the join's launch costs
+// more than the parts save (one prompt of 256 19.5 us whole, 23.0 in parts; 384
+// 24.2 and 27.5, four of 300 21.2 and 29.2; a row over 400 entries 21.5 and 18.9).
 struct PrefillPlan {
   uint64_t items, tiles;  // workgroups and tiles (of all kv heads) at most
   bool split;
@@ -504,7 +507,8 @@ PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32
   const uint64_t full = static_cast<uint64_t>(kv->n_kv) * ((s->n_rows + tq - 1u) / tq);
   // tiles: at most one that is not full a sequence, and none of a sequence without rows
   d.tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
-  d.split = 2u * full <= PF_TARGET + 128u && most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks) > PF_MIN_CHUNK;
+  const uint64_t blocks = most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks);
+  d.split = 2u * full <= PF_TARGET + 128u && blocks > PF_WHOLE;
   d.items = d.split ? PF_TARGET + d.tiles + 64u : d.tiles;  // parts of 1 / target of all blocks at least, and one a tile
   if (d.split) {
     d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
