@@ -69,8 +69,8 @@ struct PagedAttn {
   float* ml;      // of each part and column: maximum and sum
   float* part;    // of each part and column: its unnormalised output
   float* scores;  // [sequence][head][vis]: scores in base 2, where the weights are gathered
-  uint2* plan;    // of each sequence: its first part and its parts a kv head
-  uint32_t nh, G, window, sinks, q_ld, vis, min_chunk, target;
+  uint2* plan;    // decode: of each sequence its first part and its parts a kv head; prefill: of each tile (uint4)
+  uint32_t nh, G, window, sinks, q_ld, vis, min_chunk, target, tiles;
   float scale_log2;
 };
 // Blocks of 32 that a token can see of a sequence of `entries`.

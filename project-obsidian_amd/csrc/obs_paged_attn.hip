@@ -543,7 +543,7 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
   uint8_t* wb = static_cast<uint8_t*>(ws);
   const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml),
                    reinterpret_cast<float*>(wb + d.ml + d.part), reinterpret_cast<uint2*>(wb + d.ml + d.part + d.scores), n_heads, n_heads / kv->n_kv, window, sinks, q_ld,
-                   static_cast<uint32_t>(d.vis), DECODE_MIN_CHUNK, decode_target(kv, seqs),
+                   static_cast<uint32_t>(d.vis), DECODE_MIN_CHUNK, decode_target(kv, seqs), 0u,
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const Weight w = obs::weight_args(weight);
   const bool f8 = kv->dtype == OBS_KV_E4M3;

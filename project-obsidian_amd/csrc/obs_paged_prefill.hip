@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   const uint32_t lo_last = p.window && s.hi > p.window ? s.hi - p.window : 0u;
   const uint32_t q0 = s.nblk / it.splits, q1 = s.nblk % it.splits;  // parts of q0 or q0 + 1 blocks
   const uint32_t x0 = it.split * q0 + umin(it.split, q1), x1 = x0 + q0 + (it.split < q1 ? 1u : 0u);
-  if (p.target && it.split == 0u && tid == 0u)  // for the join
+  // for the join (row arrays that decrease make more tiles than rows allow: those are dropped)
+  if (p.target && it.split == 0u && tid == 0u && it.place * a.n_kv + kv < p.tiles)
     reinterpret_cast<uint4*>(p.plan)[static_cast<size_t>(it.place) * a.n_kv + kv] = make_uint4(it.first, it.splits, t0r, t1r);
   const float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
   if (tid == 0u) s_bad = 0u;
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   for (uint32_t i = 0; i < HD / 16u; ++i) {
     const uint32_t qc = 32u * wave + QR * i + lane / QC, qr = row_of(qc);
     const bool ok = is_col(qc);
-    qt[i] = *reinterpret_cast<const u32x4_v*>(p.q + static_cast<size_t>(ok ? t0r + qr : t0r) * p.q_ld +
+    qt[i] = *reinterpret_cast<const u32x4_v*>(p.q + static_cast<size_t>(ok ? t0r + qr : 0u) * p.q_ld +
                                               (kv * p.G + (ok ? qc - qr * p.G : 0u)) * HD + 8u * (lane % QC));
     if (!ok) qt[i] = u32x4_v{0u, 0u, 0u, 0u};
   }
@@ -451,8 +452,10 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedA
     tiles += wave_sum_u32(base + lane < a.n_seqs ? prefill_seq(a, p, base + lane).tiles : 0u);
   if (place >= tiles) return;  // uniform
   const uint4 plan = reinterpret_cast<const uint4*>(p.plan)[static_cast<size_t>(place) * a.n_kv + kv];
-  const uint32_t splits = uniform(plan.y), first = uniform(plan.x), t = plan.z + c / p.G, h = kv * p.G + c % p.G;
-  if (splits == 1u || c / p.G >= PF_COLS / p.G || t >= plan.w) return;
+  // (the bounds by items and rows: whatever the row array, nothing outside the buffers is met)
+  const uint32_t splits = umin(uniform(plan.y), items), first = umin(uniform(plan.x), items);
+  const uint32_t t = plan.z + c / p.G, h = kv * p.G + c % p.G;
+  if (splits == 1u || c / p.G >= PF_COLS / p.G || t >= plan.w || t >= a.n_rows) return;
   float M = NEG_INF, L = 0.0f;
   f32x4_v o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (uint32_t i0 = 0; i0 < splits; i0 += 8u) {
@@ -460,7 +463,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedA
     f32x4_v x[8];
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      // behind the last part it again, without weight (and within the launch's parts whatever the rows)
+      // behind the last part it again, without weight
       const size_t part = umin((first + umin(i0 + i, splits - 1u)) * a.n_kv + kv, items - 1u);
       ml[i] = *reinterpret_cast<const float2*>(p.ml + (part * PF_COLS + c) * 2u);
       x[i] = *reinterpret_cast<const f32x4_v*>(p.part + (part * PF_COLS + c) * HD + d);
@@ -557,7 +560,7 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
   const Paged a = obs::paged_args(ctx, kv, seqs);
   uint8_t* wb = static_cast<uint8_t*>(ws);
   const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr, reinterpret_cast<uint2*>(wb + d.ml + d.part), n_heads,
-                   n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u,
+                   n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u, static_cast<uint32_t>(d.tiles),
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const bool f8 = kv->dtype == OBS_KV_E4M3;
   if (kv->head_dim == 128u) return f8 ? launch_prefill<128, true>(ctx, a, p, d) : launch_prefill<128, false>(ctx, a, p, d);

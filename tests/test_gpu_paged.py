@@ -378,6 +378,27 @@ def test_prefill_rows_do_not_meet_hidden_nan(exe, shape, window, sinks):
                 assert np.all(np.abs(g - ref) <= bound), (what, b, r)
 
 
+@pytest.mark.parametrize("long", [False, True])
+@pytest.mark.parametrize("rows", [[0, 90, 0, 90, 0, 90], [90, 0, 90, 0, 90, 0], [-5, 40, 30, 1000, 7, 2**31 - 1],
+                                  [50, 40, 30, 20, 10, -2**31]], ids=str)
+def test_prefill_rows_out_of_order_stay_in_the_buffers(exe, rows, long):
+    """Row arrays that decrease or leave [0, n_rows] are not a batch: what the rows get is open, but
+    the call ends, and nothing beside the output and the workspace changes (in parts and whole)."""
+    nh, nkv, hd, page = 32, 4, 128, 16
+    rng = np.random.default_rng(57)
+    n = 900 if long else 300
+    pool = Pool(exe, rng, [n, n - 7, 20, n, 100], nkv, hd, page, False)
+    R, guard = 90, 4096
+    seqs = pool.seqs(rows, R)
+    need = exe.sdpa_paged_workspace(pool.kv, seqs, nh)
+    ws = exe.upload(np.full(need + guard, 0xFF, np.uint8))
+    q = exe.upload(synth.bf16_normal(rng, (R, nh, hd), 2.0))
+    out = exe.upload(np.full((R + 2, nh, hd), FILL16, np.uint16))
+    exe.sdpa_paged_prefill(pool.kv, seqs, q, out, nh, ws, ws_bytes=need)
+    exe.device_status()
+    assert np.all(out.download()[R:] == FILL16) and np.all(ws.download()[need:] == 0xFF)
+
+
 # ---- append -------------------------------------------------------------------
 
 def _prep_case(exe, shape, lens, new, seed, pos=None, rope_len=9000, pad_rows=0, weight=True, one=False):
