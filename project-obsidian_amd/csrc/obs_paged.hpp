@@ -34,6 +34,7 @@ struct DeviceGuard {
 // Shapes and pointers of kv and seqs; `pointers` false: sizes only.
 int check_paged(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs_paged_seqs* seqs, bool pointers);
 int check_heads(obs_ctx* ctx, const char* who, uint32_t n_heads, uint32_t n_kv);
+int check_grid(obs_ctx* ctx, const char* who, uint64_t workgroups, uint32_t threads);  // a launch holds less than 2^32 threads
 int check_weight(obs_ctx* ctx, const char* who, const obs_kv_weight* w, uint64_t entries, bool pointers);
 
 // The pool and the sequences as kernels take them.

@@ -535,9 +535,9 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
   rc = obs::check_attn(ctx, who, kv, seqs, weight, q, out, n_heads, &q_ld, ws, ws_bytes, d.all());
   if (rc != OBS_OK) return rc;
   if (seqs->n_seqs == 0) return OBS_OK;
-  const uint64_t grid = static_cast<uint64_t>(seqs->n_seqs) * (4ull * n_heads + kv->n_kv * ((d.vis + 1023u) / 1024u));
-  if (d.items > 0x7fffffffull || grid > 0x7fffffffull)
-    return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many sequences and heads", who);
+  const uint64_t wchunks = weight ? (d.vis + 1023u) / 1024u : 0u;
+  rc = obs::check_grid(ctx, who, std::max(d.items, seqs->n_seqs * (static_cast<uint64_t>(n_heads) * 4u + kv->n_kv * wchunks)), 256u);
+  if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   const Paged a = obs::paged_args(ctx, kv, seqs);
   uint8_t* wb = static_cast<uint8_t*>(ws);

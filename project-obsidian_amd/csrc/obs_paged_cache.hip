@@ -570,6 +570,13 @@ int check_heads(obs_ctx* ctx, const char* who, uint32_t n_heads, uint32_t n_kv) 
   return OBS_OK;
 }
 
+int check_grid(obs_ctx* ctx, const char* who, uint64_t workgroups, uint32_t threads) {
+  if (workgroups > 0xffffffffull / threads)
+    return set_error(ctx, OBS_E_SHAPE, "%s: too much for one call (%llu workgroups of %u)", who,
+                     static_cast<unsigned long long>(workgroups), threads);
+  return OBS_OK;
+}
+
 int check_weight(obs_ctx* ctx, const char* who, const obs_kv_weight* w, uint64_t entries, bool pointers) {
   if (pointers && !w->w) return set_error(ctx, OBS_E_INVALID, "%s: null weight", who);
   if (pointers && !aligned(w->w, 4)) return set_error(ctx, OBS_E_ALIGN, "%s: weight must be 4-byte aligned", who);
@@ -610,14 +617,16 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
   if (rope_len == 0 || rope_len > (1u << 24))
     return obs::set_error(ctx, OBS_E_SHAPE, "%s: rope_len must be in [1, 2^24] (got %u)", who, rope_len);
   if (seqs->n_rows == 0 || seqs->n_seqs == 0) return OBS_OK;
+  const uint32_t n_vt = seqs->row ? kv->n_kv * ((seqs->n_rows + PREP_TILE - 1u) / PREP_TILE) : 0u;
+  const uint32_t grid = n_vt + seqs->n_rows;
+  rc = obs::check_grid(ctx, who, grid, 256u);
+  if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   PrepArgs p{q, k, v, q_norm, k_norm, q_out, pos, nullptr, n_heads, rope_len, q_ld, kv_ld, q_out_ld, eps};
   rc = obs::ensure_rope_table(ctx, theta, rope_len, &p.rope);
   if (rc != OBS_OK) return rc;
   const Paged a = obs::paged_args(ctx, kv, seqs);
   const Weight w = obs::weight_args(weight);
-  const uint32_t n_vt = seqs->row ? kv->n_kv * ((seqs->n_rows + PREP_TILE - 1u) / PREP_TILE) : 0u;
-  const uint32_t grid = n_vt + seqs->n_rows;
   const bool f8 = kv->dtype == OBS_KV_E4M3;
   if (hd == 128u && !f8)
     OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, false><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
@@ -650,7 +659,9 @@ int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seq
                           who, sinks, recent, budget, dst_max_pages);
   if (seqs->n_seqs == 0) return OBS_OK;
   const uint64_t copies = static_cast<uint64_t>(seqs->n_seqs) * kv->n_kv * ((budget + 63u) / 64u);
-  if (copies > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many entries to copy", who);
+  rc = obs::check_grid(ctx, who, copies, 256u);
+  if (rc == OBS_OK) rc = obs::check_grid(ctx, who, static_cast<uint64_t>(seqs->n_seqs) * kv->n_kv, EV_THREADS);
+  if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   const Paged a = obs::paged_args(ctx, kv, seqs);
   OBS_LAUNCH(ctx, "kv_evict_select", evict_select_kernel<<<seqs->n_seqs * kv->n_kv, EV_THREADS, 0, ctx->stream>>>(

@@ -555,7 +555,9 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
   rc = obs::check_attn(ctx, who, kv, seqs, nullptr, q, out, n_heads, &q_ld, ws, ws_bytes, d.all());
   if (rc != OBS_OK) return rc;
   if (seqs->n_seqs == 0 || seqs->n_rows == 0) return OBS_OK;
-  if (d.items * 32u > 0x7fffffffull) return obs::set_error(ctx, OBS_E_SHAPE, "%s: too many rows and heads", who);
+  rc = obs::check_grid(ctx, who, d.items, PF_THREADS);
+  if (rc == OBS_OK && d.split) rc = obs::check_grid(ctx, who, d.tiles * (PF_COLS * kv->head_dim / 1024u), 256u);
+  if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   const Paged a = obs::paged_args(ctx, kv, seqs);
   uint8_t* wb = static_cast<uint8_t*>(ws);
