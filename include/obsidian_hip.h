@@ -544,7 +544,7 @@ int obs_sdpa_paged_workspace(obs_ctx* ctx, const obs_paged_kv* kv, const obs_pag
  * attention, scale 1/sqrt(head_dim), of entries j < len[b] with window == 0, or
  * j > len[b] - 1 - window (the last `window` ones), or j < sinks (the first
  * ones). What lies in hidden entries has no effect, NaN included. Nothing
- * visible, or no finite score: zeros. q bf16 rows of q_ld elements (a multiple
+ * visible, or no score above -infinity: zeros. q bf16 rows of q_ld elements (a multiple
  * of 8; 0 = dense); out bf16 [n_seqs, n_heads, head_dim]; q, out and ws 16-byte
  * aligned; row NULL. weight (nullable): every visible entry's softmax weights,
  * summed over the kv head's query heads, are added to w[slot][kv head][j].
@@ -576,7 +576,8 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
  * their old indices (-1 behind the last), dst_weight their weights; weights
  * and entries behind the last one are left alone. seqs->row is not read. The
  * destination pages and weight rows must not be among the call's source pages
- * and rows (a shared prefix stays whole for its other users). A source page id
+ * and rows (a shared prefix stays whole for its other users), and new_len must
+ * not be len. A source page id
  * that is out of range copies zeros, a destination one nothing; both are
  * reported by obs_device_status. */
 int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,

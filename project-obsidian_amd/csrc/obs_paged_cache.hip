@@ -659,6 +659,9 @@ int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seq
                           who, sinks, recent, budget, dst_max_pages);
   if (seqs->n_seqs == 0) return OBS_OK;
   const uint64_t copies = static_cast<uint64_t>(seqs->n_seqs) * kv->n_kv * ((budget + 63u) / 64u);
+  // arrays that the call's workgroups read while others write them
+  if (new_len == seqs->len || dst_pages == seqs->pages || (weight->w == dst_weight->w && weight->slot == dst_weight->slot))
+    return obs::set_error(ctx, OBS_E_INVALID, "%s: new_len, the destination's pages and its weight rows must not be the source's", who);
   rc = obs::check_grid(ctx, who, copies, 256u);
   if (rc == OBS_OK) rc = obs::check_grid(ctx, who, static_cast<uint64_t>(seqs->n_seqs) * kv->n_kv, EV_THREADS);
   if (rc != OBS_OK) return rc;

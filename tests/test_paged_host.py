@@ -179,6 +179,13 @@ def test_evict_refusals(ctx, kw, code):
     assert _evict(ctx, _kv(), _seqs(), **kw) == code
 
 
+def test_evict_refuses_arrays_it_reads_and_writes(ctx):
+    B = A + 4096
+    own = dict(dst=B, new_len=B, dw=_weight(w=B, ld=32))
+    for kw in (dict(dst=A), dict(new_len=A), dict(dw=_weight(ld=32))):
+        assert _evict(ctx, _kv(), _seqs(), **{**own, **kw}) == INV
+
+
 def test_more_than_a_launch_holds(ctx):
     """2^32 threads and more are refused before any device work."""
     rows = dict(n_seqs=4096, n_rows=1 << 24)
@@ -187,8 +194,10 @@ def test_more_than_a_launch_holds(ctx):
     assert _decode(ctx, _kv(n_kv=1024), _seqs(n_seqs=4096, n_rows=4096), nh=16 * 1024) == SHAPE
     wide = _seqs(n_seqs=512, n_rows=512, max_pages=1 << 26)
     assert _decode(ctx, _kv(), wide, _weight(n_slots=512, ld=1 << 30), nh=32, n=1 << 60) == SHAPE
-    assert _evict(ctx, _kv(n_kv=1024), _seqs(n_seqs=4096, n_rows=4096)) == SHAPE
-    assert _evict(ctx, _kv(), wide, _weight(n_slots=512, ld=1 << 30), dmax=1 << 26, dw=_weight(ld=1 << 30), budget=1 << 30) == SHAPE
+    B = A + 4096
+    assert _evict(ctx, _kv(n_kv=1024), _seqs(n_seqs=4096, n_rows=4096), dst=B, new_len=B, dw=_weight(w=B, ld=32)) == SHAPE
+    assert _evict(ctx, _kv(), wide, _weight(n_slots=512, ld=1 << 30), dst=B, new_len=B, dmax=1 << 26,
+                  dw=_weight(w=B, ld=1 << 30), budget=1 << 30) == SHAPE
 
 
 def test_nothing_to_do(ctx):
