@@ -434,6 +434,12 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, W
 // Host side
 // ---------------------------------------------------------------------------
 constexpr uint32_t DECODE_MIN_CHUNK = 4;
+// Blocks up to which a sequence is one part where no weight is gathered (no join
+// then): parts and their join cost more up to 384 entries (one sequence of 256
+// 8.9 us in parts, 6.8 whole; of 384 8.9 and 8.2, of 512 8.9 and 9.4), more rows
+// fill the chip by themselves (48 of 512 12.8 and 11.7; 64 of 1,000 22.3 and
+// 19.7, of 2,000 32.3 and 34.6; 32 of 1,000 12.8 and 18.4).
+uint32_t decode_whole(uint64_t rows) { return rows >= 256u ? 32u : rows >= 96u ? 16u : 12u; }
 // Parts of a call: three workgroups a CU are resident (768). Few rows give
 // nearly equal parts, which fill the chip once (one sequence of 100,003 entries
 // 48.2 us against 55.2 with 1,152); the parts of many sequences differ, and
@@ -443,6 +449,7 @@ uint32_t decode_target(const obs_paged_kv* kv, const obs_paged_seqs* s) { return
 struct DecodePlan {
   uint64_t items, vis, blocks;
   size_t ml, part, scores, plan;  // bytes
+  uint32_t min_chunk;
   size_t all() const { return ml + part + scores + plan; }
 };
 using obs::most_blocks;
@@ -454,8 +461,10 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
   d.blocks = most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window, sinks);
   d.vis = 32u * d.blocks;
   const uint64_t rows = static_cast<uint64_t>(s->n_seqs) * kv->n_kv;
+  const uint32_t whole = weight ? 0u : decode_whole(rows);
+  d.min_chunk = std::max(DECODE_MIN_CHUNK, d.blocks <= whole ? whole : 0u);
   // sum of the rows' rounded shares: at most target + rows (and what fp32 rounds), and at most each row's own most
-  d.items = std::min<uint64_t>(decode_target(kv, s) + rows + 64u, rows * ((d.blocks + DECODE_MIN_CHUNK - 1u) / DECODE_MIN_CHUNK));
+  d.items = std::min<uint64_t>(decode_target(kv, s) + rows + 64u, rows * ((d.blocks + d.min_chunk - 1u) / d.min_chunk));
   d.ml = up256(d.items * 32u * sizeof(float));
   d.part = up256(d.items * (n_heads / kv->n_kv) * kv->head_dim * sizeof(float));
   d.scores = weight ? up256(static_cast<size_t>(s->n_seqs) * n_heads * d.vis * sizeof(float)) : 0u;
@@ -467,7 +476,7 @@ template <uint32_t HD, bool F8, bool WEIGHT>
 int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight& w, const DecodePlan& d) {
   OBS_LAUNCH(ctx, "paged_decode",
              paged_decode_kernel<HD, F8, WEIGHT><<<static_cast<uint32_t>(d.items), 256, 0, ctx->stream>>>(a, p));
-  if (!WEIGHT && d.blocks <= DECODE_MIN_CHUNK) return OBS_OK;  // every sequence is one part
+  if (!WEIGHT && d.blocks <= d.min_chunk) return OBS_OK;  // every sequence is one part
   const uint32_t wchunks = WEIGHT ? static_cast<uint32_t>((d.vis + 1023u) / 1024u) : 0u, rows = a.n_seqs * p.nh;
   const uint32_t weights = rows / p.G * wchunks;
   // few rows have many parts each: four workgroups a row (one of 32 heads and 288
@@ -543,7 +552,7 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
   uint8_t* wb = static_cast<uint8_t*>(ws);
   const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml),
                    reinterpret_cast<float*>(wb + d.ml + d.part), reinterpret_cast<uint2*>(wb + d.ml + d.part + d.scores), n_heads, n_heads / kv->n_kv, window, sinks, q_ld,
-                   static_cast<uint32_t>(d.vis), DECODE_MIN_CHUNK, decode_target(kv, seqs), 0u,
+                   static_cast<uint32_t>(d.vis), d.min_chunk, decode_target(kv, seqs), 0u,
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const Weight w = obs::weight_args(weight);
   const bool f8 = kv->dtype == OBS_KV_E4M3;

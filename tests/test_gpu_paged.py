@@ -205,6 +205,15 @@ def test_decode_split(exe, shape, lens, weight):
     assert np.array_equal(first, out.download())  # the same call, the same bits
 
 
+@pytest.mark.parametrize("weight", [False, True])
+@pytest.mark.parametrize("shape", [(32, 4, 128, 32, False), (32, 4, 128, 64, True), (32, 8, 64, 16, False)], ids=str)
+@pytest.mark.parametrize("lens", [[1700, 3, 900, 0, 64, 33, 1300, 100, 5], [40, 512, 1, 300] * 8, [1000, 7, 250, 500] * 16],
+                         ids=["joined", "16 blocks", "32 blocks"])
+def test_decode_many_rows(exe, shape, lens, weight):
+    """Enough rows for one join workgroup each, and batches whose sequences are one part each."""
+    _decode_case(exe, shape, lens, 0, 0, weight, 20)
+
+
 def test_decode_peaked_scores_and_strides(exe):
     """Scores of several hundred (one entry takes all), a q row stride of its own."""
     _decode_case(exe, (32, 4, 128, 32, False), [777, 64], 0, 0, True, 13, k_std=30.0, q_ld=32 * 128 + 64)
