@@ -253,10 +253,10 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 constexpr uint32_t EV_THREADS = 1024, EV_WAVES = EV_THREADS / 64u, EV_KEYS = 16, EV_BINS = 2048;
 
-// Exclusive scan over the workgroup, in thread order; s_w: EV_WAVES words.
+// Exclusive scan over the workgroup, in thread order; s_w: EV_WAVES words, other
+// ones than the scan before (whose readers the barrier here does not hold back).
 __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_w, uint32_t lane, uint32_t wave, uint32_t& total) {
   const uint32_t incl = wave_scan_u32(v);
-  __syncthreads();  // what s_w held before was read
   if (lane == 63u) s_w[wave] = incl;
   __syncthreads();
   const uint32_t w = lane < EV_WAVES ? s_w[lane] : 0u, ws = wave_scan_u32(w);
@@ -271,15 +271,24 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_w, uint32
 // bits find the K-th largest key of the entries between the first and the last
 // ones: counts by digit in LDS, then a scan from the top. Attention weights
 // spread over many powers of two, so the top digit (sign, exponent, two mantissa
-// bits) has few lanes at one counter. The kept entries' places are two scans
-// over the threads (ties, then all).
+// bits) has few lanes at one counter. One more scan, of the sure entries and the
+// ties together, gives the kept ones' places; they are listed in LDS, so that the
+// stores are whole lines (from each thread by itself they took a third of the
+// kernel). The third step falls away where the second one's bin is kept whole.
+// Bound by latency and one CU's issue rate: 9.1 us for 8,192 entries (2.0 until
+// the weights are there, 3.5 for two steps, 2.1 for the places and stores),
+// 15.5 for 96 rows of up to 16,003.
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weight w, Weight wd, uint32_t sinks,
                                                                  uint32_t recent, uint32_t budget,
                                                                  int32_t* __restrict__ kept,
                                                                  int32_t* __restrict__ new_len) {
-  __shared__ uint32_t s_hist[3][EV_BINS];  // one a step, cleared together
-  __shared__ uint32_t s_w[EV_WAVES];
-  __shared__ uint32_t s_pick[2];
+  constexpr uint32_t SEG = EV_KEYS * EV_THREADS;
+  __shared__ __attribute__((aligned(16))) uint32_t s_mem[SEG / 2u];
+  uint32_t(*const s_hist)[EV_BINS] = reinterpret_cast<uint32_t(*)[EV_BINS]>(s_mem);  // one a step, cleared together
+  uint16_t* const s_list = reinterpret_cast<uint16_t*>(s_mem);                       // afterwards: a segment's kept entries
+  static_assert(SEG / 2u >= 3u * EV_BINS && SEG <= 65536u, "the counters, and places in 16 bits");
+  __shared__ uint32_t s_w[2][EV_WAVES];
+  __shared__ uint32_t s_pick[3];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
   const uint32_t b = blockIdx.x / a.n_kv, h = blockIdx.x % a.n_kv;
   const uint32_t n = uniform(paged_len(a, b)), now = umin(n, budget);
@@ -295,12 +304,17 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
   // entries a thread holds of a segment: a multiple of 4, so its loads can be 16 bytes
   const uint32_t per = umin(EV_KEYS, ((n + EV_THREADS - 1u) / EV_THREADS + 3u) & ~3u), seg = per * EV_THREADS;
   const bool vec = (reinterpret_cast<uintptr_t>(src) & 15u) == 0u;
-  float wt[EV_KEYS];
+  const uint32_t lo = n > budget ? sinks : n, hi = n > budget ? n - recent : n;  // the candidates [lo, hi)
+  auto range_bits = [&](uint32_t j0, uint32_t from, uint32_t end) {  // of the `per` entries from j0, those in [from, end)
+    return below_bits(j0, end) & ~below_bits(j0, from) & ((1u << per) - 1u);
+  };
+  uint32_t key[EV_KEYS], mid = 0u;  // mid: bits of the thread's candidates
   uint32_t held = 0xffffffffu;
   auto load = [&](uint32_t s0) __attribute__((always_inline)) {  // the segment from entry s0
     if (held == s0) return;  // uniform
     held = s0;
     const uint32_t j0 = s0 + per * tid;
+    float wt[EV_KEYS];
 #pragma unroll
     for (uint32_t i = 0; i < EV_KEYS; i += 4u) {
       if (i >= per) break;  // uniform
@@ -317,76 +331,88 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
         for (uint32_t j = 0; j < 4; ++j) wt[i + j] = j0 + i + j < n ? src[j0 + i + j] : 0.0f;
       }
     }
+#pragma unroll
+    for (uint32_t i = 0; i < EV_KEYS; ++i) {
+      if (i >= per) break;  // uniform
+      key[i] = weight_key(wt[i]);
+    }
+    mid = range_bits(j0, lo, hi);
   };
-  const uint32_t lo = n > budget ? sinks : n, hi = n > budget ? n - recent : n;  // the candidates [lo, hi)
-  uint32_t want = n > budget ? budget - sinks - recent : 0u;                     // < hi - lo
+  uint32_t want = n > budget ? budget - sinks - recent : 0u;  // < hi - lo
   uint32_t thr = 0xffffffffu, ties = 0u;  // kept: key > thr, and the first `ties` with key == thr
   if (want > 0u) {  // uniform
     uint32_t prefix = 0u;
-    for (uint32_t i = tid; i < 3u * EV_BINS; i += EV_THREADS) (&s_hist[0][0])[i] = 0u;
+    bool exact = false;  // all entries of the last digit's bin are kept (usual after two steps)
+    load(0u);
+    for (uint32_t i = tid; i < 3u * EV_BINS; i += EV_THREADS) s_mem[i] = 0u;
     __syncthreads();
 #pragma unroll
     for (uint32_t step = 0; step < 3; ++step) {
+      if (exact) break;  // uniform
       const uint32_t shift = step == 0u ? 21u : step == 1u ? 10u : 0u, bits = step == 2u ? 10u : 11u;
       for (uint32_t s0 = 0; s0 < n; s0 += seg) {
         load(s0);
 #pragma unroll
         for (uint32_t i = 0; i < EV_KEYS; ++i) {
           if (i >= per) break;  // uniform
-          const uint32_t j = s0 + per * tid + i, key = weight_key(wt[i]);
-          if (j >= lo && j < hi && (step == 0u || (key >> (shift + bits)) == (prefix >> (shift + bits))))
-            atomicAdd(&s_hist[step][(key >> shift) & ((1u << bits) - 1u)], 1u);
+          if ((mid >> i & 1u) && (step == 0u || ((key[i] ^ prefix) >> (shift + bits)) == 0u))
+            atomicAdd(&s_hist[step][(key[i] >> shift) & ((1u << bits) - 1u)], 1u);
         }
       }
       __syncthreads();
       // thread t looks at bins top - 2 t and top - 2 t - 1: the one where the count from the top reaches `want`
       const uint32_t top = EV_BINS - 1u - 2u * tid, c1 = s_hist[step][top], c0 = s_hist[step][top - 1u];
       uint32_t total;
-      const uint32_t above = group_scan(c0 + c1, s_w, lane, wave, total);
+      const uint32_t above = group_scan(c0 + c1, s_w[step & 1u], lane, wave, total);
       if (above < want && above + c0 + c1 >= want) {  // one thread
         const bool first = above + c1 >= want;
         s_pick[0] = first ? top : top - 1u;
         s_pick[1] = want - above - (first ? 0u : c1);
+        s_pick[2] = first ? c1 : c0;
       }
       __syncthreads();
       prefix |= s_pick[0] << shift;
       want = s_pick[1];  // (written again only behind the next step's barriers)
+      exact = s_pick[2] == want && prefix > 0u;
     }
-    thr = prefix;
-    ties = want;
+    thr = exact ? prefix - 1u : prefix;
+    ties = exact ? 0u : want;
   }
-  uint32_t at = 0u, tie_at = 0u;
-  for (uint32_t s0 = 0; s0 < n; s0 += seg) {
+  uint32_t sure_at = 0u, tie_at = 0u;  // of the segments before
+  for (uint32_t s0 = 0, par = 1u; s0 < n; s0 += seg, par ^= 1u) {
     load(s0);
     const uint32_t j0 = s0 + per * tid;
-    uint32_t tie = 0u, keep = 0u;  // bits of the thread's entries
+    uint32_t tie = 0u, above = 0u;  // bits of the thread's entries
 #pragma unroll
     for (uint32_t i = 0; i < EV_KEYS; ++i) {
       if (i >= per) break;  // uniform
-      const uint32_t j = j0 + i, key = weight_key(wt[i]);
-      const bool mid = j >= lo && j < hi;
-      tie |= mid && key == thr && ties > 0u ? 1u << i : 0u;
-      keep |= j < n && (!mid || key > thr) ? 1u << i : 0u;
+      tie |= key[i] == thr ? 1u << i : 0u;
+      above |= key[i] > thr ? 1u << i : 0u;
     }
-    uint32_t tsum = 0u, ksum;
-    if (ties > 0u) {  // uniform
-      uint32_t rank = tie_at + group_scan(static_cast<uint32_t>(__popc(tie)), s_w, lane, wave, tsum);
+    tie &= ties ? mid : 0u;
+    uint32_t keep = (range_bits(j0, 0u, n) & ~mid) | (above & mid);
+    uint32_t sums;
+    const uint32_t before = group_scan(static_cast<uint32_t>(__popc(keep)) << 16 | static_cast<uint32_t>(__popc(tie)), s_w[par], lane, wave, sums);
+    uint32_t rank = tie_at + (before & 0xffffu);  // of the thread's first tie
+    const uint32_t ties_before = umin(tie_at, ties);
+    uint32_t x = (before >> 16) + umin(rank, ties) - ties_before;  // place among the segment's kept entries
 #pragma unroll
-      for (uint32_t i = 0; i < EV_KEYS; ++i)
-        if (tie >> i & 1u) keep |= rank++ < ties ? 1u << i : 0u;
+    for (uint32_t i = 0; i < EV_KEYS; ++i) {
+      if (i >= per) break;  // uniform
+      if (tie >> i & 1u) keep |= rank++ < ties ? 1u << i : 0u;
+      if (keep >> i & 1u) s_list[x++] = static_cast<uint16_t>(per * tid + i);
     }
-    uint32_t e = at + group_scan(static_cast<uint32_t>(__popc(keep)), s_w, lane, wave, ksum);
-#pragma unroll
-    for (uint32_t i = 0; i < EV_KEYS; ++i)
-      if (keep >> i & 1u) {
-        if (e < budget) {
-          kp[e] = static_cast<int32_t>(j0 + i);
-          if (dslot >= 0) dst[e] = wt[i];
-        }
-        ++e;
-      }
-    at += ksum;
-    tie_at += tsum;
+    const uint32_t first = sure_at + ties_before;
+    sure_at += sums >> 16;
+    tie_at += sums & 0xffffu;
+    const uint32_t count = sure_at + umin(tie_at, ties) - first;
+    __syncthreads();
+    for (uint32_t i = tid; i < count; i += EV_THREADS) {
+      const uint32_t j = s0 + s_list[i], e = first + i;
+      if (e >= budget) break;
+      kp[e] = static_cast<int32_t>(j);
+      if (dslot >= 0) dst[e] = slot >= 0 ? src[j] : 0.0f;
+    }
   }
 }
 
