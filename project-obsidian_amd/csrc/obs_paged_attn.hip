@@ -442,8 +442,8 @@ constexpr uint32_t DECODE_MIN_CHUNK = 4;
 uint32_t decode_whole(uint64_t rows) { return rows >= 256u ? 32u : rows >= 96u ? 16u : 12u; }
 // Parts of a call: three workgroups a CU are resident (768). Few rows give
 // nearly equal parts, which fill the chip once (one sequence of 100,003 entries
-// 48.2 us against 55.2 with 1,152); the parts of many sequences differ, and
-// finer ones even out (48 sequences of up to 16,000: 69.5 us against 74.0).
+// 46.6 us against 52.8 with 1,152); the parts of many sequences differ, and
+// finer ones even out (48 sequences of up to 16,000: 72.3 us against 74.6).
 uint32_t decode_target(const obs_paged_kv* kv, const obs_paged_seqs* s) { return s->n_seqs * kv->n_kv <= 32u ? 768u : 1152u; }
 
 struct DecodePlan {
@@ -479,8 +479,8 @@ int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight
   if (!WEIGHT && d.blocks <= d.min_chunk) return OBS_OK;  // every sequence is one part
   const uint32_t wchunks = WEIGHT ? static_cast<uint32_t>((d.vis + 1023u) / 1024u) : 0u, rows = a.n_seqs * p.nh;
   const uint32_t weights = rows / p.G * wchunks;
-  // few rows have many parts each: four workgroups a row (one of 32 heads and 288
-  // parts 7.8 -> 4.3 us; 48 sequences of up to 12 parts 4.9 us against 11.5)
+  // few rows have many parts each: four workgroups a row (one sequence of 100,003
+  // entries 46.5 us against 48.2; 48 sequences of up to 16,000 77.7 against 72.3)
   if (rows < 256u)
     OBS_LAUNCH(ctx, "paged_join", paged_join_kernel<HD, F8, WEIGHT, 32><<<rows * (HD / 32u) + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
   else

@@ -58,8 +58,8 @@ __device__ __forceinline__ uint32_t seq_of_row_lane(const Paged& a, uint32_t t, 
 // Values of 64 consecutive token rows of one kv head, transposed through LDS:
 // a lane owns a row, so a store of one dim writes the runs of consecutive
 // entries that the rows are. (From each row's own workgroup, one entry of a
-// cache row at a time, the stores cost more than everything else: 43 against
-// 28 us for 5,475 rows into an e4m3 cache.)
+// cache row at a time, the stores cost more than everything else: 38.8 against
+// 28.3 us for 5,795 rows into an e4m3 cache.)
 constexpr uint32_t PREP_TILE = 64;
 template <uint32_t HD, bool F8>
 __device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs& p, uint32_t vi) {
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
 #pragma unroll
     for (uint32_t i = 0; i < 16; ++i)
       cnt += uniform(static_cast<uint32_t>(s_dst[16u * q + i])) == static_cast<uint32_t>(dp) ? 1u : 0u;
-    if constexpr (GE == 16u) {  // few entries: a load each, the shortest way (6.2 us against 8.0; of many 125 against 103)
+    if constexpr (GE == 16u) {  // few entries: a load each, the shortest way (both kernels 15.4 us against 17.1; of many 137 against 118)
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i) {
         const int32_t sp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_src[16u * q + i])));
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
 template <uint32_t HD, bool F8>
 int launch_copy(obs_ctx* ctx, const Paged& a, const int32_t* dst_pages, uint32_t dst_max_pages, uint32_t budget,
                 const int32_t* kept, uint64_t copies) {
-  // below two workgroups a CU (a few sequences): 16 entries each, one sequence of 2,048 kept entries 8.3 -> 6.0 us
+  // below two workgroups a CU (a few sequences): 16 entries each, one sequence of 2,048 kept entries 15.4 us against 19.9
   if (copies < 512u) {
     const uint32_t grid = a.n_seqs * a.n_kv * ((budget + 15u) / 16u);
     OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<HD, F8, 16><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));

@@ -27,7 +27,7 @@ using obs::up256;
 // Measured against it, at 8,192 rows under a window of 4,096 and at a prompt of
 // 5,001: one wave of 64 columns a SIMD 936 and 332 us (a wave issues an
 // instruction every four cycles), two of 32 columns with the next block's scores
-// beside this one's softmax 602 and 245, this one 577 and 220. More loads in
+// beside this one's softmax 602 and 245, this one 575 and 219. More loads in
 // flight, LDS reads earlier, two blocks a barrier, wave priorities and the other
 // machine schedulers gained nothing.
 // The running maximum follows the scores only when they pass it by 2^8 (the sums
