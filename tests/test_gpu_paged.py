@@ -620,6 +620,24 @@ def test_evict_long(exe):
     _evict_case(exe, (8, 2, 64, 256, True), [50000], 0, 0, 25000, 71, "ties")
 
 
+@pytest.mark.parametrize("weights", ["normal", "ties"])
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16, False), (32, 4, 128, 32, True), (16, 4, 64, 64, False), (16, 4, 64, 16, True)],
+                         ids=str)
+def test_evict_many(exe, shape, weights):
+    """Enough entries for the copy's large groups."""
+    _evict_case(exe, shape, [2500, 1101, 1100, 60, 1900, 2048, 1333, 0], 4, 100, 1100, 83, weights)
+
+
+def test_more_kv_heads_than_threads(exe):
+    """300 kv heads: loops over heads go round more than once."""
+    shape = (300, 300, 64, 16, False)
+    _decode_case(exe, shape, [40, 0, 17], 0, 0, True, 87)
+    _prefill_case(exe, shape, [40, 9], [11, 9], 0, 0, 87)
+    args = _prep_case(exe, shape, [40, 9], [11, 9], 87)
+    _check_prep(*args, [40, 9], [11, 9])
+    _evict_case(exe, shape, [70, 20], 2, 3, 30, 87)
+
+
 def test_evict_reports_bad_pages_and_slots(exe):
     nkv, hd, page, n, budget = 2, 64, 16, 64, 32
     rng = np.random.default_rng(73)

@@ -419,3 +419,44 @@ def test_many_sequences_at_the_limit(exe):
         for r in range(n):
             ref, bound, _, _ = _attend(_f64(pq[rows[b] + r]), k, v, np.arange(n) <= r)
             assert np.all(np.abs(pgot[rows[b] + r] - ref) <= bound)
+
+
+def test_offsets_past_32_bits(exe):
+    """Append, prompt attention and eviction in pages behind 4 GiB of keys and of values: bit for
+    bit what the same calls give in a small pool."""
+    nh, nkv, hd, page, n, R = 32, 8, 128, 256, 1000, 700
+    rng = np.random.default_rng(91)
+    n_pages = 8300  # 4.05 GiB of keys
+    per = nkv * page * hd
+    ld = (nh + 2 * nkv) * hd
+    x = exe.upload(synth.bf16_normal(rng, (R, ld), 2.0))
+    qn, kn = exe.upload(synth.bf16_normal(rng, hd)), exe.upload(synth.bf16_normal(rng, hd))
+    old = [synth.bf16_normal(rng, (8, per)) for _ in range(2)]
+    w = rng.random((1, nkv, 4 * page)).astype(np.float32)
+    results = []
+    for total in (8, n_pages):
+        dk, dv = exe.alloc((total, per), np.uint16), exe.alloc((total, per), np.uint16)
+        at = total - 8  # the last eight pages
+        for d, o in ((dk, old[0]), (dv, old[1])):
+            exe._check(oh.lib().obs_upload(exe.ctx, d.ptr + at * per * 2, o.ctypes.data, o.nbytes))
+        kv = oh.PagedKv(dk, dv, total, page, nkv, hd)
+        ids = exe.upload(np.array([at + 7, at + 2, at + 5, at], np.int32))
+        seqs = oh.PagedSeqs(ids, exe.upload(np.array([n], np.int32)), 1, 4, R, exe.upload(np.array([0, R], np.int32)))
+        q, out = exe.alloc((R, nh, hd), np.uint16), exe.alloc((R, nh, hd), np.uint16)
+        exe.attn_prep_paged(kv, seqs, x.ptr, x.ptr + 2 * nh * hd, x.ptr + 2 * (nh + nkv) * hd, qn, kn, q, nh, 1e-6, 1e7, 2048,
+                            q_ld=ld, kv_ld=ld)
+        ws = exe.alloc(exe.sdpa_paged_workspace(kv, seqs, nh), np.uint8)
+        exe.sdpa_paged_prefill(kv, seqs, q, out, nh, ws)
+        dw, dwd = exe.upload(w), exe.alloc((1, nkv, 400), np.float32)
+        kept, new_len = exe.alloc((1, nkv, 400), np.int32), exe.alloc(1, np.int32)
+        exe.kv_evict(kv, seqs, oh.KvWeight(dw, 1, 4 * page), exe.upload(np.array([at + 6, at + 1], np.int32)), 2,
+                     oh.KvWeight(dwd, 1, 400), 4, 50, 400, kept, new_len)
+        exe.device_status()
+        results.append([out.download(), kept.download(), dwd.download()] +
+                       [exe.download_raw(d.ptr + at * per * 2, (8, per), np.uint16) for d in (dk, dv)])
+        dk.free()
+        dv.free()
+    for a, b in zip(*results):
+        assert np.array_equal(a, b)
+    keys = results[0][3]  # entries 300 on were appended (pages 2, 5 and 0), kept ones copied to pages 6 and 1
+    assert np.array_equal(keys[7], old[0][7]) and not any(np.array_equal(keys[i], old[0][i]) for i in (2, 5, 0, 6, 1))
