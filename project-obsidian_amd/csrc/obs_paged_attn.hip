@@ -157,18 +157,31 @@ struct Found {
 __device__ __forceinline__ uint32_t span_blocks(const PagedAttn& p, uint32_t n) {
   return span_of(n ? n - 1u : 0u, n, p.window, p.sinks).nblk;
 }
+// Parts a block. Where the target's parts would be short, those that the chip
+// holds at once instead (DECODE_ONCE, less what rounding up adds): a second round
+// costs more than it evens out (24 sequences of up to 4,000 26.7 -> 22.4 us, 64
+// of 1,500 26.2 -> 22.8; but 48 of 6,000, 14 blocks a part, 52.0 against 56.4,
+// and 256 of 2,000, 20 blocks, 94.9 against 103.8).
+constexpr uint32_t DECODE_ONCE = 768;
+__device__ __forceinline__ float plan_rate(const Paged& a, const PagedAttn& p, float total) {
+  const float rows = static_cast<float>(a.n_seqs) * static_cast<float>(a.n_kv);
+  const float work = fmaxf(total * static_cast<float>(a.n_kv), 1.0f);
+  float target = static_cast<float>(p.target);
+  if (p.target > DECODE_ONCE && work < (rows < 256.0f ? 9.5f : 16.0f) * target) target = fmaxf(DECODE_ONCE - 0.5f * rows, 128.0f);
+  return target / work;
+}
 __device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane) {
   float rate = 0.0f;
   uint32_t n = 0, nblk = 0;
   if (a.n_seqs <= 64u) {  // uniform
     n = lane < a.n_seqs ? paged_len(a, lane) : 0u;
     nblk = span_blocks(p, n);
-    rate = static_cast<float>(p.target) / fmaxf(static_cast<float>(wave_sum_u32(nblk)) * static_cast<float>(a.n_kv), 1.0f);
+    rate = plan_rate(a, p, static_cast<float>(wave_sum_u32(nblk)));
   } else {
     float total = 0.0f;
     for (uint32_t base = 0; base < a.n_seqs; base += 64u)
       total += static_cast<float>(wave_sum_u32(base + lane < a.n_seqs ? span_blocks(p, paged_len(a, base + lane)) : 0u));
-    rate = static_cast<float>(p.target) / fmaxf(total * static_cast<float>(a.n_kv), 1.0f);
+    rate = plan_rate(a, p, total);
   }
   uint32_t acc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
@@ -438,13 +451,14 @@ constexpr uint32_t DECODE_MIN_CHUNK = 4;
 // then): parts and their join cost more up to 384 entries (one sequence of 256
 // 8.9 us in parts, 6.8 whole; of 384 8.9 and 8.2, of 512 8.9 and 9.4), more rows
 // fill the chip by themselves (48 of 512 12.8 and 11.7; 64 of 1,000 22.3 and
-// 19.7, of 2,000 32.3 and 34.6; 32 of 1,000 12.8 and 18.4).
-uint32_t decode_whole(uint64_t rows) { return rows >= 256u ? 32u : rows >= 96u ? 16u : 12u; }
-// Parts of a call: three workgroups a CU are resident (768). Few rows give
+// 19.7, of 2,000 32.3 and 34.6; 32 of 1,000 12.8 and 18.4), and blocks in e4m3
+// are half as long (256 of 2,000 59.8 and 56.1, in bf16 94.9 and 99.3).
+uint32_t decode_whole(uint64_t rows, bool f8) { return rows >= 512u && f8 ? 64u : rows >= 256u ? 32u : rows >= 96u ? 16u : 12u; }
+// Parts of a call: three workgroups a CU are resident (DECODE_ONCE). Few rows give
 // nearly equal parts, which fill the chip once (one sequence of 100,003 entries
 // 46.6 us against 52.8 with 1,152); the parts of many sequences differ, and
 // finer ones even out (48 sequences of up to 16,000: 72.3 us against 74.6).
-uint32_t decode_target(const obs_paged_kv* kv, const obs_paged_seqs* s) { return s->n_seqs * kv->n_kv <= 32u ? 768u : 1152u; }
+uint32_t decode_target(const obs_paged_kv* kv, const obs_paged_seqs* s) { return s->n_seqs * kv->n_kv <= 32u ? DECODE_ONCE : 1152u; }
 
 struct DecodePlan {
   uint64_t items, vis, blocks;
@@ -461,7 +475,7 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
   d.blocks = most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window, sinks);
   d.vis = 32u * d.blocks;
   const uint64_t rows = static_cast<uint64_t>(s->n_seqs) * kv->n_kv;
-  const uint32_t whole = weight ? 0u : decode_whole(rows);
+  const uint32_t whole = weight ? 0u : decode_whole(rows, kv->dtype == OBS_KV_E4M3);
   d.min_chunk = std::max(DECODE_MIN_CHUNK, d.blocks <= whole ? whole : 0u);
   // sum of the rows' rounded shares: at most target + rows (and what fp32 rounds), and at most each row's own most
   d.items = std::min<uint64_t>(decode_target(kv, s) + rows + 64u, rows * ((d.blocks + d.min_chunk - 1u) / d.min_chunk));
