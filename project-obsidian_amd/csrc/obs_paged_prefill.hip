@@ -27,7 +27,7 @@ using obs::up256;
 // Measured against it, at 8,192 rows under a window of 4,096 and at a prompt of
 // 5,001: one wave of 64 columns a SIMD 936 and 332 us (a wave issues an
 // instruction every four cycles), two of 32 columns with the next block's scores
-// beside this one's softmax 602 and 245, this one 575 and 219. More loads in
+// beside this one's softmax 602 and 245, this one 581 and 220. More loads in
 // flight, LDS reads earlier, two blocks a barrier, wave priorities and the other
 // machine schedulers gained nothing.
 // The running maximum follows the scores only when they pass it by 2^8 (the sums
@@ -36,69 +36,100 @@ using obs::up256;
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
 
 constexpr uint32_t PF_COLS = 384, PF_THREADS = 2u * PF_COLS, PF_TARGET = 256, PF_MIN_CHUNK = 4, PF_WHOLE = 12;
+constexpr uint32_t PF_TILES = 1024;  // tiles a kv head at most where they are cut into parts
 constexpr float PF_SLACK = 8.0f;
 
-// Tiles and blocks of the sequences, as the parts are planned by.
-struct PrefillSeq {
-  uint32_t tiles, nblk;
-};
 __device__ __forceinline__ Span tile_span(const PagedAttn& p, const RowSpan& r, uint32_t n, uint32_t t0, uint32_t t1) {
   // entry of row t is n - (r1 - t); negative: nothing to see
   const uint32_t hi0 = n + t0 + 1u > r.r1 ? n + t0 + 1u - r.r1 : 0u, hi1 = n + t1 > r.r1 ? n + t1 - r.r1 : 0u;
   return span_of(hi0 ? hi0 - 1u : 0u, hi1, p.window, p.sinks);
 }
-__device__ __forceinline__ PrefillSeq prefill_seq(const Paged& a, const PagedAttn& p, uint32_t b) {
-  const RowSpan r = paged_rows(a, b);
-  const uint32_t tq = PF_COLS / p.G, tiles = (r.r1 - r.r0 + tq - 1u) / tq;
-  return {tiles, tiles ? tile_span(p, r, paged_len(a, b), r.r0 + (tiles - 1u) * tq, r.r1).nblk : 0u};
+__device__ __forceinline__ uint32_t row_tiles(const PagedAttn& p, const RowSpan& r) {
+  const uint32_t tq = PF_COLS / p.G;
+  return (r.r1 - r.r0 + tq - 1u) / tq;
+}
+__device__ __forceinline__ uint32_t seq_tiles(const Paged& a, const PagedAttn& p, uint32_t b) {
+  return b < a.n_seqs ? row_tiles(p, paged_rows(a, b)) : 0u;
 }
 struct PrefillItem {
   uint32_t b, tile, split, splits, first, place;  // first: the part of the tile's split 0; place: the tile among all
 };
-// Part `item` of a kv head: sequences in order, in each the last tile (the
-// longest) first, a tile's parts together. With few rows (target > 0) the tiles
-// are cut into parts that fill the chip once (a workgroup fills a CU).
-__device__ __forceinline__ PrefillItem prefill_find(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane) {
-  // The shortest parts, in steps of an eighth, of which there are no more than
-  // the target: the longest one sets the time.
-  uint32_t chunk = 0xffffffffu;
-  if (p.target) {
-    PrefillSeq own{0u, 0u};
-    if (lane < a.n_seqs) own = prefill_seq(a, p, lane);
-    float total = 0.0f;
-    for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-      PrefillSeq s = own;
-      if (base) s = base + lane < a.n_seqs ? prefill_seq(a, p, base + lane) : PrefillSeq{0u, 0u};
-      total += wave_sum_asc(static_cast<float>(s.tiles) * static_cast<float>(s.nblk));
-    }
-    const float even = total * static_cast<float>(a.n_kv) / static_cast<float>(p.target);
-    for (uint32_t k = 8; k <= 16u; ++k) {
-      chunk = max(PF_MIN_CHUNK, static_cast<uint32_t>(__builtin_ceilf(even * static_cast<float>(k) * 0.125f)));
-      uint32_t parts = 0;
-      for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-        PrefillSeq s = own;
-        if (base) s = base + lane < a.n_seqs ? prefill_seq(a, p, base + lane) : PrefillSeq{0u, 0u};
-        parts += wave_sum_u32(s.tiles * plan_splits(s.nblk, chunk));
-      }
-      if (parts * a.n_kv <= p.target) break;  // uniform
-    }
-  }
-  uint32_t acc = 0, tacc = 0;
+// Tile `place` of a kv head: sequences in order, in each the last tile (the
+// longest) first. b is n_seqs behind the last one.
+__device__ __forceinline__ PrefillItem prefill_tile(const Paged& a, const PagedAttn& p, uint32_t place, uint32_t lane) {
+  uint32_t acc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-    PrefillSeq s{0u, 0u};
-    if (base + lane < a.n_seqs) s = prefill_seq(a, p, base + lane);
-    const uint32_t splits = p.target ? plan_splits(s.nblk, chunk) : 1u;
-    const uint32_t incl = wave_scan_u32(s.tiles * splits), all = __builtin_amdgcn_readlane(incl, 63);
-    const uint32_t tincl = wave_scan_u32(s.tiles);
-    if (item < acc + all) {
-      const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
-      const uint32_t tl = __builtin_amdgcn_readlane(s.tiles, l), sp = __builtin_amdgcn_readlane(splits, l);
-      const uint32_t end = acc + __builtin_amdgcn_readlane(incl, l), tend = tacc + __builtin_amdgcn_readlane(tincl, l);
-      const uint32_t at = item - (end - tl * sp), x = at / sp, split = at % sp;
-      return {uniform(base + l), uniform(tl - 1u - x), uniform(split), uniform(sp), uniform(item - split), uniform(tend - tl + x)};
+    const uint32_t tiles = seq_tiles(a, p, base + lane);
+    const uint32_t incl = wave_scan_u32(tiles), all = __builtin_amdgcn_readlane(incl, 63);
+    if (place < acc + all) {
+      const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= place)));
+      const uint32_t tile = acc + __builtin_amdgcn_readlane(incl, l) - 1u - place;
+      return {uniform(base + l), uniform(tile), 0u, 1u, uniform(place), uniform(place)};
     }
     acc += all;
-    tacc += __builtin_amdgcn_readlane(tincl, 63);
+  }
+  return {a.n_seqs, 0u, 0u, 1u, 0u, 0u};
+}
+// Part `item` of a kv head where there are few tiles: they are cut into parts of
+// nearly one length, a tile's parts together. The waves list all tiles' blocks in
+// LDS (s_tile), each wave then plans by the list. (With a sequence's tiles cut alike, by its last tile, one prompt of
+// 2,000 took 92.5 us against 68.)
+__device__ __forceinline__ PrefillItem prefill_part(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane, uint32_t wave,
+                                                    uint32_t* s_tile) {
+  const uint32_t tq = PF_COLS / p.G;
+  auto of = [](uint32_t v, uint32_t l) __attribute__((always_inline)) {
+    return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(static_cast<int>(4u * l), static_cast<int>(v)));
+  };
+  uint32_t n_tiles = 0;
+  for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
+    RowSpan r{0u, 0u};
+    uint32_t n = 0;
+    if (base + lane < a.n_seqs) {
+      r = paged_rows(a, base + lane);
+      n = paged_len(a, base + lane);
+    }
+    const uint32_t tiles = row_tiles(p, r), incl = wave_scan_u32(tiles), all = __builtin_amdgcn_readlane(incl, 63);
+    for (uint32_t x0 = 64u * wave; x0 < all; x0 += PF_THREADS) {  // uniform per wave
+      const uint32_t x = x0 + lane;
+      uint32_t l = 0;  // sequences that end at or before tile x
+#pragma unroll
+      for (uint32_t step = 32; step; step >>= 1) l += of(incl, l + step - 1u) <= x ? step : 0u;
+      const RowSpan rl{of(r.r0, l), of(r.r1, l)};
+      const uint32_t nl = of(n, l), t0 = rl.r0 + (of(incl, l) - 1u - x) * tq;
+      if (x < all && n_tiles + x < PF_TILES) s_tile[n_tiles + x] = tile_span(p, rl, nl, t0, umin(rl.r1, t0 + tq)).nblk;
+    }
+    n_tiles += all;
+  }
+  __syncthreads();
+  n_tiles = umin(n_tiles, PF_TILES);
+  float total = 0.0f;
+  for (uint32_t base = 0; base < n_tiles; base += 64u)
+    total += wave_sum_asc(base + lane < n_tiles ? static_cast<float>(s_tile[base + lane]) : 0.0f);
+  // The shortest parts, in steps of an eighth, of which there are no more than the
+  // target (a workgroup fills a CU): the longest one sets the time.
+  const float even = total * static_cast<float>(a.n_kv) / static_cast<float>(p.target);
+  uint32_t chunk = 0;
+  for (uint32_t k = 8; k <= 16u; ++k) {
+    chunk = max(PF_MIN_CHUNK, static_cast<uint32_t>(__builtin_ceilf(even * static_cast<float>(k) * 0.125f)));
+    uint32_t parts = 0;
+    for (uint32_t base = 0; base < n_tiles; base += 64u)
+      parts += wave_sum_u32(base + lane < n_tiles ? plan_splits(s_tile[base + lane], chunk) : 0u);
+    if (parts * a.n_kv <= p.target) break;  // uniform
+  }
+  uint32_t acc = 0;
+  for (uint32_t base = 0; base < n_tiles; base += 64u) {
+    const uint32_t splits = base + lane < n_tiles ? plan_splits(s_tile[base + lane], chunk) : 0u;
+    const uint32_t incl = wave_scan_u32(splits), all = __builtin_amdgcn_readlane(incl, 63);
+    if (item < acc + all) {
+      const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= item)));
+      const uint32_t sp = __builtin_amdgcn_readlane(splits, l), first = acc + __builtin_amdgcn_readlane(incl, l) - sp;
+      PrefillItem it = prefill_tile(a, p, base + l, lane);
+      it.split = uniform(item - first);
+      it.splits = uniform(sp);
+      it.first = uniform(first);
+      return it;
+    }
+    acc += all;
   }
   return {a.n_seqs, 0u, 0u, 1u, 0u, 0u};
 }
@@ -120,7 +151,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
   const uint32_t col = lane & 31u, half = lane >> 5;
   const uint32_t kv = blockIdx.x % a.n_kv;
-  const PrefillItem it = prefill_find(a, p, blockIdx.x / a.n_kv, lane);
+  __shared__ uint32_t s_tile[PF_TILES];
+  const PrefillItem it = p.target ? prefill_part(a, p, blockIdx.x / a.n_kv, lane, wave, s_tile) : prefill_tile(a, p, blockIdx.x / a.n_kv, lane);
   const uint32_t b = it.b;
   if (b >= a.n_seqs) return;  // uniform
   // everything of the tile in scalar registers: no address or branch below takes the vector unit
@@ -449,7 +481,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedA
   const uint32_t c = blockIdx.x % WG * CW + tid / (HD / 4u), d = 4u * (tid % (HD / 4u));
   uint32_t tiles = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u)
-    tiles += wave_sum_u32(base + lane < a.n_seqs ? prefill_seq(a, p, base + lane).tiles : 0u);
+    tiles += wave_sum_u32(seq_tiles(a, p, base + lane));
   if (place >= tiles) return;  // uniform
   const uint4 plan = reinterpret_cast<const uint4*>(p.plan)[static_cast<size_t>(place) * a.n_kv + kv];
   // (the bounds by items and rows: whatever the row array, nothing outside the buffers is met)
@@ -511,7 +543,7 @@ PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32
   // tiles: at most one that is not full a sequence, and none of a sequence without rows
   d.tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
   const uint64_t blocks = most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks);
-  d.split = 2u * full <= PF_TARGET + 128u && blocks > PF_WHOLE;
+  d.split = 2u * full <= PF_TARGET + 128u && d.tiles <= static_cast<uint64_t>(PF_TILES) * kv->n_kv && blocks > PF_WHOLE;
   d.items = d.split ? PF_TARGET + d.tiles + 64u : d.tiles;  // parts of 1 / target of all blocks at least, and one a tile
   if (d.split) {
     d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
