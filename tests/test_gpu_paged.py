@@ -342,6 +342,24 @@ def test_prefill_long(exe, shape, lens, new, window):
     assert np.array_equal(first, out.download())
 
 
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16, False), (6, 2, 64, 32, True)], ids=str)
+def test_prefill_many_short_prompts_in_parts(exe, shape):
+    """More sequences than a wave has lanes, some without rows, some of several tiles, over caches
+    long enough to be cut into parts."""
+    r = np.random.default_rng(95)
+    new = [int(x) for x in r.choice([0, 1, 2, 3, 60], 150, p=[0.3, 0.3, 0.2, 0.15, 0.05])]
+    lens = [max(t, int(x)) for t, x in zip(new, r.integers(0, 900, 150))]
+    _prefill_case(exe, shape, lens, new, 0, 0, 97, pad_rows=2)
+    _prefill_case(exe, shape, lens, new, 200, 3, 99)
+
+
+@pytest.mark.parametrize("shape,lens", [((32, 4, 128, 32, False), [2000]), ((32, 8, 64, 64, True), [1100]),
+                                        ((16, 1, 128, 32, False), [2900]), ((32, 4, 128, 16, True), [900, 1, 650])], ids=str)
+def test_prefill_whole_prompts_in_parts(exe, shape, lens):
+    """Prompts into an empty cache whose tiles have all lengths: the last ones in parts, the first whole."""
+    _prefill_case(exe, shape, lens, lens, 0, 0, 101, check_rows=[0, 30, 47, 48, 300, 511, 700, 1000, 1500, 10**9])
+
+
 def test_prefill_peaked_scores(exe):
     _prefill_case(exe, (32, 4, 128, 32, False), [300, 65], [129, 65], 0, 0, 37, k_std=30.0)
 
