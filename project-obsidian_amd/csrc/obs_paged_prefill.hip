@@ -72,8 +72,8 @@ __device__ __forceinline__ PrefillItem prefill_tile(const Paged& a, const PagedA
 }
 // Part `item` of a kv head where there are few tiles: they are cut into parts of
 // nearly one length, a tile's parts together. The waves list all tiles' blocks in
-// LDS (s_tile), each wave then plans by the list. (With a sequence's tiles cut alike, by its last tile, one prompt of
-// 2,000 took 92.5 us against 68.)
+// LDS (s_tile), each wave then plans by the list. (With a sequence's tiles cut
+// alike, by its last tile, one prompt of 2,000 took 92.5 us against 68.)
 __device__ __forceinline__ PrefillItem prefill_part(const Paged& a, const PagedAttn& p, uint32_t item, uint32_t lane, uint32_t wave,
                                                     uint32_t* s_tile) {
   const uint32_t tq = PF_COLS / p.G;
