@@ -257,3 +257,15 @@ def test_garbage_in_the_device_arrays_stays_in_bounds(host):
         assert bool(out[1]) == ok and out[0] == (want if ok else 0)
         assert out[2] == min(max(int(ln[b]), 0), mp << lp) and bool(out[3]) == (int(ln[b]) > mp << lp)
         assert 0 <= out[4] <= out[5] <= n_rows
+
+
+@pytest.mark.parametrize("t", [0, 32, 64, (1 << 30) - 32])
+def test_masks_of_a_block(host, t):
+    """A bit each for the entries below hi that are at or above lo or among the first tokens."""
+    edges = [0, 1, 31, 32, 33, 50, 63, 64, 65, 96, 1000, t, t + 1, t + 16, t + 31, t + 32, t + 33, 1 << 30]
+    host.seen.restype = C.c_uint32
+    for hi in edges:
+        for lo in edges:
+            for sinks in [*edges, 0xffffffff]:
+                ref = sum(1 << j for j in range(32) if t + j < hi and (t + j >= lo or t + j < sinks))
+                assert host.seen(C.c_uint32(t), C.c_uint32(hi), C.c_uint32(lo), C.c_uint32(sinks)) == ref, (hi, lo, sinks)
