@@ -18,7 +18,11 @@ using obs::Weight;
 // its own. Row r of score tile tt is entry 8 (r / 4) + 4 tt + r % 4 of the block:
 // the lane's eight scores are then entries 8 g .. 8 g + 7, the eight values that
 // one 16-byte load of a transposed value row brings.
-template <uint32_t HD, bool F8>
+// KEEP: values stay in the caches. From 64 entries on a row of a page holds several
+// blocks' values in one line; below, they are streamed like the keys (32 sequences
+// of up to 9,000, pages of 64: 69.5 us against 72.9 streamed, of 128 in e4m3 47.7
+// and 54.4; of 32 48.2 and 43.7).
+template <uint32_t HD, bool F8, bool KEEP>
 struct Block {
   static constexpr uint32_t KS = HD / 32u, NT = HD / 16u, KL = F8 ? KS / 2u : KS;
   u32x4_v k[2][KL];  // e4m3: 16 dims a load, two steps
@@ -37,13 +41,14 @@ struct Block {
 #pragma unroll
       for (uint32_t i = 0; i < KL; ++i) k[tt][i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_v*>(kr + 64u * i));
     }
+    typedef typename std::conditional<F8, u32x2_v, u32x4_v>::type V;
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; ++nt) {
-      const uint8_t* vr = vb + ((16u * nt + col) * SZ << a.lp);
-      if constexpr (F8)
-        v[nt] = __builtin_nontemporal_load(reinterpret_cast<const u32x2_v*>(vr));
+      const V* vr = reinterpret_cast<const V*>(vb + ((16u * nt + col) * SZ << a.lp));
+      if constexpr (KEEP)
+        v[nt] = *vr;
       else
-        v[nt] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_v*>(vr));
+        v[nt] = __builtin_nontemporal_load(vr);
     }
   }
   // key fragment of tile tt, step ks: the dims that query fragment ks holds
@@ -85,8 +90,8 @@ struct Column {
 // token sees (values it does not see read as zero: the pool may hold anything
 // there); ok: whether the lane's page is there; masked: whether the block needs
 // any of it.
-template <uint32_t HD, bool F8>
-__device__ __forceinline__ void block_step(const Block<HD, F8>& blk, const bf16x8_v (&qb)[HD / 32u], Column<HD>& c,
+template <uint32_t HD, bool F8, bool KEEP>
+__device__ __forceinline__ void block_step(const Block<HD, F8, KEEP>& blk, const bf16x8_v (&qb)[HD / 32u], Column<HD>& c,
                                            uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok, bool masked, float scale_log2, float (&sv)[8],
                                            uint32_t lane) {
   constexpr uint32_t KS = HD / 32u, NT = HD / 16u;
@@ -212,7 +217,7 @@ __device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, u
 // the columns. Its four waves take the part's blocks in turn and meet in LDS.
 // A part that is all of its sequence writes the output, others their maximum,
 // sum and output for paged_join_kernel.
-template <uint32_t HD, bool F8, bool WEIGHT>
+template <uint32_t HD, bool F8, bool WEIGHT, bool KEEP>
 __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn p) {
   constexpr uint32_t NT = HD / 16u;
   __shared__ float s_ml[4][16][2];
@@ -232,7 +237,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
 #pragma unroll
   for (uint32_t ks = 0; ks < HD / 32u; ++ks) {
     u32x4_v v = *reinterpret_cast<const u32x4_v*>(p.q + static_cast<size_t>(b) * p.q_ld + (kv * p.G + min(col, p.G - 1u)) * HD +
-                                                  Block<HD, F8>::q_dim(ks, g));
+                                                  Block<HD, F8, KEEP>::q_dim(ks, g));
     if (col >= p.G) v = u32x4_v{0u, 0u, 0u, 0u};
     qb[ks] = __builtin_bit_cast(bf16x8_v, v);
   }
@@ -257,11 +262,11 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
       p0 = ok0 ? p0 : 0u;
       p1 = ok1 ? p1 : 0u;
     }
-    Block<HD, F8> blk;
+    Block<HD, F8, KEEP> blk;
     blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
     __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
     float sv[8];
-    block_step<HD, F8>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
+    block_step<HD, F8, KEEP>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
                        !(whole && ok0 && ok1), scale, sv, lane);
     if constexpr (WEIGHT) {
       if (col < p.G) {
@@ -488,8 +493,11 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
 
 template <uint32_t HD, bool F8, bool WEIGHT>
 int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight& w, const DecodePlan& d) {
-  OBS_LAUNCH(ctx, "paged_decode",
-             paged_decode_kernel<HD, F8, WEIGHT><<<static_cast<uint32_t>(d.items), 256, 0, ctx->stream>>>(a, p));
+  const uint32_t items = static_cast<uint32_t>(d.items);
+  if (a.lp >= 6u)
+    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, F8, WEIGHT, true><<<items, 256, 0, ctx->stream>>>(a, p));
+  else
+    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, F8, WEIGHT, false><<<items, 256, 0, ctx->stream>>>(a, p));
   if (!WEIGHT && d.blocks <= d.min_chunk) return OBS_OK;  // every sequence is one part
   const uint32_t wchunks = WEIGHT ? static_cast<uint32_t>((d.vis + 1023u) / 1024u) : 0u, rows = a.n_seqs * p.nh;
   const uint32_t weights = rows / p.G * wchunks;
