@@ -111,19 +111,22 @@ __device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs
 }
 
 // Workgroups 0 .. n_vt - 1 bring the values of prompts (none with one token a
-// sequence). The others: a token row each; HD / 8 lanes per head with 8 dims
+// sequence). The others: one token row each, or four; HD / 8 lanes per head with 8 dims
 // each, so a wave norms and rotates 512 / HD heads at once. The sums and the
 // rotation are attn_prep_rows_kernel's, in its order. The first heads are
 // requested before the row's sequence, entry and position are known.
-template <uint32_t HD, bool F8>
+template <uint32_t HD, bool F8, uint32_t WAVES>
 __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p, Weight w, uint32_t n_vt) {
   constexpr uint32_t LPH = HD / 8u, HPW = 64u / LPH;  // lanes per head, heads per wave
   if (blockIdx.x < n_vt) {  // uniform
     prep_paged_values<HD, F8>(a, p, blockIdx.x);
     return;
   }
-  const uint32_t lane = threadIdx.x & 63u, wave = uniform(threadIdx.x >> 6), m = lane % LPH, c0 = 8u * m;
-  const uint32_t t = blockIdx.x - n_vt, heads = p.nh + a.n_kv;
+  const uint32_t lane = threadIdx.x & 63u, m = lane % LPH, c0 = 8u * m;
+  const uint32_t w4 = uniform(threadIdx.x >> 6), wave = w4 % WAVES;           // the wave among its row's
+  const uint32_t tid = threadIdx.x % (64u * WAVES), threads = 64u * WAVES;  // the thread among its row's
+  const uint32_t t = (blockIdx.x - n_vt) * (4u / WAVES) + w4 / WAVES, heads = p.nh + a.n_kv;
+  if (t >= a.n_rows) return;  // uniform per wave, as all below (no barrier)
   const uint16_t* q = p.q + static_cast<size_t>(t) * p.q_ld;
   const uint16_t* k = p.k + static_cast<size_t>(t) * p.kv_ld;
   auto load_head = [&](uint32_t head) __attribute__((always_inline)) {  // clamped: past the last head, unused
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
   const RowSpan rs = paged_rows(a, b);
   if (t < rs.r0 || t >= rs.r1) return;
   const uint32_t n = uniform(paged_len(a, b));
-  if (t == rs.r0 && threadIdx.x == 0u && paged_len_bad(a, b)) paged_flag(a.status);
+  if (t == rs.r0 && tid == 0u && paged_len_bad(a, b)) paged_flag(a.status);
   const int32_t entry = static_cast<int32_t>(n) - static_cast<int32_t>(uniform(rs.r1) - t);
   const int32_t pos = p.pos ? static_cast<int32_t>(uniform(static_cast<uint32_t>(p.pos[t]))) : entry;
   if (pos < 0 || static_cast<uint32_t>(pos) >= p.rope_len) return;  // uniform
@@ -156,24 +159,24 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
   const uint32_t e = there ? static_cast<uint32_t>(entry) : 0u;
   bool ok;
   const uint32_t page = uniform(paged_id(a, b, e, ok));
-  if (there && !ok && threadIdx.x == 0u) paged_flag(a.status);
+  if (there && !ok && tid == 0u) paged_flag(a.status);
   there = there && ok;
   const uint32_t off = e & ((1u << a.lp) - 1u);
-  if (w.w && entry >= 0 && threadIdx.x < a.n_kv) {
+  if (w.w && entry >= 0 && tid < a.n_kv) {
     const int64_t s = weight_slot(w, b);
     if (s >= 0)
-      for (uint32_t h = threadIdx.x; h < a.n_kv; h += 256u) w.w[(static_cast<size_t>(s) * a.n_kv + h) * w.ld + e] = 0.0f;
-    else if (threadIdx.x == 0u)
+      for (uint32_t h = tid; h < a.n_kv; h += threads) w.w[(static_cast<size_t>(s) * a.n_kv + h) * w.ld + e] = 0.0f;
+    else if (tid == 0u)
       paged_flag(a.status);
   }
   uint16_t* q_out = p.q_out + static_cast<size_t>(t) * p.q_out_ld;
   const size_t page0 = static_cast<size_t>(page) * a.n_kv;
   const uint32_t pg = 1u << a.lp;
   const bool first = m < LPH / 2u;
-  for (uint32_t hb = HPW * wave; hb < heads; hb += 4u * HPW) {  // uniform per wave
+  for (uint32_t hb = HPW * wave; hb < heads; hb += WAVES * HPW) {  // uniform per wave
     const uint32_t head = hb + lane / LPH;
     const bool is_q = head < p.nh;
-    const uint4 xnext = load_head(head + 4u * HPW);
+    const uint4 xnext = load_head(head + WAVES * HPW);
     const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
     const uint32_t ww[4] = {is_q ? wq.x : wk.x, is_q ? wq.y : wk.y, is_q ? wq.z : wk.z, is_q ? wq.w : wk.w};
     xv = xnext;
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
   }
   if (!there || n_vt) return;
   const uint16_t* v = p.v + static_cast<size_t>(t) * p.kv_ld;
-  for (uint32_t i = threadIdx.x; i < a.n_kv * HD; i += 256u) {  // one token: one transposed column
+  for (uint32_t i = tid; i < a.n_kv * HD; i += threads) {  // one token: one transposed column
     const uint32_t h = i / HD, d = i % HD;
     const size_t at = ((page0 + h) * HD + d) * pg + off;
     if constexpr (F8)
@@ -537,6 +540,21 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
   }
 }
 
+// Waves a token row: four, or one where rows fill the chip and it goes at most five
+// times round the heads, as the chain to a row's entry and position then runs in
+// fewer waves (6,000 rows of 36 heads of 64: 38.0 us with four, 24.8 with one; of 36
+// heads of 128, nine times round, 31.2 and 32.3).
+uint32_t prep_waves(uint32_t hd, uint32_t heads, uint32_t rows) { return heads * hd <= 2560u && rows >= 1024u ? 1u : 4u; }
+
+template <uint32_t HD, bool F8>
+int launch_prep(obs_ctx* ctx, const Paged& a, const PrepArgs& p, const Weight& w, uint32_t n_vt, uint32_t grid, uint32_t waves) {
+  if (waves == 1u)
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<HD, F8, 1><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
+  else
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<HD, F8, 4><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
+  return OBS_OK;
+}
+
 // copies: workgroups with 64 entries each.
 template <uint32_t HD, bool F8>
 int launch_copy(obs_ctx* ctx, const Paged& a, const int32_t* dst_pages, uint32_t dst_max_pages, uint32_t budget,
@@ -644,7 +662,8 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
     return obs::set_error(ctx, OBS_E_SHAPE, "%s: rope_len must be in [1, 2^24] (got %u)", who, rope_len);
   if (seqs->n_rows == 0 || seqs->n_seqs == 0) return OBS_OK;
   const uint32_t n_vt = seqs->row ? kv->n_kv * ((seqs->n_rows + PREP_TILE - 1u) / PREP_TILE) : 0u;
-  const uint32_t grid = n_vt + seqs->n_rows;
+  const uint32_t waves = prep_waves(hd, n_heads + kv->n_kv, seqs->n_rows);
+  const uint32_t grid = n_vt + (waves == 1u ? (seqs->n_rows + 3u) / 4u : seqs->n_rows);
   rc = obs::check_grid(ctx, who, grid, 256u);
   if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
@@ -654,15 +673,9 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
   const Paged a = obs::paged_args(ctx, kv, seqs);
   const Weight w = obs::weight_args(weight);
   const bool f8 = kv->dtype == OBS_KV_E4M3;
-  if (hd == 128u && !f8)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, false><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
-  else if (hd == 128u)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<128, true><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
-  else if (!f8)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, false><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
-  else
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<64, true><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
-  return OBS_OK;
+  if (hd == 128u)
+    return f8 ? launch_prep<128, true>(ctx, a, p, w, n_vt, grid, waves) : launch_prep<128, false>(ctx, a, p, w, n_vt, grid, waves);
+  return f8 ? launch_prep<64, true>(ctx, a, p, w, n_vt, grid, waves) : launch_prep<64, false>(ctx, a, p, w, n_vt, grid, waves);
 }
 
 int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,

@@ -534,6 +534,16 @@ def test_prep_many_sequences(exe):
     _check_prep(*a, lens, new, weight=False)
 
 
+@pytest.mark.parametrize("shape", [(32, 4, 64, 16, False), (8, 1, 128, 32, True), (12, 2, 64, 64, True)], ids=str)
+def test_prep_many_rows_of_few_heads(exe, shape):
+    """Rows that take one wave each: a count that is no multiple of four, sequences without rows,
+    rows behind the last one."""
+    lens, new = [700, 5, 0, 480, 9], [600, 3, 0, 480, 9]
+    a = _prep_case(exe, shape, lens, new, 103, pad_rows=3)
+    exe.device_status()
+    _check_prep(*a, lens, new)
+
+
 def test_prep_equals_the_contiguous_cache(exe):
     """bf16 at head_dim 128: q, keys and values are obs_attn_prep_rows' bit for bit."""
     nh, nkv, hd, page, T, pos0 = 32, 4, 128, 32, 75, 60
