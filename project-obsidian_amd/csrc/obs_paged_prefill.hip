@@ -102,16 +102,20 @@ __device__ __forceinline__ PrefillItem prefill_part(const Paged& a, const PagedA
   }
   __syncthreads();
   n_tiles = umin(n_tiles, PF_TILES);
-  float total = 0.0f;
-  for (uint32_t base = 0; base < n_tiles; base += 64u)
-    total += wave_sum_asc(base + lane < n_tiles ? static_cast<float>(s_tile[base + lane]) : 0.0f);
+  float total = 0.0f, longest = 0.0f;
+  for (uint32_t base = 0; base < n_tiles; base += 64u) {
+    const float v = base + lane < n_tiles ? static_cast<float>(s_tile[base + lane]) : 0.0f;
+    total += wave_sum_asc(v);
+    longest = fmaxf(longest, wave_max_f32(v));
+  }
   // The shortest parts, in steps of an eighth, of which there are no more than the
-  // target (a workgroup fills a CU): the longest one sets the time. One prompt's
-  // parts begin with the longest tile's, so a second round of its shortest ends
-  // early: there no longer than half above the even share.
+  // target (a workgroup fills a CU): the longest one sets the time. The parts of one
+  // prompt whose tiles have all lengths begin with the longest tile's, so a second
+  // round of its shortest ends early: there no longer than half above the even share.
   const float even = total * static_cast<float>(a.n_kv) / static_cast<float>(p.target);
   uint32_t chunk = 0;
-  for (uint32_t k = 8; k <= (a.n_seqs == 1u ? 12u : 16u); ++k) {
+  const uint32_t most = a.n_seqs == 1u && longest * static_cast<float>(n_tiles) > 1.5f * total ? 12u : 16u;
+  for (uint32_t k = 8; k <= most; ++k) {
     chunk = max(PF_MIN_CHUNK, static_cast<uint32_t>(__builtin_ceilf(even * static_cast<float>(k) * 0.125f)));
     uint32_t parts = 0;
     for (uint32_t base = 0; base < n_tiles; base += 64u)
@@ -533,8 +537,9 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedA
 // more than the parts save (one prompt of 256 19.5 us whole, 23.0 in parts; 384
 // 24.2 and 27.5, four of 300 21.2 and 29.2; a row over 400 entries 21.5 and 18.9).
 // More tiles than three quarters of the CUs: whole ones end as early (four prompts
-// of up to 985 48 us against 54), but for one prompt, whose tiles have all lengths
-// (2,600 107.7 whole, 96.6 in parts; 3,000 123.3 and 119.1).
+// of up to 985 48 us against 54; 2,600 rows of 5,000 entries 201 and 215), but for
+// one that the table hardly outgrows, whose tiles have all lengths (2,600 107.7
+// whole, 96.6 in parts; 3,000 123.3 and 119.1).
 struct PrefillPlan {
   uint64_t items, tiles;  // workgroups and tiles (of all kv heads) at most
   bool split;
@@ -547,8 +552,10 @@ PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32
   const uint64_t full = static_cast<uint64_t>(kv->n_kv) * ((s->n_rows + tq - 1u) / tq);
   // tiles: at most one that is not full a sequence, and none of a sequence without rows
   d.tiles = static_cast<uint64_t>(kv->n_kv) * std::min<uint64_t>(s->n_rows, (s->n_rows + tq - 1u) / tq + s->n_seqs);
-  const uint64_t blocks = most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window ? static_cast<uint64_t>(window) + tq : 0u, sinks);
-  d.split = full <= (s->n_seqs == 1u ? PF_TARGET : PF_TARGET * 3u / 4u) && d.tiles <= static_cast<uint64_t>(PF_TILES) * kv->n_kv && blocks > PF_WHOLE;
+  const uint64_t entries = static_cast<uint64_t>(s->max_pages) * kv->page;
+  const uint64_t blocks = most_blocks(entries, window ? static_cast<uint64_t>(window) + tq : 0u, sinks);
+  const bool steps = s->n_seqs == 1u && !window && 2u * entries < 3u * static_cast<uint64_t>(s->n_rows);
+  d.split = full <= (steps ? PF_TARGET : PF_TARGET * 3u / 4u) && d.tiles <= static_cast<uint64_t>(PF_TILES) * kv->n_kv && blocks > PF_WHOLE;
   d.items = d.split ? PF_TARGET + d.tiles + 64u : d.tiles;  // parts of 1 / target of all blocks at least, and one a tile
   if (d.split) {
     d.ml = up256(d.items * PF_COLS * 2u * sizeof(float));
