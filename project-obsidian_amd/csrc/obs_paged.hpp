@@ -223,7 +223,9 @@ __device__ __forceinline__ float wave_max_f32(float v) {  // uniform
   v = fmaxf(v, dpp_f32<DPP_MIRROR>(v));
   return fmaxf(fmaxf(readlane_f32(v, 0), readlane_f32(v, 16)), fmaxf(readlane_f32(v, 32), readlane_f32(v, 48)));
 }
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v))); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));
+}
 // Parts of a sequence's nblk blocks.
 __device__ __forceinline__ uint32_t plan_splits(uint32_t nblk, uint32_t chunk) { return max(1u, (nblk + chunk - 1u) / chunk); }
 

@@ -92,8 +92,8 @@ struct Column {
 // any of it.
 template <uint32_t HD, bool F8, bool KEEP>
 __device__ __forceinline__ void block_step(const Block<HD, F8, KEEP>& blk, const bf16x8_v (&qb)[HD / 32u], Column<HD>& c,
-                                           uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok, bool masked, float scale_log2, float (&sv)[8],
-                                           uint32_t lane) {
+                                           uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok, bool masked,
+                                           float scale_log2, float (&sv)[8], uint32_t lane) {
   constexpr uint32_t KS = HD / 32u, NT = HD / 16u;
 #pragma unroll
   for (uint32_t tt = 0; tt < 2; ++tt) {
@@ -504,7 +504,8 @@ int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight
   // few rows have many parts each: four workgroups a row (one sequence of 100,003
   // entries 46.5 us against 48.2; 48 sequences of up to 16,000 77.7 against 72.3)
   if (rows < 256u)
-    OBS_LAUNCH(ctx, "paged_join", paged_join_kernel<HD, F8, WEIGHT, 32><<<rows * (HD / 32u) + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
+    OBS_LAUNCH(ctx, "paged_join",
+               paged_join_kernel<HD, F8, WEIGHT, 32><<<rows * (HD / 32u) + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
   else
     OBS_LAUNCH(ctx, "paged_join", paged_join_kernel<HD, F8, WEIGHT, HD><<<rows + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
   return OBS_OK;
@@ -573,7 +574,8 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
   const Paged a = obs::paged_args(ctx, kv, seqs);
   uint8_t* wb = static_cast<uint8_t*>(ws);
   const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml),
-                   reinterpret_cast<float*>(wb + d.ml + d.part), reinterpret_cast<uint2*>(wb + d.ml + d.part + d.scores), n_heads, n_heads / kv->n_kv, window, sinks, q_ld,
+                   reinterpret_cast<float*>(wb + d.ml + d.part), reinterpret_cast<uint2*>(wb + d.ml + d.part + d.scores),
+                   n_heads, n_heads / kv->n_kv, window, sinks, q_ld,
                    static_cast<uint32_t>(d.vis), d.min_chunk, decode_target(kv, seqs), 0u,
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const Weight w = obs::weight_args(weight);

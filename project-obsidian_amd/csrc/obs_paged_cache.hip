@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
     tie &= ties ? mid : 0u;
     uint32_t keep = (range_bits(j0, 0u, n) & ~mid) | (above & mid);
     uint32_t sums;
-    const uint32_t before = group_scan(static_cast<uint32_t>(__popc(keep)) << 16 | static_cast<uint32_t>(__popc(tie)), s_w[par], lane, wave, sums);
+    const uint32_t before = group_scan(static_cast<uint32_t>(__popc(keep)) << 16 | static_cast<uint32_t>(__popc(tie)),
+                                       s_w[par], lane, wave, sums);
     uint32_t rank = tie_at + (before & 0xffffu);  // of the thread's first tie
     const uint32_t ties_before = umin(tie_at, ties);
     uint32_t x = (before >> 16) + umin(rank, ties) - ties_before;  // place among the segment's kept entries
@@ -461,14 +462,17 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
 #pragma unroll
   for (uint32_t i = 0; i < KN; ++i) {
     const uint32_t t = tid + 256u * i, e = t / CH % GE, c = t % CH;
-    kx[i] = *reinterpret_cast<const uint4*>(kb + (((static_cast<size_t>(max(s_src[e], 0)) * a.n_kv + h) << a.lp) + s_so[e]) * (HD * SZ) + 16u * c);
+    const size_t row = ((static_cast<size_t>(max(s_src[e], 0)) * a.n_kv + h) << a.lp) + s_so[e];
+    kx[i] = *reinterpret_cast<const uint4*>(kb + row * (HD * SZ) + 16u * c);
     if (s_src[e] < 0) kx[i] = make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (uint32_t i = 0; i < KN; ++i) {
     const uint32_t t = tid + 256u * i, e = t / CH % GE, c = t % CH;
-    if ((GE * CH % 256u == 0u || t < GE * CH) && s_dst[e] >= 0)
-      *reinterpret_cast<uint4*>(kb + (((static_cast<size_t>(s_dst[e]) * a.n_kv + h) << a.lp) + ((e0 + e) & mask)) * (HD * SZ) + 16u * c) = kx[i];
+    if ((GE * CH % 256u == 0u || t < GE * CH) && s_dst[e] >= 0) {
+      const size_t row = ((static_cast<size_t>(s_dst[e]) * a.n_kv + h) << a.lp) + ((e0 + e) & mask);
+      *reinterpret_cast<uint4*>(kb + row * (HD * SZ) + 16u * c) = kx[i];
+    }
   }
   constexpr uint32_t DW = HD / 64u;  // waves across the dims
   const T* vs = reinterpret_cast<const T*>(a.v);
@@ -562,9 +566,12 @@ int launch_copy(obs_ctx* ctx, const Paged& a, const int32_t* dst_pages, uint32_t
   // below two workgroups a CU (a few sequences): 16 entries each, one sequence of 2,048 kept entries 15.4 us against 19.9
   if (copies < 512u) {
     const uint32_t grid = a.n_seqs * a.n_kv * ((budget + 15u) / 16u);
-    OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<HD, F8, 16><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+    OBS_LAUNCH(ctx, "kv_evict_copy",
+               evict_copy_kernel<HD, F8, 16><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
   } else {
-    OBS_LAUNCH(ctx, "kv_evict_copy", evict_copy_kernel<HD, F8, 64><<<static_cast<uint32_t>(copies), 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+    const uint32_t grid = static_cast<uint32_t>(copies);
+    OBS_LAUNCH(ctx, "kv_evict_copy",
+               evict_copy_kernel<HD, F8, 64><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
   }
   return OBS_OK;
 }

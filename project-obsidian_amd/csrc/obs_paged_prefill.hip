@@ -158,7 +158,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   const uint32_t col = lane & 31u, half = lane >> 5;
   const uint32_t kv = blockIdx.x % a.n_kv;
   __shared__ uint32_t s_tile[PF_TILES];
-  const PrefillItem it = p.target ? prefill_part(a, p, blockIdx.x / a.n_kv, lane, wave, s_tile) : prefill_tile(a, p, blockIdx.x / a.n_kv, lane);
+  const PrefillItem it = p.target ? prefill_part(a, p, blockIdx.x / a.n_kv, lane, wave, s_tile)
+                                  : prefill_tile(a, p, blockIdx.x / a.n_kv, lane);
   const uint32_t b = it.b;
   if (b >= a.n_seqs) return;  // uniform
   // everything of the tile in scalar registers: no address or branch below takes the vector unit
@@ -449,7 +450,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       wave_sync();
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j)
-        if (to[j]) *reinterpret_cast<u32x4_v*>(to[j] + 32u * d) = *reinterpret_cast<const u32x4_v*>(slab + (ocol + 16u * j) * 80u + 16u * och);
+        if (to[j])
+          *reinterpret_cast<u32x4_v*>(to[j] + 32u * d) = *reinterpret_cast<const u32x4_v*>(slab + (ocol + 16u * j) * 80u + 16u * och);
       wave_sync();
     }
   } else {
@@ -471,7 +473,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       for (uint32_t j = 0; j < 2; ++j) {
         const uint32_t oc = 32u * wave + ocol + 16u * j;
         if (is_col(oc))
-          *reinterpret_cast<u32x4_v*>(p.part + (at + oc) * HD + 16u * d + 4u * och) = *reinterpret_cast<const u32x4_v*>(slab + (ocol + 16u * j) * 80u + 16u * och);
+          *reinterpret_cast<u32x4_v*>(p.part + (at + oc) * HD + 16u * d + 4u * och) =
+              *reinterpret_cast<const u32x4_v*>(slab + (ocol + 16u * j) * 80u + 16u * och);
       }
       wave_sync();
     }
@@ -605,8 +608,8 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
   obs::DeviceGuard guard(ctx);
   const Paged a = obs::paged_args(ctx, kv, seqs);
   uint8_t* wb = static_cast<uint8_t*>(ws);
-  const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr, reinterpret_cast<uint2*>(wb + d.ml + d.part), n_heads,
-                   n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u, static_cast<uint32_t>(d.tiles),
+  const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr,
+                   reinterpret_cast<uint2*>(wb + d.ml + d.part), n_heads, n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u, static_cast<uint32_t>(d.tiles),
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const bool f8 = kv->dtype == OBS_KV_E4M3;
   if (kv->head_dim == 128u) return f8 ? launch_prefill<128, true>(ctx, a, p, d) : launch_prefill<128, false>(ctx, a, p, d);
