@@ -53,22 +53,31 @@ __device__ __forceinline__ uint32_t seq_tiles(const Paged& a, const PagedAttn& p
 }
 struct PrefillItem {
   uint32_t b, tile, split, splits, first, place;  // first: the part of the tile's split 0; place: the tile among all
+  RowSpan r;  // the sequence's rows
+  uint32_t n;  // and entries
 };
 // Tile `place` of a kv head: sequences in order, in each the last tile (the
 // longest) first. b is n_seqs behind the last one.
 __device__ __forceinline__ PrefillItem prefill_tile(const Paged& a, const PagedAttn& p, uint32_t place, uint32_t lane) {
   uint32_t acc = 0;
   for (uint32_t base = 0; base < a.n_seqs; base += 64u) {
-    const uint32_t tiles = seq_tiles(a, p, base + lane);
-    const uint32_t incl = wave_scan_u32(tiles), all = __builtin_amdgcn_readlane(incl, 63);
+    RowSpan r{0u, 0u};
+    uint32_t n = 0;
+    if (base + lane < a.n_seqs) {
+      r = paged_rows(a, base + lane);
+      n = paged_len(a, base + lane);
+    }
+    const uint32_t incl = wave_scan_u32(row_tiles(p, r)), all = __builtin_amdgcn_readlane(incl, 63);
     if (place < acc + all) {
-      const uint32_t l = static_cast<uint32_t>(__popcll(__ballot(acc + incl <= place)));
+      const uint32_t l = uniform(static_cast<uint32_t>(__popcll(__ballot(acc + incl <= place))));
       const uint32_t tile = acc + __builtin_amdgcn_readlane(incl, l) - 1u - place;
-      return {uniform(base + l), uniform(tile), 0u, 1u, uniform(place), uniform(place)};
+      return {base + l, uniform(tile), 0u, 1u, uniform(place), uniform(place),
+              {static_cast<uint32_t>(__builtin_amdgcn_readlane(r.r0, l)), static_cast<uint32_t>(__builtin_amdgcn_readlane(r.r1, l))},
+              static_cast<uint32_t>(__builtin_amdgcn_readlane(n, l))};
     }
     acc += all;
   }
-  return {a.n_seqs, 0u, 0u, 1u, 0u, 0u};
+  return {a.n_seqs, 0u, 0u, 1u, 0u, 0u, {0u, 0u}, 0u};
 }
 // Part `item` of a kv head where there are few tiles: they are cut into parts of
 // nearly one length, a tile's parts together. The waves list all tiles' blocks in
@@ -137,7 +146,7 @@ __device__ __forceinline__ PrefillItem prefill_part(const Paged& a, const PagedA
     }
     acc += all;
   }
-  return {a.n_seqs, 0u, 0u, 1u, 0u, 0u};
+  return {a.n_seqs, 0u, 0u, 1u, 0u, 0u, {0u, 0u}, 0u};
 }
 
 template <uint32_t HD, bool F8>
@@ -163,9 +172,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   const uint32_t b = it.b;
   if (b >= a.n_seqs) return;  // uniform
   // everything of the tile in scalar registers: no address or branch below takes the vector unit
-  RowSpan r = paged_rows(a, b);
-  r = {uniform(r.r0), uniform(r.r1)};
-  const uint32_t n = uniform(paged_len(a, b));
+  const RowSpan r = it.r;
+  const uint32_t n = it.n;
   const uint32_t tq = PF_COLS / p.G, t0r = r.r0 + it.tile * tq, t1r = umin(r.r1, t0r + tq);
   if (tid == 0u && it.tile == 0u && it.split == 0u && kv == 0u && paged_len_bad(a, b)) paged_flag(a.status);
   const Span s = tile_span(p, r, n, t0r, t1r);
