@@ -586,6 +586,28 @@ def test_prep_in_place_and_bad_pages(exe):
     assert np.array_equal(after, want)
 
 
+@pytest.mark.parametrize("rows", [200, 1101])
+@pytest.mark.parametrize("shape", [(32, 4, 64, 16, False), (32, 4, 128, 32, True), (8, 1, 128, 32, False)], ids=str)
+def test_prep_of_prompts_in_place(exe, shape, rows):
+    """q_out is q, inside one projection's rows: what the call gives with a q_out of its own."""
+    nh, nkv, hd, page, f8 = shape
+    rng = np.random.default_rng(107)
+    lens, ld = [rows + 13], (nh + 2 * nkv) * hd
+    x, qn, kn = synth.bf16_normal(rng, (rows, ld), 2.0), synth.norm_weight(rng, hd), synth.norm_weight(rng, hd)
+    results = []
+    for own in (False, True):
+        pool = Pool(exe, np.random.default_rng(109), lens, nkv, hd, page, f8)
+        dx, out = exe.upload(x), exe.alloc((rows, ld), np.uint16)
+        to = out if own else dx
+        exe.attn_prep_paged(pool.kv, pool.seqs([0, rows]), dx.ptr, dx.ptr + 2 * nh * hd, dx.ptr + 2 * (nh + nkv) * hd,
+                            exe.upload(qn), exe.upload(kn), to.ptr, nh, EPS, THETA, 2048, q_ld=ld, kv_ld=ld, q_out_ld=ld)
+        exe.device_status()
+        results.append([to.download()[:, :nh * hd], pool.dk.download(), pool.dv.download()])
+    for a, b in zip(*results):
+        assert np.array_equal(a, b)
+    assert not np.array_equal(results[0][0], x[:, :nh * hd])
+
+
 # ---- eviction -------------------------------------------------------------------
 
 def _kept(w, n, sinks, recent, budget):
