@@ -678,6 +678,36 @@ def test_evict_many(exe, shape, weights):
     _evict_case(exe, shape, [2500, 1101, 1100, 60, 1900, 2048, 1333, 0], 4, 100, 1100, 83, weights)
 
 
+def test_weight_rows_of_odd_strides(exe):
+    """Weight rows that begin at any 4-byte address: gathered, cleared and evicted as in aligned ones."""
+    nh, nkv, hd, page, lens = 32, 4, 128, 32, [900, 37, 500]
+    B, budget = len(lens), 130
+    results = []
+    for pad, off in ((0, 0), (3, 1)):
+        rng = np.random.default_rng(113)
+        pool = Pool(exe, rng, lens, nkv, hd, page, False, extra=B * 5)
+        cap = pool.max_pages * page
+        w = rng.random((B, nkv, cap)).astype(np.float32)
+        flat = np.zeros(off + B * nkv * (cap + pad), np.float32)
+        flat[off:].reshape(B, nkv, cap + pad)[:, :, :cap] = w
+        dw = exe.upload(flat)
+        wt = oh.KvWeight(dw.ptr + 4 * off, B, cap + pad)
+        q, out = exe.upload(synth.bf16_normal(rng, (B, nh, hd), 2.0)), exe.alloc((B, nh, hd), np.uint16)
+        ws = exe.alloc(exe.sdpa_paged_workspace(pool.kv, pool.seqs(), nh, wt), np.uint8)
+        exe.sdpa_paged_decode(pool.kv, pool.seqs(), q, out, nh, ws, weight=wt)
+        kept, new_len = exe.alloc((B, nkv, budget), np.int32), exe.alloc(B, np.int32)
+        dwd = exe.alloc(off + B * nkv * (budget + pad), np.float32)
+        exe.kv_evict(pool.kv, pool.seqs(), wt, exe.upload(pool.free[:B * 5].reshape(B, 5).copy()), 5,
+                     oh.KvWeight(dwd.ptr + 4 * off, B, budget + pad), 2, 30, budget, kept, new_len)
+        exe.device_status()
+        after = dw.download()[off:].reshape(B, nkv, cap + pad)
+        assert not np.any(after[:, :, cap:]) and not np.any(after[1, :, 37:cap] != w[1, :, 37:])
+        gw = dwd.download()[off:].reshape(B, nkv, budget + pad)
+        results.append([out.download(), after[:, :, :cap], kept.download(), gw[[0, 2], :, :budget], gw[1, :, :37], pool.dk.download()])
+    for x, y in zip(*results):
+        assert np.array_equal(x, y)
+
+
 def test_more_kv_heads_than_threads(exe):
     """300 kv heads: loops over heads go round more than once."""
     shape = (300, 300, 64, 16, False)
