@@ -295,8 +295,9 @@ int obs_set_decode_path(obs_ctx* ctx, int path);
 /* Waits for the stream, then reports (OBS_E_HIP + message) and clears a
  * device-side failure: a bounded wait that timed out in the fused decode
  * path, the fused attention half or the grouped prefill's one-launch expert
- * FFN, or (OBS_E_INVALID) a page id, length or slot out of range that a call
- * on a paged cache met; OBS_OK otherwise. The reference never checks GPU status. */
+ * FFN, or (OBS_E_INVALID) a page id, length, slot or entry past
+ * obs_attn_prep_paged's positions that a call on a paged cache met; OBS_OK
+ * otherwise. The reference never checks GPU status. */
 int obs_device_status(obs_ctx* ctx);
 
 /* Dispatch facts and the one-launch paths they allow (no reference
@@ -524,7 +525,9 @@ typedef struct obs_kv_weight {
  * 448 to 448). q, k, v: bf16 rows of q_ld, kv_ld elements (multiples of 8; 0 =
  * dense), 16-byte aligned, so they may be column ranges of one projection's
  * output; q_out rows of q_out_ld (q_out may be q if q_out_ld == q_ld).
- * rope_len: positions lie in [0, rope_len); a row at another one writes nothing.
+ * rope_len: positions lie in [0, rope_len). A row at another one writes nothing (its
+ * entry and q_out stay as they were): with pos that is how a caller leaves rows out;
+ * with pos NULL the entry counts as one out of range, and obs_device_status reports it.
  * The context's RoPE table is built on the first call of a theta and length (run
  * one before a capture). n_heads a multiple of n_kv, at most 16 per kv head.
  * Two rows of a call must not name the same entry of a page. */

@@ -9,8 +9,8 @@
 
 namespace obs {
 
-// Word of obs_ctx::status_dev (behind the one-launch FFN's): a page id, length
-// or slot out of range that a kernel met.
+// Word of obs_ctx::status_dev (behind the one-launch FFN's): a page id, length,
+// entry past the positions or slot out of range that a kernel met.
 constexpr uint32_t CTX_ST_PAGED = 2;
 static_assert(CTX_ST_PAGED > CTX_ST_FFN_SCHED && CTX_ST_PAGED < CTX_ST_WORDS, "a word of its own");
 int paged_status(obs_ctx* ctx);  // reads and clears it (obs_device_status)

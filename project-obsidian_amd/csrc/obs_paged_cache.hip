@@ -143,7 +143,11 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
   if (t == rs.r0 && tid == 0u && paged_len_bad(a, b)) paged_flag(a.status);
   const int32_t entry = static_cast<int32_t>(n) - static_cast<int32_t>(uniform(rs.r1) - t);
   const int32_t pos = p.pos ? static_cast<int32_t>(uniform(static_cast<uint32_t>(p.pos[t]))) : entry;
-  if (pos < 0 || static_cast<uint32_t>(pos) >= p.rope_len) return;  // uniform
+  if (pos < 0 || static_cast<uint32_t>(pos) >= p.rope_len) {  // uniform
+    // without positions of the caller's own it is the length that is out of range
+    if (!p.pos && entry >= 0 && tid == 0u) paged_flag(a.status);
+    return;
+  }
   float cs[8], sn[8];  // of the lane's pairs: columns c0 .. c0 + 7 modulo HD / 2
   {
     const float* tab = p.rope + static_cast<size_t>(pos) * 128u + (HD == 128u ? 16u : 32u) * (m % (LPH / 2u));

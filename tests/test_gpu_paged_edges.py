@@ -1,0 +1,57 @@
+"""Calls on the paged cache (obs_attn_prep_paged, obs_sdpa_paged_prefill, obs_kv_evict,
+obs_device_status) that the documentation allows and that are easily answered
+wrongly: positions past the RoPE table's, far positions, tables that grow,
+padded batches, several device failures at once. Helpers, pools and bars as in
+test_gpu_paged.py; a test that needs another bar derives it beside it."""
+import numpy as np
+import pytest
+
+import obsidian_hip as oh
+from obsidian_hip import synth
+from test_gpu_paged import (E4M3, EPS, FILL16, NAN16, SHAPES, THETA, Pool, _attend, _bf16, _check_prep, _e4m3_bytes, _f64, _kept,
+                            _prep_case, _rope64, _visible)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- positions ------------------------------------------------------------------
+
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16, False), (8, 1, 128, 32, True), (12, 2, 64, 64, True)], ids=str)
+def test_entries_past_the_positions_are_reported(exe, shape, one):
+    """pos NULL: a row whose entry lies at or past rope_len writes nothing, as one whose length
+    is out of range, and that is reported once; a batch that ends right at rope_len is clean."""
+    lens = [40, 64, 65, 0] if one else [40, 64, 70, 0]
+    new = [1] * 4 if one else [40, 10, 12, 0]
+    a = _prep_case(exe, shape, lens, new, 151, rope_len=64, one=one)
+    with pytest.raises(oh.ObsError, match="paged cache") as ei:
+        exe.device_status()
+    assert ei.value.code == oh.OBS_E_INVALID
+    exe.device_status()
+    _check_prep(*a, lens, new, rope_len=64)
+    lens[2] = 64
+    a = _prep_case(exe, shape, lens, new, 151, rope_len=64, one=one)
+    exe.device_status()
+    _check_prep(*a, lens, new, rope_len=64)
+
+
+def test_many_rows_past_the_positions_are_reported(exe):
+    """The same in the form that takes one wave a row."""
+    lens, new = [1100, 30], [1100, 30]
+    a = _prep_case(exe, (32, 4, 64, 16, False), lens, new, 153, rope_len=1099)
+    with pytest.raises(oh.ObsError, match="paged cache"):
+        exe.device_status()
+    _check_prep(*a, lens, new, rope_len=1099)
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_prompt_rows_with_positions_of_their_own(exe, shape):
+    """Ragged prompts behind an eviction: positions ahead of the entries, and rows whose own position
+    is outside [0, rope_len) write nothing (that is how a caller leaves rows out; not reported)."""
+    lens, new = [40, 3, 0, 17, 200], [40, 3, 0, 1, 130]
+    rng = np.random.default_rng(157)
+    pos = rng.integers(0, 9000, sum(new))
+    pos[[0, 5, 70]], pos[[41, 100]] = [9000, 2**31 - 1, 9001], [-1, -2**31]
+    a = _prep_case(exe, shape, lens, new, 157, pos=pos, pad_rows=1)
+    exe.device_status()
+    _check_prep(*a, lens, new, pos=[int(p) for p in pos])
