@@ -199,10 +199,12 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
     const float inv = 1.0f / __builtin_sqrtf(ss / static_cast<float>(HD) + p.eps);
     float nvs[8], r[8];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {  // rounded as the stored q / k would be
-      const uint32_t pr = pack_bf16_pair_rne((bf16lo(xw[i]) * inv) * bf16lo(ww[i]), (bf16hi(xw[i]) * inv) * bf16hi(ww[i]));
-      nvs[2 * i] = bf16lo(pr);
-      nvs[2 * i + 1] = bf16hi(pr);
+    for (uint32_t i = 0; i < 4; ++i) {
+      const float n0 = (bf16lo(xw[i]) * inv) * bf16lo(ww[i]), n1 = (bf16hi(xw[i]) * inv) * bf16hi(ww[i]);
+      // what becomes bf16 is rounded as the stored q / k would be; a key in e4m3 only at its end
+      const uint32_t pr = pack_bf16_pair_rne(n0, n1);
+      nvs[2 * i] = F8 && !is_q ? n0 : bf16lo(pr);
+      nvs[2 * i + 1] = F8 && !is_q ? n1 : bf16hi(pr);
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {

@@ -55,3 +55,26 @@ def test_prompt_rows_with_positions_of_their_own(exe, shape):
     a = _prep_case(exe, shape, lens, new, 157, pos=pos, pad_rows=1)
     exe.device_status()
     _check_prep(*a, lens, new, pos=[int(p) for p in pos])
+
+
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16, True), (16, 16, 64, 32, True), (12, 2, 64, 64, True)], ids=str)
+@pytest.mark.parametrize("rows", [60, 1030])
+def test_e4m3_keys_are_rounded_once(exe, shape, rows):
+    """A key in e4m3 is the nearest to the exact value over the scale, but where the fp32
+    arithmetic's own error reaches over the middle between two. That error: at most 32 roundings
+    of 2^-24 behind each of the two products (the sum of squares as a tree of 11 levels, root,
+    quotient, two products; cosine, product, difference, division), and the angle's 2^-23 p."""
+    nh, nkv, hd, page, _ = shape
+    pos = np.arange(rows) % 61
+    pool, _, x, _, kn, _, _, _ = _prep_case(exe, shape, [rows], [rows], 163, pos=pos)
+    exe.device_status()
+    k, f, s = pool.dk.download(), _f64(x), pool.ks.astype(np.float64)[:, None]
+    for r in range(rows):
+        y = f[r, nh * hd:(nh + nkv) * hd].reshape(nkv, hd)
+        ref, _ = _rope64(y, _f64(kn), int(pos[r]))
+        y = y / np.sqrt(np.mean(y * y, -1, keepdims=True) + EPS) * _f64(kn)
+        turn = np.concatenate([np.abs(y[:, :hd // 2]) + np.abs(y[:, hd // 2:])] * 2, -1)
+        err = (2.0 ** -19 + 2.0 ** -23 * pos[r]) * turn
+        got = E4M3[k[pool.table[0, r // page], :, r % page]]
+        lo, hi = E4M3[_e4m3_bytes((ref - err) / s)], E4M3[_e4m3_bytes((ref + err) / s)]
+        assert np.all((lo <= got) & (got <= hi)), (r, np.sum((lo > got) | (got > hi)))
