@@ -18,6 +18,16 @@ int paged_status(obs_ctx* ctx);  // reads and clears it (obs_device_status)
 constexpr uint32_t PAGED_MAX_SEQS = 4096;
 constexpr uint64_t PAGED_MAX_ENTRIES = 1ull << 30;
 
+// Positions of the RoPE table that a call with rope_len takes: a power of two, 8,192
+// at least. Tables are built with a wait and kept (graphs read them), so a caller
+// whose rope_len follows its longest sequence must not get one a step.
+constexpr uint32_t ROPE_ROWS_MIN = 8192;
+inline uint32_t rope_rows(uint32_t rope_len) {
+  uint32_t n = ROPE_ROWS_MIN;
+  while (n < rope_len) n *= 2u;  // rope_len <= 2^24
+  return n;
+}
+
 // Makes the context's device current for a call's launches (a caller may work
 // on another one).
 struct DeviceGuard {

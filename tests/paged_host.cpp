@@ -30,5 +30,6 @@ void entry(const int32_t* table, const int32_t* len, const int32_t* row, uint32_
   out[0] = id; out[1] = ok; out[2] = obsd::paged_len(a, b); out[3] = obsd::paged_len_bad(a, b);
   out[4] = r.r0; out[5] = r.r1;
 }
+uint32_t rope_rows(uint32_t rope_len) { return obs::rope_rows(rope_len); }
 uint32_t seen(uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks) { return obsd::seen_bits(t, hi, lo, sinks); }
 }

@@ -78,3 +78,37 @@ def test_e4m3_keys_are_rounded_once(exe, shape, rows):
         got = E4M3[k[pool.table[0, r // page], :, r % page]]
         lo, hi = E4M3[_e4m3_bytes((ref - err) / s)], E4M3[_e4m3_bytes((ref + err) / s)]
         assert np.all((lo <= got) & (got <= hi)), (r, np.sum((lo > got) | (got > hi)))
+
+
+# ---- the RoPE table ---------------------------------------------------------------
+
+def test_a_growing_rope_len_needs_no_new_table():
+    """A caller that passes its present longest position as rope_len: no call up to the next
+    power of two builds a table, so the calls can be captured (building one cannot be)."""
+    nh, nkv, hd, page = 32, 4, 128, 16
+    with oh.ObsidianExecutor(0) as exe:
+        rng = np.random.default_rng(167)
+        pool = Pool(exe, rng, [60], nkv, hd, page, False)
+        ld = (nh + 2 * nkv) * hd
+        x, q = exe.upload(synth.bf16_normal(rng, (1, ld), 2.0)), exe.alloc((1, nh, hd), np.uint16)
+        qn, kn = exe.upload(synth.norm_weight(rng, hd)), exe.upload(synth.norm_weight(rng, hd))
+
+        def step(rope_len):
+            exe.attn_prep_paged(pool.kv, pool.seqs(), x.ptr, x.ptr + 2 * nh * hd, x.ptr + 2 * (nh + nkv) * hd, qn, kn, q, nh, EPS,
+                                THETA, rope_len, q_ld=ld, kv_ld=ld)
+
+        for first, later in ((100, (101, 4000, 8192)), (8193, (8194, 16384, 100))):
+            step(first)
+            want = q.download()
+            for n in later:
+                q.upload(np.full((1, nh, hd), FILL16, np.uint16))
+                exe.sync()
+                exe.capture_begin()
+                try:
+                    step(n)
+                finally:
+                    g = exe.capture_end()
+                exe.graph_launch(g)
+                exe.device_status()
+                exe.graph_destroy(g)
+                assert np.array_equal(q.download(), want)

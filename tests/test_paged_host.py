@@ -269,3 +269,13 @@ def test_masks_of_a_block(host, t):
             for sinks in [*edges, 0xffffffff]:
                 ref = sum(1 << j for j in range(32) if t + j < hi and (t + j >= lo or t + j < sinks))
                 assert host.seen(C.c_uint32(t), C.c_uint32(hi), C.c_uint32(lo), C.c_uint32(sinks)) == ref, (hi, lo, sinks)
+
+
+def test_rope_tables_grow_by_doubling(host):
+    """Whatever lengths a caller goes through, it meets few tables, each holding all of its positions."""
+    host.rope_rows.restype = C.c_uint32
+    assert [host.rope_rows(n) for n in (1, 8191, 8192, 8193, 16384, 16385)] == [8192, 8192, 8192, 16384, 16384, 32768]
+    sizes = {host.rope_rows(n) for n in [*range(1, 70000, 13), 1 << 20, (1 << 24) - 1, 1 << 24]}
+    assert sizes == {1 << i for i in (13, 14, 15, 16, 17, 20, 24)}
+    for n in (1, 4097, 8193, 100_003, (1 << 23) + 1, 1 << 24):
+        assert n <= host.rope_rows(n) <= max(8192, 2 * n - 1)
