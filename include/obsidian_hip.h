@@ -520,11 +520,12 @@ typedef struct obs_kv_weight {
  * (eps), NeoX RoPE at pos[row] (NULL: at the row's entry index; entries that an
  * eviction moved keep the rotation they were stored with, so such a sequence
  * needs pos), q to q_out, k and v to their entries, weight (nullable) of those
- * entries set to 0. bf16 results are obs_attn_prep_rows' bit for bit; e4m3 ones
- * are rounded once from the fp32 value over the scale (to nearest even, beyond
- * 448 to 448). q, k, v: bf16 rows of q_ld, kv_ld elements (multiples of 8; 0 =
- * dense), 16-byte aligned, so they may be column ranges of one projection's
- * output; q_out rows of q_out_ld (q_out may be q if q_out_ld == q_ld).
+ * entries set to 0. bf16 results are obs_attn_prep_rows' bit for bit at positions
+ * below 8,192; from there on the angle is formed in double, where that call rounds
+ * it to fp32. e4m3 ones are rounded once from the fp32 value over the scale (to
+ * nearest even, beyond 448 to 448). q, k, v: bf16 rows of q_ld, kv_ld elements
+ * (multiples of 8; 0 = dense), 16-byte aligned, so they may be column ranges of one
+ * projection's output; q_out rows of q_out_ld (q_out may be q if q_out_ld == q_ld).
  * rope_len: positions lie in [0, rope_len). A row at another one writes nothing (its
  * entry and q_out stay as they were): with pos that is how a caller leaves rows out;
  * with pos NULL the entry counts as one out of range, and obs_device_status reports it.

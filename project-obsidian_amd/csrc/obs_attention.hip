@@ -12,6 +12,9 @@
 // Caches (bf16): keys [n_kv, max_len, head_dim] as the reference lays them
 // out (kv_cache.rs:3), values transposed [n_kv, head_dim, max_len] so that the
 // attention's value operand reads consecutive positions of one dimension.
+
+#include <algorithm>
+
 #include "obs_internal.hpp"
 
 namespace {
@@ -998,15 +1001,18 @@ __global__ void __launch_bounds__(256) argmax_final_kernel(const unsigned long l
 constexpr uint32_t ARGMAX_PARTS = 256;
 
 // RoPE table entry (p, i) = (cos, sin) of fl32(p * fl32(theta^(-2i/128))), each
-// in double and rounded once: the values attn_prep_kernel computes.
-__global__ void __launch_bounds__(256) rope_table_kernel(float* __restrict__ table, uint32_t max_len, float theta) {
+// in double and rounded once: the values attn_prep_kernel computes. From position
+// exact_from on the angle is not rounded.
+__global__ void __launch_bounds__(256) rope_table_kernel(float* __restrict__ table, uint32_t max_len, float theta,
+                                                         uint32_t exact_from) {
   const uint32_t e = blockIdx.x * 256u + threadIdx.x;
   if (e >= max_len * 64u) return;
   const uint32_t p = e / 64u, i = e % 64u;
-  const float f = static_cast<float>(pow(static_cast<double>(theta), -2.0 * static_cast<double>(i) / 128.0));
-  const float angle = static_cast<float>(p) * f;
-  table[2u * e] = static_cast<float>(cos(static_cast<double>(angle)));
-  table[2u * e + 1u] = static_cast<float>(sin(static_cast<double>(angle)));
+  const double f = pow(static_cast<double>(theta), -2.0 * static_cast<double>(i) / 128.0);
+  const float near = static_cast<float>(p) * static_cast<float>(f);
+  const double angle = p < exact_from ? static_cast<double>(near) : static_cast<double>(p) * f;
+  table[2u * e] = static_cast<float>(cos(angle));
+  table[2u * e + 1u] = static_cast<float>(sin(angle));
 }
 
 uint32_t sdpa_splits(uint32_t max_len) {
@@ -1018,9 +1024,10 @@ uint32_t sdpa_splits(uint32_t max_len) {
 
 namespace obs {
 
-int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out) {
+int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out, uint32_t exact_from) {
+  exact_from = std::min(exact_from, max_len);
   for (const auto& r : ctx->rope_tables)
-    if (r.theta == theta && r.len >= max_len) {
+    if (r.theta == theta && r.len >= max_len && std::min(r.exact_from, max_len) == exact_from) {
       *out = r.table;
       return OBS_OK;
     }
@@ -1031,14 +1038,14 @@ int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float**
                      static_cast<double>(theta), max_len);
   float* t = nullptr;
   OBS_HIP_TRY(ctx, hipMalloc(&t, sizeof(float) * 128u * max_len));
-  rope_table_kernel<<<(max_len * 64u + 255u) / 256u, 256, 0, ctx->stream>>>(t, max_len, theta);
+  rope_table_kernel<<<(max_len * 64u + 255u) / 256u, 256, 0, ctx->stream>>>(t, max_len, theta, exact_from);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
   if (e != hipSuccess) {
     (void)hipFree(t);
     return set_error(ctx, OBS_E_HIP, "RoPE table: %s", hipGetErrorString(e));
   }
-  ctx->rope_tables.push_back({t, max_len, theta});
+  ctx->rope_tables.push_back({t, max_len, theta, exact_from});
   *out = t;
   return OBS_OK;
 }

@@ -53,6 +53,7 @@ struct obs_ctx {
     float* table;
     uint32_t len;
     float theta;
+    uint32_t exact_from;  // the angle in double from this position on (len: nowhere)
   };
   std::vector<rope_entry> rope_tables;
   // decode workspaces replaced by larger ones, kept for the same reason
@@ -195,9 +196,9 @@ int layer_fused_status(obs_ctx* ctx);
 
 // The context's RoPE table for (theta, max_len) (obs_attention.hip): entry
 // [p][i] = (cos, sin) of fl32(p * fl32(theta^(-2i/128))), each evaluated in
-// double and rounded once (attn_prep_kernel's values). Built on first use
-// (not under graph capture).
-int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out);
+// double and rounded once (attn_prep_kernel's values); from position exact_from
+// on, of theta^(-2i/128) p in double. Built on first use (not under graph capture).
+int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out, uint32_t exact_from = 0xffffffffu);
 
 }  // namespace obs
 

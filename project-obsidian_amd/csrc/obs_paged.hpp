@@ -22,6 +22,10 @@ constexpr uint64_t PAGED_MAX_ENTRIES = 1ull << 30;
 // at least. Tables are built with a wait and kept (graphs read them), so a caller
 // whose rope_len follows its longest sequence must not get one a step.
 constexpr uint32_t ROPE_ROWS_MIN = 8192;
+// From here on the table's angles are formed in double: the fp32 product of
+// obs_attn_prep_rows is off by up to 2^-24 of the angle twice, 0.0003 at 8,192, but
+// 0.004 at 100,000 and 0.035 at 10^6, beside bf16's half step of 0.002.
+constexpr uint32_t ROPE_EXACT_FROM = 8192;
 inline uint32_t rope_rows(uint32_t rope_len) {
   uint32_t n = ROPE_ROWS_MIN;
   while (n < rope_len) n *= 2u;  // rope_len <= 2^24

@@ -112,3 +112,58 @@ def test_a_growing_rope_len_needs_no_new_table():
                 exe.device_status()
                 exe.graph_destroy(g)
                 assert np.array_equal(q.download(), want)
+
+
+FAR = [8191, 8192, 8193, 100_003, 1_000_000, (1 << 20) - 1]
+
+
+@pytest.mark.parametrize("shape", [(32, 4, 128, 16, False), (16, 16, 64, 32, False), (8, 1, 128, 16, True)], ids=str)
+@pytest.mark.parametrize("one", [True, False])
+def test_far_positions(exe, shape, one):
+    """Rotations at positions up to 2^20 against 64 bits, with a bar that does not grow with the
+    position: below 8,192 the angle is an fp32 product of two fp32 factors, the largest of which
+    with a rounding is 0.78: 2^13 0.78 2^-23 < 2^-10; from there on it is formed in double, and the
+    rounded cosine and sine (2^-24 of each) are within 2^-20 like the other fp32 steps."""
+    nh, nkv, hd, page, f8 = shape
+    new = [1] * len(FAR) if one else [1, 30, 1, 2, 40, 1]
+    lens = [20, 33, 1, 500, 64, 17]
+    rows = np.concatenate([[0], np.cumsum(new)]).astype(int)
+    pos = np.concatenate([p + 1 - np.arange(t, 0, -1) for p, t in zip(FAR, new)])
+    pool, rows, x, qn, kn, q_out, w0, dw = _prep_case(exe, shape, lens, new, 173, pos=pos, rope_len=1 << 20, one=one)
+    exe.device_status()
+    got, k, f = _f64(q_out.download()), pool.dk.download(), _f64(x)
+    for b, (n, t) in enumerate(zip(lens, new)):
+        for r in range(t):
+            row, e = rows[b] + r, n - t + r
+            turn_err = 2.0 ** -10 if pos[row] < 8192 else 0.0
+            for y, w, g in ((f[row, :nh * hd].reshape(nh, hd), qn, got[row]),
+                            (f[row, nh * hd:(nh + nkv) * hd].reshape(nkv, hd), kn, k[pool.table[b, e // page], :, e % page])):
+                ref, _ = _rope64(y, _f64(w), int(pos[row]))
+                y = y / np.sqrt(np.mean(y * y, -1, keepdims=True) + EPS) * _f64(w)
+                turn = np.concatenate([np.abs(y[:, :hd // 2]) + np.abs(y[:, hd // 2:])] * 2, -1)
+                pre = (2.0 ** -8 + 2.0 ** -20 + turn_err) * turn  # the normed value's rounding, the fp32 steps
+                lim = pre + 2.0 ** -8 * (np.abs(ref) + pre)
+                if w is kn and f8:
+                    s = pool.ks.astype(np.float64)[:, None]
+                    g, ref = E4M3[g] * s, np.clip(ref, -448 * s, 448 * s)
+                    lim = pre + 2.0 ** -4 * (np.abs(ref) + pre) + 2.0 ** -10 * s
+                elif w is kn:
+                    g = _f64(g)
+                assert np.all(np.abs(g - ref) <= lim), (b, r, int(pos[row]), np.max(np.abs(g - ref)))
+
+
+@pytest.mark.parametrize("rope_len", [8192, 1 << 20])
+def test_near_positions_equal_the_contiguous_cache(exe, rope_len):
+    """Below 8,192 q and keys are obs_attn_prep_rows' bit for bit, whatever rope_len."""
+    nh, nkv, hd, page, T, ml = 32, 4, 128, 32, 60, 8192
+    pos0 = ml - T
+    a = _prep_case(exe, (nh, nkv, hd, page, False), [T], [T], 179, pos=np.arange(pos0, ml), rope_len=rope_len, weight=False)
+    pool, _, x, qn, kn, q_out = a[:6]
+    ld, dx = x.shape[1], exe.upload(x)
+    kc, vc = exe.zeros((nkv, ml, hd), np.uint16), exe.zeros((nkv, hd, ml), np.uint16)
+    exe.attn_prep_rows(dx.ptr, dx.ptr + 2 * nh * hd, dx.ptr + 2 * (nh + nkv) * hd, exe.upload(qn), exe.upload(kn), kc, vc, nh,
+                       nkv, hd, ml, EPS, THETA, pos0, T, ld, ld)
+    assert np.array_equal(dx.download()[:, :nh * hd].reshape(T, nh, hd), q_out.download())
+    j = np.arange(T)
+    p, o = pool.table[0, j // page], j % page
+    assert np.array_equal(kc.download()[:, pos0 + j].transpose(1, 0, 2), pool.dk.download()[p, :, o])
