@@ -510,7 +510,7 @@ typedef struct obs_paged_seqs {
 /* Attention weight gathered by entries: w fp32 [n_slots, n_kv, ld], sequence b
  * of a call in slot[b] (NULL: slot b), ld >= max_pages * page of the call. The
  * slots of a call's sequences are distinct; a slot outside [0, n_slots) gathers
- * nothing and is reported like a page id. */
+ * nothing and, if its sequence has entries, is reported like a page id. */
 typedef struct obs_kv_weight {
   float* w; const int32_t* slot;
   uint32_t n_slots, ld;

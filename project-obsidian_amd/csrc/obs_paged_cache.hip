@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
   const uint32_t n = uniform(paged_len(a, b)), now = umin(n, budget);
   const int64_t slot = weight_slot(w, b), dslot = weight_slot(wd, b);
   if (tid == 0u) {
-    if (paged_len_bad(a, b) || slot < 0 || dslot < 0) paged_flag(a.status);
+    if (paged_len_bad(a, b) || (n > 0u && (slot < 0 || dslot < 0))) paged_flag(a.status);  // (a padded batch needs no slots)
     if (h == 0u) new_len[b] = static_cast<int32_t>(now);
   }
   const float* src = w.w + (static_cast<size_t>(max(slot, int64_t(0))) * a.n_kv + h) * w.ld;

@@ -167,3 +167,38 @@ def test_near_positions_equal_the_contiguous_cache(exe, rope_len):
     j = np.arange(T)
     p, o = pool.table[0, j // page], j % page
     assert np.array_equal(kc.download()[:, pos0 + j].transpose(1, 0, 2), pool.dk.download()[p, :, o])
+
+
+# ---- padded batches and several reports --------------------------------------------
+
+@pytest.mark.parametrize("slots", [[-1, 0, 1, 9], None], ids=["slots", "no slots"])
+def test_evict_of_a_padded_batch(exe, slots):
+    """Sequences without entries keep nothing and need no slot, in the eviction as in the append
+    and the attention: nothing is reported. One with entries and no slot is."""
+    nkv, hd, page, budget = 2, 64, 16, 50
+    rng = np.random.default_rng(181)
+    lens = [0, 300, 40, -3] if slots else [300, 40, 0, -3]
+    pool = Pool(exe, rng, lens, nkv, hd, page, False, extra=4 * 4)
+    cap = pool.max_pages * page
+    w = rng.random((2, nkv, cap)).astype(np.float32)
+    kept, new_len = exe.upload(np.full((4, nkv, budget), 77, np.int32)), exe.upload(np.full(4, 77, np.int32))
+    dwd = exe.upload(np.full((2, nkv, budget), 5.5, np.float32))
+    ds = None if slots is None else exe.upload(np.array(slots, np.int32))
+    dst = exe.upload(pool.free[:16].reshape(4, 4).copy())
+
+    def call():
+        exe.kv_evict(pool.kv, pool.seqs(), oh.KvWeight(exe.upload(w), 2, cap, ds), dst, 4, oh.KvWeight(dwd, 2, budget, ds), 4, 10,
+                     budget, kept, new_len)
+
+    call()
+    exe.device_status()
+    gk = kept.download()
+    assert list(new_len.download()) == [min(max(n, 0), budget) for n in lens]
+    for b, n in enumerate(lens):
+        for h in range(nkv):
+            ref = _kept(w[b if slots is None else slots[b], h], n, 4, 10, budget) if n > 0 else np.arange(0)
+            assert np.array_equal(gk[b, h], np.concatenate([ref, np.full(budget - len(ref), -1)]))
+    pool.dl.upload(np.array([1] * 4, np.int32))  # now all have an entry
+    call()
+    with pytest.raises(oh.ObsError, match="paged cache"):
+        exe.device_status()
