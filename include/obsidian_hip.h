@@ -296,8 +296,8 @@ int obs_set_decode_path(obs_ctx* ctx, int path);
  * device-side failure: a bounded wait that timed out in the fused decode
  * path, the fused attention half or the grouped prefill's one-launch expert
  * FFN, or (OBS_E_INVALID) a page id, length, slot or entry past
- * obs_attn_prep_paged's positions that a call on a paged cache met; OBS_OK
- * otherwise. The reference never checks GPU status. */
+ * obs_attn_prep_paged's positions that a call on a paged cache met (behind a
+ * time-out the next call reports that one); OBS_OK otherwise. The reference never checks GPU status. */
 int obs_device_status(obs_ctx* ctx);
 
 /* Dispatch facts and the one-launch paths they allow (no reference

@@ -489,8 +489,9 @@ int obs_device_status(obs_ctx* ctx) {
   const int c = ctx->scratch_used ? obs::fused_decode_status_ws(ctx, ctx->scratch) : OBS_OK;
   const int f = obs::ffn_status(ctx);
   const int l = obs::layer_fused_status(ctx);
-  const int p = obs::paged_status(ctx);
-  return a != OBS_OK ? a : b != OBS_OK ? b : c != OBS_OK ? c : f != OBS_OK ? f : l != OBS_OK ? l : p;
+  const int w = a != OBS_OK ? a : b != OBS_OK ? b : c != OBS_OK ? c : f != OBS_OK ? f : l;
+  // behind a time-out the paged cache's report stays for the next call: it has a code and message of its own
+  return w != OBS_OK ? w : obs::paged_status(ctx);
 }
 
 }  // extern "C"

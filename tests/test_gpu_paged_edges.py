@@ -202,3 +202,32 @@ def test_evict_of_a_padded_batch(exe, slots):
     call()
     with pytest.raises(oh.ObsError, match="paged cache"):
         exe.device_status()
+
+
+def test_two_failures_are_reported_one_after_the_other():
+    """A time-out of the grouped prefill (forced by its test hook) and a bad page id in one stretch of
+    work: each has its own report, code and message together, and neither takes the other away."""
+    E, H, I, K, T = 128, 2048, 768, 8, 64
+    rng = np.random.default_rng(191)
+    with oh.ObsidianExecutor(0) as exe:
+        layer = oh.MoeLayer.upload(exe, synth.moe_layer(41, E, H, I, 64))
+        cfg = oh.MoeConfig(E, K, H, I, 64, True)
+        ids, w = synth.zipf_routing(T, E, K, 1.1, seed=5)
+        ws_bytes = exe.moe_prefill_workspace(cfg, T)
+        ws, Y = exe.alloc(ws_bytes, np.uint8), exe.alloc((T, H), np.uint16)
+        exe.debug_ffn_wait(1, 200)
+        exe.moe_prefill(cfg, layer, exe.upload(synth.bf16_normal(rng, (T, H))), Y, T, ids=exe.upload(ids), weights=exe.upload(w),
+                        ws=ws, ws_bytes=ws_bytes)
+        pool = Pool(exe, rng, [40], 4, 128, 16, False)
+        pool.dt.upload(np.full_like(pool.table, -1))
+        q, out = exe.upload(synth.bf16_normal(rng, (1, 32, 128))), exe.alloc((1, 32, 128), np.uint16)
+        pws = exe.alloc(exe.sdpa_paged_workspace(pool.kv, pool.seqs(), 32), np.uint8)
+        exe.sdpa_paged_decode(pool.kv, pool.seqs(), q, out, 32, pws)
+        with pytest.raises(oh.ObsError, match="timed out") as ei:
+            exe.device_status()
+        assert ei.value.code == oh.OBS_E_HIP
+        with pytest.raises(oh.ObsError, match="paged cache") as ei:
+            exe.device_status()
+        assert ei.value.code == oh.OBS_E_INVALID
+        exe.device_status()
+        assert not np.any(out.download())  # nothing visible: zeros
