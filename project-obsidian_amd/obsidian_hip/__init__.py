@@ -628,9 +628,11 @@ class PagedKv:
 
 class PagedSeqs:
     """The sequences of a call (obs_paged_seqs): device arrays pages [n_seqs, max_pages], len [n_seqs]
-    and, for more than one token a sequence, row [n_seqs + 1]."""
+    and, for more than one token a sequence, row [n_seqs + 1] with n_rows."""
 
     def __init__(self, pages, len_, n_seqs: int, max_pages: int, n_rows: Optional[int] = None, row=None):
+        if row is not None and n_rows is None:
+            raise ValueError("PagedSeqs: n_rows is needed with row (the call's token rows)")
         self.held = (pages, len_, row)
         self.c = ObsPagedSeqs(_ptr(pages), _ptr(len_), _ptr(row), n_seqs, max_pages,
                               n_seqs if n_rows is None else n_rows)

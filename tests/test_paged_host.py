@@ -279,3 +279,11 @@ def test_rope_tables_grow_by_doubling(host):
     assert sizes == {1 << i for i in (13, 14, 15, 16, 17, 20, 24)}
     for n in (1, 4097, 8193, 100_003, (1 << 23) + 1, 1 << 24):
         assert n <= host.rope_rows(n) <= max(8192, 2 * n - 1)
+
+
+def test_a_batch_with_rows_names_their_number():
+    """PagedSeqs takes one row a sequence only where there is no row array: with one, the rows behind
+    the first n_seqs would be left out without a word."""
+    with pytest.raises(ValueError, match="n_rows"):
+        oh.PagedSeqs(A, A, 3, 4, row=A)
+    assert oh.PagedSeqs(A, A, 3, 4, 17, A).c.n_rows == 17 and oh.PagedSeqs(A, A, 3, 4).c.n_rows == 3
