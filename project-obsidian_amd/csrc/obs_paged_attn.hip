@@ -517,7 +517,7 @@ namespace obs {
 int check_attn(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs_paged_seqs* seqs,
                const obs_kv_weight* weight, const uint16_t* q, const uint16_t* out, uint32_t n_heads, uint32_t* q_ld,
                const void* ws, size_t ws_bytes, size_t need) {
-  if (!q || !out || !ws) return set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+  if (!q || !out || (!ws && need)) return set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
   if (weight) {
     const int rc = check_weight(ctx, who, weight, static_cast<uint64_t>(seqs->max_pages) * kv->page, true);
     if (rc != OBS_OK) return rc;

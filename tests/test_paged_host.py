@@ -287,3 +287,11 @@ def test_a_batch_with_rows_names_their_number():
     with pytest.raises(ValueError, match="n_rows"):
         oh.PagedSeqs(A, A, 3, 4, row=A)
     assert oh.PagedSeqs(A, A, 3, 4, 17, A).c.n_rows == 17 and oh.PagedSeqs(A, A, 3, 4).c.n_rows == 3
+
+
+def test_an_empty_batch_needs_no_workspace(ctx):
+    """A call gets by with exactly what obs_sdpa_paged_workspace names, which for no sequences may be nothing."""
+    n, none = C.c_size_t(7), _seqs(n_seqs=0, n_rows=0)
+    assert oh.lib().obs_sdpa_paged_workspace(ctx, _kv(), none, None, 32, 0, 0, C.byref(n)) == oh.OBS_OK
+    assert n.value == 0 and _decode(ctx, _kv(), none, ws=None, n=0) == oh.OBS_OK
+    assert _decode(ctx, _kv(), _seqs(), ws=None, n=0) == INV
