@@ -8,7 +8,7 @@ import pytest
 
 import obsidian_hip as oh
 from obsidian_hip import synth
-from test_gpu_paged import (E4M3, EPS, FILL16, NAN16, SHAPES, THETA, Pool, _attend, _bf16, _check_prep, _e4m3_bytes, _f64, _kept,
+from test_gpu_paged import (E4M3, EPS, FILL16, NAN16, SHAPES, THETA, Pool, _attend, _check_prep, _e4m3_bytes, _f64, _kept,
                             _prep_case, _rope64, _visible)
 
 pytestmark = pytest.mark.gpu
@@ -231,3 +231,41 @@ def test_two_failures_are_reported_one_after_the_other():
         assert ei.value.code == oh.OBS_E_INVALID
         exe.device_status()
         assert not np.any(out.download())  # nothing visible: zeros
+
+
+# ---- values that are not finite, in parts ------------------------------------------
+
+@pytest.mark.parametrize("shape,n,new,window,bad", [
+    # a window whose low edge and whose diagonal lie in different parts
+    ((32, 4, 128, 32, False), 3000, 100, 1000, [1910, 1920, 2970, 2990]),
+    ((16, 2, 64, 64, True), 3000, 100, 1000, [1910, 1920, 2970, 2990]),
+    # parts of more than 64 blocks: page ids are fetched twice
+    ((64, 64, 64, 16, False), 9000, 100, 0, [8905, 8950, 8999])], ids=str)
+def test_prefill_values_not_finite_in_parts(exe, shape, n, new, window, bad):
+    nh, nkv, hd, page, f8 = shape
+    rng = np.random.default_rng(193)
+    pool = Pool(exe, rng, [n], nkv, hd, page, f8)
+    k, v = pool.entries(0, "k"), pool.entries(0, "v")
+    for j in bad:
+        pool.v[pool.table[0, j // page], :, :, j % page] = 0x7F if f8 else (0x7F80 if j % 4 else NAN16)
+    pool.up()
+    q = synth.bf16_normal(rng, (new, nh, hd), 2.0)
+    out = exe.upload(np.full((new, nh, hd), FILL16, np.uint16))
+    seqs = pool.seqs([0, new])
+    ws = exe.upload(np.full(exe.sdpa_paged_workspace(pool.kv, seqs, nh, None, window, 0), 0xFF, np.uint8))
+    exe.sdpa_paged_prefill(pool.kv, seqs, exe.upload(q), out, nh, ws, window=window)
+    exe.device_status()
+    got = _f64(out.download())
+    clean = 0
+    for r in range(new):
+        vis = _visible(n - new + r, n, window, 0)
+        if any(vis[j] for j in bad):
+            assert not np.any(np.isfinite(got[r])), r
+            continue
+        clean += 1
+        if r % 5 and r not in (0, new - 1):
+            assert np.all(np.isfinite(got[r])), r
+            continue
+        ref, bound, _, _ = _attend(_f64(q[r]), k, v, vis)
+        assert np.all(np.abs(got[r] - ref) <= bound), r
+    assert clean == (50 if window else 5)  # the rows between the edges, or before the first bad entry
