@@ -501,7 +501,10 @@ typedef struct obs_paged_kv {
  * sequence, row b of sequence b, n_rows == n_seqs. Page ids of entries that a
  * call does not touch may be anything; an id outside [0, n_pages) that it needs
  * hides the page's entries, appends nothing there, and is reported by
- * obs_device_status (OBS_E_INVALID). At most 4,096 sequences, 2^30 entries each. */
+ * obs_device_status (OBS_E_INVALID). At most 4,096 sequences, 2^30 entries each.
+ * The host knows the lengths by max_pages * page only: the attention's workspace and
+ * its choice between whole sequences and parts follow that, so a table not much wider
+ * than the call's longest sequence is the fastest. */
 typedef struct obs_paged_seqs {
   const int32_t* pages; const int32_t* len; const int32_t* row;
   uint32_t n_seqs, max_pages, n_rows;

@@ -453,7 +453,10 @@ __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, W
 // ---------------------------------------------------------------------------
 constexpr uint32_t DECODE_MIN_CHUNK = 4;
 // Blocks up to which a sequence is one part where no weight is gathered (no join
-// then): parts and their join cost more up to 384 entries (one sequence of 256
+// then), by what the page table can hold, as the lengths are the device's: a table of
+// 32,768 entries takes one sequence of 256 from 6.6 to 9.0 us, 64 of 1,000 from 24.2 to
+// 30.4 and, with weights, 16 of up to 8,200 from 34.4 to 40.8 (the join's workgroups
+// are as many as the table has entries for). In tables as long as the sequences, parts and their join cost more up to 384 entries (one sequence of 256
 // 8.9 us in parts, 6.8 whole; of 384 8.9 and 8.2, of 512 8.9 and 9.4), more rows
 // fill the chip by themselves (48 of 512 12.8 and 11.7; 64 of 1,000 22.3 and
 // 19.7, of 2,000 32.3 and 34.6; 32 of 1,000 12.8 and 18.4), and blocks in e4m3

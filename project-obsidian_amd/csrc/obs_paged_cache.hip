@@ -286,7 +286,8 @@ __device__ __forceinline__ uint32_t group_scan(uint32_t v, uint32_t* s_w, uint32
 // kernel). The third step falls away where the second one's bin is kept whole.
 // Bound by latency and one CU's issue rate: 9.1 us for 8,192 entries (2.0 until
 // the weights are there, 3.5 for two steps, 2.1 for the places and stores),
-// 15.5 for 96 rows of up to 16,003.
+// 16 for 96 rows of up to 16,003, 91 for one sequence of 100,003 (seven segments,
+// three or four times each).
 __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weight w, Weight wd, uint32_t sinks,
                                                                  uint32_t recent, uint32_t budget,
                                                                  int32_t* __restrict__ kept,
@@ -552,8 +553,8 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
 
 // Waves a token row: four, or one where rows fill the chip and it goes at most five
 // times round the heads, as the chain to a row's entry and position then runs in
-// fewer waves (6,000 rows of 36 heads of 64: 38.0 us with four, 24.8 with one; of 36
-// heads of 128, nine times round, 31.2 and 32.3).
+// fewer waves (6,000 rows of 36 heads of 64: 32.0 us with four, 18.0 with one, of 14
+// heads 28.2 and 11.9; of 36 heads of 128, nine times round, one gains nothing).
 uint32_t prep_waves(uint32_t hd, uint32_t heads, uint32_t rows) { return heads * hd <= 2560u && rows >= 1024u ? 1u : 4u; }
 
 template <uint32_t HD, bool F8>
