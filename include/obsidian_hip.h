@@ -532,10 +532,9 @@ typedef struct obs_kv_weight {
  * rope_len: positions lie in [0, rope_len). A row at another one writes nothing (its
  * entry and q_out stay as they were): with pos that is how a caller leaves rows out;
  * with pos NULL the entry counts as one out of range, and obs_device_status reports it.
- * The context's RoPE table (512 bytes a position) is built, with a wait, by the first
- * call of a theta (run one before a capture), for rope_len rounded up to a power of
- * two of at least 8,192; a call past that builds another, and all are kept until the
- * context ends. n_heads a multiple of n_kv, at most 16 per kv head.
+ * A call for whose theta and rope_len the context has no RoPE table (512 bytes a
+ * position) builds one, with a wait (run it before a capture), of rope_len rounded up
+ * to a power of two of at least 8,192 positions; all are kept until the context ends. n_heads a multiple of n_kv, at most 16 per kv head.
  * Two rows of a call must not name the same entry of a page. */
 int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,
                         const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_norm,

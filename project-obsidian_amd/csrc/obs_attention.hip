@@ -1024,10 +1024,10 @@ uint32_t sdpa_splits(uint32_t max_len) {
 
 namespace obs {
 
-int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out, uint32_t exact_from) {
-  exact_from = std::min(exact_from, max_len);
+int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out, uint32_t exact_from,
+                      uint32_t build_len) {
   for (const auto& r : ctx->rope_tables)
-    if (r.theta == theta && r.len >= max_len && std::min(r.exact_from, max_len) == exact_from) {
+    if (r.theta == theta && r.len >= max_len && std::min(r.exact_from, max_len) == std::min(exact_from, max_len)) {
       *out = r.table;
       return OBS_OK;
     }
@@ -1036,6 +1036,8 @@ int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float**
   if (cs != hipStreamCaptureStatusNone)
     return set_error(ctx, OBS_E_INVALID, "RoPE table: run once before capturing (table for theta %g, %u positions)",
                      static_cast<double>(theta), max_len);
+  max_len = std::max(max_len, build_len);
+  exact_from = std::min(exact_from, max_len);
   float* t = nullptr;
   OBS_HIP_TRY(ctx, hipMalloc(&t, sizeof(float) * 128u * max_len));
   rope_table_kernel<<<(max_len * 64u + 255u) / 256u, 256, 0, ctx->stream>>>(t, max_len, theta, exact_from);

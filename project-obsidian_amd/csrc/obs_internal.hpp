@@ -197,8 +197,10 @@ int layer_fused_status(obs_ctx* ctx);
 // The context's RoPE table for (theta, max_len) (obs_attention.hip): entry
 // [p][i] = (cos, sin) of fl32(p * fl32(theta^(-2i/128))), each evaluated in
 // double and rounded once (attn_prep_kernel's values); from position exact_from
-// on, of theta^(-2i/128) p in double. Built on first use (not under graph capture).
-int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out, uint32_t exact_from = 0xffffffffu);
+// on, of theta^(-2i/128) p in double. Where none holds max_len positions, one is built
+// (not under graph capture), of build_len if that is more.
+int ensure_rope_table(obs_ctx* ctx, float theta, uint32_t max_len, const float** out, uint32_t exact_from = 0xffffffffu,
+                      uint32_t build_len = 0);
 
 }  // namespace obs
 

@@ -18,7 +18,7 @@ int paged_status(obs_ctx* ctx);  // reads and clears it (obs_device_status)
 constexpr uint32_t PAGED_MAX_SEQS = 4096;
 constexpr uint64_t PAGED_MAX_ENTRIES = 1ull << 30;
 
-// Positions of the RoPE table that a call with rope_len takes: a power of two, 8,192
+// Positions of the RoPE table that a call with rope_len builds: a power of two, 8,192
 // at least. Tables are built with a wait and kept (graphs read them), so a caller
 // whose rope_len follows its longest sequence must not get one a step.
 constexpr uint32_t ROPE_ROWS_MIN = 8192;

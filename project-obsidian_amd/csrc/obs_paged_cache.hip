@@ -682,7 +682,7 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
   if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   PrepArgs p{q, k, v, q_norm, k_norm, q_out, pos, nullptr, n_heads, rope_len, q_ld, kv_ld, q_out_ld, eps};
-  rc = obs::ensure_rope_table(ctx, theta, obs::rope_rows(rope_len), &p.rope, obs::ROPE_EXACT_FROM);
+  rc = obs::ensure_rope_table(ctx, theta, rope_len, &p.rope, obs::ROPE_EXACT_FROM, obs::rope_rows(rope_len));
   if (rc != OBS_OK) return rc;
   const Paged a = obs::paged_args(ctx, kv, seqs);
   const Weight w = obs::weight_args(weight);

@@ -114,6 +114,47 @@ def test_a_growing_rope_len_needs_no_new_table():
                 assert np.array_equal(q.download(), want)
 
 
+def test_a_table_that_is_long_enough_is_taken():
+    """A context that has a table for a call's positions, from the contiguous cache or the other way
+    round, needs no other one: such a first call can be captured."""
+    nh, nkv, hd, page, ml = 32, 4, 128, 16, 160
+    rng = np.random.default_rng(197)
+    ld = (nh + 2 * nkv) * hd
+    x0 = synth.bf16_normal(rng, (1, ld), 2.0)
+    norms = [synth.norm_weight(rng, hd) for _ in range(2)]
+    results = []
+    for order in ("paged last", "paged first"):
+        with oh.ObsidianExecutor(0) as exe:
+            pool = Pool(exe, np.random.default_rng(199), [60], nkv, hd, page, False)
+            seqs, q = pool.seqs(), exe.alloc((1, nh, hd), np.uint16)
+            qn, kn = (exe.upload(w) for w in norms)
+            kc, vc = exe.zeros((nkv, ml, hd), np.uint16), exe.zeros((nkv, hd, ml), np.uint16)
+            x, y = exe.upload(x0), exe.upload(x0)  # the contiguous call norms q in place
+
+            def paged():
+                exe.attn_prep_paged(pool.kv, seqs, x.ptr, x.ptr + 2 * nh * hd, x.ptr + 2 * (nh + nkv) * hd, qn, kn, q, nh, EPS, THETA,
+                                    100, q_ld=ld, kv_ld=ld)
+
+            def contiguous():
+                exe.attn_prep_rows(y.ptr, y.ptr + 2 * nh * hd, y.ptr + 2 * (nh + nkv) * hd, qn, kn, kc, vc, nh, nkv, hd, ml, EPS, THETA,
+                                   59, 1, ld, ld)
+
+            first, later = (contiguous, paged) if order == "paged last" else (paged, contiguous)
+            first()
+            exe.sync()
+            exe.capture_begin()
+            try:
+                later()
+            finally:
+                g = exe.capture_end()
+            exe.graph_launch(g)
+            exe.device_status()
+            exe.graph_destroy(g)
+            results += [q.download().reshape(-1), y.download()[0, :nh * hd]]
+    for r in results[1:]:
+        assert np.array_equal(r, results[0])
+
+
 FAR = [8191, 8192, 8193, 100_003, 1_000_000, (1 << 20) - 1]
 
 
