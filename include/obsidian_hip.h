@@ -482,13 +482,19 @@ int obs_sdpa_prefill(obs_ctx* ctx, const uint16_t* q, const uint16_t* k_cache, c
  * 16 to 256), head_dim 64 or 128. Keys [n_pages, n_kv, page, head_dim], values
  * transposed [n_pages, n_kv, head_dim, page], both 16-byte aligned, in bf16 or
  * in e4m3 (OCP, magnitudes up to 448) with one positive fp32 scale per kv head: an
- * entry is the stored value times the scale. */
-enum { OBS_KV_BF16 = 0, OBS_KV_E4M3 = 1 };
+ * entry is the stored value times the scale. Or in 4 bits (OBS_KV_Q4), affine in
+ * groups of 64 dims as the weights are: a dim is q * scale + bias, q in 0 .. 15,
+ * scale and bias bf16 (scales up to 2^120). A (page, kv head) of keys is then
+ * [page][head_dim / 2] bytes, byte i of an entry holding dim i in its low and dim
+ * i + head_dim / 2 in its high nibble, followed by uint32 [head_dim / 64][page], the
+ * scale in the low and the bias in the high half; one of values [head_dim / 2][page]
+ * such bytes and then the same: page * 9/16 head_dim bytes each. */
+enum { OBS_KV_BF16 = 0, OBS_KV_E4M3 = 1, OBS_KV_Q4 = 4 };
 typedef struct obs_paged_kv {
   void* k_pages; void* v_pages;
   const float* k_scale; const float* v_scale; /* [n_kv] under OBS_KV_E4M3, else unused */
   uint32_t n_pages, page, n_kv, head_dim;
-  int32_t dtype; /* OBS_KV_BF16 or OBS_KV_E4M3 */
+  int32_t dtype; /* OBS_KV_BF16, OBS_KV_E4M3 or OBS_KV_Q4 */
 } obs_paged_kv;
 
 /* The sequences of a call, read on the device (a captured call follows their
@@ -526,7 +532,10 @@ typedef struct obs_kv_weight {
  * entries set to 0. bf16 results are obs_attn_prep_rows' bit for bit at positions
  * below 8,192; from there on the angle is formed in double, where that call rounds
  * it to fp32. e4m3 ones are rounded once from the fp32 value over the scale (to
- * nearest even, beyond 448 to 448). q, k, v: bf16 rows of q_ld, kv_ld elements
+ * nearest even, beyond 448 to 448). In 4 bits the fp32 values of a group of 64 dims
+ * get scale = bf16((max - min) / 15), bias = bf16(min) and q = (x - bias) / scale
+ * to nearest even within 0 .. 15 (scale 0: q 0; a group with a value that is not
+ * finite reads as NaN). q, k, v: bf16 rows of q_ld, kv_ld elements
  * (multiples of 8; 0 = dense), 16-byte aligned, so they may be column ranges of one
  * projection's output; q_out rows of q_out_ld (q_out may be q if q_out_ld == q_ld).
  * rope_len: positions lie in [0, rope_len). A row at another one writes nothing (its
@@ -569,6 +578,7 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
  * j < sinks; a row whose i is negative (len shorter than its tokens) gets zeros.
  * A row is not touched by what other rows see, NaN and infinities included.
  * The rows' own keys and values are in the pages already (obs_attn_prep_paged).
+ * Entries of 4 bits enter the products rounded to bf16.
  * out bf16 [n_rows, n_heads, head_dim]; workspace as above. */
 int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const uint16_t* q,
                            uint16_t* out, uint32_t n_heads, uint32_t window, uint32_t sinks, uint32_t q_ld, void* ws,

@@ -88,6 +88,20 @@ struct PagedAttn {
   uint32_t nh, G, window, sinks, q_ld, vis, min_chunk, target, tiles;
   float scale_log2;
 };
+// What a pool holds, as the kernels' template argument.
+constexpr uint32_t KT_BF16 = 0, KT_E4M3 = 1, KT_Q4 = 2;
+// f with the pool's head_dim and kind as constants.
+template <typename F>
+int paged_shape(const obs_paged_kv* kv, F f) {
+  typedef std::integral_constant<uint32_t, 64u> D64;
+  typedef std::integral_constant<uint32_t, 128u> D128;
+  auto of = [&](auto t) { return kv->head_dim == 128u ? f(D128{}, t) : f(D64{}, t); };
+  switch (kv->dtype) {
+    case OBS_KV_E4M3: return of(std::integral_constant<uint32_t, KT_E4M3>{});
+    case OBS_KV_Q4: return of(std::integral_constant<uint32_t, KT_Q4>{});
+    default: return of(std::integral_constant<uint32_t, KT_BF16>{});
+  }
+}
 // Blocks of 32 that a token can see of a sequence of `entries`.
 inline uint64_t most_blocks(uint64_t entries, uint64_t window, uint32_t sinks) {
   const uint64_t all = (entries + 31u) / 32u;
@@ -192,6 +206,55 @@ __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
 }
 
+// Bytes of an entry in a (page, kv head) of keys or of values: head_dim nibbles and a
+// scale and bias (bf16, one word) a group of 64 dims under OBS_KV_Q4.
+template <uint32_t HD, uint32_t KT>
+constexpr uint32_t entry_bytes() {
+  return KT == obs::KT_Q4 ? HD / 2u + HD / 16u : KT == obs::KT_E4M3 ? HD : 2u * HD;
+}
+template <uint32_t HD, uint32_t KT>
+__device__ __forceinline__ size_t page_at(const obs::Paged& a, uint32_t page, uint32_t kv) {  // a (page, kv head), in bytes
+  return ((static_cast<size_t>(page) * a.n_kv + kv) << a.lp) * entry_bytes<HD, KT>();
+}
+// Nibbles of a word, byte i holding a low and a high one, as 16 + q in bf16: the
+// nibble in the top four of seven mantissa bits under the exponent of 16, so two of
+// them are a shift and an and-or, exact. J = 0: the low ones of bytes 0 and 2, 1: of
+// bytes 1 and 3, 2 and 3: the high ones.
+template <uint32_t J>
+__device__ __forceinline__ uint32_t q4_bf16(uint32_t w) {
+  const uint32_t x = J == 0u ? w << 3 : J == 1u ? w >> 5 : J == 2u ? w >> 1 : w >> 9;
+  return and_or(x, 0x00780078u, 0x41804180u);
+}
+// Eight low (or high) nibbles of two words, in the order 0, 2, 1, 3, 4, 6, 5, 7.
+template <bool HIGH>
+__device__ __forceinline__ bf16x8_v q4_bf16x8(uint32_t w0, uint32_t w1) {
+  constexpr uint32_t J = HIGH ? 2u : 0u;
+  return __builtin_bit_cast(bf16x8_v, u32x4_v{q4_bf16<J>(w0), q4_bf16<J + 1u>(w0), q4_bf16<J>(w1), q4_bf16<J + 1u>(w1)});
+}
+// Eight bf16 in q4_bf16x8's order.
+__device__ __forceinline__ u32x4_v q4_order(const u32x4_v& v) {
+  return u32x4_v{__builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.y, v.x, 0x07060302u),
+                 __builtin_amdgcn_perm(v.w, v.z, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u)};
+}
+// The low or high nibble of byte I.
+template <uint32_t I, bool HIGH>
+__device__ __forceinline__ float q4_nibble(uint32_t w) {
+  return static_cast<float>(w >> (8u * I + (HIGH ? 4u : 0u)) & 15u);
+}
+__device__ __forceinline__ float q4_value(float q, uint32_t par) { return __builtin_fmaf(q, bf16lo(par), bf16hi(par)); }
+// Scale and bias of a group whose least and largest values are lo and hi; `bits`: the
+// largest magnitude's, which shows a value that is not finite (the group then reads
+// as NaN). (max - min) / 15, by halves, so that it cannot overflow.
+__device__ __forceinline__ uint32_t q4_params(float lo, float hi, uint32_t bits) {
+  if (bits >= 0x7f800000u) return 0x7fc07fc0u;
+  return static_cast<uint32_t>(f32_to_bf16((0.5f * hi - 0.5f * lo) / 7.5f)) | static_cast<uint32_t>(f32_to_bf16(lo)) << 16;
+}
+__device__ __forceinline__ uint32_t q4_quant(float x, uint32_t par) {
+  const float s = bf16lo(par), q = __builtin_rintf((x - bf16hi(par)) / s);
+  // (a scale of zero or NaN: any q stands for the bias, or for NaN)
+  return s > 0.0f ? static_cast<uint32_t>(__builtin_fminf(__builtin_fmaxf(q, 0.0f), 15.0f)) : 0u;
+}
+
 // The entries of the block of 32 from entry t that are below hi, and at or above
 // lo or below sinks: a bit each. Arithmetic on whole words, no branch an entry.
 __host__ __device__ __forceinline__ uint32_t below_bits(uint32_t t, uint32_t end) {  // entries below `end`
@@ -236,6 +299,24 @@ __device__ __forceinline__ float wave_max_f32(float v) {  // uniform
   v = fmaxf(v, dpp_f32<DPP_HALF_MIRROR>(v));
   v = fmaxf(v, dpp_f32<DPP_MIRROR>(v));
   return fmaxf(fmaxf(readlane_f32(v, 0), readlane_f32(v, 16)), fmaxf(readlane_f32(v, 32), readlane_f32(v, 48)));
+}
+__device__ __forceinline__ uint32_t wave_max_u31(uint32_t v) {  // uniform; below 2^31
+  return static_cast<uint32_t>(wave_max_i32(static_cast<int>(v)));
+}
+__device__ __forceinline__ float half_max_f32(float v, uint32_t lane) {  // over a wave's half
+  v = fmaxf(v, dpp_f32<DPP_XOR1>(v));
+  v = fmaxf(v, dpp_f32<DPP_XOR2>(v));
+  v = fmaxf(v, dpp_f32<DPP_HALF_MIRROR>(v));
+  v = fmaxf(v, dpp_f32<DPP_MIRROR>(v));
+  return fmaxf(v, lane_xor16_f32(v, lane));
+}
+__device__ __forceinline__ uint32_t half_max_u32(uint32_t v, uint32_t lane) {
+  auto step = [](uint32_t x, float y) __attribute__((always_inline)) { return max(x, __float_as_uint(y)); };
+  v = step(v, dpp_f32<DPP_XOR1>(__uint_as_float(v)));
+  v = step(v, dpp_f32<DPP_XOR2>(__uint_as_float(v)));
+  v = step(v, dpp_f32<DPP_HALF_MIRROR>(__uint_as_float(v)));
+  v = step(v, dpp_f32<DPP_MIRROR>(__uint_as_float(v)));
+  return step(v, lane_xor16_f32(__uint_as_float(v), lane));
 }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) {
   return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(v)));

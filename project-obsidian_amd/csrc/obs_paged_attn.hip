@@ -5,6 +5,9 @@
 
 namespace {
 using namespace obsd;
+using obs::KT_BF16;
+using obs::KT_E4M3;
+using obs::KT_Q4;
 using obs::Paged;
 using obs::PagedAttn;
 using obs::Weight;
@@ -139,6 +142,159 @@ __device__ __forceinline__ void block_step(const Block<HD, F8, KEEP>& blk, const
 }
 
 // ---------------------------------------------------------------------------
+// The same over entries of 4 bits
+// ---------------------------------------------------------------------------
+// A dim is q s + b, so a group's share of a score is s sum(q Q) + b sum(Q) and of an
+// output sum(p s q) + sum(p b): the products take the nibbles themselves, as 16 + q
+// in bf16 (exact), and scales and biases meet them in fp32 a score, not a dim.
+//   score = s (sum((16 + q) Q)) + (b - 16 s) sum(Q)
+//   O = sum(w (16 + q)) - 24 sum(w) + sum(p (b + 8 s)),  w = bf16(p s)
+// w is the one rounding: the middle of the nibbles' range is split off with the
+// bias, so it weighs values of the size that the entries have, as P's does in bf16.
+// Bytes hold dims d (low) and d + HD / 2 (high): a lane's 16 bytes of a key (8 of a
+// head of 64) are two fragments of each half, its 8 bytes of a value row the eight
+// entries of two dims. Its scales and biases are those of its own eight scores.
+template <uint32_t HD, bool KEEP>
+struct Block4 {
+  static constexpr uint32_t NG = HD / 64u, NT = HD / 16u;
+  typedef typename std::conditional<HD == 128u, u32x4_v, u32x2_v>::type K;
+  K k[2];
+  u32x2_v v[NT / 2u];
+  u32x4_v kp[NG][2], vp[NG][2];  // scale and bias of entries 8 g .. 8 g + 7
+
+  // kid, eid: page ids of the lane's key rows and of its entries
+  __device__ __forceinline__ void load(const Paged& a, uint32_t kv, uint32_t kid, uint32_t eid, uint32_t t0, uint32_t col,
+                                       uint32_t g) {
+    const uint32_t mask = (1u << a.lp) - 1u, e = (t0 + 8u * g) & mask;
+    const uint8_t* kb = a.k + page_at<HD, KT_Q4>(a, kid, kv);
+#pragma unroll
+    for (uint32_t tt = 0; tt < 2; ++tt)
+      k[tt] = __builtin_nontemporal_load(reinterpret_cast<const K*>(
+          kb + ((t0 + 8u * (col / 4u) + 4u * tt + col % 4u) & mask) * (HD / 2u) + sizeof(K) * g));
+    const uint8_t* vb = a.v + page_at<HD, KT_Q4>(a, eid, kv);
+#pragma unroll
+    for (uint32_t nt = 0; nt < NT / 2u; ++nt) {
+      const u32x2_v* vr = reinterpret_cast<const u32x2_v*>(vb + ((16u * nt + col) << a.lp) + e);
+      if constexpr (KEEP)
+        v[nt] = *vr;
+      else
+        v[nt] = __builtin_nontemporal_load(vr);
+    }
+    const uint8_t* kw = a.k + page_at<HD, KT_Q4>(a, eid, kv) + (HD / 2u << a.lp) + 4u * e;
+    const uint8_t* vw = vb + (HD / 2u << a.lp) + 4u * e;
+#pragma unroll
+    for (uint32_t q = 0; q < NG; ++q)
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        kp[q][i] = *reinterpret_cast<const u32x4_v*>(kw + (4u * q << a.lp) + 16u * i);
+        vp[q][i] = *reinterpret_cast<const u32x4_v*>(vw + (4u * q << a.lp) + 16u * i);
+      }
+  }
+  // dims of query fragment ks (in q4_order): of the low nibbles, then of the high ones
+  static __device__ __forceinline__ uint32_t q_dim(uint32_t ks, uint32_t g) {
+    return HD == 128u ? 64u * (ks / 2u) + 16u * g + 8u * (ks & 1u) : 32u * ks + 8u * g;
+  }
+};
+
+// Running sums of a column's weights beside its softmax: the lane's share.
+template <uint32_t HD>
+struct Sums4 {
+  float w[HD / 64u], b[HD / 64u];
+};
+
+template <uint32_t HD, bool KEEP>
+__device__ __forceinline__ void block_step4(const Block4<HD, KEEP>& blk, const bf16x8_v (&qb)[HD / 32u],
+                                            const float (&qs)[HD / 64u], Column<HD>& c, Sums4<HD>& u, uint32_t t, uint32_t hi,
+                                            uint32_t lo, uint32_t sinks, bool ok, bool masked, float scale_log2,
+                                            float (&sv)[8], uint32_t lane) {
+  constexpr uint32_t NG = HD / 64u, NT = HD / 16u;
+  const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (uint32_t tt = 0; tt < 2; ++tt) {
+    f32x4_v acc[NG];
+    if constexpr (HD == 128u) {
+      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].x, blk.k[tt].y), qb[0], zero, 0, 0, 0);
+      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].z, blk.k[tt].w), qb[1], acc[0], 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].x, blk.k[tt].y), qb[2], zero, 0, 0, 0);
+      acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].z, blk.k[tt].w), qb[3], acc[1], 0, 0, 0);
+    } else {
+      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].x, blk.k[tt].y), qb[0], zero, 0, 0, 0);
+      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].x, blk.k[tt].y), qb[1], acc[0], 0, 0, 0);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      float s = 0.0f;
+#pragma unroll
+      for (uint32_t q = 0; q < NG; ++q) {
+        const uint32_t par = blk.kp[q][tt][i];
+        const float sc = bf16lo(par);
+        s = __builtin_fmaf(sc, acc[q][i], __builtin_fmaf(__builtin_fmaf(sc, -16.0f, bf16hi(par)), qs[q], s));
+      }
+      sv[4 * tt + i] = s * scale_log2;
+    }
+  }
+  uint32_t bits = 0xffu;
+  if (masked) {  // uniform
+    bits = ok ? seen_bits(t, hi, lo, sinks) : 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) sv[j] = bits >> j & 1u ? sv[j] : NEG_INF;
+  }
+  float bm = sv[0];
+#pragma unroll
+  for (uint32_t j = 1; j < 8; ++j) bm = fmaxf(bm, sv[j]);
+  bm = fmaxf(bm, lane_xor16_f32(bm, lane));
+  bm = fmaxf(bm, lane_xor32_f32(bm, lane));
+  const float m_new = fmaxf(c.m, bm), m_use = m_new == NEG_INF ? 0.0f : m_new;
+  if (__any(m_new > c.m)) {  // (a column whose maximum stays has a factor of one)
+    const float corr = __builtin_amdgcn_exp2f(c.m - m_use);
+    c.l *= corr;
+#pragma unroll
+    for (uint32_t q = 0; q < NG; ++q) {
+      u.w[q] *= corr;
+      u.b[q] *= corr;
+    }
+#pragma unroll
+    for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) c.o[nt][i] *= corr;
+    c.m = m_new;
+  }
+  float p[8];
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) {
+    p[j] = __builtin_amdgcn_exp2f(sv[j] - m_use);
+    c.l += p[j];
+  }
+  typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+  const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
+  bf16x8_v pb[NG];
+#pragma unroll
+  for (uint32_t q = 0; q < NG; ++q) {
+    float w[8];
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      // what lies in hidden entries may be anything: its scale and bias read as zero
+      uint32_t par = blk.vp[q][j / 4u][j % 4u];
+      if (masked) par = bits >> j & 1u ? par : 0u;  // uniform
+      w[j] = p[j] * bf16lo(par);
+      u.b[q] = __builtin_fmaf(p[j], __builtin_fmaf(bf16lo(par), 8.0f, bf16hi(par)), u.b[q]);
+    }
+    const u32x4_v pk = {pack_bf16_pair_rne(w[0], w[2]), pack_bf16_pair_rne(w[1], w[3]), pack_bf16_pair_rne(w[4], w[6]),
+                        pack_bf16_pair_rne(w[5], w[7])};
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+      u.w[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, static_cast<uint32_t>(pk[i])), ones, u.w[q], false);
+    pb[q] = __builtin_bit_cast(bf16x8_v, pk);
+  }
+#pragma unroll
+  for (uint32_t nt = 0; nt < NT / 2u; ++nt) {
+    c.o[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.v[nt].x, blk.v[nt].y), pb[0], c.o[nt], 0, 0, 0);
+    c.o[nt + NT / 2u] =
+        __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.v[nt].x, blk.v[nt].y), pb[NG - 1u], c.o[nt + NT / 2u], 0, 0, 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // The plan: which part of which sequence a workgroup takes
 // ---------------------------------------------------------------------------
 // Every sequence's blocks are cut into equal parts, so many that the call has
@@ -217,9 +373,11 @@ __device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, u
 // the columns. Its four waves take the part's blocks in turn and meet in LDS.
 // A part that is all of its sequence writes the output, others their maximum,
 // sum and output for paged_join_kernel.
-template <uint32_t HD, bool F8, bool WEIGHT, bool KEEP>
+template <uint32_t HD, uint32_t KT, bool WEIGHT, bool KEEP>
 __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn p) {
-  constexpr uint32_t NT = HD / 16u;
+  constexpr uint32_t NT = HD / 16u, NG = HD / 64u;
+  constexpr bool F8 = KT == KT_E4M3, Q4 = KT == KT_Q4;
+  typedef typename std::conditional<Q4, Block4<HD, KEEP>, Block<HD, F8, KEEP>>::type Blk;
   __shared__ float s_ml[4][16][2];
   __shared__ float s_o[4][16][HD + 4u];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, col = lane & 15u, g = lane >> 4;
@@ -237,12 +395,29 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
 #pragma unroll
   for (uint32_t ks = 0; ks < HD / 32u; ++ks) {
     u32x4_v v = *reinterpret_cast<const u32x4_v*>(p.q + static_cast<size_t>(b) * p.q_ld + (kv * p.G + min(col, p.G - 1u)) * HD +
-                                                  Block<HD, F8, KEEP>::q_dim(ks, g));
+                                                  Blk::q_dim(ks, g));
     if (col >= p.G) v = u32x4_v{0u, 0u, 0u, 0u};
+    if constexpr (Q4) v = q4_order(v);
     qb[ks] = __builtin_bit_cast(bf16x8_v, v);
   }
   Column<HD> c;
   c.clear();
+  float qs[NG] = {};  // sums of the column's queries over each group
+  Sums4<HD> u = {};
+  if constexpr (Q4) {
+#pragma unroll
+    for (uint32_t ks = 0; ks < HD / 32u; ++ks)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t w = __builtin_bit_cast(u32x4_v, qb[ks])[i];
+        qs[ks / 2u] += bf16lo(w) + bf16hi(w);
+      }
+#pragma unroll
+    for (uint32_t q = 0; q < NG; ++q) {
+      qs[q] += lane_xor16_f32(qs[q], lane);
+      qs[q] += lane_xor32_f32(qs[q], lane);
+    }
+  }
   // page ids of the wave's next 64 blocks (both halves of each), a block a lane
   uint32_t id0 = 0, id1 = 0;
   for (uint32_t x = x0 + wave, it = 0; x < x1; x += 4u, ++it) {
@@ -262,12 +437,16 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
       p0 = ok0 ? p0 : 0u;
       p1 = ok1 ? p1 : 0u;
     }
-    Block<HD, F8, KEEP> blk;
+    Blk blk;
     blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
     __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
     float sv[8];
-    block_step<HD, F8, KEEP>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
-                       !(whole && ok0 && ok1), scale, sv, lane);
+    if constexpr (Q4)
+      block_step4<HD, KEEP>(blk, qb, qs, c, u, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, !(whole && ok0 && ok1),
+                            scale, sv, lane);
+    else
+      block_step<HD, F8, KEEP>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
+                         !(whole && ok0 && ok1), scale, sv, lane);
     if constexpr (WEIGHT) {
       if (col < p.G) {
         float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + col) * p.vis + 32u * x + 8u * g);
@@ -278,6 +457,18 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
   }
   c.l += lane_xor16_f32(c.l, lane);
   c.l += lane_xor32_f32(c.l, lane);
+  if constexpr (Q4) {
+#pragma unroll
+    for (uint32_t q = 0; q < NG; ++q) {
+      float add = __builtin_fmaf(u.w[q], -24.0f, u.b[q]);
+      add += lane_xor16_f32(add, lane);
+      add += lane_xor32_f32(add, lane);
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT / NG; ++nt)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) c.o[NT / NG * q + nt][i] += add;
+    }
+  }
   if (lane < 16u) {
     s_ml[wave][col][0] = c.m;
     s_ml[wave][col][1] = c.l;
@@ -334,8 +525,9 @@ __device__ __forceinline__ Total join_total(const float* ml, uint32_t splits, ui
 // parts in flight at once). The others (WEIGHT): 1,024 listed entries of a
 // (sequence, kv head) each, whose weights are the scores taken to the head's
 // total.
-template <uint32_t HD, bool F8, bool WEIGHT, uint32_t JD>
+template <uint32_t HD, uint32_t KT, bool WEIGHT, uint32_t JD>
 __global__ void __launch_bounds__(256) paged_join_kernel(Paged a, PagedAttn p, Weight w, uint32_t wchunks) {
+  constexpr bool F8 = KT == KT_E4M3;
   constexpr uint32_t TD = JD / 4u, PT = 256u / TD, ROUND = 8u * PT;  // threads of a part, parts at once, parts a round
   __shared__ f32x4_v s_part[PT][TD];
   __shared__ float s_tot[16][2];
@@ -483,7 +675,7 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
   d.blocks = most_blocks(static_cast<uint64_t>(s->max_pages) * kv->page, window, sinks);
   d.vis = 32u * d.blocks;
   const uint64_t rows = static_cast<uint64_t>(s->n_seqs) * kv->n_kv;
-  const uint32_t whole = weight ? 0u : decode_whole(rows, kv->dtype == OBS_KV_E4M3);
+  const uint32_t whole = weight ? 0u : decode_whole(rows, kv->dtype != OBS_KV_BF16);
   d.min_chunk = std::max(DECODE_MIN_CHUNK, d.blocks <= whole ? whole : 0u);
   // sum of the rows' rounded shares: at most target + rows (and what fp32 rounds), and at most each row's own most
   d.items = std::min<uint64_t>(decode_target(kv, s) + rows + 64u, rows * ((d.blocks + d.min_chunk - 1u) / d.min_chunk));
@@ -494,13 +686,13 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
   return d;
 }
 
-template <uint32_t HD, bool F8, bool WEIGHT>
+template <uint32_t HD, uint32_t KT, bool WEIGHT>
 int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight& w, const DecodePlan& d) {
   const uint32_t items = static_cast<uint32_t>(d.items);
   if (a.lp >= 6u)
-    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, F8, WEIGHT, true><<<items, 256, 0, ctx->stream>>>(a, p));
+    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, KT, WEIGHT, true><<<items, 256, 0, ctx->stream>>>(a, p));
   else
-    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, F8, WEIGHT, false><<<items, 256, 0, ctx->stream>>>(a, p));
+    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, KT, WEIGHT, false><<<items, 256, 0, ctx->stream>>>(a, p));
   if (!WEIGHT && d.blocks <= d.min_chunk) return OBS_OK;  // every sequence is one part
   const uint32_t wchunks = WEIGHT ? static_cast<uint32_t>((d.vis + 1023u) / 1024u) : 0u, rows = a.n_seqs * p.nh;
   const uint32_t weights = rows / p.G * wchunks;
@@ -508,9 +700,9 @@ int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight
   // entries 46.5 us against 48.2; 48 sequences of up to 16,000 77.7 against 72.3)
   if (rows < 256u)
     OBS_LAUNCH(ctx, "paged_join",
-               paged_join_kernel<HD, F8, WEIGHT, 32><<<rows * (HD / 32u) + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
+               paged_join_kernel<HD, KT, WEIGHT, 32><<<rows * (HD / 32u) + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
   else
-    OBS_LAUNCH(ctx, "paged_join", paged_join_kernel<HD, F8, WEIGHT, HD><<<rows + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
+    OBS_LAUNCH(ctx, "paged_join", paged_join_kernel<HD, KT, WEIGHT, HD><<<rows + weights, 256, 0, ctx->stream>>>(a, p, w, wchunks));
   return OBS_OK;
 }
 
@@ -582,13 +774,10 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
                    static_cast<uint32_t>(d.vis), d.min_chunk, decode_target(kv, seqs), 0u,
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
   const Weight w = obs::weight_args(weight);
-  const bool f8 = kv->dtype == OBS_KV_E4M3;
-  if (kv->head_dim == 128u) {
-    if (weight) return f8 ? launch_decode<128, true, true>(ctx, a, p, w, d) : launch_decode<128, false, true>(ctx, a, p, w, d);
-    return f8 ? launch_decode<128, true, false>(ctx, a, p, w, d) : launch_decode<128, false, false>(ctx, a, p, w, d);
-  }
-  if (weight) return f8 ? launch_decode<64, true, true>(ctx, a, p, w, d) : launch_decode<64, false, true>(ctx, a, p, w, d);
-  return f8 ? launch_decode<64, true, false>(ctx, a, p, w, d) : launch_decode<64, false, false>(ctx, a, p, w, d);
+  return obs::paged_shape(kv, [&](auto hd, auto t) {
+    return weight ? launch_decode<decltype(hd)::value, decltype(t)::value, true>(ctx, a, p, w, d)
+                  : launch_decode<decltype(hd)::value, decltype(t)::value, false>(ctx, a, p, w, d);
+  });
 }
 
 }  // extern "C"

@@ -5,6 +5,9 @@
 
 namespace {
 using namespace obsd;
+using obs::KT_BF16;
+using obs::KT_E4M3;
+using obs::KT_Q4;
 using obs::Paged;
 using obs::Weight;
 
@@ -61,8 +64,9 @@ __device__ __forceinline__ uint32_t seq_of_row_lane(const Paged& a, uint32_t t, 
 // cache row at a time, the stores cost more than everything else: 38.8 against
 // 28.3 us for 5,795 rows into an e4m3 cache.)
 constexpr uint32_t PREP_TILE = 64;
-template <uint32_t HD, bool F8>
+template <uint32_t HD, uint32_t KT>
 __device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs& p, uint32_t vi) {
+  constexpr bool F8 = KT == KT_E4M3;
   __shared__ uint32_t s_v[PREP_TILE][HD / 2u + 1u];  // rows of dim pairs (+1 word: bank spread)
   const uint32_t h = vi % a.n_kv, t0 = vi / a.n_kv * PREP_TILE, nt = umin(PREP_TILE, a.n_rows - t0);
 #pragma unroll
@@ -79,7 +83,7 @@ __device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, t = t0 + lane;
   const uint32_t b0 = seq_of_row(a, t0, lane);
   bool there = false;
-  size_t at = 0;
+  uint32_t page = 0u, off = 0u;
   if (lane < nt && b0 < a.n_seqs) {
     const uint32_t b = seq_of_row_lane(a, t, b0);
     if (b < a.n_seqs) {
@@ -87,11 +91,63 @@ __device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs
       const int32_t entry = static_cast<int32_t>(paged_len(a, b)) - static_cast<int32_t>(r.r1 - t);
       const int32_t pos = p.pos ? p.pos[t] : entry;
       if (t >= r.r0 && t < r.r1 && entry >= 0 && pos >= 0 && static_cast<uint32_t>(pos) < p.rope_len) {
-        const uint32_t page = paged_id(a, b, static_cast<uint32_t>(entry), there);  // reported by the row's workgroup
-        at = ((static_cast<size_t>(page) * a.n_kv + h) * HD << a.lp) + (static_cast<uint32_t>(entry) & ((1u << a.lp) - 1u));
+        page = paged_id(a, b, static_cast<uint32_t>(entry), there);  // reported by the row's workgroup
+        off = static_cast<uint32_t>(entry) & ((1u << a.lp) - 1u);
       }
     }
   }
+  if constexpr (KT == KT_Q4) {
+    // A wave takes a quarter of the bytes of the rows: the dims of both nibbles. The
+    // groups' ranges go through LDS, as their dims are several waves'.
+    constexpr uint32_t HALF = HD / 2u, BW = HALF / 4u;  // bytes of a row, of a wave
+    __shared__ float s_lo[4][2][PREP_TILE], s_hi[4][2][PREP_TILE];
+    __syncthreads();
+    float x[2][BW];
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      float lo = -NEG_INF, hi = NEG_INF;
+#pragma unroll
+      for (uint32_t i = 0; i < BW; i += 2u) {
+        const uint32_t w = s_v[lane][(HALF * j + BW * wave + i) / 2u];
+        x[j][i] = bf16lo(w);
+        x[j][i + 1u] = bf16hi(w);
+      }
+      bool wild = false;
+#pragma unroll
+      for (uint32_t i = 0; i < BW; ++i) {
+        lo = fminf(lo, x[j][i]);
+        hi = fmaxf(hi, x[j][i]);
+        wild |= (__float_as_uint(x[j][i]) & 0x7f800000u) == 0x7f800000u;
+      }
+      // a value that is not finite: both ends at infinity (fmin and fmax pass over NaN)
+      s_lo[wave][j][lane] = wild ? NEG_INF : lo;
+      s_hi[wave][j][lane] = hi;
+    }
+    __syncthreads();
+    if (!there) return;
+    uint8_t* const base = const_cast<uint8_t*>(a.v) + page_at<HD, KT>(a, page, h);
+    uint32_t par[2];
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      float lo = -NEG_INF, hi = NEG_INF;
+#pragma unroll
+      for (uint32_t g = 0; g < 2; ++g) {  // a head of 64 has one group of both halves
+        if (HD == 128u && g != j) continue;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          lo = fminf(lo, s_lo[i][g][lane]);
+          hi = fmaxf(hi, s_hi[i][g][lane]);
+        }
+      }
+      par[j] = q4_params(lo, hi, max(__float_as_uint(lo) & 0x7fffffffu, __float_as_uint(hi) & 0x7fffffffu));
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < BW; ++i)
+      base[(static_cast<size_t>(BW * wave + i) << a.lp) + off] = static_cast<uint8_t>(q4_quant(x[0][i], par[0]) | q4_quant(x[1][i], par[1]) << 4);
+    if (wave < HD / 64u) reinterpret_cast<uint32_t*>(base + (HALF << a.lp))[(wave << a.lp) + off] = par[wave ? 1 : 0];
+    return;
+  }
+  const size_t at = ((static_cast<size_t>(page) * a.n_kv + h) * HD << a.lp) + off;
   const float s = F8 ? a.v_scale[h] : 1.0f;
   __syncthreads();
   if (!there) return;
@@ -115,11 +171,12 @@ __device__ __forceinline__ void prep_paged_values(const Paged& a, const PrepArgs
 // each, so a wave norms and rotates 512 / HD heads at once. The sums and the
 // rotation are attn_prep_rows_kernel's, in its order. The first heads are
 // requested before the row's sequence, entry and position are known.
-template <uint32_t HD, bool F8, uint32_t WAVES>
-__global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p, Weight w, uint32_t n_vt) {
+template <uint32_t HD, uint32_t KT, uint32_t WAVES>
+__global__ void __launch_bounds__(256, KT == KT_Q4 ? 6 : 8) prep_paged_kernel(Paged a, PrepArgs p, Weight w, uint32_t n_vt) {
+  constexpr bool F8 = KT == KT_E4M3, Q4 = KT == KT_Q4;
   constexpr uint32_t LPH = HD / 8u, HPW = 64u / LPH;  // lanes per head, heads per wave
   if (blockIdx.x < n_vt) {  // uniform
-    prep_paged_values<HD, F8>(a, p, blockIdx.x);
+    prep_paged_values<HD, KT>(a, p, blockIdx.x);
     return;
   }
   const uint32_t lane = threadIdx.x & 63u, m = lane % LPH, c0 = 8u * m;
@@ -201,10 +258,10 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       const float n0 = (bf16lo(xw[i]) * inv) * bf16lo(ww[i]), n1 = (bf16hi(xw[i]) * inv) * bf16hi(ww[i]);
-      // what becomes bf16 is rounded as the stored q / k would be; a key in e4m3 only at its end
+      // what becomes bf16 is rounded as the stored q / k would be; a key in fewer bits only at its end
       const uint32_t pr = pack_bf16_pair_rne(n0, n1);
-      nvs[2 * i] = F8 && !is_q ? n0 : bf16lo(pr);
-      nvs[2 * i + 1] = F8 && !is_q ? n1 : bf16hi(pr);
+      nvs[2 * i] = KT != KT_BF16 && !is_q ? n0 : bf16lo(pr);
+      nvs[2 * i + 1] = KT != KT_BF16 && !is_q ? n1 : bf16hi(pr);
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -217,6 +274,33 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
       const float x0 = nv * cs[i], x1 = other * sn[i];
       r[i] = first ? x0 - x1 : x0 + x1;
     }
+    uint32_t par = 0u, mine = 0u, other = 0u;  // a key in 4 bits: its group's parameters, the lane's nibbles, the other half's
+    if (Q4 && hb + HPW > p.nh) {  // uniform per wave
+      float lo = r[0], hi = r[0];
+      uint32_t bits = 0u;
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) {
+        lo = fminf(lo, r[i]);
+        hi = fmaxf(hi, r[i]);
+        bits = max(bits, __float_as_uint(r[i]) & 0x7fffffffu);
+      }
+      // the group's eight lanes (NaN passes fmin and fmax, not the integer maximum)
+      auto over = [&](auto step) __attribute__((always_inline)) {
+        lo = fminf(lo, step(lo));
+        hi = fmaxf(hi, step(hi));
+        bits = max(bits, __float_as_uint(step(__uint_as_float(bits))));
+      };
+      over([](float v) { return dpp_f32<DPP_XOR1>(v); });
+      over([](float v) { return dpp_f32<DPP_XOR2>(v); });
+      over([](float v) { return dpp_f32<DPP_HALF_MIRROR>(v); });
+      par = q4_params(lo, hi, bits);
+#pragma unroll
+      for (uint32_t i = 0; i < 8; ++i) mine |= q4_quant(r[i], par) << (4u * i);
+      if constexpr (HD == 128u)
+        other = __float_as_uint(dpp_f32<DPP_ROW_ROR8>(__uint_as_float(mine)));
+      else
+        other = __float_as_uint(dpp_xor4_f32(__uint_as_float(mine)));
+    }
     if (head >= heads) continue;
     if (is_q) {
       *reinterpret_cast<uint4*>(q_out + head * HD + c0) =
@@ -225,7 +309,18 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
     } else if (there) {
       const uint32_t h = head - p.nh;
       const size_t at = ((page0 + h) * pg + off) * HD + c0;
-      if constexpr (F8) {
+      if constexpr (Q4) {
+        uint8_t* const base = const_cast<uint8_t*>(a.k) + page_at<HD, KT>(a, page, h);
+        if (m % 8u == 0u) reinterpret_cast<uint32_t*>(base + pg * (HD / 2u))[(m / 8u) * pg + off] = par;
+        if (first) {  // bytes of the lane's dims and those half a row on
+          auto spread = [](uint32_t v) __attribute__((always_inline)) {  // four nibbles to four bytes
+            v = (v | v << 8) & 0x00ff00ffu;
+            return (v | v << 4) & 0x0f0f0f0fu;
+          };
+          *reinterpret_cast<uint2*>(base + off * (HD / 2u) + c0) =
+              make_uint2(spread(mine & 0xffffu) | spread(other & 0xffffu) << 4, spread(mine >> 16) | spread(other >> 16) << 4);
+        }
+      } else if constexpr (F8) {
         const float s = a.k_scale[h];
         uint2 o;
         o.x = pack_e4m3x4(r[0] / s, r[1] / s, r[2] / s, r[3] / s);
@@ -240,6 +335,27 @@ __global__ void __launch_bounds__(256, 8) prep_paged_kernel(Paged a, PrepArgs p,
   }
   if (!there || n_vt) return;
   const uint16_t* v = p.v + static_cast<size_t>(t) * p.kv_ld;
+  if constexpr (Q4) {  // a byte of a head a lane: dims d and d + HD / 2; a head of 64 takes half a wave
+    constexpr uint32_t HALF = HD / 2u;
+    for (uint32_t i0 = 64u * wave; i0 < a.n_kv * HALF; i0 += threads) {  // uniform per wave
+      const uint32_t i = umin(i0 + lane, a.n_kv * HALF - 1u), h = i / HALF, d = i % HALF;
+      const float x0 = bf16_to_f32(v[h * HD + d]), x1 = bf16_to_f32(v[h * HD + HALF + d]);
+      const uint32_t b0 = __float_as_uint(x0) & 0x7fffffffu, b1 = __float_as_uint(x1) & 0x7fffffffu;
+      uint32_t par[2];
+      if constexpr (HD == 128u) {
+        par[0] = q4_params(-wave_max_f32(-x0), wave_max_f32(x0), wave_max_u31(b0));
+        par[1] = q4_params(-wave_max_f32(-x1), wave_max_f32(x1), wave_max_u31(b1));
+      } else {
+        par[0] = par[1] = q4_params(-half_max_f32(fmaxf(-x0, -x1), lane), half_max_f32(fmaxf(x0, x1), lane),
+                                      half_max_u32(max(b0, b1), lane));
+      }
+      if (i0 + lane >= a.n_kv * HALF) continue;  // behind the last head
+      uint8_t* const base = const_cast<uint8_t*>(a.v) + page_at<HD, KT>(a, page, h);
+      base[d * pg + off] = static_cast<uint8_t>(q4_quant(x0, par[0]) | q4_quant(x1, par[1]) << 4);
+      if (d < HD / 64u) reinterpret_cast<uint32_t*>(base + pg * HALF)[d * pg + off] = par[d ? 1 : 0];
+    }
+    return;
+  }
   for (uint32_t i = tid; i < a.n_kv * HD; i += threads) {  // one token: one transposed column
     const uint32_t h = i / HD, d = i % HD;
     const size_t at = ((page0 + h) * HD + d) * pg + off;
@@ -435,12 +551,15 @@ __global__ void __launch_bounds__(EV_THREADS) evict_select_kernel(Paged a, Weigh
 // the first is taken apart, and a lane writes 16 consecutive entries of its row.
 // A transposed value page is read whole as soon as one of its entries is kept
 // (an entry's dims lie a row apart).
-template <uint32_t HD, bool F8, uint32_t GE>
+// Entries in 4 bits are copied as bytes of half as many dims, and their words of
+// scale and bias.
+template <uint32_t HD, uint32_t KT, uint32_t GE>
 __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t* __restrict__ dst_pages,
                                                          uint32_t dst_max_pages, uint32_t budget,
                                                          const int32_t* __restrict__ kept) {
-  typedef typename std::conditional<F8, uint8_t, uint16_t>::type T;
-  constexpr uint32_t SZ = sizeof(T), CH = HD * SZ / 16u;  // 16-byte chunks of a key row
+  typedef typename std::conditional<KT == KT_BF16, uint16_t, uint8_t>::type T;
+  constexpr uint32_t ROWS = KT == KT_Q4 ? HD / 2u : HD;     // values of an entry, rows of a value page
+  constexpr uint32_t SZ = sizeof(T), CH = ROWS * SZ / 16u;  // 16-byte chunks of a key row
   __shared__ int32_t s_src[GE], s_dst[GE];                // pages of both sides, -1: none
   __shared__ uint32_t s_so[GE];                           // entries in the source pages
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), groups = (budget + GE - 1u) / GE;
@@ -469,22 +588,35 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
 #pragma unroll
   for (uint32_t i = 0; i < KN; ++i) {
     const uint32_t t = tid + 256u * i, e = t / CH % GE, c = t % CH;
-    const size_t row = ((static_cast<size_t>(max(s_src[e], 0)) * a.n_kv + h) << a.lp) + s_so[e];
-    kx[i] = *reinterpret_cast<const uint4*>(kb + row * (HD * SZ) + 16u * c);
+    const uint8_t* row = kb + page_at<HD, KT>(a, static_cast<uint32_t>(max(s_src[e], 0)), h) + s_so[e] * (ROWS * SZ);
+    kx[i] = *reinterpret_cast<const uint4*>(row + 16u * c);
     if (s_src[e] < 0) kx[i] = make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (uint32_t i = 0; i < KN; ++i) {
     const uint32_t t = tid + 256u * i, e = t / CH % GE, c = t % CH;
     if ((GE * CH % 256u == 0u || t < GE * CH) && s_dst[e] >= 0) {
-      const size_t row = ((static_cast<size_t>(s_dst[e]) * a.n_kv + h) << a.lp) + ((e0 + e) & mask);
-      *reinterpret_cast<uint4*>(kb + row * (HD * SZ) + 16u * c) = kx[i];
+      uint8_t* row = kb + page_at<HD, KT>(a, static_cast<uint32_t>(s_dst[e]), h) + ((e0 + e) & mask) * (ROWS * SZ);
+      *reinterpret_cast<uint4*>(row + 16u * c) = kx[i];
     }
   }
-  constexpr uint32_t DW = HD / 64u;  // waves across the dims
-  const T* vs = reinterpret_cast<const T*>(a.v);
-  T* vd = reinterpret_cast<T*>(const_cast<uint8_t*>(a.v));
-  const uint32_t d = 64u * (wave % DW) + lane;
+  if constexpr (KT == KT_Q4) {
+    for (uint32_t t = tid; t < 2u * GE * (HD / 64u); t += 256u) {
+      const uint32_t e = t % GE, g = t / GE % (HD / 64u);
+      uint8_t* side = const_cast<uint8_t*>(t / GE < HD / 64u ? a.k : a.v);
+      auto word = [&](int32_t page, uint32_t off) __attribute__((always_inline)) {
+        return reinterpret_cast<uint32_t*>(side + page_at<HD, KT>(a, static_cast<uint32_t>(page), h) + (ROWS << a.lp)) + (g << a.lp) + off;
+      };
+      const uint32_t x = s_src[e] < 0 ? 0u : *word(s_src[e], s_so[e]);
+      if (s_dst[e] >= 0) *word(s_dst[e], (e0 + e) & mask) = x;
+    }
+  }
+  constexpr uint32_t DW = ROWS < 64u ? 1u : ROWS / 64u;  // waves across the rows
+  auto values = [&](uint32_t page) __attribute__((always_inline)) {
+    return reinterpret_cast<T*>(const_cast<uint8_t*>(a.v) + page_at<HD, KT>(a, page, h));
+  };
+  const uint32_t d = umin(64u * (wave % DW) + lane, ROWS - 1u);
+  const bool has_row = ROWS >= 64u || lane < ROWS;
   for (uint32_t q = wave / DW; q < GE / 16u; q += 4u / DW) {  // 16 entries, of one destination page
     const int32_t dp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_dst[16u * q])));
     if (dp < 0) continue;  // uniform: no page, or behind the last entry
@@ -498,7 +630,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
       for (uint32_t i = 0; i < 16; ++i) {
         const int32_t sp = static_cast<int32_t>(uniform(static_cast<uint32_t>(s_src[16u * q + i])));
         // (a page that is not there reads page 0)
-        const T* row = vs + ((static_cast<size_t>(max(sp, 0)) * a.n_kv + h) * HD << a.lp) + uniform(s_so[16u * q + i]);
+        const T* row = values(static_cast<uint32_t>(max(sp, 0))) + uniform(s_so[16u * q + i]);
         x[i] = row[d << a.lp];
         if (sp < 0) x[i] = 0;  // uniform
       }
@@ -514,7 +646,7 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
         if (i == 0u || sp != ps || c != pc) {  // uniform
           fresh |= 1u << i;
           // (a page that is not there reads page 0)
-          const T* row = vs + ((static_cast<size_t>(static_cast<int32_t>(sp) < 0 ? 0u : sp) * a.n_kv + h) * HD << a.lp) + CE * c;
+          const T* row = values(static_cast<int32_t>(sp) < 0 ? 0u : sp) + CE * c;
           ch[i] = *reinterpret_cast<const u32x4_v*>(row + (d << a.lp));
           if (static_cast<int32_t>(sp) < 0) ch[i] = u32x4_v{0u, 0u, 0u, 0u};
         }
@@ -531,12 +663,13 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
         x[i] = static_cast<T>(k * SZ < 8u ? lo : hi);
       }
     }
-    T* to = vd + ((static_cast<size_t>(dp) * a.n_kv + h) * HD << a.lp) + (static_cast<size_t>(d) << a.lp) + ((e0 + 16u * q) & mask);
+    if (!has_row) continue;
+    T* to = values(static_cast<uint32_t>(dp)) + (static_cast<size_t>(d) << a.lp) + ((e0 + 16u * q) & mask);
     if (cnt == 16u) {  // uniform
       uint32_t o[4 * SZ];
 #pragma unroll
       for (uint32_t i = 0; i < 4 * SZ; ++i) {
-        if constexpr (F8)
+        if constexpr (SZ == 1u)
           o[i] = x[4 * i] | x[4 * i + 1] << 8 | x[4 * i + 2] << 16 | static_cast<uint32_t>(x[4 * i + 3]) << 24;
         else
           o[i] = x[2 * i] | static_cast<uint32_t>(x[2 * i + 1]) << 16;
@@ -557,28 +690,28 @@ __global__ void __launch_bounds__(256) evict_copy_kernel(Paged a, const int32_t*
 // heads 28.2 and 11.9; of 36 heads of 128, nine times round, one gains nothing).
 uint32_t prep_waves(uint32_t hd, uint32_t heads, uint32_t rows) { return heads * hd <= 2560u && rows >= 1024u ? 1u : 4u; }
 
-template <uint32_t HD, bool F8>
+template <uint32_t HD, uint32_t KT>
 int launch_prep(obs_ctx* ctx, const Paged& a, const PrepArgs& p, const Weight& w, uint32_t n_vt, uint32_t grid, uint32_t waves) {
   if (waves == 1u)
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<HD, F8, 1><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<HD, KT, 1><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
   else
-    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<HD, F8, 4><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
+    OBS_LAUNCH(ctx, "attn_prep_paged", prep_paged_kernel<HD, KT, 4><<<grid, 256, 0, ctx->stream>>>(a, p, w, n_vt));
   return OBS_OK;
 }
 
 // copies: workgroups with 64 entries each.
-template <uint32_t HD, bool F8>
+template <uint32_t HD, uint32_t KT>
 int launch_copy(obs_ctx* ctx, const Paged& a, const int32_t* dst_pages, uint32_t dst_max_pages, uint32_t budget,
                 const int32_t* kept, uint64_t copies) {
   // below two workgroups a CU (a few sequences): 16 entries each, one sequence of 2,048 kept entries 15.4 us against 19.9
   if (copies < 512u) {
     const uint32_t grid = a.n_seqs * a.n_kv * ((budget + 15u) / 16u);
     OBS_LAUNCH(ctx, "kv_evict_copy",
-               evict_copy_kernel<HD, F8, 16><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+               evict_copy_kernel<HD, KT, 16><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
   } else {
     const uint32_t grid = static_cast<uint32_t>(copies);
     OBS_LAUNCH(ctx, "kv_evict_copy",
-               evict_copy_kernel<HD, F8, 64><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
+               evict_copy_kernel<HD, KT, 64><<<grid, 256, 0, ctx->stream>>>(a, dst_pages, dst_max_pages, budget, kept));
   }
   return OBS_OK;
 }
@@ -599,8 +732,8 @@ int paged_status(obs_ctx* ctx) {
 
 int check_paged(obs_ctx* ctx, const char* who, const obs_paged_kv* kv, const obs_paged_seqs* s, bool pointers) {
   if (!kv || !s) return set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
-  if (kv->dtype != OBS_KV_BF16 && kv->dtype != OBS_KV_E4M3)
-    return set_error(ctx, OBS_E_INVALID, "%s: dtype must be OBS_KV_BF16 or OBS_KV_E4M3 (got %d)", who, kv->dtype);
+  if (kv->dtype != OBS_KV_BF16 && kv->dtype != OBS_KV_E4M3 && kv->dtype != OBS_KV_Q4)
+    return set_error(ctx, OBS_E_INVALID, "%s: dtype must be OBS_KV_BF16, OBS_KV_E4M3 or OBS_KV_Q4 (got %d)", who, kv->dtype);
   if (pointers) {
     if (!kv->k_pages || !kv->v_pages || !s->pages || !s->len || (kv->dtype == OBS_KV_E4M3 && (!kv->k_scale || !kv->v_scale)))
       return set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
@@ -686,10 +819,9 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
   if (rc != OBS_OK) return rc;
   const Paged a = obs::paged_args(ctx, kv, seqs);
   const Weight w = obs::weight_args(weight);
-  const bool f8 = kv->dtype == OBS_KV_E4M3;
-  if (hd == 128u)
-    return f8 ? launch_prep<128, true>(ctx, a, p, w, n_vt, grid, waves) : launch_prep<128, false>(ctx, a, p, w, n_vt, grid, waves);
-  return f8 ? launch_prep<64, true>(ctx, a, p, w, n_vt, grid, waves) : launch_prep<64, false>(ctx, a, p, w, n_vt, grid, waves);
+  return obs::paged_shape(kv, [&](auto d, auto t) {
+    return launch_prep<decltype(d)::value, decltype(t)::value>(ctx, a, p, w, n_vt, grid, waves);
+  });
 }
 
 int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const obs_kv_weight* weight,
@@ -723,11 +855,9 @@ int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seq
   OBS_LAUNCH(ctx, "kv_evict_select", evict_select_kernel<<<seqs->n_seqs * kv->n_kv, EV_THREADS, 0, ctx->stream>>>(
                                          a, obs::weight_args(weight), obs::weight_args(dst_weight), sinks, recent, budget,
                                          kept, new_len));
-  const bool f8 = kv->dtype == OBS_KV_E4M3, d128 = kv->head_dim == 128u;
-  return d128 ? (f8 ? launch_copy<128, true>(ctx, a, dst_pages, dst_max_pages, budget, kept, copies)
-                    : launch_copy<128, false>(ctx, a, dst_pages, dst_max_pages, budget, kept, copies))
-              : (f8 ? launch_copy<64, true>(ctx, a, dst_pages, dst_max_pages, budget, kept, copies)
-                    : launch_copy<64, false>(ctx, a, dst_pages, dst_max_pages, budget, kept, copies));
+  return obs::paged_shape(kv, [&](auto d, auto t) {
+    return launch_copy<decltype(d)::value, decltype(t)::value>(ctx, a, dst_pages, dst_max_pages, budget, kept, copies);
+  });
 }
 
 }  // extern "C"

@@ -5,6 +5,9 @@
 
 namespace {
 using namespace obsd;
+using obs::KT_BF16;
+using obs::KT_E4M3;
+using obs::KT_Q4;
 using obs::most_blocks;
 using obs::Paged;
 using obs::PagedAttn;
@@ -149,12 +152,17 @@ __device__ __forceinline__ PrefillItem prefill_part(const Paged& a, const PagedA
   return {a.n_seqs, 0u, 0u, 1u, 0u, 0u, {0u, 0u}, 0u};
 }
 
-template <uint32_t HD, bool F8>
+template <uint32_t HD, uint32_t KT>
 __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, PagedAttn p) {
-  constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = F8 ? 1u : 2u;
+  constexpr bool F8 = KT == KT_E4M3, Q4 = KT == KT_Q4;
+  constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = KT == KT_BF16 ? 2u : 1u;
   constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
   constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
-  constexpr uint32_t KN = 32u * KC, VN = HD * VC;       // chunks of a block: 512, 256 or 128, at most one a thread
+  // In 4 bits chunks are 8 bytes, eight dims of either half of a key row, or eight
+  // entries of two value rows; a chunk of keys needs the scale and bias of one entry
+  // (two groups), one of values those of its eight entries.
+  constexpr uint32_t NG = HD / 64u, KC4 = HD / 16u, VC4 = 4u;
+  constexpr uint32_t KN = Q4 ? 32u * KC4 : 32u * KC, VN = Q4 ? HD / 2u * VC4 : HD * VC;  // chunks of a block: 128 to 512, at most one a thread
   // Keys and values of two blocks; before and after them a slab a wave, through
   // which queries come in and outputs go out by whole 64-byte runs.
   constexpr uint32_t SLAB = 32u * 80u;  // 32 columns of 64 bytes (+16: bank spread)
@@ -265,15 +273,42 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     k.edge = !(k.ok0 && k.ok1 && k.t + 32u <= hi_first && (k.t >= lo_last || k.t + 32u <= p.sinks));
     return k;
   };
-  const uint32_t v_dim = vc % (VN / 2u) / (VC / 2u), v_ent = 16u * vh + (16u / SZ) * (vc % (VC / 2u));
-  const uint32_t koff = ((kc / KC) & pmask) * (HD * SZ) + 16u * (kc % KC);
+  const uint32_t v_dim = Q4 ? vc % (VN / 2u) / 2u : vc % (VN / 2u) / (VC / 2u);
+  const uint32_t v_ent = 16u * vh + (Q4 ? 8u * (vc % 2u) : (16u / SZ) * (vc % (VC / 2u)));
+  const uint32_t koff = Q4 ? ((kc / KC4) & pmask) * (HD / 2u) + 8u * (kc % KC4) : ((kc / KC) & pmask) * (HD * SZ) + 16u * (kc % KC);
   const uint32_t voff = ((v_dim << a.lp) + (v_ent & pmask)) * SZ;
   u32x4_v kr, vr;
+  u32x2_v xr;              // in 4 bits: a chunk of keys or of values (a wave brings one of them)
+  u32x4_v xp[NG][2];       // and its scales and biases (of keys: the first word)
   auto load_k = [&](const Blk& k) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      if (has_k) {
+        const uint8_t* base = a.k + (static_cast<size_t>(k.ik) << a.lp) * entry_bytes<HD, KT>();
+        xr = *reinterpret_cast<const u32x2_v*>(base + (k.t & pmask) * (HD / 2u) + koff);
+#pragma unroll
+        for (uint32_t q = 0; q < NG; ++q)
+          xp[q][0].x = *reinterpret_cast<const uint32_t*>(base + (HD / 2u << a.lp) + (4u * q << a.lp) +
+                                                          4u * ((k.t & pmask) + ((kc / KC4) & pmask)));
+      }
+      return;
+    }
     const uint8_t* base = a.k + ((static_cast<size_t>(k.ik) << a.lp) + (k.t & pmask)) * (HD * SZ);
     if (has_k) kr = *reinterpret_cast<const u32x4_v*>(base + koff);
   };
   auto load_v = [&](const Blk& k) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      if (has_v) {
+        const uint8_t* base = a.v + (static_cast<size_t>(k.iv) << a.lp) * entry_bytes<HD, KT>();
+        xr = *reinterpret_cast<const u32x2_v*>(base + (k.t & pmask) + voff);
+#pragma unroll
+        for (uint32_t q = 0; q < NG; ++q)
+#pragma unroll
+          for (uint32_t i = 0; i < 2; ++i)
+            xp[q][i] = *reinterpret_cast<const u32x4_v*>(base + (HD / 2u << a.lp) + (4u * q << a.lp) +
+                                                         4u * ((k.t & pmask) + (v_ent & pmask)) + 16u * i);
+      }
+      return;
+    }
     const uint8_t* base = a.v + ((static_cast<size_t>(k.iv) * HD << a.lp) + (k.t & pmask)) * SZ;
     if (has_v) vr = *reinterpret_cast<const u32x4_v*>(base + voff);
   };
@@ -289,7 +324,34 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       return w;
     }
   };
+  // Eight nibbles (low or high ones) as bf16: q s + b in fp32, rounded once. The
+  // products of a prompt take bf16 operands (a rounding of 2^-8 at most, as a cache in
+  // bf16 has it), so that a block is widened once for all of its 384 columns.
+  auto widen4 = [&](bool high, auto par) __attribute__((always_inline)) {
+    const uint32_t w0 = high ? xr.x >> 4 : xr.x, w1 = high ? xr.y >> 4 : xr.y;
+    float f[8];
+    f[0] = q4_value(q4_nibble<0, false>(w0), par(0));
+    f[1] = q4_value(q4_nibble<1, false>(w0), par(1));
+    f[2] = q4_value(q4_nibble<2, false>(w0), par(2));
+    f[3] = q4_value(q4_nibble<3, false>(w0), par(3));
+    f[4] = q4_value(q4_nibble<0, false>(w1), par(4));
+    f[5] = q4_value(q4_nibble<1, false>(w1), par(5));
+    f[6] = q4_value(q4_nibble<2, false>(w1), par(6));
+    f[7] = q4_value(q4_nibble<3, false>(w1), par(7));
+    return u32x4_v{pack_bf16_pair_rne(f[0], f[1]), pack_bf16_pair_rne(f[2], f[3]), pack_bf16_pair_rne(f[4], f[5]),
+                   pack_bf16_pair_rne(f[6], f[7])};
+  };
   auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
+    if constexpr (Q4) {
+      if (has_k) {
+        uint16_t* to = &s_k[buf][(kc / KC4) * KROW + 8u * (kc % KC4)];
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j)
+          *reinterpret_cast<u32x4_v*>(to + HD / 2u * j) =
+              widen4(j == 1u, [&](uint32_t) __attribute__((always_inline)) { return xp[j * (NG - 1u)][0].x; });
+      }
+      return;
+    }
     if (has_k) {
       uint16_t* to = &s_k[buf][(kc / KC) * KROW + (16u / SZ) * (kc % KC)];
 #pragma unroll
@@ -303,13 +365,18 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     if (has_v) {
       u32x4_v w[2u / SZ];
 #pragma unroll
-      for (uint32_t j = 0; j < 2u / SZ; ++j) w[j] = widen(vr, j);
+      for (uint32_t j = 0; j < 2u / SZ; ++j) {
+        if constexpr (Q4)
+          w[j] = widen4(j == 1u, [&](uint32_t e) __attribute__((always_inline)) { return xp[j * (NG - 1u)][e / 4u][e % 4u]; });
+        else
+          w[j] = widen(vr, j);
+      }
       if (k.edge) {  // uniform
         const uint32_t bits = seen_bits(k.t, s.hi, s.lo, p.sinks) & page_bits(k);
         uint32_t bad = 0u;
 #pragma unroll
         for (uint32_t j = 0; j < 2u / SZ; ++j) {
-          w[j] &= word_masks(bits >> (v_ent + 8u * j));
+          w[j] &= word_masks(bits >> (v_ent + (Q4 ? 0u : 8u * j)));
 #pragma unroll
           for (uint32_t q = 0; q < 4; ++q) {
             // all ones in the exponent: adding one in its last place carries into the sign's
@@ -322,7 +389,8 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
         if (bad) s_bad = 1u;
       }
 #pragma unroll
-      for (uint32_t j = 0; j < 2u / SZ; ++j) *reinterpret_cast<u32x4_v*>(&s_v[buf][v_dim * VROW + v_ent + 8u * j]) = w[j];
+      for (uint32_t j = 0; j < 2u / SZ; ++j)  // in 4 bits: the other nibbles' row
+        *reinterpret_cast<u32x4_v*>(&s_v[buf][(v_dim + (Q4 ? HD / 2u * j : 0u)) * VROW + v_ent + (Q4 ? 0u : 8u * j)]) = w[j];
     }
   };
   auto sees = [&](uint32_t e) __attribute__((always_inline)) { return e < hi && (e >= lo || e < p.sinks); };
@@ -423,7 +491,17 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
           for (uint32_t d = 0; d < DT; ++d)
 #pragma unroll
             for (uint32_t j = 0; j < 16; ++j) {
-              const size_t at = ((base + 32u * d + 8u * (j / 4u) + 4u * half + j % 4u) << a.lp) + (e & pmask);
+              const uint32_t dim = 32u * d + 8u * (j / 4u) + 4u * half + j % 4u;
+              const size_t at = ((base + dim) << a.lp) + (e & pmask);
+              if constexpr (Q4) {
+                const uint8_t* page = a.v + page_at<HD, KT>(a, i < 16u ? p0 : p1, kv);
+                const uint32_t byte = page[((dim % (HD / 2u)) << a.lp) + (e & pmask)];
+                const uint32_t par = reinterpret_cast<const uint32_t*>(page + (HD / 2u << a.lp))[(dim / 64u << a.lp) + (e & pmask)];
+                // rounded as in the tile: what is not finite there
+                const float v = bf16_to_f32(f32_to_bf16(q4_value(static_cast<float>(byte >> (dim < HD / 2u ? 0u : 4u) & 15u), par)));
+                o[d][j] += seen && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.0f;
+                continue;
+              }
               const uint32_t w = F8 ? e4m3x2_bf16<false>(a.v[at]) << 16
                                     : static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(a.v)[at]) << 16;
               const float v = (w & 0x7f800000u) == 0x7f800000u ? __uint_as_float(w) : 0.0f;
@@ -491,8 +569,9 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
 
 // A tile's parts joined in order: 1024 / HD columns a workgroup, four dims a
 // thread, eight parts in flight at once.
-template <uint32_t HD, bool F8>
+template <uint32_t HD, uint32_t KT>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(Paged a, PagedAttn p, uint32_t items) {
+  constexpr bool F8 = KT == KT_E4M3;
   constexpr uint32_t CW = 1024u / HD, WG = PF_COLS / CW;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, place = blockIdx.x / (WG * a.n_kv), kv = blockIdx.x / WG % a.n_kv;
   const uint32_t c = blockIdx.x % WG * CW + tid / (HD / 4u), d = 4u * (tid % (HD / 4u));
@@ -578,13 +657,13 @@ PrefillPlan prefill_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, uint32
   return d;
 }
 
-template <uint32_t HD, bool F8>
+template <uint32_t HD, uint32_t KT>
 int launch_prefill(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const PrefillPlan& d) {
   const uint32_t grid = static_cast<uint32_t>(d.items);
-  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, F8><<<grid, PF_THREADS, 0, ctx->stream>>>(a, p));
+  OBS_LAUNCH(ctx, "paged_prefill", paged_prefill_kernel<HD, KT><<<grid, PF_THREADS, 0, ctx->stream>>>(a, p));
   if (d.split)
     OBS_LAUNCH(ctx, "paged_prefill_join",
-               paged_prefill_join_kernel<HD, F8><<<static_cast<uint32_t>(d.tiles) * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
+               paged_prefill_join_kernel<HD, KT><<<static_cast<uint32_t>(d.tiles) * (PF_COLS * HD / 1024u), 256, 0, ctx->stream>>>(a, p, grid));
   return OBS_OK;
 }
 
@@ -621,9 +700,7 @@ int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged
   const PagedAttn p{q, out, reinterpret_cast<float*>(wb), reinterpret_cast<float*>(wb + d.ml), nullptr,
                    reinterpret_cast<uint2*>(wb + d.ml + d.part), n_heads, n_heads / kv->n_kv, window, sinks, q_ld, 0u, 0u, d.split ? PF_TARGET : 0u, static_cast<uint32_t>(d.tiles),
                    1.4426950408889634f / __builtin_sqrtf(static_cast<float>(kv->head_dim))};
-  const bool f8 = kv->dtype == OBS_KV_E4M3;
-  if (kv->head_dim == 128u) return f8 ? launch_prefill<128, true>(ctx, a, p, d) : launch_prefill<128, false>(ctx, a, p, d);
-  return f8 ? launch_prefill<64, true>(ctx, a, p, d) : launch_prefill<64, false>(ctx, a, p, d);
+  return obs::paged_shape(kv, [&](auto hd, auto t) { return launch_prefill<decltype(hd)::value, decltype(t)::value>(ctx, a, p, d); });
 }
 
 }  // extern "C"

@@ -35,7 +35,7 @@ OBS_E_UNSUPPORTED = -6
 
 OBS_DECODE_AUTO, OBS_DECODE_MULTI, OBS_DECODE_FUSED = 0, 1, 2
 OBS_PATH_FUSED_DECODE, OBS_PATH_FUSED_ATTN, OBS_PATH_FFN_ONE_LAUNCH = 1, 2, 4  # obs_dispatch_gate bits
-KV_BF16, KV_E4M3 = 0, 1  # OBS_KV_*: what a paged cache holds (PagedKv.dtype)
+KV_BF16, KV_E4M3, KV_Q4 = 0, 1, 4  # OBS_KV_*: what a paged cache holds (PagedKv.dtype)
 # routing rules (obs_route_topk, MoeConfig.route_rule)
 ROUTE_REF, ROUTE_F32 = 0, 1
 
@@ -616,7 +616,8 @@ class ObsidianExecutor:
 
 class PagedKv:
     """One layer's pool of key/value pages (obs_paged_kv): keys [n_pages, n_kv, page, head_dim],
-    values [n_pages, n_kv, head_dim, page], bf16 or e4m3 bytes with fp32 scales [n_kv]."""
+    values [n_pages, n_kv, head_dim, page], bf16 or e4m3 bytes with fp32 scales [n_kv]; KV_Q4: bytes
+    [n_pages, n_kv, page * head_dim * 9 / 16] of nibbles and, behind them, scales and biases."""
 
     def __init__(self, k_pages, v_pages, n_pages: int, page: int, n_kv: int, head_dim: int, dtype: int = KV_BF16,
                  k_scale=None, v_scale=None):
