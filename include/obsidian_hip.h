@@ -603,6 +603,40 @@ int obs_kv_evict(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seq
                  uint32_t recent, uint32_t budget, int32_t* kept, int32_t* new_len);
 
 /* ------------------------------------------------------------------ */
+/* Log probabilities of given tokens, entropy, most likely alternatives  */
+/* (no reference counterpart: run_one_token takes the argmax alone,      */
+/* forward.rs:563-566)                                                   */
+/* ------------------------------------------------------------------ */
+/* Of each of T rows of logits [T, vocab] (fp32 or bf16, row stride ld elements, 0 =
+ * dense, aligned to their type), in fp32 and natural units:
+ *   logprob[t] = x[tokens[t]] - log sum exp x, 0 for a token outside [0, vocab)
+ *     (padding); tokens and logprob both or neither;
+ *   entropy[t] (nullable) = -sum p log p;
+ *   top_ids, top_logprobs [T, top_k]: the top_k (at most 64 and at most vocab; 0: none)
+ *     largest logits, equal ones by the lower id, and their log probabilities; -1 and
+ *     -infinity where fewer are above -infinity.
+ * -infinity forbids a token; where all are, log probabilities are -infinity and the
+ * entropy 0. NaN and +infinity make a row's log probabilities and entropy NaN (NaN is
+ * never an alternative). ws: device workspace of obs_token_logprobs_workspace bytes
+ * (by sizes alone, no device work), 16-byte aligned, for one call at a time. */
+enum { OBS_LOGITS_F32 = 0, OBS_LOGITS_BF16 = 1 };
+int obs_token_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t vocab, int dtype, uint32_t top_k, size_t* bytes);
+int obs_token_logprobs(obs_ctx* ctx, const void* logits, int dtype, uint32_t T, uint32_t vocab, uint32_t ld,
+                       const int32_t* tokens, float* logprob, float* entropy, uint32_t top_k, int32_t* top_ids,
+                       float* top_logprobs, void* ws, size_t ws_bytes);
+
+/* The same of the logits x . dequant(W)^T of T rows x bf16 [T, in] (after the final
+ * norm) and a 4-bit [vocab, in] matrix (the lm_head); the logits are not the caller's.
+ * No weight is rounded (q * scale + bias enters in fp32, as in obs_q4_gemv). group 64,
+ * in a multiple of 512 up to 16,384; x, w, scales, biases and ws 16-byte aligned.
+ * With alternatives the rows of more than 32 tokens pass by 256 at a time, whose logits
+ * are in the workspace. */
+int obs_lm_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t in, uint32_t vocab, uint32_t top_k, size_t* bytes);
+int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
+                    uint32_t T, uint32_t in, uint32_t vocab, uint32_t group, const int32_t* tokens, float* logprob,
+                    float* entropy, uint32_t top_k, int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes);
+
+/* ------------------------------------------------------------------ */
 /* Checkpoint loading: safetensors -> HBM-resident expert table        */
 /* (replaces Qwen3MoeConfig::from_file model.rs:26-30,                 */
 /*  Weights::load_non_expert weight_loader.rs:19-71, ExpertIndex::open */

@@ -1,0 +1,798 @@
+// obs_logprobs.hip — log probabilities of given tokens, the entropy and the most
+// likely alternatives, from logits (obs_token_logprobs) or from hidden rows and the
+// 4-bit output matrix (obs_lm_logprobs).
+//
+// With m the largest of a set of logits, s = sum e and w = sum e (x - m),
+// e = exp(x - m), sets are joined by taking s and w to the larger maximum
+// (w' = f (w + s (m - m')), f = exp(m - m')). Of the whole row
+//   log p(t) = x_t - m - log s,   entropy = log s - w / s,
+// sums of one sign each. The k largest of a row lie in the k tiles of 256 (512)
+// logits with the largest maxima, ties to the lower tile, so only those are looked
+// through.
+#include <algorithm>
+
+#include "obs_internal.hpp"
+#include "obs_paged.hpp"
+
+namespace {
+using namespace obsd;
+
+constexpr float LOG2E = 1.44269504088896341f, FAR = -1.0e4f;
+constexpr uint32_t MAX_TOP = 64;
+
+struct Stat {
+  float m = NEG_INF, s = 0.0f, w = 0.0f;
+};
+__device__ __forceinline__ Stat stat_of(const float4& v) {
+  Stat r;
+  r.m = v.x;
+  r.s = v.y;
+  r.w = v.z;
+  return r;
+}
+// s and w taken to the maximum m (a set without a logit above -inf has s = w = 0; NaN stays)
+__device__ __forceinline__ void stat_to(Stat& a, float m) {
+  const float d = fmaxf(a.m - (m == NEG_INF ? 0.0f : m), FAR), f = __builtin_amdgcn_exp2f(d * LOG2E);
+  a.w = f * __builtin_fmaf(a.s, d, a.w);
+  a.s *= f;
+  a.m = m;
+}
+template <uint32_t N>
+__device__ __forceinline__ void stat_add(Stat& a, const float (&x)[N], float top) {  // top: the largest of x
+  const float m = fmaxf(a.m, top);
+  if (m > a.m) stat_to(a, m);
+  const float mu = a.m == NEG_INF ? 0.0f : a.m;
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    const float d = x[i] - mu, e = __builtin_amdgcn_exp2f(d * LOG2E);
+    a.s += e;
+    a.w = __builtin_fmaf(e, fmaxf(d, FAR), a.w);
+  }
+}
+// Over the workgroup's four waves; s_st: four words each of three, another barrier before their next use.
+__device__ __forceinline__ Stat stat_group(Stat a, float (*s_st)[4], uint32_t lane, uint32_t wave) {
+  stat_to(a, wave_max_f32(a.m));
+  const float s = wave_sum_asc(a.s), w = wave_sum_asc(a.w);
+  if (lane == 0u) {
+    s_st[0][wave] = a.m;
+    s_st[1][wave] = s;
+    s_st[2][wave] = w;
+  }
+  __syncthreads();
+  Stat r;
+  r.m = fmaxf(fmaxf(s_st[0][0], s_st[0][1]), fmaxf(s_st[0][2], s_st[0][3]));
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) {
+    Stat b;
+    b.m = s_st[0][i];
+    b.s = s_st[1][i];
+    b.w = s_st[2][i];
+    stat_to(b, r.m);
+    r.s += b.s;
+    r.w += b.w;
+  }
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// The k largest of what a wave sees
+// ---------------------------------------------------------------------------
+// A key is a value's order-preserving image above the complement of its index:
+// larger value, larger key; of equal ones the lower index. Lane i holds the i-th
+// largest key met (0: none yet); `edge` keeps out what cannot be among the k.
+__device__ __forceinline__ uint64_t top_key(float v, uint32_t index) {
+  const uint32_t u = __float_as_uint(v + 0.0f);  // (-0 as +0)
+  return static_cast<uint64_t>((u >> 31) ? ~u : u | 0x80000000u) << 32 | ~index;
+}
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float((u >> 31) ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return ~static_cast<uint32_t>(key); }
+__device__ __forceinline__ uint64_t lane_u64(uint64_t v, uint32_t l) {
+  const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(l)));
+  const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), static_cast<int>(l)));
+  return static_cast<uint64_t>(hi) << 32 | lo;
+}
+constexpr uint64_t NONE_KEY = 0x007fffffffffffffull;  // of -inf (0x007fffff in the upper word): nothing at or below it counts
+struct Top {
+  uint64_t key = 0u, edge = NONE_KEY;
+  // every lane offers a key (0: none)
+  __device__ __forceinline__ void offer(uint64_t c, uint32_t k, uint32_t lane) {
+    for (;;) {
+      const uint64_t mask = __ballot(c > edge);
+      if (!mask) break;  // uniform
+      const uint32_t l = static_cast<uint32_t>(__builtin_ctzll(mask));
+      const uint64_t x = lane_u64(c, l);
+      const uint32_t at = static_cast<uint32_t>(__popcll(__ballot(key > x)));
+      const uint32_t lo = static_cast<uint32_t>(__shfl_up(static_cast<int>(key), 1)),
+                     hi = static_cast<uint32_t>(__shfl_up(static_cast<int>(key >> 32), 1));
+      key = lane > at ? (static_cast<uint64_t>(hi) << 32 | lo) : lane == at ? x : key;
+      const uint64_t last = lane_u64(key, k - 1u);
+      edge = last > edge ? last : edge;
+      if (lane == l) c = 0u;
+    }
+  }
+  // the k-th largest of the lanes' own largest values cannot be above the k-th of all
+  __device__ __forceinline__ void edge_from(float own, uint32_t k, uint32_t lane) {
+    int v = f32_order(own);
+    int m = 0;
+    for (uint32_t i = 0; i < k; ++i) {
+      m = wave_max_i32(v);
+      const uint32_t l = static_cast<uint32_t>(__builtin_ctzll(__ballot(v == m)));
+      if (lane == l) v = -0x7fffffff - 1;
+    }
+    const uint64_t e = top_key(f32_unorder(m), ~0u) - 1u;  // below every index of that value
+    edge = e > edge ? e : edge;
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Logits
+// ---------------------------------------------------------------------------
+// A workgroup takes one part of a row, a wave 64 * 16 logits at once: their sums,
+// and of each tile (one load of the wave: 256 logits in fp32, 512 in bf16) the
+// maximum. One pass; bound by the reading.
+template <bool BF16>
+struct Logits {
+  static constexpr uint32_t TILE = BF16 ? 512u : 256u, PER = TILE / 64u, STEP = 1024u, N = STEP / TILE;
+  // PER logits from i on (behind the row's end: -inf)
+  static __device__ __forceinline__ void load(const void* row, uint32_t i, uint32_t n, bool vec, float* x) {
+    if constexpr (BF16) {
+      const uint16_t* p = static_cast<const uint16_t*>(row) + i;
+      if (vec && i + PER <= n) {
+        const uint4 v = load_stream(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          x[2 * j] = bf16lo(w[j]);
+          x[2 * j + 1] = bf16hi(w[j]);
+        }
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) x[j] = i + j < n ? bf16_to_f32(p[j]) : NEG_INF;
+      }
+    } else {
+      const float* p = static_cast<const float*>(row) + i;
+      if (vec && i + PER <= n) {
+        const uint4 v = load_stream(p);
+        x[0] = __uint_as_float(v.x);
+        x[1] = __uint_as_float(v.y);
+        x[2] = __uint_as_float(v.z);
+        x[3] = __uint_as_float(v.w);
+      } else {
+#pragma unroll
+        for (uint32_t j = 0; j < PER; ++j) x[j] = i + j < n ? p[j] : NEG_INF;
+      }
+    }
+  }
+};
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) logits_part_kernel(const uint8_t* __restrict__ logits, size_t row_bytes,
+                                                          uint32_t vocab, uint32_t parts, float4* __restrict__ stat,
+                                                          float* __restrict__ tmax, uint32_t tiles) {
+  typedef Logits<BF16> L;
+  __shared__ float s_st[3][4];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6);
+  const uint32_t t = blockIdx.x / parts, part = blockIdx.x % parts;
+  const uint8_t* row = logits + t * row_bytes;
+  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15u) == 0u;
+  const uint32_t steps = (vocab + L::STEP - 1u) / L::STEP;
+  Stat a;
+  for (uint32_t s = 4u * part + wave; s < steps; s += 4u * parts) {
+    float x[L::N][L::PER];
+#pragma unroll
+    for (uint32_t j = 0; j < L::N; ++j) L::load(row, s * L::STEP + j * L::TILE + L::PER * lane, vocab, vec, x[j]);
+    float top[L::N];
+#pragma unroll
+    for (uint32_t j = 0; j < L::N; ++j) {
+      top[j] = x[j][0];
+#pragma unroll
+      for (uint32_t i = 1; i < L::PER; ++i) top[j] = fmaxf(top[j], x[j][i]);
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < L::N; ++j) stat_add<L::PER>(a, x[j], top[j]);
+    if (tmax) {  // uniform
+#pragma unroll
+      for (uint32_t j = 0; j < L::N; ++j) {
+        const float m = fmaxf(wave_max_f32(top[j]), NEG_INF);  // (a tile of NaN alone: -inf)
+        if (lane == 0u && L::N * s + j < tiles) tmax[static_cast<size_t>(t) * tiles + L::N * s + j] = m;
+      }
+    }
+  }
+  const Stat r = stat_group(a, s_st, lane, wave);
+  if (tid == 0u) stat[static_cast<size_t>(t) * parts + part] = make_float4(r.m, r.s, r.w, 0.0f);
+}
+
+struct JoinArgs {
+  const float4* stat;  // [rows][n_stat]
+  const float* tmax;   // maximum of tile i of row t at [t * tiles + i] * tstride
+  const uint8_t* logits;
+  const float* xt;  // the tokens' logits, or null: from the logits
+  const int32_t* tokens;
+  float* logprob;
+  float* entropy;
+  int32_t* top_ids;
+  float* top_lp;
+  size_t row_bytes;
+  uint32_t n_stat, tiles, tstride, vocab, k;
+};
+
+// A workgroup a row: the parts' sums joined, then the k largest.
+template <bool BF16, uint32_t TILE>
+__global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
+  constexpr uint32_t PER = TILE / 64u;
+  __shared__ float s_st[3][4];
+  __shared__ uint32_t s_tile[MAX_TOP];
+  __shared__ uint64_t s_key[4][MAX_TOP];
+  __shared__ uint64_t s_edge;
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), t = blockIdx.x;
+  const uint8_t* row = p.logits + t * p.row_bytes;
+  auto logit = [&](uint32_t i) __attribute__((always_inline)) {
+    return BF16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[i]) : reinterpret_cast<const float*>(row)[i];
+  };
+  if (p.k && wave == 3u) {  // the tiles with the k largest maxima
+    const float* tm = p.tmax + static_cast<size_t>(t) * p.tiles * p.tstride;
+    Top top;
+    float own = NEG_INF;
+    for (uint32_t i = lane; i < p.tiles; i += 64u) own = fmaxf(own, tm[static_cast<size_t>(i) * p.tstride]);
+    top.edge_from(own, p.k, lane);
+    for (uint32_t i0 = 0; i0 < p.tiles; i0 += 64u) {
+      const uint32_t i = i0 + lane;
+      top.offer(i < p.tiles ? top_key(tm[static_cast<size_t>(i) * p.tstride], i) : 0u, p.k, lane);
+    }
+    if (lane < p.k) s_tile[lane] = top.key ? key_index(top.key) : 0xffffffffu;
+    // k tiles have a logit at least as large as the last of them has
+    const uint64_t last = lane_u64(top.key, p.k - 1u);
+    if (lane == 0u) s_edge = last ? top_key(key_value(last), ~0u) - 1u : NONE_KEY;
+  }
+  Stat a;
+  for (uint32_t i = tid; i < p.n_stat; i += 256u) {
+    Stat b = stat_of(p.stat[static_cast<size_t>(t) * p.n_stat + i]);
+    const float m = fmaxf(a.m, b.m);
+    stat_to(a, m);
+    stat_to(b, m);
+    a.s += b.s;
+    a.w += b.w;
+  }
+  const Stat r = stat_group(a, s_st, lane, wave);
+  const float ls = logf(r.s);
+  const bool none = r.m == NEG_INF && r.s == 0.0f;  // no logit above -inf
+  if (tid == 0u) {
+    if (p.entropy) p.entropy[t] = none ? 0.0f : ls - r.w / r.s;
+    if (p.logprob) {
+      const int32_t tok = p.tokens[t];
+      const bool there = tok >= 0 && static_cast<uint32_t>(tok) < p.vocab;
+      const float x = !there ? 0.0f : p.xt ? p.xt[t] : logit(static_cast<uint32_t>(tok));
+      p.logprob[t] = !there ? 0.0f : none ? NEG_INF : (x - r.m) - ls;
+    }
+  }
+  if (!p.k) return;
+  Top top;
+  top.edge = s_edge;
+  for (uint32_t j = wave; j < p.k; j += 4u) {
+    const uint32_t tile = uniform(s_tile[j]);
+    if (tile == 0xffffffffu) break;
+    float x[PER];
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+      const uint32_t v = tile * TILE + 64u * i + lane;
+      x[i] = v < p.vocab ? logit(v) : NEG_INF;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) top.offer(x[i] == x[i] ? top_key(x[i], tile * TILE + 64u * i + lane) : 0u, p.k, lane);
+  }
+  s_key[wave][lane] = top.key;
+  __syncthreads();
+  if (wave) return;
+  for (uint32_t i = 1; i < 4; ++i) top.offer(s_key[i][lane], p.k, lane);
+  if (lane < p.k) {
+    const bool there = top.key != 0u;
+    p.top_ids[static_cast<size_t>(t) * p.k + lane] = there ? static_cast<int32_t>(key_index(top.key)) : -1;
+    p.top_lp[static_cast<size_t>(t) * p.k + lane] = there ? (key_value(top.key) - r.m) - ls : NEG_INF;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Hidden rows and the 4-bit output matrix
+// ---------------------------------------------------------------------------
+// logit[t][v] = sum_g s (sum q x) + b (sum x) over the groups g of 64 columns, s and b
+// of (v, g). The products take q as 16 + q in bf16, exact, and the sums over a group
+// are taken to fp32 with the scale: no weight is rounded.
+// A lane (col = lane % 32, half = lane / 32) has one vocabulary row of each product
+// (v_mfma_f32_32x32x16_bf16, tokens x vocabulary), so a scale is one factor of its 16
+// sums. It loads 16 bytes of the row a group: 32 columns, the operands of four steps;
+// step s has columns 32 half + 8 s + 0, 4, 1, 5, 2, 6, 3, 7, as the nibbles come apart.
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
+constexpr uint32_t LM_COLS = 256;  // vocabulary rows of a workgroup, 64 a wave
+
+// The operands of four steps of 32 nibbles.
+__device__ __forceinline__ bf16x8_v lm_weights(uint32_t w) {
+  return __builtin_bit_cast(bf16x8_v, u32x4_v{q4_bf16<0>(w), q4_bf16<2>(w), q4_bf16<1>(w), q4_bf16<3>(w)});
+}
+// Eight columns in that order.
+__device__ __forceinline__ u32x4_v lm_order(const uint4& v) {
+  return u32x4_v{__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
+                 __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u)};
+}
+__device__ __forceinline__ float sum8(const uint4& v) {
+  return ((bf16lo(v.x) + bf16hi(v.x)) + (bf16lo(v.y) + bf16hi(v.y))) + ((bf16lo(v.z) + bf16hi(v.z)) + (bf16lo(v.w) + bf16hi(v.w)));
+}
+__device__ __forceinline__ float sum_of_8_lanes(float v) {
+  v += dpp_f32<DPP_XOR1>(v);
+  v += dpp_f32<DPP_XOR2>(v);
+  return v + dpp_f32<DPP_HALF_MIRROR>(v);
+}
+
+struct LmArgs {
+  const uint16_t* x;
+  const uint32_t* w;
+  const uint16_t* s;
+  const uint16_t* b;
+  const int32_t* tokens;
+  float* xt;
+  float4* stat;   // [T][tiles]
+  float* logits;  // [T][ld], or null
+  uint32_t T, in, vocab, tiles, ld;
+};
+
+// A row's 256 logits of the workgroup in LDS: the sums of them, the token's own, and
+// the logits where they are wanted. A wave takes a row.
+__device__ __forceinline__ void lm_row(const LmArgs& p, const float* row, uint32_t t, uint32_t v0, uint32_t lane) {
+  const float4 v = *reinterpret_cast<const float4*>(row + 4u * lane);
+  float x[4] = {v.x, v.y, v.z, v.w};
+  const uint32_t at = v0 + 4u * lane;
+  if (p.logits && at < p.ld) *reinterpret_cast<float4*>(p.logits + static_cast<size_t>(t) * p.ld + at) = v;
+  if (p.tokens) {
+    const uint32_t k = static_cast<uint32_t>(p.tokens[t]) - at;
+    if (k < 4u && at + k < p.vocab) p.xt[t] = x[k];
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < 4; ++i) x[i] = at + i < p.vocab ? x[i] : NEG_INF;
+  const float m = fmaxf(wave_max_f32(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))), NEG_INF);  // (of NaN alone: -inf)
+  Stat a;
+  a.m = m;
+  stat_add<4>(a, x, m);
+  const float s = wave_sum_asc(a.s), w = wave_sum_asc(a.w);
+  if (lane == 0u) p.stat[static_cast<size_t>(t) * p.tiles + v0 / LM_COLS] = make_float4(m, s, w, 0.0f);
+}
+
+// Up to RT tokens: the weights go through once, 256 vocabulary rows a workgroup, and
+// bound the call. The rows come in by 256 columns through LDS.
+template <uint32_t RT>
+__global__ void __launch_bounds__(256, 2) lm_few_kernel(LmArgs p) {
+  constexpr uint32_t NR = RT / 2u;                            // sums of a lane that are some token's
+  constexpr uint32_t CH = RT * 32u, CT = (CH + 255u) / 256u;  // 16-byte chunks of 256 columns, a thread's
+  constexpr uint32_t XB = RT * 512u, OB = RT * (LM_COLS + 8u) * 4u;
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[2u * XB > OB ? 2u * XB : OB];
+  __shared__ float s_sum[2][4][RT];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 31u, half = lane >> 5;
+  const uint32_t v0 = blockIdx.x * LM_COLS, groups = p.in / 64u, chunks = p.in / 256u;
+  const uint32_t* wp[2];
+  const uint16_t *sp[2], *bp[2];
+#pragma unroll
+  for (uint32_t n = 0; n < 2; ++n) {
+    const size_t v = umin(v0 + 64u * wave + 32u * n + col, p.vocab - 1u);  // (behind the last row it again)
+    wp[n] = p.w + v * (p.in / 8u) + 4u * half;
+    sp[n] = p.s + v * groups;
+    bp[n] = p.b + v * groups;
+  }
+  uint4 xr[CT];
+  auto load_x = [&](uint32_t c) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < CT; ++i) {
+      const uint32_t j = tid + 256u * i, r = j / 32u;
+      xr[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (j < CH && r < p.T) xr[i] = *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(r) * p.in + 256u * c + 8u * (j % 32u));
+    }
+  };
+  auto store_x = [&](uint32_t buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < CT; ++i) {
+      const uint32_t j = tid + 256u * i, r = j / 32u, c = j % 32u;  // chunk c: group c / 8, half c / 4 % 2, step c % 4
+      const float sum = sum_of_8_lanes(sum8(xr[i]));
+      if (j < CH) {
+        *reinterpret_cast<u32x4_v*>(s_mem + buf * XB + 16u * (((c / 8u * 4u + c % 4u) * 2u + c / 4u % 2u) * RT + r)) = lm_order(xr[i]);
+        if (c % 8u == 0u) s_sum[buf][c / 8u][r] = sum;
+      }
+    }
+  };
+  f32x16_v acc[2] = {};
+  u32x4_v wr[4][2];  // the weights of four groups (a line of each row), scales and biases of them
+  u32x2_v sr[2], br[2];
+  auto load_w = [&](uint32_t c, uint32_t g) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) wr[g][n] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_v*>(wp[n] + 32u * c + 8u * g));
+  };
+  auto load_s = [&](uint32_t c) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+      sr[n] = *reinterpret_cast<const u32x2_v*>(sp[n] + 4u * c);
+      br[n] = *reinterpret_cast<const u32x2_v*>(bp[n] + 4u * c);
+    }
+  };
+  load_x(0u);
+#pragma unroll
+  for (uint32_t g = 0; g < 4; ++g) load_w(0u, g);
+  load_s(0u);
+  store_x(0u);
+  __syncthreads();
+  for (uint32_t c = 0; c < chunks; ++c) {
+    const uint32_t buf = c & 1u;
+    const uint32_t next = umin(c + 1u, chunks - 1u);
+    if (c + 1u < chunks) load_x(c + 1u);  // uniform
+    u32x2_v s0[2] = {sr[0], sr[1]}, b0[2] = {br[0], br[1]};
+    load_s(next);
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g) {
+      bf16x8_v xa[4];
+#pragma unroll
+      for (uint32_t s = 0; s < 4; ++s)
+        xa[s] = *reinterpret_cast<const bf16x8_v*>(s_mem + buf * XB + 16u * (((g * 4u + s) * 2u + half) * RT + col % RT));
+      float xs[NR];
+#pragma unroll
+      for (uint32_t i = 0; i < NR; ++i) xs[i] = s_sum[buf][g][8u * (i / 4u) + 4u * half + i % 4u];
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n) {
+        f32x16_v y = {};
+#pragma unroll
+        for (uint32_t s = 0; s < 4; ++s)
+          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[s], lm_weights(wr[g][n][s]), y, 0, 0, 0);
+        const uint32_t sw = g < 2u ? s0[n].x : s0[n].y, bw = g < 2u ? b0[n].x : b0[n].y;
+        const float sc = g & 1u ? bf16hi(sw) : bf16lo(sw), bi = g & 1u ? bf16hi(bw) : bf16lo(bw);
+        const float off = __builtin_fmaf(sc, -16.0f, bi);
+#pragma unroll
+        for (uint32_t i = 0; i < NR; ++i) acc[n][i] = __builtin_fmaf(sc, y[i], __builtin_fmaf(off, xs[i], acc[n][i]));
+      }
+      load_w(next, g);  // the next four groups', as soon as this one is used (behind the last chunk it again)
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (c + 1u < chunks) store_x(buf ^ 1u);  // uniform
+    __syncthreads();
+  }
+  float(*const s_out)[LM_COLS + 8u] = reinterpret_cast<float(*)[LM_COLS + 8u]>(s_mem);
+#pragma unroll
+  for (uint32_t n = 0; n < 2; ++n)
+#pragma unroll
+    for (uint32_t i = 0; i < NR; ++i) s_out[8u * (i / 4u) + 4u * half + i % 4u][64u * wave + 32u * n + col] = acc[n][i];
+  __syncthreads();
+  for (uint32_t t = wave; t < p.T; t += 4u) lm_row(p, s_out[t], t, v0, lane);
+}
+
+// Many tokens. First their rows in the order of the products' operands, [tile of 32 MT
+// rows][group][32 rows][step][lane] 16 bytes, and the sums of every group in three bf16
+// parts (24 bits), once as they are and once times -16: at the end of a tile they meet
+// the biases and the scales in products of their own, 12 instead of 2 * 16 sums a group.
+constexpr uint32_t LM_SUMS = 6;
+template <uint32_t MT>
+__global__ void __launch_bounds__(256) lm_rows_kernel(const uint16_t* __restrict__ x, uint32_t T, uint32_t in, uint8_t* __restrict__ xp,
+                                                      uint8_t* __restrict__ xs) {
+  const uint32_t tid = threadIdx.x, groups = in / 64u, gpad = (groups + 15u) & ~15u;
+  const uint32_t mt = blockIdx.x / (gpad / 8u), c0 = blockIdx.x % (gpad / 8u) * 64u;  // 32 rows, 512 columns
+#pragma unroll
+  for (uint32_t i = 0; i < 8; ++i) {
+    const uint32_t r = (tid + 256u * i) / 64u, c = c0 + (tid + 256u * i) % 64u, t = 32u * mt + r, g = c / 8u;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (t < T && g < groups) v = *reinterpret_cast<const uint4*>(x + static_cast<size_t>(t) * in + 8u * c);
+    const float sum = sum_of_8_lanes(sum8(v));
+    if (g < groups)
+      *reinterpret_cast<u32x4_v*>(xp + 16u * (((static_cast<size_t>(mt / MT) * groups + g) * MT + mt % MT) * 256u + c % 4u * 64u +
+                                              32u * (c / 4u % 2u) + r)) = lm_order(v);
+    if (c % 8u == 0u) {
+      float rest = sum;
+#pragma unroll
+      for (uint32_t k = 0; k < 3; ++k) {
+        const uint16_t part = f32_to_bf16(rest);
+        rest -= bf16_to_f32(part);
+        // steps of 16 groups, eight a lane's half
+        uint16_t* to = reinterpret_cast<uint16_t*>(xs + 16u * ((static_cast<size_t>(mt) * LM_SUMS * (gpad / 16u) + k * (gpad / 16u) + g / 16u) * 64u +
+                                                               32u * (g / 8u % 2u) + r)) + g % 8u;
+        to[0] = part;
+        to[3u * (gpad / 16u) * 512u] = f32_to_bf16(-16.0f * bf16_to_f32(part));
+      }
+    }
+  }
+}
+
+// 32 MT tokens x 256 vocabulary rows a workgroup, 64 a wave; two workgroups a CU.
+template <uint32_t MT>
+__global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t* __restrict__ xp, const uint8_t* __restrict__ xs,
+                                                         uint32_t ttiles) {
+  constexpr uint32_t XB = MT * 4096u, OROW = LM_COLS + 8u, OB = 32u * OROW * 4u;  // bytes of a group's rows; of 32 rows of logits
+  __shared__ __attribute__((aligned(16))) uint8_t s_mem[2u * XB > OB ? 2u * XB : OB];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 31u, half = lane >> 5;
+  // an XCD (blockIdx.x % 8) takes all token tiles of one column tile after another: its weights stay in its L2
+  const uint32_t at = blockIdx.x / 8u, vt = at / ttiles * 8u + blockIdx.x % 8u, tt = at % ttiles;
+  if (vt >= p.tiles) return;  // uniform
+  const uint32_t v0 = vt * LM_COLS, groups = p.in / 64u, gpad = (groups + 15u) & ~15u;
+  const uint32_t* wp[2];
+  const uint16_t *sp[2], *bp[2];
+#pragma unroll
+  for (uint32_t n = 0; n < 2; ++n) {
+    const size_t v = umin(v0 + 64u * wave + 32u * n + col, p.vocab - 1u);
+    wp[n] = p.w + v * (p.in / 8u) + 4u * half;
+    sp[n] = p.s + v * groups;
+    bp[n] = p.b + v * groups;
+  }
+  const uint8_t* xg = xp + static_cast<size_t>(tt) * groups * XB + 16u * tid;
+  u32x4_v xr[MT];
+  auto load_x = [&](uint32_t g) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < MT; ++i) xr[i] = *reinterpret_cast<const u32x4_v*>(xg + static_cast<size_t>(g) * XB + 4096u * i);
+  };
+  auto store_x = [&](uint32_t buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < MT; ++i) *reinterpret_cast<u32x4_v*>(s_mem + buf * XB + 16u * tid + 4096u * i) = xr[i];
+  };
+  f32x16_v acc[MT][2];
+#pragma unroll
+  for (uint32_t m = 0; m < MT; ++m)
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) acc[m][n] = f32x16_v{};
+  u32x4_v wr[2][2];  // two groups ahead
+  uint32_t sr[2][2];
+  auto load_w = [&](uint32_t g, uint32_t slot) __attribute__((always_inline)) {
+    const uint32_t gc = umin(g, groups - 1u);
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+      wr[slot][n] = *reinterpret_cast<const u32x4_v*>(wp[n] + 8u * gc);
+      sr[slot][n] = sp[n][gc];
+    }
+  };
+  load_x(0u);
+  load_w(0u, 0u);
+  load_w(1u, 1u);
+  store_x(0u);
+  __syncthreads();
+  auto step = [&](uint32_t g, uint32_t slot) __attribute__((always_inline)) {
+    load_x(umin(g + 1u, groups - 1u));
+    bf16x8_v wb[2][4];
+    float sc[2];
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+      sc[n] = __uint_as_float(sr[slot][n] << 16);
+#pragma unroll
+      for (uint32_t s = 0; s < 4; ++s) wb[n][s] = lm_weights(wr[slot][n][s]);
+    }
+    load_w(g + 2u, slot);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (uint32_t m = 0; m < MT; ++m) {
+      bf16x8_v xa[4];
+#pragma unroll
+      for (uint32_t s = 0; s < 4; ++s) xa[s] = *reinterpret_cast<const bf16x8_v*>(s_mem + slot * XB + 16u * ((m * 4u + s) * 64u + lane));
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n) {
+        f32x16_v y = {};
+#pragma unroll
+        for (uint32_t s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[s], wb[n][s], y, 0, 0, 0);
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) acc[m][n][i] = __builtin_fmaf(sc[n], y[i], acc[m][n][i]);
+      }
+    }
+    store_x(slot ^ 1u);
+    __syncthreads();
+  };
+  for (uint32_t g = 0; g < groups; g += 2u) {  // groups is a multiple of 8
+    step(g, 0u);
+    step(g + 1u, 1u);
+  }
+  // the groups' sums with the biases, and (times -16) with the scales
+  const uint32_t steps = gpad / 16u;
+#pragma unroll
+  for (uint32_t kind = 0; kind < 2; ++kind)
+    for (uint32_t s = 0; s < steps; ++s) {
+      const uint32_t g = 16u * s + 8u * half;
+      bf16x8_v wb[2];
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n) {
+        u32x4_v v = *reinterpret_cast<const u32x4_v*>((kind ? sp[n] : bp[n]) + umin(g, groups - 8u));
+        if (g >= groups) v = u32x4_v{0u, 0u, 0u, 0u};
+        wb[n] = __builtin_bit_cast(bf16x8_v, v);
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 3; ++k)
+#pragma unroll
+        for (uint32_t m = 0; m < MT; ++m) {
+          const bf16x8_v xa = *reinterpret_cast<const bf16x8_v*>(
+              xs + 16u * (((static_cast<size_t>(tt) * MT + m) * LM_SUMS * steps + (3u * kind + k) * steps + s) * 64u + lane));
+#pragma unroll
+          for (uint32_t n = 0; n < 2; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa, wb[n], acc[m][n], 0, 0, 0);
+        }
+    }
+  float(*const s_out)[OROW] = reinterpret_cast<float(*)[OROW]>(s_mem);
+#pragma unroll
+  for (uint32_t m = 0; m < MT; ++m) {
+    if (m) __syncthreads();
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) s_out[8u * (i / 4u) + 4u * half + i % 4u][64u * wave + 32u * n + col] = acc[m][n][i];
+    __syncthreads();
+    for (uint32_t r = wave; r < 32u; r += 4u) {
+      const uint32_t t = 32u * (tt * MT + m) + r;
+      if (t < p.T) lm_row(p, s_out[r], t, v0, lane);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+using obs::up256;
+
+struct LogitsPlan {
+  uint32_t parts, tiles;
+  size_t stat, tmax;  // bytes
+};
+LogitsPlan logits_plan(uint32_t T, uint32_t vocab, int dtype, uint32_t k) {
+  LogitsPlan d{};
+  const uint32_t tile = dtype == OBS_LOGITS_BF16 ? 512u : 256u;
+  // eight workgroups a CU, of 4,096 logits at least
+  d.parts = std::max(1u, std::min((2047u + T) / std::max(T, 1u), (vocab + 4095u) / 4096u));
+  d.tiles = (vocab + tile - 1u) / tile;
+  d.stat = up256(static_cast<size_t>(T) * d.parts * sizeof(float4));
+  d.tmax = k ? up256(static_cast<size_t>(T) * d.tiles * sizeof(float)) : 0u;
+  return d;
+}
+
+constexpr uint32_t LM_FEW = 32;
+struct LmPlan {
+  uint32_t rows, mt, tiles, ld;  // token rows of a pass, 32-row blocks of a workgroup
+  size_t stat, xt, logits, xp, xs;
+  size_t all() const { return stat + xt + logits + xp + xs; }
+};
+LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
+  LmPlan d{};
+  d.tiles = (vocab + LM_COLS - 1u) / LM_COLS;
+  d.ld = (vocab + 3u) & ~3u;
+  // the logits of a pass where alternatives are wanted, and its sums, are of a bounded size
+  d.rows = T <= LM_FEW ? T : std::min(T, k ? 256u : 4096u);
+  d.mt = d.rows <= 64u ? 2u : 4u;
+  const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = (d.rows + 32u * d.mt - 1u) / (32u * d.mt) * d.mt;
+  d.stat = up256(static_cast<size_t>(d.rows) * d.tiles * sizeof(float4));
+  d.xt = up256(static_cast<size_t>(d.rows) * sizeof(float));
+  d.logits = k ? up256(static_cast<size_t>(d.rows) * d.ld * sizeof(float)) : 0u;
+  if (T > LM_FEW) {
+    d.xp = up256(blocks * 64u * in);
+    d.xs = up256(blocks * LM_SUMS * gpad * 64u);
+  }
+  return d;
+}
+
+int check_outputs(obs_ctx* ctx, const char* who, const int32_t* tokens, const float* logprob, uint32_t top_k, uint32_t vocab,
+                  const int32_t* top_ids, const float* top_logprobs) {
+  if ((tokens == nullptr) != (logprob == nullptr) || (top_k && (!top_ids || !top_logprobs)))
+    return obs::set_error(ctx, OBS_E_INVALID, "%s: tokens and logprob go together, and top_k needs its outputs", who);
+  if (top_k > MAX_TOP || top_k > vocab)
+    return obs::set_error(ctx, OBS_E_SHAPE, "%s: top_k must be at most %u and at most vocab (got %u)", who, MAX_TOP, top_k);
+  return OBS_OK;
+}
+int check_logits(obs_ctx* ctx, const char* who, uint32_t T, uint32_t vocab, int dtype) {
+  if (dtype != OBS_LOGITS_F32 && dtype != OBS_LOGITS_BF16)
+    return obs::set_error(ctx, OBS_E_INVALID, "%s: dtype must be OBS_LOGITS_F32 or OBS_LOGITS_BF16 (got %d)", who, dtype);
+  if (vocab == 0 || vocab > (1u << 24) || T > (1u << 24))
+    return obs::set_error(ctx, OBS_E_SHAPE, "%s: vocab must be in [1, 2^24], rows at most 2^24 (got %u, %u)", who, vocab, T);
+  return OBS_OK;
+}
+int check_lm(obs_ctx* ctx, const char* who, uint32_t T, uint32_t in, uint32_t vocab, uint32_t group) {
+  if (group != 64u || in == 0 || in % 512u || in > 16384u || vocab == 0 || vocab > (1u << 24) || T > (1u << 24))
+    return obs::set_error(ctx, OBS_E_SHAPE,
+                          "%s: group must be 64, in a multiple of 512 up to 16,384, vocab in [1, 2^24], rows at most 2^24 (got %u, %u, %u, %u)",
+                          who, group, in, vocab, T);
+  return OBS_OK;
+}
+
+template <uint32_t MT>
+int launch_many(obs_ctx* ctx, const LmArgs& a, uint8_t* xp, uint8_t* xs) {
+  const uint32_t ttiles = (a.T + 32u * MT - 1u) / (32u * MT), gpad = (a.in / 64u + 15u) & ~15u;
+  OBS_LAUNCH(ctx, "lm_rows", lm_rows_kernel<MT><<<ttiles * MT * (gpad / 8u), 256, 0, ctx->stream>>>(a.x, a.T, a.in, xp, xs));
+  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT><<<(a.tiles + 7u) / 8u * 8u * ttiles, 256, 0, ctx->stream>>>(a, xp, xs, ttiles));
+  return OBS_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int obs_token_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t vocab, int dtype, uint32_t top_k, size_t* bytes) {
+  if (!ctx || !bytes) return OBS_E_INVALID;
+  *bytes = 0;
+  const char* who = "obs_token_logprobs_workspace";
+  int rc = check_logits(ctx, who, T, vocab, dtype);
+  if (rc != OBS_OK) return rc;
+  const LogitsPlan d = logits_plan(T, vocab, dtype, top_k);
+  *bytes = d.stat + d.tmax;
+  return OBS_OK;
+}
+
+int obs_token_logprobs(obs_ctx* ctx, const void* logits, int dtype, uint32_t T, uint32_t vocab, uint32_t ld, const int32_t* tokens,
+                       float* logprob, float* entropy, uint32_t top_k, int32_t* top_ids, float* top_logprobs, void* ws,
+                       size_t ws_bytes) {
+  if (!ctx) return OBS_E_INVALID;
+  const char* who = "obs_token_logprobs";
+  int rc = check_logits(ctx, who, T, vocab, dtype);
+  if (rc == OBS_OK) rc = check_outputs(ctx, who, tokens, logprob, top_k, vocab, top_ids, top_logprobs);
+  if (rc != OBS_OK) return rc;
+  ld = ld ? ld : vocab;
+  if (ld < vocab) return obs::set_error(ctx, OBS_E_SHAPE, "%s: row stride %u holds no row of %u", who, ld, vocab);
+  const LogitsPlan d = logits_plan(T, vocab, dtype, top_k);
+  if (T == 0) return OBS_OK;
+  if (!logits || !ws) return obs::set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+  const bool bf16 = dtype == OBS_LOGITS_BF16;
+  if (!obs::aligned(logits, bf16 ? 2 : 4) || !obs::aligned(ws, 16))
+    return obs::set_error(ctx, OBS_E_ALIGN, "%s: logits must be aligned to their type, the workspace to 16 bytes", who);
+  if (ws_bytes < d.stat + d.tmax)
+    return obs::set_error(ctx, OBS_E_NOMEM, "%s: workspace %zu bytes < %zu needed", who, ws_bytes, d.stat + d.tmax);
+  rc = obs::check_grid(ctx, who, static_cast<uint64_t>(T) * d.parts, 256u);
+  if (rc != OBS_OK) return rc;
+  obs::DeviceGuard guard(ctx);
+  uint8_t* wb = static_cast<uint8_t*>(ws);
+  float4* stat = reinterpret_cast<float4*>(wb);
+  float* tmax = top_k ? reinterpret_cast<float*>(wb + d.stat) : nullptr;
+  const uint8_t* lp = static_cast<const uint8_t*>(logits);
+  const size_t row_bytes = static_cast<size_t>(ld) * (bf16 ? 2u : 4u);
+  const JoinArgs j{stat, tmax, lp, nullptr, tokens, logprob, entropy, top_ids, top_logprobs, row_bytes, d.parts, d.tiles, 1u, vocab, top_k};
+  if (bf16) {
+    OBS_LAUNCH(ctx, "logits_part", logits_part_kernel<true><<<T * d.parts, 256, 0, ctx->stream>>>(lp, row_bytes, vocab, d.parts, stat, tmax, d.tiles));
+    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<true, 512><<<T, 256, 0, ctx->stream>>>(j));
+  } else {
+    OBS_LAUNCH(ctx, "logits_part", logits_part_kernel<false><<<T * d.parts, 256, 0, ctx->stream>>>(lp, row_bytes, vocab, d.parts, stat, tmax, d.tiles));
+    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, 256><<<T, 256, 0, ctx->stream>>>(j));
+  }
+  return OBS_OK;
+}
+
+int obs_lm_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t in, uint32_t vocab, uint32_t top_k, size_t* bytes) {
+  if (!ctx || !bytes) return OBS_E_INVALID;
+  *bytes = 0;
+  int rc = check_lm(ctx, "obs_lm_logprobs_workspace", T, in, vocab, 64u);
+  if (rc != OBS_OK) return rc;
+  *bytes = lm_plan(T, in, vocab, top_k).all();
+  return OBS_OK;
+}
+
+int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const uint16_t* scales, const uint16_t* biases, uint32_t T,
+                    uint32_t in, uint32_t vocab, uint32_t group, const int32_t* tokens, float* logprob, float* entropy,
+                    uint32_t top_k, int32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes) {
+  if (!ctx) return OBS_E_INVALID;
+  const char* who = "obs_lm_logprobs";
+  int rc = check_lm(ctx, who, T, in, vocab, group);
+  if (rc == OBS_OK) rc = check_outputs(ctx, who, tokens, logprob, top_k, vocab, top_ids, top_logprobs);
+  if (rc != OBS_OK) return rc;
+  if (T == 0) return OBS_OK;
+  if (!x || !w || !scales || !biases || !ws) return obs::set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
+  if (!obs::aligned(x, 16) || !obs::aligned(w, 16) || !obs::aligned(scales, 16) || !obs::aligned(biases, 16) || !obs::aligned(ws, 16))
+    return obs::set_error(ctx, OBS_E_ALIGN, "%s: x, the weight, scales, biases and the workspace must be 16-byte aligned", who);
+  const LmPlan d = lm_plan(T, in, vocab, top_k);
+  if (ws_bytes < d.all()) return obs::set_error(ctx, OBS_E_NOMEM, "%s: workspace %zu bytes < %zu needed", who, ws_bytes, d.all());
+  rc = obs::check_grid(ctx, who, static_cast<uint64_t>(d.tiles + 7u) * ((d.rows + 63u) / 64u), 256u);
+  if (rc != OBS_OK) return rc;
+  obs::DeviceGuard guard(ctx);
+  uint8_t* wb = static_cast<uint8_t*>(ws);
+  float4* stat = reinterpret_cast<float4*>(wb);
+  float* xt = reinterpret_cast<float*>(wb + d.stat);
+  float* logits = top_k ? reinterpret_cast<float*>(wb + d.stat + d.xt) : nullptr;
+  uint8_t *xp = wb + d.stat + d.xt + d.logits, *xs = xp + d.xp;
+  for (uint32_t t0 = 0; t0 < T; t0 += d.rows) {
+    const uint32_t n = std::min(d.rows, T - t0);
+    const LmArgs a{x + static_cast<size_t>(t0) * in, w, scales, biases, tokens ? tokens + t0 : nullptr, xt, stat, logits, n, in, vocab, d.tiles, d.ld};
+    if (T <= 8u)
+      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<8><<<d.tiles, 256, 0, ctx->stream>>>(a));
+    else if (T <= 16u)
+      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<16><<<d.tiles, 256, 0, ctx->stream>>>(a));
+    else if (T <= LM_FEW)
+      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<32><<<d.tiles, 256, 0, ctx->stream>>>(a));
+    else if ((rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xs) : launch_many<4>(ctx, a, xp, xs)) != OBS_OK)
+      return rc;
+    const JoinArgs j{stat, reinterpret_cast<const float*>(stat), reinterpret_cast<const uint8_t*>(logits), xt, a.tokens,
+                     logprob ? logprob + t0 : nullptr, entropy ? entropy + t0 : nullptr,
+                     top_k ? top_ids + static_cast<size_t>(t0) * top_k : nullptr,
+                     top_k ? top_logprobs + static_cast<size_t>(t0) * top_k : nullptr, static_cast<size_t>(d.ld) * sizeof(float),
+                     d.tiles, d.tiles, 4u, vocab, top_k};
+    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, LM_COLS><<<n, 256, 0, ctx->stream>>>(j));
+  }
+  return OBS_OK;
+}
+
+}  // extern "C"

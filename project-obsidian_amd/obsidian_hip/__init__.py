@@ -36,6 +36,7 @@ OBS_E_UNSUPPORTED = -6
 OBS_DECODE_AUTO, OBS_DECODE_MULTI, OBS_DECODE_FUSED = 0, 1, 2
 OBS_PATH_FUSED_DECODE, OBS_PATH_FUSED_ATTN, OBS_PATH_FFN_ONE_LAUNCH = 1, 2, 4  # obs_dispatch_gate bits
 KV_BF16, KV_E4M3, KV_Q4 = 0, 1, 4  # OBS_KV_*: what a paged cache holds (PagedKv.dtype)
+LOGITS_F32, LOGITS_BF16 = 0, 1  # OBS_LOGITS_*: the type of token_logprobs' logits
 # routing rules (obs_route_topk, MoeConfig.route_rule)
 ROUTE_REF, ROUTE_F32 = 0, 1
 
@@ -65,6 +66,7 @@ EXPORTS = (
     "obs_attn_decode", "obs_layer_decode", "obs_dispatch_gate", "obs_dispatch_info", "obs_set_dispatch_facts", "obs_debug_ffn_wait",
     "obs_measure_read", "obs_measure_mfma",
     "obs_attn_prep_paged", "obs_sdpa_paged_workspace", "obs_sdpa_paged_decode", "obs_sdpa_paged_prefill", "obs_kv_evict",
+    "obs_token_logprobs_workspace", "obs_token_logprobs", "obs_lm_logprobs_workspace", "obs_lm_logprobs",
 )
 
 
@@ -220,6 +222,10 @@ def lib() -> C.CDLL:
                                          u32, vp, sz]),
         "obs_kv_evict": (i32, [vp, C.POINTER(ObsPagedKv), C.POINTER(ObsPagedSeqs), C.POINTER(ObsKvWeight), vp, u32,
                                C.POINTER(ObsKvWeight), u32, u32, u32, vp, vp]),
+        "obs_token_logprobs_workspace": (i32, [vp, u32, u32, i32, u32, C.POINTER(sz)]),
+        "obs_token_logprobs": (i32, [vp, vp, i32, u32, u32, u32, vp, vp, vp, u32, vp, vp, vp, sz]),
+        "obs_lm_logprobs_workspace": (i32, [vp, u32, u32, u32, u32, C.POINTER(sz)]),
+        "obs_lm_logprobs": (i32, [vp, vp, vp, vp, vp, u32, u32, u32, u32, vp, vp, vp, u32, vp, vp, vp, sz]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -583,6 +589,34 @@ class ObsidianExecutor:
         gathered weight) and copies them to other pages."""
         self._check(lib().obs_kv_evict(self.ctx, kv.ref, seqs.ref, weight.ref, _ptr(dst_pages), dst_max_pages,
                                        dst_weight.ref, sinks, recent, budget, _ptr(kept), _ptr(new_len)))
+
+    # -- log probabilities (no reference counterpart) ----------------------
+    def token_logprobs_workspace(self, T: int, vocab: int, top_k: int = 0, dtype: int = LOGITS_F32) -> int:
+        n = C.c_size_t()
+        self._check(lib().obs_token_logprobs_workspace(self.ctx, T, vocab, dtype, top_k, C.byref(n)))
+        return n.value
+
+    def token_logprobs(self, logits, T: int, vocab: int, ws, ws_bytes: Optional[int] = None, tokens=None, logprob=None,
+                       entropy=None, top_k: int = 0, top_ids=None, top_logprobs=None, dtype: int = LOGITS_F32,
+                       ld: int = 0) -> None:
+        """Of T rows of logits: the tokens' log probabilities, the entropies, and the top_k most likely
+        ids with theirs."""
+        ws_bytes = ws.nbytes if ws_bytes is None else ws_bytes
+        self._check(lib().obs_token_logprobs(self.ctx, _ptr(logits), dtype, T, vocab, ld, _ptr(tokens), _ptr(logprob),
+                                             _ptr(entropy), top_k, _ptr(top_ids), _ptr(top_logprobs), _ptr(ws), ws_bytes))
+
+    def lm_logprobs_workspace(self, T: int, in_f: int, vocab: int, top_k: int = 0) -> int:
+        n = C.c_size_t()
+        self._check(lib().obs_lm_logprobs_workspace(self.ctx, T, in_f, vocab, top_k, C.byref(n)))
+        return n.value
+
+    def lm_logprobs(self, x, w, s, b, T: int, in_f: int, vocab: int, ws, ws_bytes: Optional[int] = None, tokens=None,
+                    logprob=None, entropy=None, top_k: int = 0, top_ids=None, top_logprobs=None, group: int = 64) -> None:
+        """token_logprobs of the logits of T normalised hidden rows and a 4-bit output matrix."""
+        ws_bytes = ws.nbytes if ws_bytes is None else ws_bytes
+        self._check(lib().obs_lm_logprobs(self.ctx, _ptr(x), _ptr(w), _ptr(s), _ptr(b), T, in_f, vocab, group, _ptr(tokens),
+                                          _ptr(logprob), _ptr(entropy), top_k, _ptr(top_ids), _ptr(top_logprobs),
+                                          _ptr(ws), ws_bytes))
 
     def download_raw(self, ptr: int, shape, dtype) -> np.ndarray:
         """Copies device bytes at `ptr` into a new host array (Buffer::contents after a drain)."""
