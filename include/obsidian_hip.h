@@ -484,7 +484,7 @@ int obs_sdpa_prefill(obs_ctx* ctx, const uint16_t* q, const uint16_t* k_cache, c
  * in e4m3 (OCP, magnitudes up to 448) with one positive fp32 scale per kv head: an
  * entry is the stored value times the scale. Or in 4 bits (OBS_KV_Q4), affine in
  * groups of 64 dims as the weights are: a dim is q * scale + bias, q in 0 .. 15,
- * scale and bias bf16 (scales up to 2^120). A (page, kv head) of keys is then
+ * scale and bias bf16, values up to 65,504 in magnitude. A (page, kv head) of keys is then
  * [page][head_dim / 2] bytes, byte i of an entry holding dim i in its low and dim
  * i + head_dim / 2 in its high nibble, followed by uint32 [head_dim / 64][page], the
  * scale in the low and the bias in the high half; one of values [head_dim / 2][page]
@@ -535,7 +535,8 @@ typedef struct obs_kv_weight {
  * nearest even, beyond 448 to 448). In 4 bits the fp32 values of a group of 64 dims
  * get scale = bf16((max - min) / 15), bias = bf16(min) and q = (x - bias) / scale
  * to nearest even within 0 .. 15 (scale 0: q 0; a group with a value that is not
- * finite reads as NaN). q, k, v: bf16 rows of q_ld, kv_ld elements
+ * finite reads as NaN), q_out is rounded once and all
+ * angles are formed in double. q, k, v: bf16 rows of q_ld, kv_ld elements
  * (multiples of 8; 0 = dense), 16-byte aligned, so they may be column ranges of one
  * projection's output; q_out rows of q_out_ld (q_out may be q if q_out_ld == q_ld).
  * rope_len: positions lie in [0, rope_len). A row at another one writes nothing (its
@@ -578,7 +579,7 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
  * j < sinks; a row whose i is negative (len shorter than its tokens) gets zeros.
  * A row is not touched by what other rows see, NaN and infinities included.
  * The rows' own keys and values are in the pages already (obs_attn_prep_paged).
- * Entries of 4 bits enter the products rounded to bf16.
+ * Entries of 4 bits enter the products rounded to fp16.
  * out bf16 [n_rows, n_heads, head_dim]; workspace as above. */
 int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const uint16_t* q,
                            uint16_t* out, uint32_t n_heads, uint32_t window, uint32_t sinks, uint32_t q_ld, void* ws,

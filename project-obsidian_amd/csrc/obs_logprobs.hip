@@ -358,104 +358,126 @@ __device__ __forceinline__ void lm_row(const LmArgs& p, const float* row, uint32
   if (lane == 0u) p.stat[static_cast<size_t>(t) * p.tiles + v0 / LM_COLS] = make_float4(m, s, w, 0.0f);
 }
 
-// Up to RT tokens: the weights go through once, 256 vocabulary rows a workgroup, and
-// bound the call. The rows come in by 256 columns through LDS.
-template <uint32_t RT>
+// Up to 16 NT tokens: the weights go through once, 256 vocabulary rows a workgroup, and
+// bound the call, so they are loaded by whole 64-byte runs: a lane (col = lane % 16, q =
+// lane / 16) takes 16 bytes of its row, the four 128 columns. Those are two groups, so a
+// product (v_mfma_f32_16x16x32_bf16) of either takes rows that are zero where the other's
+// columns stand; the matrix units have the time. The rows of 256 columns come in
+// through LDS, the weights a chunk ahead in registers.
+template <uint32_t NT>
 __global__ void __launch_bounds__(256, 2) lm_few_kernel(LmArgs p) {
-  constexpr uint32_t NR = RT / 2u;                            // sums of a lane that are some token's
-  constexpr uint32_t CH = RT * 32u, CT = (CH + 255u) / 256u;  // 16-byte chunks of 256 columns, a thread's
+  constexpr uint32_t RT = 16u * NT, CT = 2u * NT;  // 16-byte chunks of 256 columns that a thread brings
   constexpr uint32_t XB = RT * 512u, OB = RT * (LM_COLS + 8u) * 4u;
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[2u * XB > OB ? 2u * XB : OB];
-  __shared__ float s_sum[2][4][RT];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 31u, half = lane >> 5;
+  __shared__ __attribute__((aligned(16))) float s_sum[2][4][RT];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 15u, q = lane >> 4;
   const uint32_t v0 = blockIdx.x * LM_COLS, groups = p.in / 64u, chunks = p.in / 256u;
-  const uint32_t* wp[2];
-  const uint16_t *sp[2], *bp[2];
+  uint32_t vrow[4];
 #pragma unroll
-  for (uint32_t n = 0; n < 2; ++n) {
-    const size_t v = umin(v0 + 64u * wave + 32u * n + col, p.vocab - 1u);  // (behind the last row it again)
-    wp[n] = p.w + v * (p.in / 8u) + 4u * half;
-    sp[n] = p.s + v * groups;
-    bp[n] = p.b + v * groups;
-  }
+  for (uint32_t n = 0; n < 4; ++n) vrow[n] = umin(v0 + 64u * wave + 16u * n + col, p.vocab - 1u);  // (behind the last row it again)
   uint4 xr[CT];
   auto load_x = [&](uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t i = 0; i < CT; ++i) {
       const uint32_t j = tid + 256u * i, r = j / 32u;
       xr[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (j < CH && r < p.T) xr[i] = *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(r) * p.in + 256u * c + 8u * (j % 32u));
+      if (r < p.T) xr[i] = *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(r) * p.in + 256u * c + 8u * (j % 32u));
     }
   };
   auto store_x = [&](uint32_t buf) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t i = 0; i < CT; ++i) {
-      const uint32_t j = tid + 256u * i, r = j / 32u, c = j % 32u;  // chunk c: group c / 8, half c / 4 % 2, step c % 4
+      const uint32_t j = tid + 256u * i, r = j / 32u, c = j % 32u;  // columns 128 (c / 16) + 32 (c / 4 % 4) + 8 (c % 4)
       const float sum = sum_of_8_lanes(sum8(xr[i]));
-      if (j < CH) {
-        *reinterpret_cast<u32x4_v*>(s_mem + buf * XB + 16u * (((c / 8u * 4u + c % 4u) * 2u + c / 4u % 2u) * RT + r)) = lm_order(xr[i]);
-        if (c % 8u == 0u) s_sum[buf][c / 8u][r] = sum;
-      }
+      *reinterpret_cast<u32x4_v*>(s_mem + buf * XB + 16u * (((c / 16u * 4u + c % 4u) * NT + r / 16u) * 64u + 16u * (c / 4u % 4u) + r % 16u)) =
+          lm_order(xr[i]);
+      if (c % 8u == 0u) s_sum[buf][c / 8u][r] = sum;
     }
   };
-  f32x16_v acc[2] = {};
-  u32x4_v wr[4][2];  // the weights of four groups (a line of each row), scales and biases of them
-  u32x2_v sr[2], br[2];
-  auto load_w = [&](uint32_t c, uint32_t g) __attribute__((always_inline)) {
+  f32x4_v acc[4][NT] = {};
+  struct Chunk {
+    u32x4_v w[4][2];     // 128 columns each
+    u32x2_v s[4], b[4];  // of four groups
+  } cur, nxt;
+  auto load_w = [&](Chunk& k, uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) wr[g][n] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_v*>(wp[n] + 32u * c + 8u * g));
-  };
-  auto load_s = [&](uint32_t c) __attribute__((always_inline)) {
+    for (uint32_t n = 0; n < 4; ++n) {
+      const u32x4_v* wp = reinterpret_cast<const u32x4_v*>(p.w + static_cast<size_t>(vrow[n]) * (p.in / 8u)) + 8u * c + q;
+      k.w[n][0] = wp[0];
+      k.w[n][1] = wp[4];
+    }
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) {
-      sr[n] = *reinterpret_cast<const u32x2_v*>(sp[n] + 4u * c);
-      br[n] = *reinterpret_cast<const u32x2_v*>(bp[n] + 4u * c);
+    for (uint32_t n = 0; n < 4; ++n) {
+      const size_t at = static_cast<size_t>(vrow[n]) * groups + 4u * c;
+      k.s[n] = *reinterpret_cast<const u32x2_v*>(p.s + at);
+      k.b[n] = *reinterpret_cast<const u32x2_v*>(p.b + at);
     }
   };
   load_x(0u);
-#pragma unroll
-  for (uint32_t g = 0; g < 4; ++g) load_w(0u, g);
-  load_s(0u);
+  load_w(cur, 0u);
   store_x(0u);
   __syncthreads();
+  const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
   for (uint32_t c = 0; c < chunks; ++c) {
     const uint32_t buf = c & 1u;
-    const uint32_t next = umin(c + 1u, chunks - 1u);
     if (c + 1u < chunks) load_x(c + 1u);  // uniform
-    u32x2_v s0[2] = {sr[0], sr[1]}, b0[2] = {br[0], br[1]};
-    load_s(next);
+    load_w(nxt, umin(c + 1u, chunks - 1u));
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (uint32_t g = 0; g < 4; ++g) {
-      bf16x8_v xa[4];
+    for (uint32_t h = 0; h < 2; ++h) {  // 128 columns, groups 2 h and 2 h + 1
+      f32x4_v y[2][4][NT];
 #pragma unroll
-      for (uint32_t s = 0; s < 4; ++s)
-        xa[s] = *reinterpret_cast<const bf16x8_v*>(s_mem + buf * XB + 16u * (((g * 4u + s) * 2u + half) * RT + col % RT));
-      float xs[NR];
+      for (uint32_t s = 0; s < 4; ++s) {
+        bf16x8_v xa[2][NT];
 #pragma unroll
-      for (uint32_t i = 0; i < NR; ++i) xs[i] = s_sum[buf][g][8u * (i / 4u) + 4u * half + i % 4u];
+        for (uint32_t m = 0; m < NT; ++m) {
+          const u32x4_v x = *reinterpret_cast<const u32x4_v*>(s_mem + buf * XB + 16u * (((h * 4u + s) * NT + m) * 64u + lane));
+          u32x4_v x0 = x, x1 = x;
 #pragma unroll
-      for (uint32_t n = 0; n < 2; ++n) {
-        f32x16_v y = {};
+          for (uint32_t i = 0; i < 4; ++i) {
+            x0[i] = q < 2u ? x[i] : 0u;
+            x1[i] = q < 2u ? 0u : x[i];
+          }
+          xa[0][m] = __builtin_bit_cast(bf16x8_v, x0);
+          xa[1][m] = __builtin_bit_cast(bf16x8_v, x1);
+        }
 #pragma unroll
-        for (uint32_t s = 0; s < 4; ++s)
-          y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[s], lm_weights(wr[g][n][s]), y, 0, 0, 0);
-        const uint32_t sw = g < 2u ? s0[n].x : s0[n].y, bw = g < 2u ? b0[n].x : b0[n].y;
-        const float sc = g & 1u ? bf16hi(sw) : bf16lo(sw), bi = g & 1u ? bf16hi(bw) : bf16lo(bw);
-        const float off = __builtin_fmaf(sc, -16.0f, bi);
+        for (uint32_t n = 0; n < 4; ++n) {
+          const bf16x8_v wb = lm_weights(cur.w[n][h][s]);
 #pragma unroll
-        for (uint32_t i = 0; i < NR; ++i) acc[n][i] = __builtin_fmaf(sc, y[i], __builtin_fmaf(off, xs[i], acc[n][i]));
+          for (uint32_t m = 0; m < NT; ++m)
+#pragma unroll
+            for (uint32_t g = 0; g < 2; ++g)
+              y[g][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[g][m], wb, s ? y[g][n][m] : zero, 0, 0, 0);
+        }
       }
-      load_w(next, g);  // the next four groups', as soon as this one is used (behind the last chunk it again)
-      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (uint32_t g = 0; g < 2; ++g) {
+        f32x4_v xs[NT];
+#pragma unroll
+        for (uint32_t m = 0; m < NT; ++m) xs[m] = *reinterpret_cast<const f32x4_v*>(&s_sum[buf][2u * h + g][16u * m + 4u * q]);
+#pragma unroll
+        for (uint32_t n = 0; n < 4; ++n) {
+          const uint32_t sw = cur.s[n][h], bw = cur.b[n][h];
+          const float sc = g ? bf16hi(sw) : bf16lo(sw), off = __builtin_fmaf(sc, -16.0f, g ? bf16hi(bw) : bf16lo(bw));
+#pragma unroll
+          for (uint32_t m = 0; m < NT; ++m)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) acc[n][m][i] = __builtin_fmaf(sc, y[g][n][m][i], __builtin_fmaf(off, xs[m][i], acc[n][m][i]));
+        }
+      }
     }
     if (c + 1u < chunks) store_x(buf ^ 1u);  // uniform
     __syncthreads();
+    cur = nxt;
   }
   float(*const s_out)[LM_COLS + 8u] = reinterpret_cast<float(*)[LM_COLS + 8u]>(s_mem);
 #pragma unroll
-  for (uint32_t n = 0; n < 2; ++n)
+  for (uint32_t n = 0; n < 4; ++n)
 #pragma unroll
-    for (uint32_t i = 0; i < NR; ++i) s_out[8u * (i / 4u) + 4u * half + i % 4u][64u * wave + 32u * n + col] = acc[n][i];
+    for (uint32_t m = 0; m < NT; ++m)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) s_out[16u * m + 4u * q + i][64u * wave + 16u * n + col] = acc[n][m][i];
   __syncthreads();
   for (uint32_t t = wave; t < p.T; t += 4u) lm_row(p, s_out[t], t, v0, lane);
 }
@@ -777,12 +799,10 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
   for (uint32_t t0 = 0; t0 < T; t0 += d.rows) {
     const uint32_t n = std::min(d.rows, T - t0);
     const LmArgs a{x + static_cast<size_t>(t0) * in, w, scales, biases, tokens ? tokens + t0 : nullptr, xt, stat, logits, n, in, vocab, d.tiles, d.ld};
-    if (T <= 8u)
-      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<8><<<d.tiles, 256, 0, ctx->stream>>>(a));
-    else if (T <= 16u)
-      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<16><<<d.tiles, 256, 0, ctx->stream>>>(a));
+    if (T <= 16u)
+      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<1><<<d.tiles, 256, 0, ctx->stream>>>(a));
     else if (T <= LM_FEW)
-      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<32><<<d.tiles, 256, 0, ctx->stream>>>(a));
+      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<2><<<d.tiles, 256, 0, ctx->stream>>>(a));
     else if ((rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xs) : launch_many<4>(ctx, a, xp, xs)) != OBS_OK)
       return rc;
     const JoinArgs j{stat, reinterpret_cast<const float*>(stat), reinterpret_cast<const uint8_t*>(logits), xt, a.tokens,

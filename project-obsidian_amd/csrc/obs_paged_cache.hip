@@ -258,10 +258,12 @@ __global__ void __launch_bounds__(256, KT == KT_Q4 ? 6 : 8) prep_paged_kernel(Pa
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
       const float n0 = (bf16lo(xw[i]) * inv) * bf16lo(ww[i]), n1 = (bf16hi(xw[i]) * inv) * bf16hi(ww[i]);
-      // what becomes bf16 is rounded as the stored q / k would be; a key in fewer bits only at its end
+      // what becomes bf16 is rounded as the stored q / k would be; a key in fewer bits only
+      // at its end, and so is q beside a cache in 4 bits, which equals no call without pages
       const uint32_t pr = pack_bf16_pair_rne(n0, n1);
-      nvs[2 * i] = KT != KT_BF16 && !is_q ? n0 : bf16lo(pr);
-      nvs[2 * i + 1] = KT != KT_BF16 && !is_q ? n1 : bf16hi(pr);
+      const bool once = Q4 || (F8 && !is_q);
+      nvs[2 * i] = once ? n0 : bf16lo(pr);
+      nvs[2 * i + 1] = once ? n1 : bf16hi(pr);
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -815,7 +817,8 @@ int obs_attn_prep_paged(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_se
   if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   PrepArgs p{q, k, v, q_norm, k_norm, q_out, pos, nullptr, n_heads, rope_len, q_ld, kv_ld, q_out_ld, eps};
-  rc = obs::ensure_rope_table(ctx, theta, rope_len, &p.rope, obs::ROPE_EXACT_FROM, obs::rope_rows(rope_len));
+  const uint32_t exact_from = kv->dtype == OBS_KV_Q4 ? 0u : obs::ROPE_EXACT_FROM;
+  rc = obs::ensure_rope_table(ctx, theta, rope_len, &p.rope, exact_from, obs::rope_rows(rope_len));
   if (rc != OBS_OK) return rc;
   const Paged a = obs::paged_args(ctx, kv, seqs);
   const Weight w = obs::weight_args(weight);

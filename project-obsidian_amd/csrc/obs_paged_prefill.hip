@@ -152,9 +152,38 @@ __device__ __forceinline__ PrefillItem prefill_part(const Paged& a, const PagedA
   return {a.n_seqs, 0u, 0u, 1u, 0u, 0u, {0u, 0u}, 0u};
 }
 
+// The products' operands: bf16, or fp16 over entries of 4 bits.
+typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
+template <bool F16>
+struct Ops {
+  typedef bf16x8_v V;
+  static __device__ __forceinline__ f32x16_v mfma(V a, V b, const f32x16_v& c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16_pair_rne(lo, hi); }
+  static __device__ __forceinline__ float add_pair(uint32_t w, float acc) {
+    typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, w), __builtin_bit_cast(bf16x2_v, 0x3f803f80u), acc, false);
+  }
+  static constexpr uint32_t EXP = 0x7f807f80u, ULP = 0x00800080u;  // exponents of a pair, one in their last places
+};
+template <>
+struct Ops<true> {
+  typedef f16x8_v V;
+  static __device__ __forceinline__ f32x16_v mfma(V a, V b, const f32x16_v& c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    typedef float f32x2_v __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_v{lo, hi}), f16x2_t));
+  }
+  static __device__ __forceinline__ float add_pair(uint32_t w, float acc) {
+    return __builtin_amdgcn_fdot2(as_f16x2(w), as_f16x2(0x3c003c00u), acc, false);
+  }
+  static constexpr uint32_t EXP = 0x7c007c00u, ULP = 0x04000400u;
+};
+
 template <uint32_t HD, uint32_t KT>
 __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, PagedAttn p) {
   constexpr bool F8 = KT == KT_E4M3, Q4 = KT == KT_Q4;
+  typedef Ops<Q4> O;
+  typedef typename O::V OpV;
   constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = KT == KT_BF16 ? 2u : 1u;
   constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
   constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
@@ -192,7 +221,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   // for the join (row arrays that decrease make more tiles than rows allow: those are dropped)
   if (p.target && it.split == 0u && tid == 0u && it.place * a.n_kv + kv < p.tiles)
     reinterpret_cast<uint4*>(p.plan)[static_cast<size_t>(it.place) * a.n_kv + kv] = make_uint4(it.first, it.splits, t0r, t1r);
-  const float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
+  float scale = F8 ? __uint_as_float(uniform(__float_as_uint(p.scale_log2 * a.k_scale[kv]))) : p.scale_log2;
   if (tid == 0u) s_bad = 0u;
 
   // the wave's columns: limits, state
@@ -220,7 +249,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
   };
-  bf16x8_v qb[KS];
+  OpV qb[KS];
   auto take_queries = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t k4 = 0; k4 < HD / 32u; ++k4) {  // 32 dims at a time
@@ -232,8 +261,30 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       wave_sync();
 #pragma unroll
       for (uint32_t j = 0; j < 2; ++j)
-        qb[2u * k4 + j] = *reinterpret_cast<const bf16x8_v*>(slab + col * 80u + 32u * j + 16u * half);
+        qb[2u * k4 + j] = *reinterpret_cast<const OpV*>(slab + col * 80u + 32u * j + 16u * half);
       wave_sync();
+    }
+    if constexpr (Q4) {
+      // queries keep bf16's range: a power of two brings the column's largest to 2^14
+      float most = 0.0f;
+#pragma unroll
+      for (uint32_t ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const uint32_t w = __builtin_bit_cast(u32x4_v, qb[ks])[i];
+          most = fmaxf(most, fmaxf(fabsf(bf16lo(w)), fabsf(bf16hi(w))));
+        }
+      most = fmaxf(most, lane_xor32_f32(most, lane));
+      const uint32_t e = max(__float_as_uint(most) >> 23, 15u);
+      const float up = __uint_as_float((268u - e) << 23);
+      scale *= __uint_as_float((e - 14u) << 23);
+#pragma unroll
+      for (uint32_t ks = 0; ks < KS; ++ks) {
+        u32x4_v w = __builtin_bit_cast(u32x4_v, qb[ks]);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) w[i] = O::pack(bf16lo(w[i]) * up, bf16hi(w[i]) * up);
+        qb[ks] = __builtin_bit_cast(OpV, w);
+      }
     }
   };
   float m = NEG_INF, l = 0.0f;
@@ -324,9 +375,10 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       return w;
     }
   };
-  // Eight nibbles (low or high ones) as bf16: q s + b in fp32, rounded once. The
-  // products of a prompt take bf16 operands (a rounding of 2^-8 at most, as a cache in
-  // bf16 has it), so that a block is widened once for all of its 384 columns.
+  // Eight nibbles (low or high ones) as fp16: q s + b in fp32, rounded once (2^-11 of
+  // it at most; in bf16 the keys' roundings were most of an output's error, 0.0043 of
+  // it where fp16 leaves the output's own 0.0017). A block is widened once for all of
+  // its 384 columns.
   auto widen4 = [&](bool high, auto par) __attribute__((always_inline)) {
     const uint32_t w0 = high ? xr.x >> 4 : xr.x, w1 = high ? xr.y >> 4 : xr.y;
     float f[8];
@@ -338,8 +390,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     f[5] = q4_value(q4_nibble<1, false>(w1), par(5));
     f[6] = q4_value(q4_nibble<2, false>(w1), par(6));
     f[7] = q4_value(q4_nibble<3, false>(w1), par(7));
-    return u32x4_v{pack_bf16_pair_rne(f[0], f[1]), pack_bf16_pair_rne(f[2], f[3]), pack_bf16_pair_rne(f[4], f[5]),
-                   pack_bf16_pair_rne(f[6], f[7])};
+    return u32x4_v{O::pack(f[0], f[1]), O::pack(f[2], f[3]), O::pack(f[4], f[5]), O::pack(f[6], f[7])};
   };
   auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
     if constexpr (Q4) {
@@ -380,7 +431,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
 #pragma unroll
           for (uint32_t q = 0; q < 4; ++q) {
             // all ones in the exponent: adding one in its last place carries into the sign's
-            const uint32_t e = (w[j][q] & 0x7f807f80u) + 0x00800080u;
+            const uint32_t e = (w[j][q] & O::EXP) + O::ULP;
             const uint32_t wild = (e & 0x80008000u) >> 15;  // bit 0, bit 16
             bad |= wild;
             w[j][q] &= ~(wild * 0xffffu);
@@ -401,8 +452,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     to = f32x16_v{};
 #pragma unroll
     for (uint32_t ks = 0; ks < KS; ++ks)
-      to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-          *reinterpret_cast<const bf16x8_v*>(&s_k[buf][krow * KROW + 16u * ks + 8u * half]), qb[ks], to, 0, 0, 0);
+      to = O::mfma(*reinterpret_cast<const OpV*>(&s_k[buf][krow * KROW + 16u * ks + 8u * half]), qb[ks], to);
   };
   auto maximum = [&](const f32x16_v& v) __attribute__((always_inline)) {
     float t = fmaxf(v[0], v[1]);
@@ -448,26 +498,23 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
           for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
       }
       const float mu = m == NEG_INF ? 0.0f : m;
-      typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
-      const bf16x2_v ones = __builtin_bit_cast(bf16x2_v, 0x3f803f80u);
-      bf16x8_v pb[2];
+      OpV pb[2];
 #pragma unroll
       for (uint32_t k2 = 0; k2 < 2; ++k2) {
         uint32_t pk[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-          pk[i] = pack_bf16_pair_rne(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i], scale, -mu)),
-                                     __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i + 1], scale, -mu)));
-          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, pk[i]), ones, l, false);
+          pk[i] = O::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i], scale, -mu)),
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i + 1], scale, -mu)));
+          l = O::add_pair(pk[i], l);
         }
-        pb[k2] = __builtin_bit_cast(bf16x8_v, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
+        pb[k2] = __builtin_bit_cast(OpV, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
       }
 #pragma unroll
       for (uint32_t k2 = 0; k2 < 2; ++k2)
 #pragma unroll
         for (uint32_t d = 0; d < DT; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              *reinterpret_cast<const bf16x8_v*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]), pb[k2], o[d], 0, 0, 0);
+          o[d] = O::mfma(*reinterpret_cast<const OpV*>(&s_v[x & 1u][(32u * d + col) * VROW + 16u * k2 + 8u * half]), pb[k2], o[d]);
       const Blk kn = block_of(x + 2u);
       // the slots of block x - 1, last read before the barrier that began this iteration
       store_k((x + 1u) & 1u);
@@ -498,7 +545,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
                 const uint32_t byte = page[((dim % (HD / 2u)) << a.lp) + (e & pmask)];
                 const uint32_t par = reinterpret_cast<const uint32_t*>(page + (HD / 2u << a.lp))[(dim / 64u << a.lp) + (e & pmask)];
                 // rounded as in the tile: what is not finite there
-                const float v = bf16_to_f32(f32_to_bf16(q4_value(static_cast<float>(byte >> (dim < HD / 2u ? 0u : 4u) & 15u), par)));
+                const float v = round_f16(q4_value(static_cast<float>(byte >> (dim < HD / 2u ? 0u : 4u) & 15u), par));
                 o[d][j] += seen && (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u ? v : 0.0f;
                 continue;
               }

@@ -10,13 +10,14 @@ to join the groups), and what they add is s (16 + q) |Q| and |b - 16 s| |Q|. P s
 enters the value product in bf16 (2^-8 of sum p s |q - 8|, the middle being split
 off), the rest of an output is fp32, off by 2^-24 of sum p s (40 + q) + p |b + 8 s| an
 addition; the output is rounded once (2^-8 of it). Prompts take entries rounded to
-bf16, which the reference does too; beyond that the bars of test_gpu_paged.py."""
+fp16, which the reference does too, and P in fp16 (2^-11 of sum p |v|, and half its
+least step, 2^-25, of every |v| where that is more); scores and the output as above."""
 import numpy as np
 import pytest
 
 import obsidian_hip as oh
 from obsidian_hip import synth
-from test_gpu_paged import (EPS, FILL16, LENS, NAN16, PREFILL, THETA, WINDOWS, _attend, _f64, _kept, _visible)
+from test_gpu_paged import (EPS, FILL16, LENS, NAN16, PREFILL, THETA, WINDOWS, _f64, _kept, _visible)
 
 pytestmark = pytest.mark.gpu
 
@@ -270,13 +271,42 @@ def test_decode_bad_pages(exe, page):
 
 # ---- prompts ------------------------------------------------------------------
 
-def _prefill_case(exe, shape, lens, new, window, sinks, seed, pad_rows=0, check_rows=None, k_std=1.0):
+def _f16(x):
+    """float64 -> nearest float32 -> nearest fp16, as float64."""
+    with np.errstate(over="ignore"):
+        return np.asarray(x, np.float32).astype(np.float16).astype(np.float64)
+
+
+def _attend16(q, k, v, vis):
+    """q [nh, hd], k, v [n, nkv, hd] -> (out, bound)."""
+    nh, hd = q.shape
+    per = nh // k.shape[1]
+    out, bound = np.zeros((nh, hd)), np.zeros((nh, hd))
+    idx = np.flatnonzero(vis)
+    if len(idx) == 0:
+        return out, bound
+    for h in range(nh):
+        kk, vv = k[idx, h // per], v[idx, h // per]
+        s = kk @ q[h] / np.sqrt(hd)
+        e = np.exp(s - s.max())
+        p = e / e.sum()
+        mag = np.max(np.abs(kk) @ np.abs(q[h])) / np.sqrt(hd)
+        err = 2 * (hd * 2.0 ** -24 * mag + 2.0 ** -21 * np.max(np.abs(s)) + 2.0 ** -20)
+        out[h] = p @ vv
+        A = p @ np.abs(vv)
+        # p is at least 1 / n of its largest: the least step is taken of that, in numerator and sum
+        bound[h] = 1.01 * (2 * 2.0 ** -11 + err) * A + 2.0 ** -24 * p.max() * (np.sum(np.abs(vv), 0) + len(idx) * A) + \
+            2.0 ** -8 * np.abs(out[h]) + 1e-30
+    return out, bound
+
+
+def _prefill_case(exe, shape, lens, new, window, sinks, seed, pad_rows=0, check_rows=None, k_std=1.0, q_std=2.0):
     nh, nkv, hd, page = shape
     rng = np.random.default_rng(seed)
     pool = Pool(exe, rng, lens, nkv, hd, page, k_std=k_std)
     rows = np.concatenate([[0], np.cumsum(new)]).astype(int)
     R = int(rows[-1])
-    q = synth.bf16_normal(rng, (R + pad_rows, nh, hd), 2.0)
+    q = synth.bf16_normal(rng, (R + pad_rows, nh, hd), q_std)
     out = exe.upload(np.full((R + pad_rows, nh, hd), FILL16, np.uint16))
     seqs = pool.seqs(rows, R + pad_rows)
     ws = exe.upload(np.full(exe.sdpa_paged_workspace(pool.kv, seqs, nh, None, window, sinks), 0xFF, np.uint8))
@@ -288,11 +318,11 @@ def _prefill_case(exe, shape, lens, new, window, sinks, seed, pad_rows=0, check_
     got = _f64(raw)
     assert np.all(raw[R:] == FILL16)
     for b, (n, t) in enumerate(zip(lens, new)):
-        k, v = (_bf(x[0] * x[1] + x[2]) for x in (pool.parts(b, "k"), pool.parts(b, "v")))
+        k, v = (_f16(x[0] * x[1] + x[2]) for x in (pool.parts(b, "k"), pool.parts(b, "v")))
         for r in (range(t) if check_rows is None else sorted({min(r, t - 1) for r in check_rows})):
             i = n - t + r
             vis = _visible(i, n, window, sinks) if i >= 0 else np.zeros(n, bool)
-            ref, bound, _, _ = _attend(_f64(q[rows[b] + r]), k, v, vis)
+            ref, bound = _attend16(_f64(q[rows[b] + r]), k, v, vis)
             g = got[rows[b] + r]
             assert np.all(np.abs(g - ref) <= bound), (b, r, i, np.max(np.abs(g - ref)))
     return call, out, pool
@@ -320,6 +350,12 @@ def test_prefill_peaked_scores(exe):
     _prefill_case(exe, (32, 4, 128, 32), [300], [300], 0, 0, 33, k_std=30.0)
 
 
+@pytest.mark.parametrize("q_std", [1e-30, 3e4, 1e30])
+def test_prefill_queries_of_any_size(exe, q_std):
+    """Queries keep bf16's range (they are brought into fp16's by a power of two a head)."""
+    _prefill_case(exe, (8, 2, 128, 16), [70], [70], 0, 0, 35, q_std=q_std, k_std=min(1.0, 1.0 / q_std))
+
+
 @pytest.mark.parametrize("window,sinks", [(0, 0), (24, 2), (90, 40)])
 @pytest.mark.parametrize("shape", [(32, 4, 128, 16), (16, 16, 64, 32), (12, 2, 128, 32)], ids=str)
 def test_hidden_entries_that_are_not_finite(exe, shape, window, sinks):
@@ -344,14 +380,15 @@ def test_hidden_entries_that_are_not_finite(exe, shape, window, sinks):
     ws1 = exe.alloc(exe.sdpa_paged_workspace(pool.kv, one, nh, None, window, sinks), np.uint8)
     exe.sdpa_paged_decode(pool.kv, one, exe.upload(q[-1:]), out1, nh, ws1, window=window, sinks=sinks)
     step = _f64(out1.download())
-    k, v = ([_bf(x[0] * x[1] + x[2]) for x in [pool.parts(0, w)]][0] for w in "kv")
+    with np.errstate(invalid="ignore"):
+        k, v = (_f16(x[0] * x[1] + x[2]) for x in (pool.parts(0, "k"), pool.parts(0, "v")))
     v[j] = 0.0
     for r in range(t):
         vis = _visible(n - t + r, n, window, sinks)
         if np.any(vis[j]):
             assert not np.any(np.isfinite(got[r])), r
         else:
-            ref, bound, _, _ = _attend(_f64(q[r]), k, v, vis)
+            ref, bound = _attend16(_f64(q[r]), k, v, vis)
             assert np.all(np.abs(got[r] - ref) <= bound), r
     assert np.any(np.isfinite(step)) != np.any(_visible(n - 1, n, window, sinks)[j])
 
@@ -359,7 +396,7 @@ def test_hidden_entries_that_are_not_finite(exe, shape, window, sinks):
 # ---- append -------------------------------------------------------------------
 
 def _rope(x, w, pos):
-    """Normed and rotated x, and what fp32 (its angles among it, as in test_gpu_paged.py) may be off."""
+    """Normed and rotated x, and what fp32 may be off (the norm and a few products; angles are formed in double)."""
     hd = x.shape[-1]
     y = x / np.sqrt(np.mean(x * x, -1, keepdims=True) + EPS) * w
     ang = pos * THETA ** (-np.arange(hd // 2) / (hd // 2))
@@ -367,7 +404,7 @@ def _rope(x, w, pos):
     a, b = y[..., :hd // 2], y[..., hd // 2:]
     r = np.concatenate([a * c - b * s, b * c + a * s], -1)
     turn = np.concatenate([np.abs(a) + np.abs(b)] * 2, -1)
-    return r, (2.0 ** -22 * max(pos, 1) + 2.0 ** -20) * turn
+    return r, 2.0 ** -20 * turn
 
 
 def _check_appended(side, raw, p, o, ref, off):
@@ -403,7 +440,8 @@ def _append_case(exe, shape, lens, new, seed, one=False, weight=True, pad_rows=0
                         EPS, THETA, 9000, weight=oh.KvWeight(dw, len(lens), cap) if weight else None, q_ld=ld, kv_ld=ld,
                         pos=None if pos is None else exe.upload(np.array(pos, np.int32)))
     exe.device_status()
-    raw_k, raw_v, w = pool.dk.download(), pool.dv.download(), dw.download()
+    raw_k, raw_v, w, got_q = pool.dk.download(), pool.dv.download(), dw.download(), q.download()
+    assert np.all(got_q[R:] == FILL16)
     xf = _f64(x)
     keep_k, keep_v = np.ones(raw_k.shape, bool), np.ones(raw_v.shape, bool)
     for b, (n, t) in enumerate(zip(lens, new)):
@@ -414,6 +452,8 @@ def _append_case(exe, shape, lens, new, seed, one=False, weight=True, pad_rows=0
             row = rows[b] + r
             at = i if pos is None else pos[row]
             k, off = _rope(xf[row, qd:qd + kd].reshape(nkv, hd), _f64(kn), at)
+            want, qoff = _rope(xf[row, :qd].reshape(nh, hd), _f64(qn), at)
+            assert np.all(np.abs(_f64(got_q[row]) - want) <= 2.0 ** -8 * np.abs(want) + 1.01 * qoff)  # rounded once
             v = xf[row, qd + kd:].reshape(nkv, hd)
             p, o = pool.table[b, i // page:i // page + 1], np.array([i % page])
             _check_appended(pool.k, raw_k, p, o, k[None], off[None])
@@ -428,7 +468,6 @@ def _append_case(exe, shape, lens, new, seed, one=False, weight=True, pad_rows=0
                 keep[p[0], :, :page * hd // 2] = d.reshape(nkv, -1)
                 keep[p[0], :, page * hd // 2:] = g.reshape(nkv, -1)
     assert np.array_equal(raw_k[keep_k], pool.k.raw[keep_k]) and np.array_equal(raw_v[keep_v], pool.v.raw[keep_v])
-    return pool, q.download(), raw_k, raw_v
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=str)
@@ -448,21 +487,9 @@ def test_append_many_rows_of_few_heads(exe, shape):
     _append_case(exe, shape, [900, 333], [800, 333], 47, weight=False)
 
 
-def test_append_positions_and_equal_queries(exe):
-    """The rotated queries are those of a cache in bf16, bit for bit; keys at positions of the caller's own."""
-    shape, lens, new = (32, 4, 128, 32), [40, 7], [9, 7]
-    pos = [100 + 3 * i for i in range(16)]
-    _, q4, _, _ = _append_case(exe, shape, lens, new, 53, pos=pos)
-    rng = np.random.default_rng(53)
-    pool = Pool(exe, rng, lens, 4, 128, 32)
-    x = synth.bf16_normal(rng, (16, 40 * 128), 2.0)
-    qn, kn = synth.norm_weight(rng, 128), synth.norm_weight(rng, 128)
-    dk, dv = (exe.zeros((pool.n_pages, 4, 32, 128), np.uint16) for _ in range(2))
-    kv = oh.PagedKv(dk, dv, pool.n_pages, 32, 4, 128)
-    dx, q = exe.upload(x), exe.alloc((16, 32, 128), np.uint16)
-    exe.attn_prep_paged(kv, pool.seqs([0, 9, 16]), dx.ptr, dx.ptr + 2 * 4096, dx.ptr + 2 * 4608, exe.upload(qn), exe.upload(kn),
-                        q, 32, EPS, THETA, 9000, q_ld=5120, kv_ld=5120, pos=exe.upload(np.array(pos, np.int32)))
-    assert np.array_equal(q.download(), q4)
+def test_append_positions(exe):
+    """Keys at positions of the caller's own."""
+    _append_case(exe, (32, 4, 128, 32), [40, 7], [9, 7], 53, pos=[100 + 3 * i for i in range(16)])
 
 
 @pytest.mark.parametrize("one", [False, True])
