@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 // sums. It loads 16 bytes of the row a group: 32 columns, the operands of four steps;
 // step s has columns 32 half + 8 s + 0, 4, 1, 5, 2, 6, 3, 7, as the nibbles come apart.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
-constexpr uint32_t LM_COLS = 256;  // vocabulary rows of a workgroup, 64 a wave
+constexpr uint32_t LM_COLS = 256, LM_FEW_COLS = 64;  // vocabulary rows of a workgroup
 
 // The operands of four steps of 32 nibbles.
 __device__ __forceinline__ bf16x8_v lm_weights(uint32_t w) {
@@ -337,149 +337,166 @@ struct LmArgs {
   uint32_t T, in, vocab, tiles, ld;
 };
 
-// A row's 256 logits of the workgroup in LDS: the sums of them, the token's own, and
-// the logits where they are wanted. A wave takes a row.
-__device__ __forceinline__ void lm_row(const LmArgs& p, const float* row, uint32_t t, uint32_t v0, uint32_t lane) {
-  const float4 v = *reinterpret_cast<const float4*>(row + 4u * lane);
-  float x[4] = {v.x, v.y, v.z, v.w};
-  const uint32_t at = v0 + 4u * lane;
-  if (p.logits && at < p.ld) *reinterpret_cast<float4*>(p.logits + static_cast<size_t>(t) * p.ld + at) = v;
+// A row's 64 N logits of the workgroup, N a lane: the sums of them, the token's own, and
+// the logits where they are wanted.
+template <uint32_t N>
+__device__ __forceinline__ void lm_row(const LmArgs& p, const float (&v)[N], uint32_t t, uint32_t v0, uint32_t lane) {
+  typedef float vec __attribute__((ext_vector_type(N)));
+  vec out;
+  float x[N];
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) x[i] = out[i] = v[i];
+  const uint32_t at = v0 + N * lane;
+  if (p.logits && at < p.ld) *reinterpret_cast<vec*>(p.logits + static_cast<size_t>(t) * p.ld + at) = out;
   if (p.tokens) {
     const uint32_t k = static_cast<uint32_t>(p.tokens[t]) - at;
-    if (k < 4u && at + k < p.vocab) p.xt[t] = x[k];
-  }
 #pragma unroll
-  for (uint32_t i = 0; i < 4; ++i) x[i] = at + i < p.vocab ? x[i] : NEG_INF;
-  const float m = fmaxf(wave_max_f32(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]))), NEG_INF);  // (of NaN alone: -inf)
+    for (uint32_t i = 0; i < N; ++i)
+      if (k == i && at + i < p.vocab) p.xt[t] = x[i];
+  }
+  float m = NEG_INF;
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    x[i] = at + i < p.vocab ? x[i] : NEG_INF;
+    m = fmaxf(m, x[i]);
+  }
+  m = fmaxf(wave_max_f32(m), NEG_INF);  // (of NaN alone: -inf)
   Stat a;
   a.m = m;
-  stat_add<4>(a, x, m);
+  stat_add<N>(a, x, m);
   const float s = wave_sum_asc(a.s), w = wave_sum_asc(a.w);
-  if (lane == 0u) p.stat[static_cast<size_t>(t) * p.tiles + v0 / LM_COLS] = make_float4(m, s, w, 0.0f);
+  if (lane == 0u) p.stat[static_cast<size_t>(t) * p.tiles + v0 / (64u * N)] = make_float4(m, s, w, 0.0f);
 }
 
-// Up to 16 NT tokens: the weights go through once, 256 vocabulary rows a workgroup, and
-// bound the call, so they are loaded by whole 64-byte runs: a lane (col = lane % 16, q =
-// lane / 16) takes 16 bytes of its row, the four 128 columns. Those are two groups, so a
-// product (v_mfma_f32_16x16x32_bf16) of either takes rows that are zero where the other's
-// columns stand; the matrix units have the time. The rows of 256 columns come in
-// through LDS, the weights a chunk ahead in registers.
-template <uint32_t NT>
-__global__ void __launch_bounds__(256, 2) lm_few_kernel(LmArgs p) {
-  constexpr uint32_t RT = 16u * NT, CT = 2u * NT;  // 16-byte chunks of 256 columns that a thread brings
-  constexpr uint32_t XB = RT * 512u, OB = RT * (LM_COLS + 8u) * 4u;
-  __shared__ __attribute__((aligned(16))) uint8_t s_mem[2u * XB > OB ? 2u * XB : OB];
-  __shared__ __attribute__((aligned(16))) float s_sum[2][4][RT];
+// Up to 16 NT tokens: the weights go through once and bound the call. A workgroup a CU
+// takes 64 vocabulary rows after another, each of its eight waves a slice of 256 columns
+// (of more than 2,048 several in turn), with the next weights in flight beside this one's
+// products; the slices meet in LDS. (Workgroups of one tile each loaded, computed and
+// ended together: 75 to 94 us a token in three shapes of them.) A lane (col = lane % 16, q
+// = lane / 16) of a product (v_mfma_f32_16x16x32_bf16) loads 16 bytes of its row, the four
+// 64, two groups; a swap of the wave's halves gives each lane 8 bytes of either (of the
+// group's 32, those from 16 (q % 2) + 8 (q / 2) on). The sums over a group's columns are a
+// product with ones. HELD: a wave has one slice, whose rows of x stay in registers.
+template <uint32_t NT, bool HELD>
+__global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
+  constexpr uint32_t RT = 16u * NT, OROW = LM_FEW_COLS + 4u, WAVES = 8;
+  __shared__ __attribute__((aligned(16))) float s_out[2][WAVES][RT][OROW];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 15u, q = lane >> 4;
-  const uint32_t v0 = blockIdx.x * LM_COLS, groups = p.in / 64u, chunks = p.in / 256u;
-  uint32_t vrow[4];
+  const uint32_t groups = p.in / 64u, slices = p.in / 256u, per = HELD ? 1u : (slices + WAVES - 1u) / WAVES;
+  uint32_t xoff[NT];
 #pragma unroll
-  for (uint32_t n = 0; n < 4; ++n) vrow[n] = umin(v0 + 64u * wave + 16u * n + col, p.vocab - 1u);  // (behind the last row it again)
-  uint4 xr[CT];
-  auto load_x = [&](uint32_t c) __attribute__((always_inline)) {
-#pragma unroll
-    for (uint32_t i = 0; i < CT; ++i) {
-      const uint32_t j = tid + 256u * i, r = j / 32u;
-      xr[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < p.T) xr[i] = *reinterpret_cast<const uint4*>(p.x + static_cast<size_t>(r) * p.in + 256u * c + 8u * (j % 32u));
-    }
+  for (uint32_t m = 0; m < NT; ++m) xoff[m] = umin(16u * m + col, p.T - 1u) * (2u * p.in) + 64u * (q & 1u) + 32u * (q >> 1);  // (behind the last token it again)
+  const u32x4_v one4 = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  const bf16x8_v ones = __builtin_bit_cast(bf16x8_v, one4);
+  const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  auto load_x = [&](uint32_t slice, uint32_t g, uint32_t s, uint32_t m) __attribute__((always_inline)) {
+    const uint8_t* xb = reinterpret_cast<const uint8_t*>(p.x) + 512u * slice;
+    return __builtin_bit_cast(bf16x8_v, lm_order(*reinterpret_cast<const uint4*>(xb + (xoff[m] + 128u * g + 16u * s))));
   };
-  auto store_x = [&](uint32_t buf) __attribute__((always_inline)) {
+  bf16x8_v xh[HELD ? 4 : 1][2][NT];
+  if constexpr (HELD) {
 #pragma unroll
-    for (uint32_t i = 0; i < CT; ++i) {
-      const uint32_t j = tid + 256u * i, r = j / 32u, c = j % 32u;  // columns 128 (c / 16) + 32 (c / 4 % 4) + 8 (c % 4)
-      const float sum = sum_of_8_lanes(sum8(xr[i]));
-      *reinterpret_cast<u32x4_v*>(s_mem + buf * XB + 16u * (((c / 16u * 4u + c % 4u) * NT + r / 16u) * 64u + 16u * (c / 4u % 4u) + r % 16u)) =
-          lm_order(xr[i]);
-      if (c % 8u == 0u) s_sum[buf][c / 8u][r] = sum;
+    for (uint32_t g = 0; g < 4; ++g)
+#pragma unroll
+      for (uint32_t s = 0; s < 2; ++s)
+#pragma unroll
+        for (uint32_t m = 0; m < NT; ++m) xh[g][s][m] = load_x(umin(wave, slices - 1u), g, s, m);
+  }
+  struct Rows {
+    u32x4_v w[4][2];     // two groups each
+    u32x2_v s[4], b[4];  // of four
+  } cur, nxt;
+  // a slice behind the last one reads the last one's, without use
+  auto load_w = [&](Rows& k, uint32_t tile, uint32_t slice) __attribute__((always_inline)) {
+    const uint32_t v0 = tile * LM_FEW_COLS;
+    const uint8_t *wb = reinterpret_cast<const uint8_t*>(p.w) + static_cast<size_t>(v0) * (p.in / 2u) + 128u * slice,
+                  *sb = reinterpret_cast<const uint8_t*>(p.s) + static_cast<size_t>(v0) * (2u * groups) + 8u * slice,
+                  *bb = reinterpret_cast<const uint8_t*>(p.b) + static_cast<size_t>(v0) * (2u * groups) + 8u * slice;
+#pragma unroll
+    for (uint32_t n = 0; n < 4; ++n) {
+      const uint32_t r = umin(16u * n + col, p.vocab - 1u - v0);  // (behind the last row it again)
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) k.w[n][h] = *reinterpret_cast<const u32x4_v*>(wb + (r * (p.in / 2u) + 16u * q + 64u * h));
+      k.s[n] = *reinterpret_cast<const u32x2_v*>(sb + r * (2u * groups));
+      k.b[n] = *reinterpret_cast<const u32x2_v*>(bb + r * (2u * groups));
     }
   };
   f32x4_v acc[4][NT] = {};
-  struct Chunk {
-    u32x4_v w[4][2];     // 128 columns each
-    u32x2_v s[4], b[4];  // of four groups
-  } cur, nxt;
-  auto load_w = [&](Chunk& k, uint32_t c) __attribute__((always_inline)) {
-#pragma unroll
-    for (uint32_t n = 0; n < 4; ++n) {
-      const u32x4_v* wp = reinterpret_cast<const u32x4_v*>(p.w + static_cast<size_t>(vrow[n]) * (p.in / 8u)) + 8u * c + q;
-      k.w[n][0] = wp[0];
-      k.w[n][1] = wp[4];
-    }
-#pragma unroll
-    for (uint32_t n = 0; n < 4; ++n) {
-      const size_t at = static_cast<size_t>(vrow[n]) * groups + 4u * c;
-      k.s[n] = *reinterpret_cast<const u32x2_v*>(p.s + at);
-      k.b[n] = *reinterpret_cast<const u32x2_v*>(p.b + at);
-    }
-  };
-  load_x(0u);
-  load_w(cur, 0u);
-  store_x(0u);
-  __syncthreads();
-  const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t c = 0; c < chunks; ++c) {
-    const uint32_t buf = c & 1u;
-    if (c + 1u < chunks) load_x(c + 1u);  // uniform
-    load_w(nxt, umin(c + 1u, chunks - 1u));
+  uint32_t tile = blockIdx.x, j = 0, buf = 0;
+  load_w(cur, tile, umin(wave, slices - 1u));
+  for (;;) {
+    // the next slice of these rows, or the first of the next ones
+    const bool end = j + 1u == per;
+    const uint32_t ntile = end ? tile + gridDim.x : tile, nj = end ? 0u : j + 1u;
+    load_w(nxt, umin(ntile, p.tiles - 1u), umin(wave + WAVES * nj, slices - 1u));
     __builtin_amdgcn_sched_barrier(0);
+    const uint32_t slice = wave + WAVES * j;
+    if (slice < slices) {  // uniform
 #pragma unroll
-    for (uint32_t h = 0; h < 2; ++h) {  // 128 columns, groups 2 h and 2 h + 1
-      f32x4_v y[2][4][NT];
+      for (uint32_t n = 0; n < 4; ++n)
 #pragma unroll
-      for (uint32_t s = 0; s < 4; ++s) {
-        bf16x8_v xa[2][NT];
+        for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-        for (uint32_t m = 0; m < NT; ++m) {
-          const u32x4_v x = *reinterpret_cast<const u32x4_v*>(s_mem + buf * XB + 16u * (((h * 4u + s) * NT + m) * 64u + lane));
-          u32x4_v x0 = x, x1 = x;
-#pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            x0[i] = q < 2u ? x[i] : 0u;
-            x1[i] = q < 2u ? 0u : x[i];
+          for (uint32_t i = 0; i < 2; ++i) {
+            const auto r = __builtin_amdgcn_permlane32_swap(cur.w[n][h][i], cur.w[n][h][i + 2u], false, false);
+            cur.w[n][h][i] = r[0];
+            cur.w[n][h][i + 2u] = r[1];
           }
-          xa[0][m] = __builtin_bit_cast(bf16x8_v, x0);
-          xa[1][m] = __builtin_bit_cast(bf16x8_v, x1);
-        }
 #pragma unroll
-        for (uint32_t n = 0; n < 4; ++n) {
-          const bf16x8_v wb = lm_weights(cur.w[n][h][s]);
-#pragma unroll
-          for (uint32_t m = 0; m < NT; ++m)
-#pragma unroll
-            for (uint32_t g = 0; g < 2; ++g)
-              y[g][n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[g][m], wb, s ? y[g][n][m] : zero, 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (uint32_t g = 0; g < 2; ++g) {
+      for (uint32_t g = 0; g < 4; ++g) {
+        bf16x8_v xa[2][NT];
         f32x4_v xs[NT];
 #pragma unroll
-        for (uint32_t m = 0; m < NT; ++m) xs[m] = *reinterpret_cast<const f32x4_v*>(&s_sum[buf][2u * h + g][16u * m + 4u * q]);
+        for (uint32_t s = 0; s < 2; ++s)
+#pragma unroll
+          for (uint32_t m = 0; m < NT; ++m) {
+            if constexpr (HELD)
+              xa[s][m] = xh[g][s][m];
+            else
+              xa[s][m] = load_x(slice, g, s, m);
+            xs[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[s][m], ones, s ? xs[m] : zero, 0, 0, 0);
+          }
 #pragma unroll
         for (uint32_t n = 0; n < 4; ++n) {
-          const uint32_t sw = cur.s[n][h], bw = cur.b[n][h];
-          const float sc = g ? bf16hi(sw) : bf16lo(sw), off = __builtin_fmaf(sc, -16.0f, g ? bf16hi(bw) : bf16lo(bw));
+          f32x4_v y[NT];
+#pragma unroll
+          for (uint32_t s = 0; s < 2; ++s) {
+            const bf16x8_v wb = lm_weights(cur.w[n][g / 2u][2u * (g & 1u) + s]);
+#pragma unroll
+            for (uint32_t m = 0; m < NT; ++m) y[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[s][m], wb, s ? y[m] : zero, 0, 0, 0);
+          }
+          const uint32_t sw = cur.s[n][g / 2u], bw = cur.b[n][g / 2u];
+          const float sc = g & 1u ? bf16hi(sw) : bf16lo(sw), off = __builtin_fmaf(sc, -16.0f, g & 1u ? bf16hi(bw) : bf16lo(bw));
 #pragma unroll
           for (uint32_t m = 0; m < NT; ++m)
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) acc[n][m][i] = __builtin_fmaf(sc, y[g][n][m][i], __builtin_fmaf(off, xs[m][i], acc[n][m][i]));
+            for (uint32_t i = 0; i < 4; ++i) acc[n][m][i] = __builtin_fmaf(sc, y[m][i], __builtin_fmaf(off, xs[m][i], acc[n][m][i]));
         }
       }
     }
-    if (c + 1u < chunks) store_x(buf ^ 1u);  // uniform
-    __syncthreads();
+    if (end) {  // uniform
+#pragma unroll
+      for (uint32_t n = 0; n < 4; ++n)
+#pragma unroll
+        for (uint32_t m = 0; m < NT; ++m) {
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) s_out[buf][wave][16u * m + 4u * q + i][16u * n + col] = acc[n][m][i];
+          acc[n][m] = zero;
+        }
+      __syncthreads();
+      for (uint32_t t = wave; t < p.T; t += WAVES) {
+        float x[1] = {0.0f};
+#pragma unroll
+        for (uint32_t w = 0; w < WAVES; ++w) x[0] += s_out[buf][w][t][lane];
+        lm_row<1>(p, x, t, tile * LM_FEW_COLS, lane);
+      }
+      buf ^= 1u;  // (read again two tiles on, behind a barrier that its readers pass first)
+      if (ntile >= p.tiles) break;
+    }
+    tile = ntile;
+    j = nj;
     cur = nxt;
   }
-  float(*const s_out)[LM_COLS + 8u] = reinterpret_cast<float(*)[LM_COLS + 8u]>(s_mem);
-#pragma unroll
-  for (uint32_t n = 0; n < 4; ++n)
-#pragma unroll
-    for (uint32_t m = 0; m < NT; ++m)
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) s_out[16u * m + 4u * q + i][64u * wave + 16u * n + col] = acc[n][m][i];
-  __syncthreads();
-  for (uint32_t t = wave; t < p.T; t += 4u) lm_row(p, s_out[t], t, v0, lane);
 }
 
 // Many tokens. First their rows in the order of the products' operands, [tile of 32 MT
@@ -634,7 +651,9 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
     __syncthreads();
     for (uint32_t r = wave; r < 32u; r += 4u) {
       const uint32_t t = 32u * (tt * MT + m) + r;
-      if (t < p.T) lm_row(p, s_out[r], t, v0, lane);
+      const float4 v = *reinterpret_cast<const float4*>(&s_out[r][4u * lane]);
+      const float x[4] = {v.x, v.y, v.z, v.w};
+      if (t < p.T) lm_row<4>(p, x, t, v0, lane);
     }
   }
 }
@@ -667,7 +686,8 @@ struct LmPlan {
 };
 LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   LmPlan d{};
-  d.tiles = (vocab + LM_COLS - 1u) / LM_COLS;
+  const uint32_t cols = T <= LM_FEW ? LM_FEW_COLS : LM_COLS;
+  d.tiles = (vocab + cols - 1u) / cols;
   d.ld = (vocab + 3u) & ~3u;
   // the logits of a pass where alternatives are wanted, and its sums, are of a bounded size
   d.rows = T <= LM_FEW ? T : std::min(T, k ? 256u : 4096u);
@@ -706,6 +726,15 @@ int check_lm(obs_ctx* ctx, const char* who, uint32_t T, uint32_t in, uint32_t vo
   return OBS_OK;
 }
 
+int launch_few(obs_ctx* ctx, const LmArgs& a) {
+  const uint32_t grid = std::min(a.tiles, static_cast<uint32_t>(std::max(ctx->num_cus, 1)));
+  auto go = [&](auto kernel) {
+    OBS_LAUNCH(ctx, "lm_few", kernel<<<grid, 512, 0, ctx->stream>>>(a));
+    return int(OBS_OK);
+  };
+  if (a.T <= 16u) return a.in <= 2048u ? go(lm_few_kernel<1, true>) : go(lm_few_kernel<1, false>);
+  return a.in <= 2048u ? go(lm_few_kernel<2, true>) : go(lm_few_kernel<2, false>);
+}
 template <uint32_t MT>
 int launch_many(obs_ctx* ctx, const LmArgs& a, uint8_t* xp, uint8_t* xs) {
   const uint32_t ttiles = (a.T + 32u * MT - 1u) / (32u * MT), gpad = (a.in / 64u + 15u) & ~15u;
@@ -799,18 +828,20 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
   for (uint32_t t0 = 0; t0 < T; t0 += d.rows) {
     const uint32_t n = std::min(d.rows, T - t0);
     const LmArgs a{x + static_cast<size_t>(t0) * in, w, scales, biases, tokens ? tokens + t0 : nullptr, xt, stat, logits, n, in, vocab, d.tiles, d.ld};
-    if (T <= 16u)
-      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<1><<<d.tiles, 256, 0, ctx->stream>>>(a));
-    else if (T <= LM_FEW)
-      OBS_LAUNCH(ctx, "lm_few", lm_few_kernel<2><<<d.tiles, 256, 0, ctx->stream>>>(a));
-    else if ((rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xs) : launch_many<4>(ctx, a, xp, xs)) != OBS_OK)
-      return rc;
+    if (T <= LM_FEW)
+      rc = launch_few(ctx, a);
+    else
+      rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xs) : launch_many<4>(ctx, a, xp, xs);
+    if (rc != OBS_OK) return rc;
     const JoinArgs j{stat, reinterpret_cast<const float*>(stat), reinterpret_cast<const uint8_t*>(logits), xt, a.tokens,
                      logprob ? logprob + t0 : nullptr, entropy ? entropy + t0 : nullptr,
                      top_k ? top_ids + static_cast<size_t>(t0) * top_k : nullptr,
                      top_k ? top_logprobs + static_cast<size_t>(t0) * top_k : nullptr, static_cast<size_t>(d.ld) * sizeof(float),
                      d.tiles, d.tiles, 4u, vocab, top_k};
-    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, LM_COLS><<<n, 256, 0, ctx->stream>>>(j));
+    if (T <= LM_FEW)
+      OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, LM_FEW_COLS><<<n, 256, 0, ctx->stream>>>(j));
+    else
+      OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, LM_COLS><<<n, 256, 0, ctx->stream>>>(j));
   }
   return OBS_OK;
 }
