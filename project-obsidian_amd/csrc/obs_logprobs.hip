@@ -113,18 +113,6 @@ struct Top {
       if (lane == l) c = 0u;
     }
   }
-  // the k-th largest of the lanes' own largest values cannot be above the k-th of all
-  __device__ __forceinline__ void edge_from(float own, uint32_t k, uint32_t lane) {
-    int v = f32_order(own);
-    int m = 0;
-    for (uint32_t i = 0; i < k; ++i) {
-      m = wave_max_i32(v);
-      const uint32_t l = static_cast<uint32_t>(__builtin_ctzll(__ballot(v == m)));
-      if (lane == l) v = -0x7fffffff - 1;
-    }
-    const uint64_t e = top_key(f32_unorder(m), ~0u) - 1u;  // below every index of that value
-    edge = e > edge ? e : edge;
-  }
 };
 
 // ---------------------------------------------------------------------------
@@ -219,78 +207,184 @@ struct JoinArgs {
   uint32_t n_stat, tiles, tstride, vocab, k;
 };
 
-// A workgroup a row: the parts' sums joined, then the k largest.
+// The largest value with its lower 16 bits clear that at least k of the lanes' keys
+// reach: two scalar instructions a bit. Keys: f32_order above the least int.
+__device__ __forceinline__ float lanes_edge(float own, uint32_t k) {
+  const uint32_t key = static_cast<uint32_t>(f32_order(own)) ^ 0x80000000u;
+  uint32_t e = 0u;
+#pragma unroll
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+    const uint32_t at = e | bit;
+    if (static_cast<uint32_t>(__popcll(__ballot(key >= at))) >= k) e = at;  // uniform
+  }
+  // (nothing below -inf)
+  return e < 0x00800000u ? NEG_INF : f32_unorder(static_cast<int>(e ^ 0x80000000u));
+}
+
+// A workgroup a row: the parts' sums joined, then the k largest. Of the tiles: what k
+// lanes of a wave reach with their own maxima keeps out all but a few, which are listed in
+// LDS and ranked by counting; the same of the k tiles' logits. Where more are listed than
+// there is room for (equal values in masses), a wave takes them one by one. The code runs
+// once, so its length counts. (A wave's lists from the start took 21 us a row of 2,374
+// tiles at k = 5; ranks of all 256 threads' maxima, and every load's listing unrolled, 17.)
 template <bool BF16, uint32_t TILE>
 __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
-  constexpr uint32_t PER = TILE / 64u;
+  constexpr uint32_t CAP = 1024, PER = TILE / 64u;
   __shared__ float s_st[3][4];
-  __shared__ uint32_t s_tile[MAX_TOP];
-  __shared__ uint64_t s_key[4][MAX_TOP];
-  __shared__ uint64_t s_edge;
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), t = blockIdx.x;
+  __shared__ uint32_t s_tile[MAX_TOP], s_n[2];
+  __shared__ uint64_t s_list[CAP];
+  __shared__ float s_edge[5];  // of the waves; the k-th tile's maximum
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), t = blockIdx.x, k = p.k;
   const uint8_t* row = p.logits + t * p.row_bytes;
+  const float* tm = p.tmax + static_cast<size_t>(t) * p.tiles * p.tstride;
+  const float4* st = p.stat + static_cast<size_t>(t) * p.n_stat;
   auto logit = [&](uint32_t i) __attribute__((always_inline)) {
     return BF16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(row)[i]) : reinterpret_cast<const float*>(row)[i];
   };
-  if (p.k && wave == 3u) {  // the tiles with the k largest maxima
-    const float* tm = p.tmax + static_cast<size_t>(t) * p.tiles * p.tstride;
-    Top top;
-    float own = NEG_INF;
-    for (uint32_t i = lane; i < p.tiles; i += 64u) own = fmaxf(own, tm[static_cast<size_t>(i) * p.tstride]);
-    top.edge_from(own, p.k, lane);
-    for (uint32_t i0 = 0; i0 < p.tiles; i0 += 64u) {
-      const uint32_t i = i0 + lane;
-      top.offer(i < p.tiles ? top_key(tm[static_cast<size_t>(i) * p.tstride], i) : 0u, p.k, lane);
-    }
-    if (lane < p.k) s_tile[lane] = top.key ? key_index(top.key) : 0xffffffffu;
-    // k tiles have a logit at least as large as the last of them has
-    const uint64_t last = lane_u64(top.key, p.k - 1u);
-    if (lane == 0u) s_edge = last ? top_key(key_value(last), ~0u) - 1u : NONE_KEY;
+  // the token's logit is on its way before anything waits
+  const int32_t tok = p.tokens ? p.tokens[t] : -1;
+  const bool there = tok >= 0 && static_cast<uint32_t>(tok) < p.vocab;
+  const float own_x = !there ? 0.0f : p.xt ? p.xt[t] : logit(static_cast<uint32_t>(tok));
+  // v[i]: maximum of tile i0 + 256 i + tid, -inf behind the last
+  auto maxima = [&](uint32_t i0, float (&v)[8]) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = tm[static_cast<size_t>(umin(i0 + 256u * i + tid, p.tiles - 1u)) * p.tstride];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = i0 + 256u * i + tid < p.tiles ? v[i] : NEG_INF;
+  };
+  float first[8], own = NEG_INF;  // of the first 2,048 tiles
+  if (k) {
+    if (tid < 2u) s_n[tid] = 0u;
+    if (tid < MAX_TOP) s_tile[tid] = 0xffffffffu;
+    if (tid == 0u) s_edge[4] = NEG_INF;
+    maxima(0u, first);
   }
   Stat a;
-  for (uint32_t i = tid; i < p.n_stat; i += 256u) {
-    Stat b = stat_of(p.stat[static_cast<size_t>(t) * p.n_stat + i]);
-    const float m = fmaxf(a.m, b.m);
+  for (uint32_t i0 = 0; i0 < p.n_stat; i0 += 1024u) {
+    float4 v[4];
+    float m = a.m;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t at = i0 + 256u * i + tid;
+      v[i] = st[umin(at, p.n_stat - 1u)];
+      if (at >= p.n_stat) v[i] = make_float4(NEG_INF, 0.0f, 0.0f, 0.0f);
+      m = fmaxf(m, v[i].x);
+    }
     stat_to(a, m);
-    stat_to(b, m);
-    a.s += b.s;
-    a.w += b.w;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      Stat b = stat_of(v[i]);
+      stat_to(b, m);
+      a.s += b.s;
+      a.w += b.w;
+    }
   }
-  const Stat r = stat_group(a, s_st, lane, wave);
+  if (k) {
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) own = fmaxf(own, first[i]);
+    for (uint32_t i = 2048u + tid; i < p.tiles; i += 256u) own = fmaxf(own, tm[static_cast<size_t>(i) * p.tstride]);
+    const float e = lanes_edge(own, k);
+    if (lane == 0u) s_edge[wave] = e;
+  }
+  const Stat r = stat_group(a, s_st, lane, wave);  // a barrier: the waves' edges are there
   const float ls = logf(r.s);
   const bool none = r.m == NEG_INF && r.s == 0.0f;  // no logit above -inf
   if (tid == 0u) {
     if (p.entropy) p.entropy[t] = none ? 0.0f : ls - r.w / r.s;
-    if (p.logprob) {
-      const int32_t tok = p.tokens[t];
-      const bool there = tok >= 0 && static_cast<uint32_t>(tok) < p.vocab;
-      const float x = !there ? 0.0f : p.xt ? p.xt[t] : logit(static_cast<uint32_t>(tok));
-      p.logprob[t] = !there ? 0.0f : none ? NEG_INF : (x - r.m) - ls;
-    }
+    if (p.logprob) p.logprob[t] = !there ? 0.0f : none ? NEG_INF : (own_x - r.m) - ls;
   }
-  if (!p.k) return;
-  Top top;
-  top.edge = s_edge;
-  for (uint32_t j = wave; j < p.k; j += 4u) {
-    const uint32_t tile = uniform(s_tile[j]);
-    if (tile == 0xffffffffu) break;
-    float x[PER];
+  if (!k) return;
+  auto list = [&](uint32_t which, uint64_t key) __attribute__((always_inline)) {
+    const uint32_t at = atomicAdd(&s_n[which], 1u);
+    if (at < CAP) s_list[at] = key;
+  };
+  // the place of a listed key among the n: how many are larger
+  auto place = [&](uint64_t key, uint32_t n) __attribute__((always_inline)) {
+    uint32_t above = 0;
+    for (uint32_t i = 0; i < n; i += 4u)
 #pragma unroll
-    for (uint32_t i = 0; i < PER; ++i) {
-      const uint32_t v = tile * TILE + 64u * i + lane;
-      x[i] = v < p.vocab ? logit(v) : NEG_INF;
+      for (uint32_t j = 0; j < 4; ++j) above += s_list[i + j] > key && i + j < n;  // (read before it is known to count: in flight together)
+    return above;
+  };
+  const float edge = fmaxf(fmaxf(s_edge[0], s_edge[1]), fmaxf(s_edge[2], s_edge[3]));
+  for (uint32_t i0 = 0;;) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) mask |= first[i] >= edge && first[i] > NEG_INF ? 1u << i : 0u;
+    while (mask) {  // few
+      const uint32_t i = static_cast<uint32_t>(__builtin_ctz(mask)), at = i0 + 256u * i + tid;
+      mask &= mask - 1u;
+      list(0u, top_key(tm[static_cast<size_t>(at) * p.tstride], at));
     }
-#pragma unroll
-    for (uint32_t i = 0; i < PER; ++i) top.offer(x[i] == x[i] ? top_key(x[i], tile * TILE + 64u * i + lane) : 0u, p.k, lane);
+    i0 += 2048u;
+    if (i0 >= p.tiles) break;
+    maxima(i0, first);
   }
-  s_key[wave][lane] = top.key;
   __syncthreads();
-  if (wave) return;
-  for (uint32_t i = 1; i < 4; ++i) top.offer(s_key[i][lane], p.k, lane);
-  if (lane < p.k) {
-    const bool there = top.key != 0u;
-    p.top_ids[static_cast<size_t>(t) * p.k + lane] = there ? static_cast<int32_t>(key_index(top.key)) : -1;
-    p.top_lp[static_cast<size_t>(t) * p.k + lane] = there ? (key_value(top.key) - r.m) - ls : NEG_INF;
+  uint32_t n = uniform(s_n[0]);
+  if (n <= CAP) {  // uniform
+    for (uint32_t i = tid; i < n; i += 256u) {
+      const uint64_t key = s_list[i];
+      const uint32_t at = place(key, n);
+      if (at < k) s_tile[at] = key_index(key);
+      if (at == k - 1u) s_edge[4] = key_value(key);
+    }
+  } else if (wave == 0u) {
+    Top top;
+    for (uint32_t i0 = 0; i0 < p.tiles; i0 += 64u)
+      top.offer(i0 + lane < p.tiles ? top_key(tm[static_cast<size_t>(i0 + lane) * p.tstride], i0 + lane) : 0u, k, lane);
+    if (lane < k && top.key) s_tile[lane] = key_index(top.key);
+    if (lane == k - 1u && top.key) s_edge[4] = key_value(top.key);
+  }
+  __syncthreads();
+  // the logits of those tiles that are as large as the last one's maximum: a wave takes
+  // every fourth tile, four of them in flight
+  const float low = s_edge[4];
+  const bool vec = (reinterpret_cast<uintptr_t>(row) & 15u) == 0u;
+  auto load = [&](uint32_t j, float (&x)[PER]) __attribute__((always_inline)) {  // -inf where there is none
+    const uint32_t tile = uniform(s_tile[umin(j, MAX_TOP - 1u)]), v = tile * TILE + PER * lane;
+    const bool is = j < k && tile != 0xffffffffu;  // uniform
+    if constexpr (PER == 1u)
+      x[0] = is && v < p.vocab ? logit(v) : NEG_INF;
+    else
+      Logits<BF16>::load(row, is ? v : p.vocab, p.vocab, vec, x);
+  };
+  for (uint32_t j0 = wave; j0 < k; j0 += 16u) {
+    float x[4][PER];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) load(j0 + 4u * i, x[i]);
+    uint32_t mask = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+      for (uint32_t e = 0; e < PER; ++e) mask |= x[i][e] >= low && x[i][e] > NEG_INF ? 1u << (PER * i + e) : 0u;  // (not NaN)
+    while (mask) {  // few
+      const uint32_t b = static_cast<uint32_t>(__builtin_ctz(mask)), v = s_tile[j0 + 4u * (b / PER)] * TILE + PER * lane + b % PER;
+      mask &= mask - 1u;
+      list(1u, top_key(logit(v), v));
+    }
+  }
+  __syncthreads();
+  n = uniform(s_n[1]);
+  auto write = [&](uint32_t at, uint64_t key) __attribute__((always_inline)) {
+    p.top_ids[static_cast<size_t>(t) * k + at] = key ? static_cast<int32_t>(key_index(key)) : -1;
+    p.top_lp[static_cast<size_t>(t) * k + at] = key ? (key_value(key) - r.m) - ls : NEG_INF;
+  };
+  if (n <= CAP) {  // uniform
+    for (uint32_t i = tid; i < n; i += 256u) {
+      const uint64_t key = s_list[i];
+      const uint32_t at = place(key, n);
+      if (at < k) write(at, key);
+    }
+    if (tid >= n && tid < k) write(tid, 0u);  // fewer than k
+  } else if (wave == 0u) {
+    Top top;
+    for (uint32_t i = 0; i < k * PER; ++i) {
+      const uint32_t tile = uniform(s_tile[i / PER]), v = tile * TILE + 64u * (i % PER) + lane;
+      const float x = tile != 0xffffffffu && v < p.vocab ? logit(v) : NEG_INF;
+      top.offer(x > NEG_INF ? top_key(x, v) : 0u, k, lane);
+    }
+    if (lane < k) write(lane, top.key);
   }
 }
 
