@@ -6,9 +6,8 @@
 // e = exp(x - m), sets are joined by taking s and w to the larger maximum
 // (w' = f (w + s (m - m')), f = exp(m - m')). Of the whole row
 //   log p(t) = x_t - m - log s,   entropy = log s - w / s,
-// sums of one sign each. The k largest of a row lie in the k tiles of 256 (512)
-// logits with the largest maxima, ties to the lower tile, so only those are looked
-// through.
+// sums of one sign each. The k largest of a row lie in the k tiles with the largest
+// maxima, ties to the lower tile, so only those are looked through.
 #include <algorithm>
 
 #include "obs_internal.hpp"
@@ -118,12 +117,12 @@ struct Top {
 // ---------------------------------------------------------------------------
 // Logits
 // ---------------------------------------------------------------------------
-// A workgroup takes one part of a row, a wave 64 * 16 logits at once: their sums,
-// and of each tile (one load of the wave: 256 logits in fp32, 512 in bf16) the
-// maximum. One pass; bound by the reading.
+// A workgroup takes one part of a row, a wave a step of 1,024 logits at once: their sums,
+// and the maxima of its four tiles, of 16 lanes each (a wave's whole maximum of every
+// load cost 7 of 57 us for 777 rows in bf16). One pass; bound by the reading.
 template <bool BF16>
 struct Logits {
-  static constexpr uint32_t TILE = BF16 ? 512u : 256u, PER = TILE / 64u, STEP = 1024u, N = STEP / TILE;
+  static constexpr uint32_t LOAD = BF16 ? 512u : 256u, PER = LOAD / 64u, STEP = 1024u, N = STEP / LOAD;
   // PER logits from i on (behind the row's end: -inf)
   static __device__ __forceinline__ void load(const void* row, uint32_t i, uint32_t n, bool vec, float* x) {
     if constexpr (BF16) {
@@ -171,7 +170,7 @@ __global__ void __launch_bounds__(256) logits_part_kernel(const uint8_t* __restr
   for (uint32_t s = 4u * part + wave; s < steps; s += 4u * parts) {
     float x[L::N][L::PER];
 #pragma unroll
-    for (uint32_t j = 0; j < L::N; ++j) L::load(row, s * L::STEP + j * L::TILE + L::PER * lane, vocab, vec, x[j]);
+    for (uint32_t j = 0; j < L::N; ++j) L::load(row, s * L::STEP + j * L::LOAD + L::PER * lane, vocab, vec, x[j]);
     float top[L::N];
 #pragma unroll
     for (uint32_t j = 0; j < L::N; ++j) {
@@ -182,11 +181,15 @@ __global__ void __launch_bounds__(256) logits_part_kernel(const uint8_t* __restr
 #pragma unroll
     for (uint32_t j = 0; j < L::N; ++j) stat_add<L::PER>(a, x[j], top[j]);
     if (tmax) {  // uniform
+      float m = top[0];
 #pragma unroll
-      for (uint32_t j = 0; j < L::N; ++j) {
-        const float m = fmaxf(wave_max_f32(top[j]), NEG_INF);  // (a tile of NaN alone: -inf)
-        if (lane == 0u && L::N * s + j < tiles) tmax[static_cast<size_t>(t) * tiles + L::N * s + j] = m;
-      }
+      for (uint32_t j = 1; j < L::N; ++j) m = fmaxf(m, top[j]);
+      m = fmaxf(m, dpp_f32<DPP_XOR1>(m));
+      m = fmaxf(m, dpp_f32<DPP_XOR2>(m));
+      m = fmaxf(m, dpp_f32<DPP_HALF_MIRROR>(m));
+      m = fmaxf(m, dpp_f32<DPP_MIRROR>(m));
+      // (of NaN alone: -inf)
+      if (lane % 16u == 0u) tmax[static_cast<size_t>(t) * tiles + 4u * s + lane / 16u] = fmaxf(m, NEG_INF);
     }
   }
   const Stat r = stat_group(a, s_st, lane, wave);
@@ -227,11 +230,14 @@ __device__ __forceinline__ float lanes_edge(float own, uint32_t k) {
 // there is room for (equal values in masses), a wave takes them one by one. The code runs
 // once, so its length counts. (A wave's lists from the start took 21 us a row of 2,374
 // tiles at k = 5; ranks of all 256 threads' maxima, and every load's listing unrolled, 17.)
+// TILE: tile i has the TILE logits from TILE i on; 0: logits_part_kernel's, 256 logits
+// each, four interleaved in a step. Steps are in order, so with the k-th tile come those of
+// its step, the next three at most.
 template <bool BF16, uint32_t TILE>
 __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
-  constexpr uint32_t CAP = 1024, PER = TILE / 64u;
+  constexpr uint32_t CAP = 1024, SUBS = TILE ? 1u : 4u, PER = TILE == 64u ? 1u : 4u;
   __shared__ float s_st[3][4];
-  __shared__ uint32_t s_tile[MAX_TOP], s_n[2];
+  __shared__ uint32_t s_tile[MAX_TOP + 4u], s_n[2];
   __shared__ uint64_t s_list[CAP];
   __shared__ float s_edge[5];  // of the waves; the k-th tile's maximum
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), t = blockIdx.x, k = p.k;
@@ -255,7 +261,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
   float first[8], own = NEG_INF;  // of the first 2,048 tiles
   if (k) {
     if (tid < 2u) s_n[tid] = 0u;
-    if (tid < MAX_TOP) s_tile[tid] = 0xffffffffu;
+    if (tid < MAX_TOP + 4u) s_tile[tid] = 0xffffffffu;
     if (tid == 0u) s_edge[4] = NEG_INF;
     maxima(0u, first);
   }
@@ -322,17 +328,23 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
   }
   __syncthreads();
   uint32_t n = uniform(s_n[0]);
-  if (n <= CAP) {  // uniform
+  const bool room = n <= CAP;  // else s_tile holds steps
+  if (room) {  // uniform
     for (uint32_t i = tid; i < n; i += 256u) {
       const uint64_t key = s_list[i];
       const uint32_t at = place(key, n);
-      if (at < k) s_tile[at] = key_index(key);
+      if (at < k + SUBS - 1u) s_tile[at] = key_index(key);
       if (at == k - 1u) s_edge[4] = key_value(key);
     }
   } else if (wave == 0u) {
     Top top;
-    for (uint32_t i0 = 0; i0 < p.tiles; i0 += 64u)
-      top.offer(i0 + lane < p.tiles ? top_key(tm[static_cast<size_t>(i0 + lane) * p.tstride], i0 + lane) : 0u, k, lane);
+    for (uint32_t i0 = 0; i0 < p.tiles; i0 += 64u * SUBS) {
+      const uint32_t at = i0 + SUBS * lane;
+      float m = NEG_INF;
+#pragma unroll
+      for (uint32_t i = 0; i < SUBS; ++i) m = fmaxf(m, at + i < p.tiles ? tm[static_cast<size_t>(at + i) * p.tstride] : NEG_INF);
+      top.offer(at < p.tiles ? top_key(m, at / SUBS) : 0u, k, lane);
+    }
     if (lane < k && top.key) s_tile[lane] = key_index(top.key);
     if (lane == k - 1u && top.key) s_edge[4] = key_value(top.key);
   }
@@ -341,15 +353,41 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
   // every fourth tile, four of them in flight
   const float low = s_edge[4];
   const bool vec = (reinterpret_cast<uintptr_t>(row) & 15u) == 0u;
-  auto load = [&](uint32_t j, float (&x)[PER]) __attribute__((always_inline)) {  // -inf where there is none
-    const uint32_t tile = uniform(s_tile[umin(j, MAX_TOP - 1u)]), v = tile * TILE + PER * lane;
-    const bool is = j < k && tile != 0xffffffffu;  // uniform
-    if constexpr (PER == 1u)
-      x[0] = is && v < p.vocab ? logit(v) : NEG_INF;
+  auto first_of = [&](uint32_t tile) __attribute__((always_inline)) {  // of the lane's PER logits
+    if constexpr (TILE)
+      return tile * TILE + PER * lane;
+    else if constexpr (BF16)
+      return tile / 4u * 1024u + 512u * (lane / 32u) + 128u * (tile % 4u) + 4u * (lane % 32u);
     else
-      Logits<BF16>::load(row, is ? v : p.vocab, p.vocab, vec, x);
+      return tile / 4u * 1024u + 256u * (lane / 16u) + 64u * (tile % 4u) + 4u * (lane % 16u);
   };
-  for (uint32_t j0 = wave; j0 < k; j0 += 16u) {
+  const uint32_t rows = room ? k + SUBS - 1u : k * SUBS;
+  auto tile_of = [&](uint32_t j) __attribute__((always_inline)) {
+    if (room) return s_tile[umin(j, MAX_TOP + 3u)];
+    const uint32_t step = s_tile[umin(j / SUBS, MAX_TOP - 1u)];
+    return step == 0xffffffffu ? step : step * SUBS + j % SUBS;
+  };
+  auto load = [&](uint32_t j, float (&x)[PER]) __attribute__((always_inline)) {  // -inf where there is none
+    const uint32_t tile = uniform(tile_of(j)), v = first_of(tile);
+    const bool is = j < rows && tile != 0xffffffffu;  // uniform
+    if (PER == 4u && is && vec && v + PER <= p.vocab) {
+      if constexpr (BF16) {
+        const uint2 w = *reinterpret_cast<const uint2*>(row + 2u * static_cast<size_t>(v));
+        const uint32_t u[2] = {w.x, w.y};
+#pragma unroll
+        for (uint32_t e = 0; e < PER; ++e) x[e] = e & 1u ? bf16hi(u[e / 2u]) : bf16lo(u[e / 2u]);
+      } else {
+        const float4 w = *reinterpret_cast<const float4*>(row + 4u * static_cast<size_t>(v));
+        const float u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (uint32_t e = 0; e < PER; ++e) x[e] = u[e];
+      }
+    } else {
+#pragma unroll
+      for (uint32_t e = 0; e < PER; ++e) x[e] = is && v + e < p.vocab ? logit(v + e) : NEG_INF;
+    }
+  };
+  for (uint32_t j0 = wave; j0 < rows; j0 += 16u) {
     float x[4][PER];
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) load(j0 + 4u * i, x[i]);
@@ -359,7 +397,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 #pragma unroll
       for (uint32_t e = 0; e < PER; ++e) mask |= x[i][e] >= low && x[i][e] > NEG_INF ? 1u << (PER * i + e) : 0u;  // (not NaN)
     while (mask) {  // few
-      const uint32_t b = static_cast<uint32_t>(__builtin_ctz(mask)), v = s_tile[j0 + 4u * (b / PER)] * TILE + PER * lane + b % PER;
+      const uint32_t b = static_cast<uint32_t>(__builtin_ctz(mask)), v = first_of(tile_of(j0 + 4u * (b / PER))) + b % PER;
       mask &= mask - 1u;
       list(1u, top_key(logit(v), v));
     }
@@ -379,10 +417,12 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
     if (tid >= n && tid < k) write(tid, 0u);  // fewer than k
   } else if (wave == 0u) {
     Top top;
-    for (uint32_t i = 0; i < k * PER; ++i) {
-      const uint32_t tile = uniform(s_tile[i / PER]), v = tile * TILE + 64u * (i % PER) + lane;
-      const float x = tile != 0xffffffffu && v < p.vocab ? logit(v) : NEG_INF;
-      top.offer(x > NEG_INF ? top_key(x, v) : 0u, k, lane);
+    for (uint32_t j = 0; j < rows; ++j) {
+      float x[PER];
+      load(j, x);
+      const uint32_t v = first_of(tile_of(j));
+#pragma unroll
+      for (uint32_t e = 0; e < PER; ++e) top.offer(x[e] > NEG_INF ? top_key(x[e], v + e) : 0u, k, lane);
     }
     if (lane < k) write(lane, top.key);
   }
@@ -761,12 +801,11 @@ struct LogitsPlan {
   uint32_t parts, tiles;
   size_t stat, tmax;  // bytes
 };
-LogitsPlan logits_plan(uint32_t T, uint32_t vocab, int dtype, uint32_t k) {
+LogitsPlan logits_plan(uint32_t T, uint32_t vocab, uint32_t k) {
   LogitsPlan d{};
-  const uint32_t tile = dtype == OBS_LOGITS_BF16 ? 512u : 256u;
   // eight workgroups a CU, of 4,096 logits at least
   d.parts = std::max(1u, std::min((2047u + T) / std::max(T, 1u), (vocab + 4095u) / 4096u));
-  d.tiles = (vocab + tile - 1u) / tile;
+  d.tiles = (vocab + 1023u) / 1024u * 4u;
   d.stat = up256(static_cast<size_t>(T) * d.parts * sizeof(float4));
   d.tmax = k ? up256(static_cast<size_t>(T) * d.tiles * sizeof(float)) : 0u;
   return d;
@@ -846,7 +885,7 @@ int obs_token_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t vocab, int d
   const char* who = "obs_token_logprobs_workspace";
   int rc = check_logits(ctx, who, T, vocab, dtype);
   if (rc != OBS_OK) return rc;
-  const LogitsPlan d = logits_plan(T, vocab, dtype, top_k);
+  const LogitsPlan d = logits_plan(T, vocab, top_k);
   *bytes = d.stat + d.tmax;
   return OBS_OK;
 }
@@ -861,7 +900,7 @@ int obs_token_logprobs(obs_ctx* ctx, const void* logits, int dtype, uint32_t T, 
   if (rc != OBS_OK) return rc;
   ld = ld ? ld : vocab;
   if (ld < vocab) return obs::set_error(ctx, OBS_E_SHAPE, "%s: row stride %u holds no row of %u", who, ld, vocab);
-  const LogitsPlan d = logits_plan(T, vocab, dtype, top_k);
+  const LogitsPlan d = logits_plan(T, vocab, top_k);
   if (T == 0) return OBS_OK;
   if (!logits || !ws) return obs::set_error(ctx, OBS_E_INVALID, "%s: null pointer", who);
   const bool bf16 = dtype == OBS_LOGITS_BF16;
@@ -880,10 +919,10 @@ int obs_token_logprobs(obs_ctx* ctx, const void* logits, int dtype, uint32_t T, 
   const JoinArgs j{stat, tmax, lp, nullptr, tokens, logprob, entropy, top_ids, top_logprobs, row_bytes, d.parts, d.tiles, 1u, vocab, top_k};
   if (bf16) {
     OBS_LAUNCH(ctx, "logits_part", logits_part_kernel<true><<<T * d.parts, 256, 0, ctx->stream>>>(lp, row_bytes, vocab, d.parts, stat, tmax, d.tiles));
-    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<true, 512><<<T, 256, 0, ctx->stream>>>(j));
+    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<true, 0><<<T, 256, 0, ctx->stream>>>(j));
   } else {
     OBS_LAUNCH(ctx, "logits_part", logits_part_kernel<false><<<T * d.parts, 256, 0, ctx->stream>>>(lp, row_bytes, vocab, d.parts, stat, tmax, d.tiles));
-    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, 256><<<T, 256, 0, ctx->stream>>>(j));
+    OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, 0><<<T, 256, 0, ctx->stream>>>(j));
   }
   return OBS_OK;
 }
