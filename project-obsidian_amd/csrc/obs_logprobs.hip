@@ -432,16 +432,13 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 // Hidden rows and the 4-bit output matrix
 // ---------------------------------------------------------------------------
 // logit[t][v] = sum_g s (sum q x) + b (sum x) over the groups g of 64 columns, s and b
-// of (v, g). The products take q as 16 + q in bf16, exact, and the sums over a group
-// are taken to fp32 with the scale: no weight is rounded.
-// A lane (col = lane % 32, half = lane / 32) has one vocabulary row of each product
-// (v_mfma_f32_32x32x16_bf16, tokens x vocabulary), so a scale is one factor of its 16
-// sums. It loads 16 bytes of the row a group: 32 columns, the operands of four steps;
-// step s has columns 32 half + 8 s + 0, 4, 1, 5, 2, 6, 3, 7, as the nibbles come apart.
+// of (v, g). The products take the nibbles themselves, exact, in products of tokens x
+// vocabulary, so that a lane has one vocabulary row and the scale is one factor of its sums
+// over a group, in fp32: no weight is rounded.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
 constexpr uint32_t LM_COLS = 256, LM_FEW_COLS = 64;  // vocabulary rows of a workgroup
 
-// The operands of four steps of 32 nibbles.
+// Eight nibbles as 16 + q in bf16, columns 0, 4, 1, 5, 2, 6, 3, 7.
 __device__ __forceinline__ bf16x8_v lm_weights(uint32_t w) {
   return __builtin_bit_cast(bf16x8_v, u32x4_v{q4_bf16<0>(w), q4_bf16<2>(w), q4_bf16<1>(w), q4_bf16<3>(w)});
 }
@@ -471,35 +468,44 @@ struct LmArgs {
   uint32_t T, in, vocab, tiles, ld;
 };
 
-// A row's 64 N logits of the workgroup, N a lane: the sums of them, the token's own, and
-// the logits where they are wanted.
-template <uint32_t N>
-__device__ __forceinline__ void lm_row(const LmArgs& p, const float (&v)[N], uint32_t t, uint32_t v0, uint32_t lane) {
-  typedef float vec __attribute__((ext_vector_type(N)));
-  vec out;
-  float x[N];
+// The token of row t, or one that is no column's (padding).
+__device__ __forceinline__ uint32_t lm_token(const LmArgs& p, uint32_t t) {
+  const uint32_t tok = static_cast<uint32_t>(p.tokens[t]);
+  return tok < p.vocab ? tok : 0xffffffffu;
+}
+// A row's COLS logits x of the workgroup, L lanes of N each (the lane's V-th at column
+// STEP (V / 4) + 4 lane + V % 4): their sums, and the logits where they are wanted. L is 8
+// or 16 lanes of a row of lanes; `first` is the row's first.
+template <uint32_t COLS, uint32_t L, uint32_t N>
+__device__ __forceinline__ void lm_sums(const LmArgs& p, float (&x)[N], uint32_t t, uint32_t v0, uint32_t part, bool is) {
+  static_assert(L * N == COLS && (L == 8u || L == 16u), "whole rows");
+  constexpr uint32_t STEP = 4u * L;
+  const uint32_t at = v0 + 4u * part;
+  if (p.logits) {  // uniform
 #pragma unroll
-  for (uint32_t i = 0; i < N; ++i) x[i] = out[i] = v[i];
-  const uint32_t at = v0 + N * lane;
-  if (p.logits && at < p.ld) *reinterpret_cast<vec*>(p.logits + static_cast<size_t>(t) * p.ld + at) = out;
-  if (p.tokens) {
-    const uint32_t k = static_cast<uint32_t>(p.tokens[t]) - at;
-#pragma unroll
-    for (uint32_t i = 0; i < N; ++i)
-      if (k == i && at + i < p.vocab) p.xt[t] = x[i];
+    for (uint32_t i = 0; i < N; i += 4)
+      if (is && at + STEP * (i / 4u) < p.ld)
+        *reinterpret_cast<float4*>(p.logits + static_cast<size_t>(t) * p.ld + at + STEP * (i / 4u)) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
   }
-  float m = NEG_INF;
+  if (v0 + COLS > p.vocab) {  // uniform: the last columns
 #pragma unroll
-  for (uint32_t i = 0; i < N; ++i) {
-    x[i] = at + i < p.vocab ? x[i] : NEG_INF;
-    m = fmaxf(m, x[i]);
+    for (uint32_t i = 0; i < N; ++i) x[i] = at + STEP * (i / 4u) + i % 4u < p.vocab ? x[i] : NEG_INF;
   }
-  m = fmaxf(wave_max_f32(m), NEG_INF);  // (of NaN alone: -inf)
+  float m = x[0];
+#pragma unroll
+  for (uint32_t i = 1; i < N; ++i) m = fmaxf(m, x[i]);
+  auto over = [&](float v, auto op) __attribute__((always_inline)) {
+    v = op(v, dpp_f32<DPP_XOR1>(v));
+    v = op(v, dpp_f32<DPP_XOR2>(v));
+    v = op(v, dpp_f32<DPP_HALF_MIRROR>(v));
+    return L == 16u ? op(v, dpp_f32<DPP_MIRROR>(v)) : v;
+  };
+  m = fmaxf(over(m, [](float a, float b) { return fmaxf(a, b); }), NEG_INF);  // (of NaN alone: -inf)
   Stat a;
   a.m = m;
   stat_add<N>(a, x, m);
-  const float s = wave_sum_asc(a.s), w = wave_sum_asc(a.w);
-  if (lane == 0u) p.stat[static_cast<size_t>(t) * p.tiles + v0 / (64u * N)] = make_float4(m, s, w, 0.0f);
+  const float s = over(a.s, [](float a, float b) { return a + b; }), w = over(a.w, [](float a, float b) { return a + b; });
+  if (is && part == 0u) p.stat[static_cast<size_t>(t) * p.tiles + v0 / COLS] = make_float4(m, s, w, 0.0f);
 }
 
 // Up to 16 NT tokens: the weights go through once and bound the call. A workgroup a CU
@@ -557,6 +563,8 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
   };
   f32x4_v acc[4][NT] = {};
   uint32_t tile = blockIdx.x, j = 0, buf = 0;
+  // the token of the thread's row, as below
+  const uint32_t token = p.tokens && tid / 16u < p.T ? lm_token(p, tid / 16u) : 0xffffffffu;
   load_w(cur, tile, umin(wave, slices - 1u));
   for (;;) {
     // the next slice of these rows, or the first of the next ones
@@ -618,11 +626,21 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
           acc[n][m] = zero;
         }
       __syncthreads();
-      for (uint32_t t = wave; t < p.T; t += WAVES) {
-        float x[1] = {0.0f};
+      // sixteen threads a row, four columns each
+      const uint32_t t = tid / 16u, part = tid % 16u;
+      if (t / 4u < (p.T + 3u) / 4u) {  // whole waves
+        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (uint32_t w = 0; w < WAVES; ++w) x[0] += s_out[buf][w][t][lane];
-        lm_row<1>(p, x, t, tile * LM_FEW_COLS, lane);
+        for (uint32_t w = 0; w < WAVES; ++w) {
+          const f32x4_v v = *reinterpret_cast<const f32x4_v*>(&s_out[buf][w][umin(t, RT - 1u)][4u * part]);
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) x[i] += v[i];
+        }
+        const uint32_t k = token - tile * LM_FEW_COLS - 4u * part;  // (a token behind the last one is no row's)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (k == i) p.xt[t] = x[i];
+        lm_sums<LM_FEW_COLS, 16>(p, x, t, tile * LM_FEW_COLS, part, t < p.T);
       }
       buf ^= 1u;  // (read again two tiles on, behind a barrier that its readers pass first)
       if (ntile >= p.tiles) break;
@@ -633,45 +651,71 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
   }
 }
 
-// Many tokens. First their rows in the order of the products' operands, [tile of 32 MT
-// rows][group][32 rows][step][lane] 16 bytes, and the sums of every group in three bf16
-// parts (24 bits), once as they are and once times -16: at the end of a tile they meet
-// the biases and the scales in products of their own, 12 instead of 2 * 16 sums a group.
-constexpr uint32_t LM_SUMS = 6;
+// Many tokens: bound by the matrix units, beside which the weights come apart and one
+// product a sum and group goes with the scale, in the vector unit. A nibble masked in
+// place at bits 3:0 (7:4) of a half word is the fp16 number q 2^-24 (q 2^-20), subnormal,
+// which the products (v_mfma_f32_32x32x16_f16) take as it is: five instructions for eight
+// nibbles, and no offset. The rows are brought into fp16 by a power of two a row, its
+// largest to 2^14: exact from 2^-29 of that on (the columns of upper nibbles 2^-25, as they
+// get a sixteenth), off by 2^-38 of it below. (Products of 8-bit numbers, of which a bf16 x
+// has two, would need masks alone, but they drop what lies 2^-13 below the largest of eight
+// products.)
+//
+// First the rows in the order of the products' operands, [tile of 32 MT rows][group][32
+// rows][step][lane] 16 bytes, each row's factor back, and the sums of every group in three
+// bf16 parts (24 bits), which meet the biases in products of their own at the end of a
+// tile. A wave takes a row.
+constexpr uint32_t LM_SUMS = 3;
 template <uint32_t MT>
-__global__ void __launch_bounds__(256) lm_rows_kernel(const uint16_t* __restrict__ x, uint32_t T, uint32_t in, uint8_t* __restrict__ xp,
-                                                      uint8_t* __restrict__ xs) {
-  const uint32_t tid = threadIdx.x, groups = in / 64u, gpad = (groups + 15u) & ~15u;
-  const uint32_t mt = blockIdx.x / (gpad / 8u), c0 = blockIdx.x % (gpad / 8u) * 64u;  // 32 rows, 512 columns
+__global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict__ x, uint32_t T, uint32_t in, uint8_t* __restrict__ xp,
+                                                      float* __restrict__ xf, uint8_t* __restrict__ xs) {
+  const uint32_t lane = threadIdx.x & 63u, t = blockIdx.x * 8u + uniform(threadIdx.x >> 6), mt = t / 32u, r = t % 32u;
+  const uint32_t groups = in / 64u, gpad = (groups + 15u) & ~15u, chunks = in / 8u;  // a multiple of 64
+  const uint16_t* row = x + static_cast<size_t>(t < T ? t : 0u) * in;
+  uint32_t most = 0u;
+  for (uint32_t c = lane; c < chunks; c += 64u) {
+    const uint4 v = *reinterpret_cast<const uint4*>(row + 8u * c);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) {
-    const uint32_t r = (tid + 256u * i) / 64u, c = c0 + (tid + 256u * i) % 64u, t = 32u * mt + r, g = c / 8u;
+    for (uint32_t e = 0; e < 4; ++e) most = max(most, max(w[e] & 0x7fffu, w[e] >> 16 & 0x7fffu));
+  }
+  const uint32_t ex = max(wave_max_u31(most) >> 7, 15u);
+  const float up = __uint_as_float((268u - ex) << 23);
+  if (lane == 0u) xf[t] = t < T ? __uint_as_float((ex - 2u) << 23) : 0.0f;  // back, and 2^12 of the nibbles' 2^24
+  for (uint32_t c = lane; c < gpad * 8u; c += 64u) {
+    const uint32_t g = c / 8u;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (t < T && g < groups) v = *reinterpret_cast<const uint4*>(x + static_cast<size_t>(t) * in + 8u * c);
+    if (t < T && g < groups) v = *reinterpret_cast<const uint4*>(row + 8u * c);
     const float sum = sum_of_8_lanes(sum8(v));
-    if (g < groups)
-      *reinterpret_cast<u32x4_v*>(xp + 16u * (((static_cast<size_t>(mt / MT) * groups + g) * MT + mt % MT) * 256u + c % 4u * 64u +
-                                              32u * (c / 4u % 2u) + r)) = lm_order(v);
+    if (g < groups) {
+      // half c / 4 % 2, step c % 4: columns 0, 4 | 1, 5 | 2, 6 | 3, 7 of the eight
+      auto pair = [&](float a, float b, float f) __attribute__((always_inline)) {
+        return __builtin_bit_cast(uint32_t, f16x2_of(a * f, b * f));
+      };
+      const float od = up * 0.0625f;
+      *reinterpret_cast<uint4*>(xp + 16u * (((static_cast<size_t>(mt / MT) * groups + g) * MT + mt % MT) * 256u + c % 4u * 64u + 32u * (c / 4u % 2u) + r)) =
+          make_uint4(pair(bf16lo(v.x), bf16lo(v.z), up), pair(bf16hi(v.x), bf16hi(v.z), od), pair(bf16lo(v.y), bf16lo(v.w), up),
+                     pair(bf16hi(v.y), bf16hi(v.w), od));
+    }
     if (c % 8u == 0u) {
       float rest = sum;
 #pragma unroll
-      for (uint32_t k = 0; k < 3; ++k) {
+      for (uint32_t k = 0; k < LM_SUMS; ++k) {
         const uint16_t part = f32_to_bf16(rest);
         rest -= bf16_to_f32(part);
         // steps of 16 groups, eight a lane's half
-        uint16_t* to = reinterpret_cast<uint16_t*>(xs + 16u * ((static_cast<size_t>(mt) * LM_SUMS * (gpad / 16u) + k * (gpad / 16u) + g / 16u) * 64u +
-                                                               32u * (g / 8u % 2u) + r)) + g % 8u;
-        to[0] = part;
-        to[3u * (gpad / 16u) * 512u] = f32_to_bf16(-16.0f * bf16_to_f32(part));
+        reinterpret_cast<uint16_t*>(xs + 16u * ((static_cast<size_t>(mt) * LM_SUMS * (gpad / 16u) + k * (gpad / 16u) + g / 16u) * 64u +
+                                                32u * (g / 8u % 2u) + r))[g % 8u] = part;
       }
     }
   }
 }
 
 // 32 MT tokens x 256 vocabulary rows a workgroup, 64 a wave; two workgroups a CU.
+typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
 template <uint32_t MT>
-__global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t* __restrict__ xp, const uint8_t* __restrict__ xs,
-                                                         uint32_t ttiles) {
+__global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t* __restrict__ xp, const float* __restrict__ xf,
+                                                         const uint8_t* __restrict__ xs, uint32_t ttiles) {
   constexpr uint32_t XB = MT * 4096u, OROW = LM_COLS + 8u, OB = 32u * OROW * 4u;  // bytes of a group's rows; of 32 rows of logits
   __shared__ __attribute__((aligned(16))) uint8_t s_mem[2u * XB > OB ? 2u * XB : OB];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 31u, half = lane >> 5;
@@ -679,20 +723,22 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   const uint32_t at = blockIdx.x / 8u, vt = at / ttiles * 8u + blockIdx.x % 8u, tt = at % ttiles;
   if (vt >= p.tiles) return;  // uniform
   const uint32_t v0 = vt * LM_COLS, groups = p.in / 64u, gpad = (groups + 15u) & ~15u;
-  const uint32_t* wp[2];
-  const uint16_t *sp[2], *bp[2];
+  // scalar bases and 32-bit offsets of the lane's rows
+  const uint8_t *wb0 = reinterpret_cast<const uint8_t*>(p.w) + static_cast<size_t>(v0) * (p.in / 2u),
+                *sb0 = reinterpret_cast<const uint8_t*>(p.s) + static_cast<size_t>(v0) * (2u * groups),
+                *bb0 = reinterpret_cast<const uint8_t*>(p.b) + static_cast<size_t>(v0) * (2u * groups);
+  uint32_t woff[2], soff[2];
 #pragma unroll
   for (uint32_t n = 0; n < 2; ++n) {
-    const size_t v = umin(v0 + 64u * wave + 32u * n + col, p.vocab - 1u);
-    wp[n] = p.w + v * (p.in / 8u) + 4u * half;
-    sp[n] = p.s + v * groups;
-    bp[n] = p.b + v * groups;
+    const uint32_t r = umin(v0 + 64u * wave + 32u * n + col, p.vocab - 1u) - v0;  // (behind the last row it again)
+    woff[n] = r * (p.in / 2u) + 16u * half;
+    soff[n] = r * (2u * groups);
   }
-  const uint8_t* xg = xp + static_cast<size_t>(tt) * groups * XB + 16u * tid;
+  const uint8_t* xg = xp + static_cast<size_t>(tt) * groups * XB;
   u32x4_v xr[MT];
   auto load_x = [&](uint32_t g) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t i = 0; i < MT; ++i) xr[i] = *reinterpret_cast<const u32x4_v*>(xg + static_cast<size_t>(g) * XB + 4096u * i);
+    for (uint32_t i = 0; i < MT; ++i) xr[i] = *reinterpret_cast<const u32x4_v*>(xg + static_cast<size_t>(g) * XB + (16u * tid + 4096u * i));
   };
   auto store_x = [&](uint32_t buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -703,47 +749,62 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   for (uint32_t m = 0; m < MT; ++m)
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) acc[m][n] = f32x16_v{};
-  u32x4_v wr[2][2];  // two groups ahead
-  uint32_t sr[2][2];
-  auto load_w = [&](uint32_t g, uint32_t slot) __attribute__((always_inline)) {
+  u32x4_v wr[2];  // a group ahead
+  uint32_t sr[2];
+  auto load_w = [&](uint32_t g) __attribute__((always_inline)) {
     const uint32_t gc = umin(g, groups - 1u);
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) {
-      wr[slot][n] = *reinterpret_cast<const u32x4_v*>(wp[n] + 8u * gc);
-      sr[slot][n] = sp[n][gc];
+      wr[n] = *reinterpret_cast<const u32x4_v*>(wb0 + 32u * gc + woff[n]);
+      sr[n] = *reinterpret_cast<const uint16_t*>(sb0 + 2u * gc + soff[n]);
     }
   };
   load_x(0u);
-  load_w(0u, 0u);
-  load_w(1u, 1u);
+  load_w(0u);
   store_x(0u);
   __syncthreads();
   auto step = [&](uint32_t g, uint32_t slot) __attribute__((always_inline)) {
-    load_x(umin(g + 1u, groups - 1u));
-    bf16x8_v wb[2][4];
+    f16x8_v xa[4], wb[2][4];
     float sc[2];
+    auto load_a = [&](uint32_t m, uint32_t s) __attribute__((always_inline)) {
+      xa[s] = *reinterpret_cast<const f16x8_v*>(s_mem + slot * XB + 16u * ((m * 4u + s) * 64u + lane));
+    };
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s) load_a(0u, s);
+    load_x(umin(g + 1u, groups - 1u));
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) {
-      sc[n] = __uint_as_float(sr[slot][n] << 16);
+      sc[n] = __uint_as_float(sr[n] << 16) * 4096.0f;
 #pragma unroll
-      for (uint32_t s = 0; s < 4; ++s) wb[n][s] = lm_weights(wr[slot][n][s]);
-    }
-    load_w(g + 2u, slot);
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (uint32_t m = 0; m < MT; ++m) {
-      bf16x8_v xa[4];
-#pragma unroll
-      for (uint32_t s = 0; s < 4; ++s) xa[s] = *reinterpret_cast<const bf16x8_v*>(s_mem + slot * XB + 16u * ((m * 4u + s) * 64u + lane));
-#pragma unroll
-      for (uint32_t n = 0; n < 2; ++n) {
-        f32x16_v y = {};
-#pragma unroll
-        for (uint32_t s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[s], wb[n][s], y, 0, 0, 0);
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) acc[m][n][i] = __builtin_fmaf(sc[n], y[i], acc[m][n][i]);
+      for (uint32_t s = 0; s < 4; ++s) {
+        const uint32_t w = wr[n][s], w8 = w >> 8;
+        wb[n][s] = __builtin_bit_cast(f16x8_v, u32x4_v{w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u});
       }
     }
+    load_w(g + 1u);
+    __builtin_amdgcn_sched_barrier(0);
+    // Products of one 32 x 32 tile, each beside a quarter of the sums of the tile before and,
+    // with the last use of its rows, the read of the next ones: left to itself the compiler
+    // puts a tile's sums behind its products, and the two units take turns.
+    f32x16_v y[2];
+    const f32x16_v zero = {};
+#pragma unroll
+    for (uint32_t m = 0; m < MT; ++m)
+#pragma unroll
+      for (uint32_t n = 0; n < 2; ++n)
+#pragma unroll
+        for (uint32_t s = 0; s < 4; ++s) {
+          y[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[s], wb[n][s], s ? y[n] : zero, 0, 0, 0);
+          if (n == 1u && m + 1u < MT) load_a(m + 1u, s);
+          if (m || n) {
+            const uint32_t pm = n ? m : m - 1u, pn = 1u - n;
+#pragma unroll
+            for (uint32_t i = 4u * s; i < 4u * s + 4u; ++i) acc[pm][pn][i] = __builtin_fmaf(sc[pn], y[pn][i], acc[pm][pn][i]);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) acc[MT - 1u][1][i] = __builtin_fmaf(sc[1], y[1][i], acc[MT - 1u][1][i]);
     store_x(slot ^ 1u);
     __syncthreads();
   };
@@ -751,30 +812,48 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
     step(g, 0u);
     step(g + 1u, 1u);
   }
-  // the groups' sums with the biases, and (times -16) with the scales
-  const uint32_t steps = gpad / 16u;
+  uint32_t token[MT];  // of the rows that the thread has below
 #pragma unroll
-  for (uint32_t kind = 0; kind < 2; ++kind)
-    for (uint32_t s = 0; s < steps; ++s) {
-      const uint32_t g = 16u * s + 8u * half;
-      bf16x8_v wb[2];
+  for (uint32_t m = 0; m < MT; ++m) {
+    const uint32_t t = 32u * (tt * MT + m) + tid / 8u;
+    token[m] = p.tokens && t < p.T ? lm_token(p, t) : 0xffffffffu;
+  }
+  // the rows' factors back (and 2^12 of the nibbles'), then the groups' sums with the biases
 #pragma unroll
-      for (uint32_t n = 0; n < 2; ++n) {
-        u32x4_v v = *reinterpret_cast<const u32x4_v*>((kind ? sp[n] : bp[n]) + umin(g, groups - 8u));
-        if (g >= groups) v = u32x4_v{0u, 0u, 0u, 0u};
-        wb[n] = __builtin_bit_cast(bf16x8_v, v);
+  for (uint32_t m = 0; m < MT; ++m)
+#pragma unroll
+    for (uint32_t i = 0; i < 16; i += 4) {
+      const f32x4_v f = *reinterpret_cast<const f32x4_v*>(xf + 32u * (tt * MT + m) + 2u * i + 4u * half);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        acc[m][0][i + e] *= f[e];
+        acc[m][1][i + e] *= f[e];
       }
-#pragma unroll
-      for (uint32_t k = 0; k < 3; ++k)
-#pragma unroll
-        for (uint32_t m = 0; m < MT; ++m) {
-          const bf16x8_v xa = *reinterpret_cast<const bf16x8_v*>(
-              xs + 16u * (((static_cast<size_t>(tt) * MT + m) * LM_SUMS * steps + (3u * kind + k) * steps + s) * 64u + lane));
-#pragma unroll
-          for (uint32_t n = 0; n < 2; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa, wb[n], acc[m][n], 0, 0, 0);
-        }
     }
+  const uint32_t steps = gpad / 16u;
+  for (uint32_t s = 0; s < steps; ++s) {
+    const uint32_t g = 16u * s + 8u * half;
+    bf16x8_v bb[2];
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+      u32x4_v v = *reinterpret_cast<const u32x4_v*>(bb0 + (soff[n] + 2u * umin(g, groups - 8u)));
+      if (g >= groups) v = u32x4_v{0u, 0u, 0u, 0u};
+      bb[n] = __builtin_bit_cast(bf16x8_v, v);
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < LM_SUMS; ++k)
+#pragma unroll
+      for (uint32_t m = 0; m < MT; ++m) {
+        const bf16x8_v xa = *reinterpret_cast<const bf16x8_v*>(
+            xs + 16u * (((static_cast<size_t>(tt) * MT + m) * LM_SUMS * steps + k * steps + s) * 64u + lane));
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa, bb[n], acc[m][n], 0, 0, 0);
+      }
+  }
+  // 32 rows at a time through LDS, eight threads a row. (A wave a row, one after another, took
+  // as long as the products: 740 us of 1,470 for 2,000 tokens.)
   float(*const s_out)[OROW] = reinterpret_cast<float(*)[OROW]>(s_mem);
+  const uint32_t orow = tid / 8u, part = tid % 8u;
 #pragma unroll
   for (uint32_t m = 0; m < MT; ++m) {
     if (m) __syncthreads();
@@ -783,12 +862,16 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
 #pragma unroll
       for (uint32_t i = 0; i < 16; ++i) s_out[8u * (i / 4u) + 4u * half + i % 4u][64u * wave + 32u * n + col] = acc[m][n][i];
     __syncthreads();
-    for (uint32_t r = wave; r < 32u; r += 4u) {
-      const uint32_t t = 32u * (tt * MT + m) + r;
-      const float4 v = *reinterpret_cast<const float4*>(&s_out[r][4u * lane]);
-      const float x[4] = {v.x, v.y, v.z, v.w};
-      if (t < p.T) lm_row<4>(p, x, t, v0, lane);
+    const uint32_t t = 32u * (tt * MT + m) + orow, k = token[m] - v0;
+    if (part == 0u && k < LM_COLS) p.xt[t] = s_out[orow][k];
+    float x[32];
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+      const f32x4_v v = *reinterpret_cast<const f32x4_v*>(&s_out[orow][32u * i + 4u * part]);
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) x[4 * i + e] = v[e];
     }
+    lm_sums<LM_COLS, 8>(p, x, t, v0, part, t < p.T);
   }
 }
 
@@ -814,8 +897,8 @@ LogitsPlan logits_plan(uint32_t T, uint32_t vocab, uint32_t k) {
 constexpr uint32_t LM_FEW = 32;
 struct LmPlan {
   uint32_t rows, mt, tiles, ld;  // token rows of a pass, 32-row blocks of a workgroup
-  size_t stat, xt, logits, xp, xs;
-  size_t all() const { return stat + xt + logits + xp + xs; }
+  size_t stat, xt, logits, xp, xf, xs;
+  size_t all() const { return stat + xt + logits + xp + xf + xs; }
 };
 LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   LmPlan d{};
@@ -824,13 +907,14 @@ LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   d.ld = (vocab + 3u) & ~3u;
   // the logits of a pass where alternatives are wanted, and its sums, are of a bounded size
   d.rows = T <= LM_FEW ? T : std::min(T, k ? 256u : 4096u);
-  d.mt = d.rows <= 64u ? 2u : 4u;
+  d.mt = d.rows <= 64u ? 2u : 3u;
   const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = (d.rows + 32u * d.mt - 1u) / (32u * d.mt) * d.mt;
   d.stat = up256(static_cast<size_t>(d.rows) * d.tiles * sizeof(float4));
   d.xt = up256(static_cast<size_t>(d.rows) * sizeof(float));
   d.logits = k ? up256(static_cast<size_t>(d.rows) * d.ld * sizeof(float)) : 0u;
   if (T > LM_FEW) {
     d.xp = up256(blocks * 64u * in);
+    d.xf = up256(blocks * 32u * sizeof(float));
     d.xs = up256(blocks * LM_SUMS * gpad * 64u);
   }
   return d;
@@ -869,10 +953,10 @@ int launch_few(obs_ctx* ctx, const LmArgs& a) {
   return a.in <= 2048u ? go(lm_few_kernel<2, true>) : go(lm_few_kernel<2, false>);
 }
 template <uint32_t MT>
-int launch_many(obs_ctx* ctx, const LmArgs& a, uint8_t* xp, uint8_t* xs) {
-  const uint32_t ttiles = (a.T + 32u * MT - 1u) / (32u * MT), gpad = (a.in / 64u + 15u) & ~15u;
-  OBS_LAUNCH(ctx, "lm_rows", lm_rows_kernel<MT><<<ttiles * MT * (gpad / 8u), 256, 0, ctx->stream>>>(a.x, a.T, a.in, xp, xs));
-  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT><<<(a.tiles + 7u) / 8u * 8u * ttiles, 256, 0, ctx->stream>>>(a, xp, xs, ttiles));
+int launch_many(obs_ctx* ctx, const LmArgs& a, uint8_t* xp, float* xf, uint8_t* xs) {
+  const uint32_t ttiles = (a.T + 32u * MT - 1u) / (32u * MT);
+  OBS_LAUNCH(ctx, "lm_rows", lm_rows_kernel<MT><<<ttiles * MT * 4u, 512, 0, ctx->stream>>>(a.x, a.T, a.in, xp, xf, xs));
+  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT><<<(a.tiles + 7u) / 8u * 8u * ttiles, 256, 0, ctx->stream>>>(a, xp, xf, xs, ttiles));
   return OBS_OK;
 }
 }  // namespace
@@ -957,14 +1041,15 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
   float4* stat = reinterpret_cast<float4*>(wb);
   float* xt = reinterpret_cast<float*>(wb + d.stat);
   float* logits = top_k ? reinterpret_cast<float*>(wb + d.stat + d.xt) : nullptr;
-  uint8_t *xp = wb + d.stat + d.xt + d.logits, *xs = xp + d.xp;
+  uint8_t *xp = wb + d.stat + d.xt + d.logits, *xs = xp + d.xp + d.xf;
+  float* xf = reinterpret_cast<float*>(xp + d.xp);
   for (uint32_t t0 = 0; t0 < T; t0 += d.rows) {
     const uint32_t n = std::min(d.rows, T - t0);
     const LmArgs a{x + static_cast<size_t>(t0) * in, w, scales, biases, tokens ? tokens + t0 : nullptr, xt, stat, logits, n, in, vocab, d.tiles, d.ld};
     if (T <= LM_FEW)
       rc = launch_few(ctx, a);
     else
-      rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xs) : launch_many<4>(ctx, a, xp, xs);
+      rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xf, xs) : launch_many<3>(ctx, a, xp, xf, xs);
     if (rc != OBS_OK) return rc;
     const JoinArgs j{stat, reinterpret_cast<const float*>(stat), reinterpret_cast<const uint8_t*>(logits), xt, a.tokens,
                      logprob ? logprob + t0 : nullptr, entropy ? entropy + t0 : nullptr,

@@ -8,7 +8,8 @@ wave's and workgroup's trees, the parts or tiles of a row, five a thread, again 
 So log s is off by (ADDS + 2 + 3 W) u and its own rounding, w / s by (2 ADDS + 4) u W +
 3 u Q, and log p = (x - m) - log s by what its terms have and round. From hidden rows a
 logit is off by the fp32 sums of a group, 64 additions of s (16 + q) |x| and
-|b - 16 s| |x|, and of the groups: (64 + in / 64 + 8) u of the sum of those; log p by
+|b - 16 s| |x|, and of the groups: (64 + in / 64 + 8) u of the sum of those; beyond 32 rows
+an x below 2^-24 of its row's largest is held to within 2^-35 of that; log p by
 twice the worst of them, an entropy by that times sum p |log p + H|."""
 import ctypes as C
 
@@ -151,6 +152,17 @@ def test_logits_of_the_kinds_that_go_wrong(exe):
     _logits_case(exe, synth.bf16_bits_to_f32(synth.f32_to_bf16_bits(y)), np.arange(14), k, True)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+def test_logits_equal_in_masses(exe, bf16):
+    """More equal tiles and logits than the lists hold; the lowest ids win, also where the last tile is cut."""
+    V = 700001
+    x = np.zeros((3, V), np.float32)
+    x[1, V - 1] = 1.0
+    x[2] = np.where(np.arange(V) < 300000, -np.inf, -2.0)
+    _logits_case(exe, x, np.array([V - 1, 7, 300000]), 64, bf16, pad=3)
+    _logits_case(exe, x, np.array([V - 1, 7, 299999]), 1, bf16, pad=0)
+
+
 def test_logits_every_row_its_own_offset(exe):
     """Rows of a long prompt whose tensor passes 4 GiB."""
     T, V, ld = 2100, 151936, 520000
@@ -185,12 +197,14 @@ def _logits64(x, w, s, b):
     """Logits and what their fp32 sums may be off."""
     H = x.shape[1]
     out, off = np.empty((x.shape[0], w.shape[0])), np.empty((x.shape[0], w.shape[0]))
+    top = np.abs(x).max(1, keepdims=True)
+    small = np.where((np.abs(x) < 2.0 ** -24 * top) & (x != 0) & (x.shape[0] > 32), 2.0 ** -35 * top, 0)
     for v in range(0, w.shape[0], 4096):
         q = ((w[v:v + 4096, :, None] >> np.arange(0, 32, 4, dtype=np.uint32)) & 15).reshape(-1, H).astype(np.float64)
         ss, bb = (np.repeat(_f64(y[v:v + 4096]), 64, 1) for y in (s, b))
         out[:, v:v + 4096] = x @ (q * ss + bb).T
-        off[:, v:v + 4096] = np.abs(x) @ (ss * (16 + q) + np.abs(bb - 16 * ss)).T
-    return out, off * (64 + H // 64 + 8) * 2.0 ** -24
+        off[:, v:v + 4096] = np.abs(x) @ (ss * (16 + q) + np.abs(bb - 16 * ss)).T * ((64 + H // 64 + 8) * U) + small @ (q * ss).T
+    return out, off
 
 
 def _lm_case(exe, T, H, V, k, seed, scale=1.0, tokens=None):
@@ -230,6 +244,29 @@ def test_lm_rows(exe, T):
                                      (600, 512, 5003, 2), (260, 1536, 513, 0), (1, 2048, 40000, 5), (24, 2048, 40001, 20), (200, 2048, 20000, 3)])
 def test_lm_shapes(exe, T, H, V, k):
     _lm_case(exe, T, H, V, k, T + H + V)
+
+
+@pytest.mark.parametrize("T", [5, 40])
+def test_lm_columns_of_all_sizes(exe, T):
+    """Columns from 2^-40 to 2^40 of the others', whole blocks of them, zeros, and rows at the ends of bf16's range."""
+    rng = np.random.default_rng(6)
+    H, V = 1024, 999
+    w, s, b = _matrix(rng, V, H)
+    x = rng.standard_normal((T, H)) * np.exp2(rng.integers(-14, 15, (T, H)))
+    x[0, ::2] = 0
+    x[1] = 0
+    x[2] *= np.exp2(np.repeat(rng.integers(-40, 41, H // 32), 32))
+    x[3] *= 2.0 ** -120
+    x[4] *= 2.0 ** 90 * (np.arange(H) < 32)
+    xb = synth.f32_to_bf16_bits(x.astype(np.float32))
+    args = [exe.upload(a) for a in (xb, w, s, b)]
+    tokens = rng.integers(0, V, T)
+    got = _run(exe, T, 1, tokens, lambda **kw: exe.lm_logprobs(*args, T, H, V, **kw), exe.lm_logprobs_workspace(T, H, V, 1))
+    logits, off = _logits64(_f64(xb), w, s, b)
+    lp, ent, ids, tlp, bs, be = _reference(logits, tokens, 1)
+    assert np.all(np.abs(got[0] - lp) <= bs + 4 * U * np.abs(lp) + 2 * off.max(1))
+    t = np.arange(T)
+    assert np.all(logits[t, got[2][:, 0]] >= logits[t, ids[:, 0]] - 2 * off.max(1))
 
 
 def test_lm_large_rows(exe):
