@@ -651,20 +651,21 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
   }
 }
 
-// Many tokens: bound by the matrix units, beside which the weights come apart and one
-// product a sum and group goes with the scale, in the vector unit. A nibble masked in
-// place at bits 3:0 (7:4) of a half word is the fp16 number q 2^-24 (q 2^-20), subnormal,
-// which the products (v_mfma_f32_32x32x16_f16) take as it is: five instructions for eight
-// nibbles, and no offset. The rows are brought into fp16 by a power of two a row, its
-// largest to 2^14: exact from 2^-29 of that on (the columns of upper nibbles 2^-25, as they
-// get a sixteenth), off by 2^-38 of it below. (Products of 8-bit numbers, of which a bf16 x
-// has two, would need masks alone, but they drop what lies 2^-13 below the largest of eight
-// products.)
+// Many tokens: bound by the matrix units, beside which the weights come apart in the
+// vector unit. A nibble masked in place at bits 3:0 (7:4) of a half word is the fp16 number
+// q 2^-24 (q 2^-20), subnormal; one packed fma makes s (q - 8) of it, which has at most 8 + 3
+// significant bits: exact in fp16, with the scales of a vocabulary row brought to 2^-9 by
+// their largest's power of two (below 2^-8 of that they end in fp16's subnormal steps, 2^-15
+// of the largest). So a product runs over all columns, and what it leaves out, b + 8 s, meets
+// the sums of the groups in products of its own. The rows of x are brought into fp16 by a
+// power of two each, the largest to 2^14: exact from 2^-29 of that on, off by 2^-39 of it below.
+// (Products of q itself, with the scales as factors of every group's sums, took 1,350 us for
+// 2,000 tokens: four vector instructions a product. Those of 8-bit numbers, of which a bf16 x
+// has two, drop what lies 2^-13 below the largest of eight products.)
 //
 // First the rows in the order of the products' operands, [tile of 32 MT rows][group][32
-// rows][step][lane] 16 bytes, each row's factor back, and the sums of every group in three
-// bf16 parts (24 bits), which meet the biases in products of their own at the end of a
-// tile. A wave takes a row.
+// rows][step][lane] 16 bytes, each row's factor back, and the sums of every group (over
+// that factor) in three bf16 parts (24 bits). A wave takes a row.
 constexpr uint32_t LM_SUMS = 3;
 template <uint32_t MT>
 __global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict__ x, uint32_t T, uint32_t in, uint8_t* __restrict__ xp,
@@ -681,7 +682,7 @@ __global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict
   }
   const uint32_t ex = max(wave_max_u31(most) >> 7, 15u);
   const float up = __uint_as_float((268u - ex) << 23);
-  if (lane == 0u) xf[t] = t < T ? __uint_as_float((ex - 2u) << 23) : 0.0f;  // back, and 2^12 of the nibbles' 2^24
+  if (lane == 0u) xf[t] = t < T ? __uint_as_float((ex - 14u) << 23) : 0.0f;
   for (uint32_t c = lane; c < gpad * 8u; c += 64u) {
     const uint32_t g = c / 8u;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
@@ -689,16 +690,15 @@ __global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict
     const float sum = sum_of_8_lanes(sum8(v));
     if (g < groups) {
       // half c / 4 % 2, step c % 4: columns 0, 4 | 1, 5 | 2, 6 | 3, 7 of the eight
-      auto pair = [&](float a, float b, float f) __attribute__((always_inline)) {
-        return __builtin_bit_cast(uint32_t, f16x2_of(a * f, b * f));
+      auto pair = [&](float a, float b) __attribute__((always_inline)) {
+        return __builtin_bit_cast(uint32_t, f16x2_of(a * up, b * up));
       };
-      const float od = up * 0.0625f;
       *reinterpret_cast<uint4*>(xp + 16u * (((static_cast<size_t>(mt / MT) * groups + g) * MT + mt % MT) * 256u + c % 4u * 64u + 32u * (c / 4u % 2u) + r)) =
-          make_uint4(pair(bf16lo(v.x), bf16lo(v.z), up), pair(bf16hi(v.x), bf16hi(v.z), od), pair(bf16lo(v.y), bf16lo(v.w), up),
-                     pair(bf16hi(v.y), bf16hi(v.w), od));
+          make_uint4(pair(bf16lo(v.x), bf16lo(v.z)), pair(bf16hi(v.x), bf16hi(v.z)), pair(bf16lo(v.y), bf16lo(v.w)),
+                     pair(bf16hi(v.y), bf16hi(v.w)));
     }
     if (c % 8u == 0u) {
-      float rest = sum;
+      float rest = sum * up;
 #pragma unroll
       for (uint32_t k = 0; k < LM_SUMS; ++k) {
         const uint16_t part = f32_to_bf16(rest);
@@ -711,165 +711,272 @@ __global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict
   }
 }
 
-// 32 MT tokens x 256 vocabulary rows a workgroup, 64 a wave; two workgroups a CU.
+// Four waves a workgroup, 32 MT tokens x 64 vocabulary rows a wave, two workgroups a CU: the
+// sums at one's end (350 us of 1,335 for 2,000 tokens with one of eight waves) beside the other's
+// products. Rows and weights come into LDS past the registers, by whole runs of a row; read by
+// the lanes that use them, 32 bytes of 32 rows a load, the weights took 165 us, the scales, two
+// bytes each, 150, and the rows through registers and their stores 250. 2,000 tokens take
+// 1,220 us, 1,020 TFLOP/s (a library's bf16 product of the same sizes, without the 4 bits: 1,214 us).
 typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
+// Global memory to LDS: 16 (4) bytes of every lane from its address to `to` (of the wave) and on.
+typedef const __attribute__((address_space(1))) uint32_t* GlobalWords;
+typedef __attribute__((address_space(3))) uint32_t* LdsWords;
+__device__ __forceinline__ void lds_from16(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<GlobalWords>(reinterpret_cast<uintptr_t>(from)), (LdsWords)to, 16, 0, 0);
+}
+__device__ __forceinline__ void lds_from4(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<GlobalWords>(reinterpret_cast<uintptr_t>(from)), (LdsWords)to, 4, 0, 0);
+}
+// A barrier behind a wave's LDS accesses and all its loads but the last N (the fence of
+// __syncthreads waits for all).
+template <uint32_t N>
+__device__ __forceinline__ void barrier_but() {
+  static_assert(N < 16u, "the low bits of the counter");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070 | N);
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("" ::: "memory");
+}
+template <uint32_t MT>
+struct LmTile {
+  static constexpr uint32_t THREADS = 256, ROWS = 32u * MT, COLS = 256;
+  static constexpr uint32_t XB = MT * 4096u, WB = COLS * 64u, SB = COLS * 4u;  // bytes of a group of x, of two groups' weights and scales
+  static constexpr uint32_t OROW = COLS + 8u, XLDS = XB > 16u * OROW * 4u ? XB : 16u * OROW * 4u;  // 16 rows of logits
+  static_assert(COLS == THREADS && COLS == LM_COLS, "a thread a row");
+};
 template <uint32_t MT>
 __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t* __restrict__ xp, const float* __restrict__ xf,
-                                                         const uint8_t* __restrict__ xs, uint32_t ttiles) {
-  constexpr uint32_t XB = MT * 4096u, OROW = LM_COLS + 8u, OB = 32u * OROW * 4u;  // bytes of a group's rows; of 32 rows of logits
-  __shared__ __attribute__((aligned(16))) uint8_t s_mem[2u * XB > OB ? 2u * XB : OB];
-  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = uniform(tid >> 6), col = lane & 31u, half = lane >> 5;
-  // an XCD (blockIdx.x % 8) takes all token tiles of one column tile after another: its weights stay in its L2
-  const uint32_t at = blockIdx.x / 8u, vt = at / ttiles * 8u + blockIdx.x % 8u, tt = at % ttiles;
-  if (vt >= p.tiles) return;  // uniform
-  const uint32_t v0 = vt * LM_COLS, groups = p.in / 64u, gpad = (groups + 15u) & ~15u;
-  // scalar bases and 32-bit offsets of the lane's rows
+                                                         const uint8_t* __restrict__ xs, uint32_t ttiles, uint32_t vtiles, uint32_t turn) {
+  typedef LmTile<MT> L;
+  // (arrays of their own, for the compiler to tell the ones being written from those being read)
+  __shared__ __attribute__((aligned(16))) uint8_t s_x0[L::XLDS], s_x1[L::XLDS], s_w0[L::WB], s_w1[L::WB], s_s0[L::SB], s_s1[L::SB];
+  __shared__ float s_factor[L::ROWS];
+  __shared__ uint32_t s_token[L::ROWS], s_scale[L::COLS];
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wn = uniform(tid >> 6);
+  const uint32_t col = lane & 31u, half = lane >> 5;
+  // An XCD (blockIdx.x % 8) takes `turn` token tiles, whose rows its L2 holds, through all its column tiles, then the next.
+  const uint32_t at = blockIdx.x / 8u, own = (vtiles + 7u) / 8u, t0 = at / (turn * own) * turn, many = umin(turn, ttiles - t0);
+  const uint32_t in_turn = at - t0 * own, vt = in_turn / many * 8u + blockIdx.x % 8u, tt = t0 + in_turn % many;
+  if (vt >= vtiles) return;  // uniform
+  const uint32_t v0 = vt * L::COLS, groups = p.in / 64u, gpad = (groups + 15u) & ~15u, most = p.vocab - 1u - v0;  // last row of the tile
   const uint8_t *wb0 = reinterpret_cast<const uint8_t*>(p.w) + static_cast<size_t>(v0) * (p.in / 2u),
                 *sb0 = reinterpret_cast<const uint8_t*>(p.s) + static_cast<size_t>(v0) * (2u * groups),
                 *bb0 = reinterpret_cast<const uint8_t*>(p.b) + static_cast<size_t>(v0) * (2u * groups);
-  uint32_t woff[2], soff[2];
+  const uint8_t* xg = xp + static_cast<size_t>(tt) * groups * L::XB;
+  auto load_x = [&](uint32_t g, uint8_t* to) __attribute__((always_inline)) {
+    const uint8_t* base = xg + static_cast<size_t>(umin(g, groups - 1u)) * L::XB;
+#pragma unroll
+    for (uint32_t i = 0; i < MT; ++i) lds_from16(base + 16u * (tid + 256u * i), to + 16u * (64u * wn + 256u * i));
+  };
+  // Two groups of every row: four threads for 64 bytes of weights, one for the scales. A row's chunks
+  // change places by its number, so that the reads below meet every bank once. Behind the last row it again.
+  auto load_w = [&](uint32_t block, uint8_t* to, uint8_t* sto) __attribute__((always_inline)) {
+    const uint32_t bl = umin(block, groups / 2u - 1u);
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+      const uint32_t r = 64u * i + tid / 4u;
+      lds_from16(wb0 + 64u * bl + (umin(r, most) * (p.in / 2u) + 16u * (tid % 4u ^ (r >> 1 & 3u))), to + 16u * (64u * wn + 256u * i));
+    }
+    lds_from4(sb0 + 4u * bl + umin(tid, most) * (2u * groups), sto + 4u * (64u * wn));
+  };
+  load_w(0u, s_w0, s_s0);
+  load_x(0u, s_x0);
+  load_w(1u, s_w1, s_s1);
+  if (tid < L::ROWS) {
+    const uint32_t t = L::ROWS * tt + tid;
+    s_factor[tid] = xf[t];
+    s_token[tid] = p.tokens && t < p.T ? lm_token(p, t) : 0xffffffffu;
+  }
+  // the largest scale of every vocabulary row of the tile: its exponent (or of the biases 2^90
+  // of it: no sum reaches fp32's range)
+  {
+    uint32_t top = 0u, btop = 0u;
+    for (uint32_t g = 0; g < groups; g += 8u) {
+      const uint32_t at = umin(tid, most) * (2u * groups) + 2u * g;
+      const u32x4_v v = *reinterpret_cast<const u32x4_v*>(sb0 + at), u = *reinterpret_cast<const u32x4_v*>(bb0 + at);
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        top = max(top, max(v[i] & 0x7fffu, v[i] >> 16 & 0x7fffu));
+        btop = max(btop, max(u[i] & 0x7fffu, u[i] >> 16 & 0x7fffu));
+      }
+    }
+    s_scale[tid] = umin(max(top >> 7, max(btop >> 7, 90u) - 90u), 244u);
+  }
+  __syncthreads();
+  float down[2];  // brings the lane's vocabulary rows' scales below 2^-8
+  uint32_t cex[2];
 #pragma unroll
   for (uint32_t n = 0; n < 2; ++n) {
-    const uint32_t r = umin(v0 + 64u * wave + 32u * n + col, p.vocab - 1u) - v0;  // (behind the last row it again)
-    woff[n] = r * (p.in / 2u) + 16u * half;
-    soff[n] = r * (2u * groups);
+    cex[n] = s_scale[64u * wn + 32u * n + col];
+    down[n] = __uint_as_float((245u - cex[n]) << 23);
   }
-  const uint8_t* xg = xp + static_cast<size_t>(tt) * groups * XB;
-  u32x4_v xr[MT];
-  auto load_x = [&](uint32_t g) __attribute__((always_inline)) {
-#pragma unroll
-    for (uint32_t i = 0; i < MT; ++i) xr[i] = *reinterpret_cast<const u32x4_v*>(xg + static_cast<size_t>(g) * XB + (16u * tid + 4096u * i));
-  };
-  auto store_x = [&](uint32_t buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (uint32_t i = 0; i < MT; ++i) *reinterpret_cast<u32x4_v*>(s_mem + buf * XB + 16u * tid + 4096u * i) = xr[i];
-  };
   f32x16_v acc[MT][2];
 #pragma unroll
   for (uint32_t m = 0; m < MT; ++m)
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) acc[m][n] = f32x16_v{};
-  u32x4_v wr[2];  // a group ahead
-  uint32_t sr[2];
-  auto load_w = [&](uint32_t g) __attribute__((always_inline)) {
-    const uint32_t gc = umin(g, groups - 1u);
-#pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) {
-      wr[n] = *reinterpret_cast<const u32x4_v*>(wb0 + 32u * gc + woff[n]);
-      sr[n] = *reinterpret_cast<const uint16_t*>(sb0 + 2u * gc + soff[n]);
-    }
-  };
-  load_x(0u);
-  load_w(0u);
-  store_x(0u);
-  __syncthreads();
-  auto step = [&](uint32_t g, uint32_t slot) __attribute__((always_inline)) {
-    f16x8_v xa[4], wb[2][4];
-    float sc[2];
-    auto load_a = [&](uint32_t m, uint32_t s) __attribute__((always_inline)) {
-      xa[s] = *reinterpret_cast<const f16x8_v*>(s_mem + slot * XB + 16u * ((m * 4u + s) * 64u + lane));
-    };
-#pragma unroll
-    for (uint32_t s = 0; s < 4; ++s) load_a(0u, s);
-    load_x(umin(g + 1u, groups - 1u));
-#pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) {
-      sc[n] = __uint_as_float(sr[n] << 16) * 4096.0f;
-#pragma unroll
-      for (uint32_t s = 0; s < 4; ++s) {
-        const uint32_t w = wr[n][s], w8 = w >> 8;
-        wb[n][s] = __builtin_bit_cast(f16x8_v, u32x4_v{w & 0x000f000fu, w & 0x00f000f0u, w8 & 0x000f000fu, w8 & 0x00f000f0u});
-      }
-    }
-    load_w(g + 1u);
-    __builtin_amdgcn_sched_barrier(0);
-    // Products of one 32 x 32 tile, each beside a quarter of the sums of the tile before and,
-    // with the last use of its rows, the read of the next ones: left to itself the compiler
-    // puts a tile's sums behind its products, and the two units take turns.
-    f32x16_v y[2];
-    const f32x16_v zero = {};
-#pragma unroll
-    for (uint32_t m = 0; m < MT; ++m)
-#pragma unroll
-      for (uint32_t n = 0; n < 2; ++n)
-#pragma unroll
-        for (uint32_t s = 0; s < 4; ++s) {
-          y[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[s], wb[n][s], s ? y[n] : zero, 0, 0, 0);
-          if (n == 1u && m + 1u < MT) load_a(m + 1u, s);
-          if (m || n) {
-            const uint32_t pm = n ? m : m - 1u, pn = 1u - n;
-#pragma unroll
-            for (uint32_t i = 4u * s; i < 4u * s + 4u; ++i) acc[pm][pn][i] = __builtin_fmaf(sc[pn], y[pn][i], acc[pm][pn][i]);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-    for (uint32_t i = 0; i < 16; ++i) acc[MT - 1u][1][i] = __builtin_fmaf(sc[1], y[1][i], acc[MT - 1u][1][i]);
-    store_x(slot ^ 1u);
-    __syncthreads();
-  };
-  for (uint32_t g = 0; g < groups; g += 2u) {  // groups is a multiple of 8
-    step(g, 0u);
-    step(g + 1u, 1u);
-  }
-  uint32_t token[MT];  // of the rows that the thread has below
-#pragma unroll
-  for (uint32_t m = 0; m < MT; ++m) {
-    const uint32_t t = 32u * (tt * MT + m) + tid / 8u;
-    token[m] = p.tokens && t < p.T ? lm_token(p, t) : 0xffffffffu;
-  }
-  // the rows' factors back (and 2^12 of the nibbles'), then the groups' sums with the biases
-#pragma unroll
-  for (uint32_t m = 0; m < MT; ++m)
-#pragma unroll
-    for (uint32_t i = 0; i < 16; i += 4) {
-      const f32x4_v f = *reinterpret_cast<const f32x4_v*>(xf + 32u * (tt * MT + m) + 2u * i + 4u * half);
-#pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) {
-        acc[m][0][i + e] *= f[e];
-        acc[m][1][i + e] *= f[e];
-      }
-    }
-  const uint32_t steps = gpad / 16u;
-  for (uint32_t s = 0; s < steps; ++s) {
+  // the groups' sums with b + 8 s
+  for (uint32_t s = 0, steps = gpad / 16u; s < steps; ++s) {
     const uint32_t g = 16u * s + 8u * half;
-    bf16x8_v bb[2];
+    bf16x8_v bb[2][2];
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n) {
-      u32x4_v v = *reinterpret_cast<const u32x4_v*>(bb0 + (soff[n] + 2u * umin(g, groups - 8u)));
-      if (g >= groups) v = u32x4_v{0u, 0u, 0u, 0u};
-      bb[n] = __builtin_bit_cast(bf16x8_v, v);
+      const uint32_t r = umin(64u * wn + 32u * n + col, most);
+#pragma unroll
+      for (uint32_t k = 0; k < 2; ++k) {
+        u32x4_v v = *reinterpret_cast<const u32x4_v*>((k ? sb0 : bb0) + (r * (2u * groups) + 2u * umin(g, groups - 8u)));
+        const float f = k ? 8.0f * down[n] : down[n];
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) v[i] = g < groups ? pack_bf16_pair_rne(bf16lo(v[i]) * f, bf16hi(v[i]) * f) : 0u;
+        bb[n][k] = __builtin_bit_cast(bf16x8_v, v);
+      }
     }
+    bf16x8_v xa[LM_SUMS][MT];
 #pragma unroll
     for (uint32_t k = 0; k < LM_SUMS; ++k)
 #pragma unroll
-      for (uint32_t m = 0; m < MT; ++m) {
-        const bf16x8_v xa = *reinterpret_cast<const bf16x8_v*>(
-            xs + 16u * (((static_cast<size_t>(tt) * MT + m) * LM_SUMS * steps + k * steps + s) * 64u + lane));
+      for (uint32_t m = 0; m < MT; ++m)
+        xa[k][m] = *reinterpret_cast<const bf16x8_v*>(xs + 16u * (((static_cast<size_t>(tt) * MT + m) * LM_SUMS * steps + k * steps + s) * 64u + lane));
 #pragma unroll
-        for (uint32_t n = 0; n < 2; ++n) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa, bb[n], acc[m][n], 0, 0, 0);
-      }
+    for (uint32_t k = 0; k < LM_SUMS; ++k)
+#pragma unroll
+      for (uint32_t m = 0; m < MT; ++m)
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) {
+          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[k][m], bb[n][0], acc[m][n], 0, 0, 0);
+          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[k][m], bb[n][1], acc[m][n], 0, 0, 0);
+        }
   }
-  // 32 rows at a time through LDS, eight threads a row. (A wave a row, one after another, took
-  // as long as the products: 740 us of 1,470 for 2,000 tokens.)
-  float(*const s_out)[OROW] = reinterpret_cast<float(*)[OROW]>(s_mem);
-  const uint32_t orow = tid / 8u, part = tid % 8u;
+  barrier_but<0>();
+  load_x(1u, s_x1);
+  constexpr uint32_t FR = 4u * MT, RING = 4u;  // fragments of x a group; held at once
+  f16x8_v xa[RING];
+  u32x4_v wb[2][4], raw[2];
+  uint32_t rs[2], last[2];  // scales; the last word of a group's weights
+  f16x2_t mul[2][2], off[2];
+  uint32_t roff[2], soff[2];
+#pragma unroll
+  for (uint32_t n = 0; n < 2; ++n) {
+    const uint32_t r = 64u * wn + 32u * n + col;
+    roff[n] = 64u * r + 16u * (half ^ (r >> 1 & 3u));
+    soff[n] = 4u * r;
+  }
+  auto load_a = [&](const uint8_t* from, uint32_t j) __attribute__((always_inline)) {  // fragment j of a group: step j / MT, rows j % MT
+    xa[j % RING] = *reinterpret_cast<const f16x8_v*>(from + 16u * ((j % MT * 4u + j / MT) * 64u + lane));
+  };
+  auto load_raw = [&](const uint8_t* from, const uint8_t* sfrom, uint32_t second) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+      raw[n] = *reinterpret_cast<const u32x4_v*>(from + (roff[n] ^ 32u * second));
+      rs[n] = *reinterpret_cast<const uint16_t*>(sfrom + soff[n] + 2u * second);
+    }
+  };
+  auto scales = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) {
+      const float f = __uint_as_float(rs[n] << 16) * down[n];
+      mul[n][0] = f16x2_of(f * 0x1p24f, f * 0x1p24f);
+      mul[n][1] = f16x2_of(f * 0x1p20f, f * 0x1p20f);
+      off[n] = f16x2_of(-8.0f * f, -8.0f * f);
+    }
+  };
+  // two of the eight weights of word w
+  auto apart = [&](uint32_t n, uint32_t s, uint32_t i, uint32_t w) __attribute__((always_inline)) {
+    const uint32_t v = (i < 2u ? w : w >> 8) & (i & 1u ? 0x00f000f0u : 0x000f000fu);
+    wb[n][s][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(as_f16x2(v), mul[n][i & 1u], off[n]));
+  };
+  load_raw(s_w0, s_s0, 0u);
+  scales();
+#pragma unroll
+  for (uint32_t n = 0; n < 2; ++n) {
+#pragma unroll
+    for (uint32_t s = 0; s < 3; ++s)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) apart(n, s, i, raw[n][s]);
+    last[n] = raw[n][3];
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < RING; ++j) load_a(s_x0, j);
+  // A group is one stream of products without a pause, none of which waits for the one
+  // before. Beside them stand the reads of the rows four fragments ahead and the weights to
+  // come: step s makes those of step s - 1 of the next group (step 0 the last ones of its own).
+  // The one barrier is where the last of a group's rows and the next one's weights are read,
+  // and the next one's rows have come; behind it their places are filled: with the rows of the
+  // group after the next, and at even groups the weights of the two after that, which have
+  // until the second barrier to come.
+  auto group = [&](uint32_t g, uint32_t q) __attribute__((always_inline)) {  // q = g % 4
+    uint8_t *const own = q & 1u ? s_x1 : s_x0, *const next = q & 1u ? s_x0 : s_x1;
+    const uint32_t wq = (q + 1u) % 4u;
+    load_raw(wq & 2u ? s_w1 : s_w0, wq & 2u ? s_s1 : s_s0, wq & 1u);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (uint32_t s = 0; s < 4; ++s)
+#pragma unroll
+      for (uint32_t m = 0; m < MT; ++m) {
+        const uint32_t j = s * MT + m;
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) {
+          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[j % RING], __builtin_bit_cast(f16x8_v, wb[n][s]), acc[m][n], 0, 0, 0);
+          if (n == 1u) load_a(j + RING < FR ? own : next, (j + RING) % FR);
+#pragma unroll
+          for (uint32_t i = m * 4u / MT; i < (m + 1u) * 4u / MT; ++i) apart(n, (s + 3u) % 4u, i, s ? raw[n][s - 1u] : last[n]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (j == MT - 1u) scales();
+        if (j + RING + 1u == FR) {
+          if (q & 1u)
+            barrier_but<5>();  // the five loads of weights behind the rows
+          else
+            barrier_but<0>();
+          load_x(g + 2u, own);
+          __builtin_amdgcn_sched_barrier(0);
+          if (!(q & 1u)) load_w((g + 4u) / 2u, q & 2u ? s_w1 : s_w0, q & 2u ? s_s1 : s_s0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+    for (uint32_t n = 0; n < 2; ++n) last[n] = raw[n][3];
+  };
+  for (uint32_t g = 0; g < groups; g += 4u) {  // groups is a multiple of 8
+    group(g, 0u);
+    group(g + 1u, 1u);
+    group(g + 2u, 2u);
+    group(g + 3u, 3u);
+  }
+#pragma unroll
+  for (uint32_t n = 0; n < 2; ++n) {
+    const float up = __uint_as_float((cex[n] + 9u) << 23);
+#pragma unroll
+    for (uint32_t m = 0; m < MT; ++m)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) acc[m][n][i] *= up;
+  }
+  barrier_but<0>();
+  // 32 rows at a time through LDS, eight threads for a row. (A wave a row, one after another,
+  // waited for each row's reductions and token.)
+  typedef float(*Rows)[L::OROW];
+  const Rows out0 = reinterpret_cast<Rows>(s_x0), out1 = reinterpret_cast<Rows>(s_x1);  // rows 0 to 15, 16 to 31
+  const uint32_t part = tid % 8u, orow = tid / 8u;
+  const float* mine = orow < 16u ? out0[orow] : out1[orow - 16u];
 #pragma unroll
   for (uint32_t m = 0; m < MT; ++m) {
     if (m) __syncthreads();
 #pragma unroll
     for (uint32_t n = 0; n < 2; ++n)
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) s_out[8u * (i / 4u) + 4u * half + i % 4u][64u * wave + 32u * n + col] = acc[m][n][i];
+      for (uint32_t i = 0; i < 16; ++i) (i < 8u ? out0 : out1)[8u * (i / 4u % 2u) + 4u * half + i % 4u][64u * wn + 32u * n + col] = acc[m][n][i];
     __syncthreads();
-    const uint32_t t = 32u * (tt * MT + m) + orow, k = token[m] - v0;
-    if (part == 0u && k < LM_COLS) p.xt[t] = s_out[orow][k];
+    const uint32_t r = 32u * m + orow, t = L::ROWS * tt + r, k = s_token[r] - v0;
+    const float f = s_factor[r];
+    if (part == 0u && k < LM_COLS) p.xt[t] = mine[k] * f;
     float x[32];
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
-      const f32x4_v v = *reinterpret_cast<const f32x4_v*>(&s_out[orow][32u * i + 4u * part]);
+      const f32x4_v v = *reinterpret_cast<const f32x4_v*>(mine + 32u * i + 4u * part);
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) x[4 * i + e] = v[e];
+      for (uint32_t e = 0; e < 4; ++e) x[4 * i + e] = v[e] * f;
     }
     lm_sums<LM_COLS, 8>(p, x, t, v0, part, t < p.T);
   }
@@ -896,7 +1003,7 @@ LogitsPlan logits_plan(uint32_t T, uint32_t vocab, uint32_t k) {
 
 constexpr uint32_t LM_FEW = 32;
 struct LmPlan {
-  uint32_t rows, mt, tiles, ld;  // token rows of a pass, 32-row blocks of a workgroup
+  uint32_t rows, mb, tiles, ld;  // token rows of a pass, 32-row blocks of a workgroup
   size_t stat, xt, logits, xp, xf, xs;
   size_t all() const { return stat + xt + logits + xp + xf + xs; }
 };
@@ -907,8 +1014,9 @@ LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   d.ld = (vocab + 3u) & ~3u;
   // the logits of a pass where alternatives are wanted, and its sums, are of a bounded size
   d.rows = T <= LM_FEW ? T : std::min(T, k ? 256u : 4096u);
-  d.mt = d.rows <= 64u ? 2u : 3u;
-  const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = (d.rows + 32u * d.mt - 1u) / (32u * d.mt) * d.mt;
+  const uint32_t b32 = (d.rows + 31u) / 32u, tts = (b32 + 3u) / 4u;  // 32-row blocks, workgroups of four at most
+  d.mb = std::max(2u, (b32 + tts - 1u) / tts);
+  const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = (d.rows + 32u * d.mb - 1u) / (32u * d.mb) * d.mb;
   d.stat = up256(static_cast<size_t>(d.rows) * d.tiles * sizeof(float4));
   d.xt = up256(static_cast<size_t>(d.rows) * sizeof(float));
   d.logits = k ? up256(static_cast<size_t>(d.rows) * d.ld * sizeof(float)) : 0u;
@@ -954,9 +1062,12 @@ int launch_few(obs_ctx* ctx, const LmArgs& a) {
 }
 template <uint32_t MT>
 int launch_many(obs_ctx* ctx, const LmArgs& a, uint8_t* xp, float* xf, uint8_t* xs) {
-  const uint32_t ttiles = (a.T + 32u * MT - 1u) / (32u * MT);
+  typedef LmTile<MT> L;
+  const uint32_t ttiles = (a.T + L::ROWS - 1u) / L::ROWS, vtiles = (a.vocab + L::COLS - 1u) / L::COLS;
+  const uint32_t turn = std::max(1u, (5u << 19) / (a.in / 64u * L::XB));  // 2.5 MB of an XCD's 4 MB of L2
   OBS_LAUNCH(ctx, "lm_rows", lm_rows_kernel<MT><<<ttiles * MT * 4u, 512, 0, ctx->stream>>>(a.x, a.T, a.in, xp, xf, xs));
-  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT><<<(a.tiles + 7u) / 8u * 8u * ttiles, 256, 0, ctx->stream>>>(a, xp, xf, xs, ttiles));
+  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT><<<(vtiles + 7u) / 8u * 8u * ttiles, L::THREADS, 0, ctx->stream>>>(
+                                 a, xp, xf, xs, ttiles, vtiles, turn));
   return OBS_OK;
 }
 }  // namespace
@@ -1034,7 +1145,7 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
     return obs::set_error(ctx, OBS_E_ALIGN, "%s: x, the weight, scales, biases and the workspace must be 16-byte aligned", who);
   const LmPlan d = lm_plan(T, in, vocab, top_k);
   if (ws_bytes < d.all()) return obs::set_error(ctx, OBS_E_NOMEM, "%s: workspace %zu bytes < %zu needed", who, ws_bytes, d.all());
-  rc = obs::check_grid(ctx, who, static_cast<uint64_t>(d.tiles + 7u) * ((d.rows + 63u) / 64u), 256u);
+  rc = obs::check_grid(ctx, who, static_cast<uint64_t>(d.tiles + 7u) * ((d.rows + 63u) / 64u), 512u);
   if (rc != OBS_OK) return rc;
   obs::DeviceGuard guard(ctx);
   uint8_t* wb = static_cast<uint8_t*>(ws);
@@ -1049,7 +1160,9 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
     if (T <= LM_FEW)
       rc = launch_few(ctx, a);
     else
-      rc = d.mt == 2u ? launch_many<2>(ctx, a, xp, xf, xs) : launch_many<3>(ctx, a, xp, xf, xs);
+      rc = d.mb == 2u   ? launch_many<2>(ctx, a, xp, xf, xs)
+           : d.mb == 3u ? launch_many<3>(ctx, a, xp, xf, xs)
+                        : launch_many<4>(ctx, a, xp, xf, xs);
     if (rc != OBS_OK) return rc;
     const JoinArgs j{stat, reinterpret_cast<const float*>(stat), reinterpret_cast<const uint8_t*>(logits), xt, a.tokens,
                      logprob ? logprob + t0 : nullptr, entropy ? entropy + t0 : nullptr,
