@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
   __syncthreads();
   // the logits of those tiles that are as large as the last one's maximum: a wave takes
   // every fourth tile, four of them in flight
-  const float low = s_edge[4];
+  float low = s_edge[4];
   const bool vec = (reinterpret_cast<uintptr_t>(row) & 15u) == 0u;
   auto first_of = [&](uint32_t tile) __attribute__((always_inline)) {  // of the lane's PER logits
     if constexpr (TILE)
@@ -387,6 +387,19 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
       for (uint32_t e = 0; e < PER; ++e) x[e] = is && v + e < p.vocab ? logit(v + e) : NEG_INF;
     }
   };
+  if (low == NEG_INF) {  // uniform: fewer than k tiles; what k lanes of a wave reach with all of its logits
+    float m = NEG_INF;
+    for (uint32_t j = wave; j < rows; j += 4u) {
+      float x[PER];
+      load(j, x);
+#pragma unroll
+      for (uint32_t e = 0; e < PER; ++e) m = fmaxf(m, x[e]);
+    }
+    const float e = lanes_edge(m, k);
+    if (lane == 0u) s_edge[wave] = e;
+    __syncthreads();
+    low = fmaxf(fmaxf(s_edge[0], s_edge[1]), fmaxf(s_edge[2], s_edge[3]));
+  }
   for (uint32_t j0 = wave; j0 < rows; j0 += 16u) {
     float x[4][PER];
 #pragma unroll
@@ -404,6 +417,32 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
   }
   __syncthreads();
   n = uniform(s_n[1]);
+  // Of many the k largest by their upper bits, every wave over all (433 rows of 984 logits, k = 15: 13 us,
+  // with all of them ranked 90).
+  if (n > 128u && n <= CAP) {  // uniform
+    constexpr uint32_t PER_LANE = CAP / 64u;
+    uint64_t mine[CAP / 256u];
+    uint32_t keys[PER_LANE], e = 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < PER_LANE; ++i) keys[i] = 64u * i + lane < n ? static_cast<uint32_t>(s_list[64u * i + lane] >> 32) : 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < CAP / 256u; ++i) mine[i] = 256u * i + tid < n ? s_list[256u * i + tid] : 0u;
+#pragma unroll 1
+    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1) {
+      uint32_t c = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < PER_LANE; ++i) c += static_cast<uint32_t>(__popcll(__ballot(keys[i] >= (e | bit))));
+      if (c >= k) e |= bit;  // uniform
+    }
+    __syncthreads();
+    if (tid == 0u) s_n[1] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < CAP / 256u; ++i)
+      if (mine[i] && static_cast<uint32_t>(mine[i] >> 32) >= e) list(1u, mine[i]);
+    __syncthreads();
+    n = uniform(s_n[1]);
+  }
   auto write = [&](uint32_t at, uint64_t key) __attribute__((always_inline)) {
     p.top_ids[static_cast<size_t>(t) * k + at] = key ? static_cast<int32_t>(key_index(key)) : -1;
     p.top_lp[static_cast<size_t>(t) * k + at] = key ? (key_value(key) - r.m) - ls : NEG_INF;

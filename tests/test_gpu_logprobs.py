@@ -9,7 +9,9 @@ So log s is off by (ADDS + 2 + 3 W) u and its own rounding, w / s by (2 ADDS + 4
 3 u Q, and log p = (x - m) - log s by what its terms have and round. From hidden rows a
 logit is off by the fp32 sums of a group, 64 additions of s (16 + q) |x| and
 |b - 16 s| |x|, and of the groups: (64 + in / 64 + 8) u of the sum of those; beyond 32 rows
-an x below 2^-24 of its row's largest is held to within 2^-35 of that; log p by
+an x below 2^-24 of its row's largest is held to within 2^-35 of that, a weight whose
+scale is below 2^-8 of its vocabulary row's largest to within 2^-15 of that (the sums run over
+all columns there, and are held to the same bar); log p by
 twice the worst of them, an entropy by that times sum p |log p + H|."""
 import ctypes as C
 
@@ -163,6 +165,18 @@ def test_logits_equal_in_masses(exe, bf16):
     _logits_case(exe, x, np.array([V - 1, 7, 299999]), 1, bf16, pad=0)
 
 
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("T,V,k,kinds", [(40, 984, 15, 0), (6, 2000, 20, 0), (3, 5000, 64, 0), (3, 16000, 64, 0), (2, 16200, 63, 0), (5, 700, 64, 9),
+                                         (3, 5000, 30, 3), (2, 129, 64, 0)])
+def test_logits_more_alternatives_than_tiles(exe, T, V, k, kinds, bf16):
+    """All tiles are looked through; `kinds` different values, or all different."""
+    rng = np.random.default_rng(V + k)
+    x = rng.integers(0, kinds, (T, V)).astype(np.float32) if kinds else (rng.standard_normal((T, V)) * 3).astype(np.float32)
+    if bf16:
+        x = synth.bf16_bits_to_f32(synth.f32_to_bf16_bits(x))
+    _logits_case(exe, x, rng.integers(0, V, T), k, bf16)
+
+
 def test_logits_every_row_its_own_offset(exe):
     """Rows of a long prompt whose tensor passes 4 GiB."""
     T, V, ld = 2100, 151936, 520000
@@ -265,6 +279,37 @@ def test_lm_columns_of_all_sizes(exe, T):
     logits, off = _logits64(_f64(xb), w, s, b)
     lp, ent, ids, tlp, bs, be = _reference(logits, tokens, 1)
     assert np.all(np.abs(got[0] - lp) <= bs + 4 * U * np.abs(lp) + 2 * off.max(1))
+    t = np.arange(T)
+    assert np.all(logits[t, got[2][:, 0]] >= logits[t, ids[:, 0]] - 2 * off.max(1))
+
+
+@pytest.mark.parametrize("T", [5, 40, 100])
+def test_lm_scales_of_all_sizes(exe, T):
+    """Groups' scales from 2^-20 to 2^20 of each other in a vocabulary row, zeros, rows of zeros alone, biases far above them."""
+    rng = np.random.default_rng(16)
+    H, V = 1024, 530
+    w, s, b = _matrix(rng, V, H)
+    s64, b64 = _f64(s), _f64(b)
+    f = np.exp2(rng.integers(-10, 11, s.shape) * (np.arange(V) % 2)[:, None])
+    s64, b64 = s64 * f, b64 * f
+    s64[7::50, ::3] = 0
+    s64[9::50] = 0
+    b64[9::50] = np.exp2(rng.integers(-30, 3, b64[9::50].shape))
+    b64[11::50] *= 2.0 ** 6
+    s64[13::50] *= 2.0 ** -60
+    s, b = (synth.f32_to_bf16_bits(y.astype(np.float32)) for y in (s64, b64))
+    x = synth.bf16_normal(rng, (T, H), 0.02)
+    x[T - 1, H // 2:] = 0
+    args = [exe.upload(a) for a in (x, w, s, b)]
+    tokens = rng.integers(0, V, T)
+    got = _run(exe, T, 2, tokens, lambda **kw: exe.lm_logprobs(*args, T, H, V, **kw), exe.lm_logprobs_workspace(T, H, V, 2))
+    logits, off = _logits64(_f64(x), w, s, b)
+    if T > 32:
+        most = _f64(s).max(1, keepdims=True)
+        rough = np.repeat(np.where(_f64(s) < most * 2.0 ** -8, most * 2.0 ** -15, 0), 64, 1)
+        off += np.abs(_f64(x)) @ rough.T
+    lp, ent, ids, tlp, bs, be = _reference(logits, tokens, 2)
+    assert _near(got[0], lp, bs + 4 * U * np.abs(lp) + 2 * off.max(1))
     t = np.arange(T)
     assert np.all(logits[t, got[2][:, 0]] >= logits[t, ids[:, 0]] - 2 * off.max(1))
 
