@@ -21,11 +21,11 @@ using obs::Weight;
 // its own. Row r of score tile tt is entry 8 (r / 4) + 4 tt + r % 4 of the block:
 // the lane's eight scores are then entries 8 g .. 8 g + 7, the eight values that
 // one 16-byte load of a transposed value row brings.
-// KEEP: values stay in the caches. From 64 entries on a row of a page holds several
+// KEEPS: values stay in the caches. From 64 entries on a row of a page holds several
 // blocks' values in one line; below, they are streamed like the keys (32 sequences
 // of up to 9,000, pages of 64: 69.5 us against 72.9 streamed, of 128 in e4m3 47.7
 // and 54.4; of 32 48.2 and 43.7).
-template <uint32_t HD, bool F8, bool KEEP>
+template <uint32_t HD, bool F8, bool KEEPS>
 struct Block {
   static constexpr uint32_t KS = HD / 32u, NT = HD / 16u, KL = F8 ? KS / 2u : KS;
   u32x4_v k[2][KL];  // e4m3: 16 dims a load, two steps
@@ -48,7 +48,7 @@ struct Block {
 #pragma unroll
     for (uint32_t nt = 0; nt < NT; ++nt) {
       const V* vr = reinterpret_cast<const V*>(vb + ((16u * nt + col) * SZ << a.lp));
-      if constexpr (KEEP)
+      if constexpr (KEEPS)
         v[nt] = *vr;
       else
         v[nt] = __builtin_nontemporal_load(vr);
@@ -93,8 +93,8 @@ struct Column {
 // token sees (values it does not see read as zero: the pool may hold anything
 // there); ok: whether the lane's page is there; masked: whether the block needs
 // any of it.
-template <uint32_t HD, bool F8, bool KEEP>
-__device__ __forceinline__ void block_step(const Block<HD, F8, KEEP>& blk, const bf16x8_v (&qb)[HD / 32u], Column<HD>& c,
+template <uint32_t HD, bool F8, bool KEEPS>
+__device__ __forceinline__ void block_step(const Block<HD, F8, KEEPS>& blk, const bf16x8_v (&qb)[HD / 32u], Column<HD>& c,
                                            uint32_t t, uint32_t hi, uint32_t lo, uint32_t sinks, bool ok, bool masked,
                                            float scale_log2, float (&sv)[8], uint32_t lane) {
   constexpr uint32_t KS = HD / 32u, NT = HD / 16u;
@@ -153,41 +153,55 @@ __device__ __forceinline__ void block_step(const Block<HD, F8, KEEP>& blk, const
 // bias, so it weighs values of the size that the entries have, as P's does in bf16.
 // Bytes hold dims d (low) and d + HD / 2 (high): a lane's 16 bytes of a key (8 of a
 // head of 64) are two fragments of each half, its 8 bytes of a value row the eight
-// entries of two dims. Its scales and biases are those of its own eight scores.
-template <uint32_t HD, bool KEEP>
+// entries of two dims. Its scales and biases are those of its own scores.
+// MODE, of this form alone but for KEEP. WIDE: pages of 32 entries and more, a block is in
+// one: its addresses are one place a wave and a lane's own offset. HALF: eight query heads
+// at most, eight columns of the products: of the second score tile columns 8 to 15 take
+// what 0 to 7 have, so that a lane has four scores of column col % 8 and not eight, or none.
+constexpr uint32_t KEEP = 1, WIDE = 2, HALF = 4;
+template <uint32_t HD, uint32_t MODE>
 struct Block4 {
-  static constexpr uint32_t NG = HD / 64u, NT = HD / 16u;
+  static constexpr uint32_t NG = HD / 64u, NT = HD / 16u, PER = MODE & HALF ? 4u : 8u;  // scores a lane
   typedef typename std::conditional<HD == 128u, u32x4_v, u32x2_v>::type K;
   K k[2];
   u32x2_v v[NT / 2u];
-  u32x4_v kp[NG][2], vp[NG][2];  // scale and bias of entries 8 g .. 8 g + 7
+  u32x4_v kp[NG][PER / 4u], vp[NG][PER / 4u];  // scale and bias of the entries of its scores
 
-  // kid, eid: page ids of the lane's key rows and of its entries
-  __device__ __forceinline__ void load(const Paged& a, uint32_t kv, uint32_t kid, uint32_t eid, uint32_t t0, uint32_t col,
-                                       uint32_t g) {
-    const uint32_t mask = (1u << a.lp) - 1u, e = (t0 + 8u * g) & mask;
-    const uint8_t* kb = a.k + page_at<HD, KT_Q4>(a, kid, kv);
+  // at0, at1: bytes of the pages (of the kv head) of both halves; first: the block's first entry in its page (WIDE)
+  __device__ __forceinline__ void load(const Paged& a, size_t at0, size_t at1, uint32_t first, uint32_t col, uint32_t g) {
+    const uint32_t row = 8u * (col / 4u) + col % 4u, e = 8u * g, own = MODE & HALF ? col / 8u * 4u : 0u;
+    const uint8_t *kb = a.k, *kw = a.k, *vb = a.v;
+    uint32_t kr = row, ke = e;  // the lane's own
+    if constexpr (MODE & WIDE) {
+      kb += at0 + first * (HD / 2u);
+      kw += at0 + (HD / 2u << a.lp) + 4u * first;
+      vb += at0;
+    } else {
+      const size_t at = g & 2u ? at1 : at0;
+      kb += col & 8u ? at1 : at0;
+      kw += at + (HD / 2u << a.lp);
+      vb += at;
+      kr &= 15u, ke &= 15u;
+    }
+    const uint8_t* vw = vb + (HD / 2u << a.lp) + (MODE & WIDE ? 4u * first : 0u);
+    if constexpr (MODE & WIDE) vb += first;
+    const uint32_t ko = kr * (HD / 2u) + sizeof(K) * g, vo = (col << a.lp) + ke, wo = 4u * (ke + own);
 #pragma unroll
-    for (uint32_t tt = 0; tt < 2; ++tt)
-      k[tt] = __builtin_nontemporal_load(reinterpret_cast<const K*>(
-          kb + ((t0 + 8u * (col / 4u) + 4u * tt + col % 4u) & mask) * (HD / 2u) + sizeof(K) * g));
-    const uint8_t* vb = a.v + page_at<HD, KT_Q4>(a, eid, kv);
+    for (uint32_t tt = 0; tt < 2; ++tt) k[tt] = __builtin_nontemporal_load(reinterpret_cast<const K*>(kb + 4u * tt * (HD / 2u) + ko));
 #pragma unroll
     for (uint32_t nt = 0; nt < NT / 2u; ++nt) {
-      const u32x2_v* vr = reinterpret_cast<const u32x2_v*>(vb + ((16u * nt + col) << a.lp) + e);
-      if constexpr (KEEP)
+      const u32x2_v* vr = reinterpret_cast<const u32x2_v*>(vb + (16u * nt << a.lp) + vo);
+      if constexpr (MODE & KEEP)
         v[nt] = *vr;
       else
         v[nt] = __builtin_nontemporal_load(vr);
     }
-    const uint8_t* kw = a.k + page_at<HD, KT_Q4>(a, eid, kv) + (HD / 2u << a.lp) + 4u * e;
-    const uint8_t* vw = vb + (HD / 2u << a.lp) + 4u * e;
 #pragma unroll
     for (uint32_t q = 0; q < NG; ++q)
 #pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        kp[q][i] = *reinterpret_cast<const u32x4_v*>(kw + (4u * q << a.lp) + 16u * i);
-        vp[q][i] = *reinterpret_cast<const u32x4_v*>(vw + (4u * q << a.lp) + 16u * i);
+      for (uint32_t i = 0; i < PER / 4u; ++i) {
+        kp[q][i] = *reinterpret_cast<const u32x4_v*>(kw + (4u * q << a.lp) + 16u * i + wo);
+        vp[q][i] = *reinterpret_cast<const u32x4_v*>(vw + (4u * q << a.lp) + 16u * i + wo);
       }
   }
   // dims of query fragment ks (in q4_order): of the low nibbles, then of the high ones
@@ -202,46 +216,60 @@ struct Sums4 {
   float w[HD / 64u], b[HD / 64u];
 };
 
-template <uint32_t HD, bool KEEP>
-__device__ __forceinline__ void block_step4(const Block4<HD, KEEP>& blk, const bf16x8_v (&qb)[HD / 32u],
+constexpr int ROW_ROR8 = 0x128;  // lane i <- lane i ^ 8 of its 16
+// own, but in lanes 8 to 15 of 16 what other has in lanes 0 to 7
+__device__ __forceinline__ float upper_from(float own, float other) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(own), __float_as_int(other), ROW_ROR8, 0xf, 0xc, false));
+}
+template <uint32_t MODE>
+__device__ __forceinline__ float column_sum(float v, uint32_t lane) {
+  if constexpr (MODE & HALF) v += dpp_f32<ROW_ROR8>(v);
+  v += lane_xor16_f32(v, lane);
+  return v + lane_xor32_f32(v, lane);
+}
+
+// t: the lane's first entry
+template <uint32_t HD, uint32_t MODE>
+__device__ __forceinline__ void block_step4(const Block4<HD, MODE>& blk, const bf16x8_v (&qb)[HD / 32u],
                                             const float (&qs)[HD / 64u], Column<HD>& c, Sums4<HD>& u, uint32_t t, uint32_t hi,
                                             uint32_t lo, uint32_t sinks, bool ok, bool masked, float scale_log2,
-                                            float (&sv)[8], uint32_t lane) {
-  constexpr uint32_t NG = HD / 64u, NT = HD / 16u;
+                                            float (&sv)[Block4<HD, MODE>::PER], uint32_t lane) {
+  constexpr uint32_t NG = HD / 64u, NT = HD / 16u, PER = Block4<HD, MODE>::PER;
   const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4_v acc[2][NG];
 #pragma unroll
   for (uint32_t tt = 0; tt < 2; ++tt) {
-    f32x4_v acc[NG];
     if constexpr (HD == 128u) {
-      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].x, blk.k[tt].y), qb[0], zero, 0, 0, 0);
-      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].z, blk.k[tt].w), qb[1], acc[0], 0, 0, 0);
-      acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].x, blk.k[tt].y), qb[2], zero, 0, 0, 0);
-      acc[1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].z, blk.k[tt].w), qb[3], acc[1], 0, 0, 0);
+      acc[tt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].x, blk.k[tt].y), qb[0], zero, 0, 0, 0);
+      acc[tt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].z, blk.k[tt].w), qb[1], acc[tt][0], 0, 0, 0);
+      acc[tt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].x, blk.k[tt].y), qb[2], zero, 0, 0, 0);
+      acc[tt][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].z, blk.k[tt].w), qb[3], acc[tt][1], 0, 0, 0);
     } else {
-      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].x, blk.k[tt].y), qb[0], zero, 0, 0, 0);
-      acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].x, blk.k[tt].y), qb[1], acc[0], 0, 0, 0);
+      acc[tt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<false>(blk.k[tt].x, blk.k[tt].y), qb[0], zero, 0, 0, 0);
+      acc[tt][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(q4_bf16x8<true>(blk.k[tt].x, blk.k[tt].y), qb[1], acc[tt][0], 0, 0, 0);
     }
+  }
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      float s = 0.0f;
+  for (uint32_t j = 0; j < PER; ++j) {
+    float s = 0.0f;
 #pragma unroll
-      for (uint32_t q = 0; q < NG; ++q) {
-        const uint32_t par = blk.kp[q][tt][i];
-        const float sc = bf16lo(par);
-        s = __builtin_fmaf(sc, acc[q][i], __builtin_fmaf(__builtin_fmaf(sc, -16.0f, bf16hi(par)), qs[q], s));
-      }
-      sv[4 * tt + i] = s * scale_log2;
+    for (uint32_t q = 0; q < NG; ++q) {
+      const uint32_t par = blk.kp[q][j / 4u][j % 4u];
+      const float sc = bf16lo(par), x = PER == 4u ? upper_from(acc[0][q][j % 4u], acc[1][q][j % 4u]) : acc[j / 4u][q][j % 4u];
+      s = __builtin_fmaf(sc, x, __builtin_fmaf(__builtin_fmaf(sc, -16.0f, bf16hi(par)), qs[q], s));
     }
+    sv[j] = s * scale_log2;
   }
   uint32_t bits = 0xffu;
   if (masked) {  // uniform
     bits = ok ? seen_bits(t, hi, lo, sinks) : 0u;
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) sv[j] = bits >> j & 1u ? sv[j] : NEG_INF;
+    for (uint32_t j = 0; j < PER; ++j) sv[j] = bits >> j & 1u ? sv[j] : NEG_INF;
   }
   float bm = sv[0];
 #pragma unroll
-  for (uint32_t j = 1; j < 8; ++j) bm = fmaxf(bm, sv[j]);
+  for (uint32_t j = 1; j < PER; ++j) bm = fmaxf(bm, sv[j]);
+  if constexpr (PER == 4u) bm = fmaxf(bm, dpp_f32<ROW_ROR8>(bm));
   bm = fmaxf(bm, lane_xor16_f32(bm, lane));
   bm = fmaxf(bm, lane_xor32_f32(bm, lane));
   const float m_new = fmaxf(c.m, bm), m_use = m_new == NEG_INF ? 0.0f : m_new;
@@ -259,9 +287,9 @@ __device__ __forceinline__ void block_step4(const Block4<HD, KEEP>& blk, const b
       for (uint32_t i = 0; i < 4; ++i) c.o[nt][i] *= corr;
     c.m = m_new;
   }
-  float p[8];
+  float p[PER];
 #pragma unroll
-  for (uint32_t j = 0; j < 8; ++j) {
+  for (uint32_t j = 0; j < PER; ++j) {
     p[j] = __builtin_amdgcn_exp2f(sv[j] - m_use);
     c.l += p[j];
   }
@@ -270,20 +298,32 @@ __device__ __forceinline__ void block_step4(const Block4<HD, KEEP>& blk, const b
   bf16x8_v pb[NG];
 #pragma unroll
   for (uint32_t q = 0; q < NG; ++q) {
-    float w[8];
+    uint32_t par[PER];
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      // what lies in hidden entries may be anything: its scale and bias read as zero
-      uint32_t par = blk.vp[q][j / 4u][j % 4u];
-      if (masked) par = bits >> j & 1u ? par : 0u;  // uniform
-      w[j] = p[j] * bf16lo(par);
-      u.b[q] = __builtin_fmaf(p[j], __builtin_fmaf(bf16lo(par), 8.0f, bf16hi(par)), u.b[q]);
+    for (uint32_t j = 0; j < PER; ++j) par[j] = blk.vp[q][j / 4u][j % 4u];
+    if (masked) {  // uniform: what lies in hidden entries may be anything, its scale and bias read as zero
+#pragma unroll
+      for (uint32_t j = 0; j < PER; ++j) par[j] = bits >> j & 1u ? par[j] : 0u;
     }
-    const u32x4_v pk = {pack_bf16_pair_rne(w[0], w[2]), pack_bf16_pair_rne(w[1], w[3]), pack_bf16_pair_rne(w[4], w[6]),
-                        pack_bf16_pair_rne(w[5], w[7])};
+    u32x4_v pk;
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-      u.w[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, static_cast<uint32_t>(pk[i])), ones, u.w[q], false);
+    for (uint32_t i = 0; i < PER; i += 4u) {
+      float w[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        w[j] = p[i + j] * bf16lo(par[i + j]);
+        u.b[q] = __builtin_fmaf(p[i + j], __builtin_fmaf(bf16lo(par[i + j]), 8.0f, bf16hi(par[i + j])), u.b[q]);
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        pk[i / 2u + j] = pack_bf16_pair_rne(w[j], w[j + 2]);
+        u.w[q] = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_v, static_cast<uint32_t>(pk[i / 2u + j])), ones, u.w[q], false);
+      }
+    }
+    if constexpr (PER == 4u) {
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) pk[2u + j] = static_cast<uint32_t>(dpp_i32<ROW_ROR8>(static_cast<int>(pk[j])));
+    }
     pb[q] = __builtin_bit_cast(bf16x8_v, pk);
   }
 #pragma unroll
@@ -373,13 +413,14 @@ __device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, u
 // the columns. Its four waves take the part's blocks in turn and meet in LDS.
 // A part that is all of its sequence writes the output, others their maximum,
 // sum and output for paged_join_kernel.
-template <uint32_t HD, uint32_t KT, bool WEIGHT, bool KEEP>
-__global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn p) {
+template <uint32_t HD, uint32_t KT, bool WEIGHT, uint32_t MODE>
+__global__ void __launch_bounds__(256, MODE& HALF ? 4 : 3) paged_decode_kernel(Paged a, PagedAttn p) {
   constexpr uint32_t NT = HD / 16u, NG = HD / 64u;
   constexpr bool F8 = KT == KT_E4M3, Q4 = KT == KT_Q4;
-  typedef typename std::conditional<Q4, Block4<HD, KEEP>, Block<HD, F8, KEEP>>::type Blk;
-  __shared__ float s_ml[4][16][2];
-  __shared__ float s_o[4][16][HD + 4u];
+  typedef typename std::conditional<Q4, Block4<HD, MODE>, Block<HD, F8, bool(MODE & KEEP)>>::type Blk;
+  constexpr uint32_t COLS = MODE & HALF ? 8u : 16u;
+  __shared__ float s_ml[4][COLS][2];
+  __shared__ float s_o[4][COLS][HD + 4u];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, col = lane & 15u, g = lane >> 4;
   const Found f = plan_find(a, p, blockIdx.x, lane);
   const uint32_t b = f.b, splits = f.splits, at = blockIdx.x - f.first;
@@ -413,10 +454,7 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
         qs[ks / 2u] += bf16lo(w) + bf16hi(w);
       }
 #pragma unroll
-    for (uint32_t q = 0; q < NG; ++q) {
-      qs[q] += lane_xor16_f32(qs[q], lane);
-      qs[q] += lane_xor32_f32(qs[q], lane);
-    }
+    for (uint32_t q = 0; q < NG; ++q) qs[q] = column_sum<MODE>(qs[q], lane);  // (columns 8 to 15 of HALF are zero)
   }
   // page ids of the wave's next 64 blocks (both halves of each), a block a lane
   uint32_t id0 = 0, id1 = 0;
@@ -438,45 +476,57 @@ __global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn
       p1 = ok1 ? p1 : 0u;
     }
     Blk blk;
-    blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
-    __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
-    float sv[8];
-    if constexpr (Q4)
-      block_step4<HD, KEEP>(blk, qb, qs, c, u, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, !(whole && ok0 && ok1),
-                            scale, sv, lane);
-    else
-      block_step<HD, F8, KEEP>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0,
-                         !(whole && ok0 && ok1), scale, sv, lane);
-    if constexpr (WEIGHT) {
-      if (col < p.G) {
-        float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + col) * p.vis + 32u * x + 8u * g);
-        to[0] = make_float4(sv[0], sv[1], sv[2], sv[3]);
-        to[1] = make_float4(sv[4], sv[5], sv[6], sv[7]);
+    const bool masked = !(whole && ok0 && ok1);
+    if constexpr (Q4) {
+      constexpr uint32_t PER = Blk::PER;
+      const uint32_t own = 8u * g + (PER == 4u ? col / 8u * 4u : 0u);
+      blk.load(a, page_at<HD, KT_Q4>(a, p0, kv), page_at<HD, KT_Q4>(a, p1, kv), t0 & ((1u << a.lp) - 1u), col, g);
+      __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
+      float sv[PER];
+      block_step4<HD, MODE>(blk, qb, qs, c, u, t0 + own, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, masked, scale, sv, lane);
+      if constexpr (WEIGHT) {
+        const uint32_t h = MODE & HALF ? col % 8u : col;
+        if (h < p.G) {
+          float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + h) * p.vis + 32u * x + own);
+#pragma unroll
+          for (uint32_t i = 0; i < PER / 4u; ++i) to[i] = make_float4(sv[4 * i], sv[4 * i + 1], sv[4 * i + 2], sv[4 * i + 3]);
+        }
+      }
+    } else {
+      blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
+      __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
+      float sv[8];
+      block_step<HD, F8, bool(MODE & KEEP)>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, masked, scale, sv, lane);
+      if constexpr (WEIGHT) {
+        if (col < p.G) {
+          float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + col) * p.vis + 32u * x + 8u * g);
+          to[0] = make_float4(sv[0], sv[1], sv[2], sv[3]);
+          to[1] = make_float4(sv[4], sv[5], sv[6], sv[7]);
+        }
       }
     }
   }
-  c.l += lane_xor16_f32(c.l, lane);
-  c.l += lane_xor32_f32(c.l, lane);
+  c.l = column_sum<MODE>(c.l, lane);
   if constexpr (Q4) {
 #pragma unroll
     for (uint32_t q = 0; q < NG; ++q) {
-      float add = __builtin_fmaf(u.w[q], -24.0f, u.b[q]);
-      add += lane_xor16_f32(add, lane);
-      add += lane_xor32_f32(add, lane);
+      const float add = column_sum<MODE>(__builtin_fmaf(u.w[q], -24.0f, u.b[q]), lane);
 #pragma unroll
       for (uint32_t nt = 0; nt < NT / NG; ++nt)
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) c.o[NT / NG * q + nt][i] += add;
     }
   }
-  if (lane < 16u) {
+  if (lane < COLS) {
     s_ml[wave][col][0] = c.m;
     s_ml[wave][col][1] = c.l;
   }
+  if (col < COLS) {
 #pragma unroll
-  for (uint32_t nt = 0; nt < NT; ++nt)
+    for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) s_o[wave][col][16u * nt + 4u * g + i] = c.o[nt][i];
+      for (uint32_t i = 0; i < 4; ++i) s_o[wave][col][16u * nt + 4u * g + i] = c.o[nt][i];
+  }
   __syncthreads();
   for (uint32_t i = tid; i < p.G * HD; i += 256u) {
     const uint32_t h = i / HD, d = i % HD;
@@ -689,10 +739,22 @@ DecodePlan decode_plan(const obs_paged_kv* kv, const obs_paged_seqs* s, bool wei
 template <uint32_t HD, uint32_t KT, bool WEIGHT>
 int launch_decode(obs_ctx* ctx, const Paged& a, const PagedAttn& p, const Weight& w, const DecodePlan& d) {
   const uint32_t items = static_cast<uint32_t>(d.items);
-  if (a.lp >= 6u)
-    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, KT, WEIGHT, true><<<items, 256, 0, ctx->stream>>>(a, p));
-  else
-    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, KT, WEIGHT, false><<<items, 256, 0, ctx->stream>>>(a, p));
+  auto go = [&](auto mode) {
+    OBS_LAUNCH(ctx, "paged_decode", paged_decode_kernel<HD, KT, WEIGHT, decltype(mode)::value><<<items, 256, 0, ctx->stream>>>(a, p));
+    return int(OBS_OK);
+  };
+  int rc;
+  if constexpr (KT == KT_Q4) {
+    auto pages = [&](auto half) {
+      constexpr uint32_t H = decltype(half)::value;
+      return a.lp >= 6u ? go(std::integral_constant<uint32_t, H | WIDE | KEEP>{})
+             : a.lp == 5u ? go(std::integral_constant<uint32_t, H | WIDE>{}) : go(std::integral_constant<uint32_t, H>{});
+    };
+    rc = p.G <= 8u ? pages(std::integral_constant<uint32_t, HALF>{}) : pages(std::integral_constant<uint32_t, 0u>{});
+  } else {
+    rc = a.lp >= 6u ? go(std::integral_constant<uint32_t, KEEP>{}) : go(std::integral_constant<uint32_t, 0u>{});
+  }
+  if (rc != OBS_OK) return rc;
   if (!WEIGHT && d.blocks <= d.min_chunk) return OBS_OK;  // every sequence is one part
   const uint32_t wchunks = WEIGHT ? static_cast<uint32_t>((d.vis + 1023u) / 1024u) : 0u, rows = a.n_seqs * p.nh;
   const uint32_t weights = rows / p.G * wchunks;
