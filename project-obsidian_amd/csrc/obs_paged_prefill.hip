@@ -187,9 +187,9 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   constexpr uint32_t KS = HD / 16u, DT = HD / 32u, SZ = KT == KT_BF16 ? 2u : 1u;
   constexpr uint32_t KROW = HD + 8u, VROW = 40u;  // padded rows (bf16): no bank is hit twice by eight lanes
   constexpr uint32_t KC = HD * SZ / 16u, VC = 2u * SZ;  // 16-byte chunks of a key row, of a block's value row
-  // In 4 bits chunks are 8 bytes, eight dims of either half of a key row, or eight
-  // entries of two value rows; a chunk of keys needs the scale and bias of one entry
-  // (two groups), one of values those of its eight entries.
+  // In 4 bits chunks are 8 bytes, eight dims of either half of a key row, or four
+  // entries of four value rows (two of bytes); a chunk of keys needs the scale and bias
+  // of one entry (two groups), one of values those of its four entries.
   constexpr uint32_t NG = HD / 64u, KC4 = HD / 16u, VC4 = 4u;
   constexpr uint32_t KN = Q4 ? 32u * KC4 : 32u * KC, VN = Q4 ? HD / 2u * VC4 : HD * VC;  // chunks of a block: 128 to 512, at most one a thread
   // Keys and values of two blocks; before and after them a slab a wave, through
@@ -324,13 +324,13 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     k.edge = !(k.ok0 && k.ok1 && k.t + 32u <= hi_first && (k.t >= lo_last || k.t + 32u <= p.sinks));
     return k;
   };
-  const uint32_t v_dim = Q4 ? vc % (VN / 2u) / 2u : vc % (VN / 2u) / (VC / 2u);
-  const uint32_t v_ent = 16u * vh + (Q4 ? 8u * (vc % 2u) : (16u / SZ) * (vc % (VC / 2u)));
+  const uint32_t v_dim = Q4 ? vc % (VN / 2u) / 4u * 2u : vc % (VN / 2u) / (VC / 2u);
+  const uint32_t v_ent = 16u * vh + (Q4 ? 4u * (vc % 4u) : (16u / SZ) * (vc % (VC / 2u)));
   const uint32_t koff = Q4 ? ((kc / KC4) & pmask) * (HD / 2u) + 8u * (kc % KC4) : ((kc / KC) & pmask) * (HD * SZ) + 16u * (kc % KC);
   const uint32_t voff = ((v_dim << a.lp) + (v_ent & pmask)) * SZ;
   u32x4_v kr, vr;
   u32x2_v xr;              // in 4 bits: a chunk of keys or of values (a wave brings one of them)
-  u32x4_v xp[NG][2];       // and its scales and biases (of keys: the first word)
+  u32x4_v xp[NG];          // and its scales and biases (of keys: the first word)
   auto load_k = [&](const Blk& k) __attribute__((always_inline)) {
     if constexpr (Q4) {
       if (has_k) {
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
         xr = *reinterpret_cast<const u32x2_v*>(base + (k.t & pmask) * (HD / 2u) + koff);
 #pragma unroll
         for (uint32_t q = 0; q < NG; ++q)
-          xp[q][0].x = *reinterpret_cast<const uint32_t*>(base + (HD / 2u << a.lp) + (4u * q << a.lp) +
+          xp[q].x = *reinterpret_cast<const uint32_t*>(base + (HD / 2u << a.lp) + (4u * q << a.lp) +
                                                           4u * ((k.t & pmask) + ((kc / KC4) & pmask)));
       }
       return;
@@ -350,13 +350,12 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
     if constexpr (Q4) {
       if (has_v) {
         const uint8_t* base = a.v + (static_cast<size_t>(k.iv) << a.lp) * entry_bytes<HD, KT>();
-        xr = *reinterpret_cast<const u32x2_v*>(base + (k.t & pmask) + voff);
+        const uint8_t* at = base + (k.t & pmask) + voff;
+        xr = u32x2_v{*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + (size_t(1) << a.lp))};
 #pragma unroll
         for (uint32_t q = 0; q < NG; ++q)
-#pragma unroll
-          for (uint32_t i = 0; i < 2; ++i)
-            xp[q][i] = *reinterpret_cast<const u32x4_v*>(base + (HD / 2u << a.lp) + (4u * q << a.lp) +
-                                                         4u * ((k.t & pmask) + (v_ent & pmask)) + 16u * i);
+          xp[q] = *reinterpret_cast<const u32x4_v*>(base + (HD / 2u << a.lp) + (4u * q << a.lp) +
+                                                    4u * ((k.t & pmask) + (v_ent & pmask)));
       }
       return;
     }
@@ -375,31 +374,33 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
       return w;
     }
   };
-  // Eight nibbles (low or high ones) as fp16: q s + b in fp32, rounded once (2^-11 of
+  // Four nibbles (low or high ones) as fp16: q s + b in fp32, rounded once (2^-11 of
   // it at most; in bf16 the keys' roundings were most of an output's error, 0.0043 of
   // it where fp16 leaves the output's own 0.0017). A block is widened once for all of
   // its 384 columns.
-  auto widen4 = [&](bool high, auto par) __attribute__((always_inline)) {
-    const uint32_t w0 = high ? xr.x >> 4 : xr.x, w1 = high ? xr.y >> 4 : xr.y;
-    float f[8];
-    f[0] = q4_value(q4_nibble<0, false>(w0), par(0));
-    f[1] = q4_value(q4_nibble<1, false>(w0), par(1));
-    f[2] = q4_value(q4_nibble<2, false>(w0), par(2));
-    f[3] = q4_value(q4_nibble<3, false>(w0), par(3));
-    f[4] = q4_value(q4_nibble<0, false>(w1), par(4));
-    f[5] = q4_value(q4_nibble<1, false>(w1), par(5));
-    f[6] = q4_value(q4_nibble<2, false>(w1), par(6));
-    f[7] = q4_value(q4_nibble<3, false>(w1), par(7));
-    return u32x4_v{O::pack(f[0], f[1]), O::pack(f[2], f[3]), O::pack(f[4], f[5]), O::pack(f[6], f[7])};
+  // A nibble masked in place is the fp16 number q 2^-24 (2^-20 four bits up): a fused
+  // multiply-add of it with fp32 factors, rounded to fp16, is one instruction (a prompt of
+  // 5,001 262 us; by conversions, and with eight entries of one byte row a thread, 273).
+  auto widen4 = [](uint32_t w, bool high, auto par) __attribute__((always_inline)) {
+    const uint32_t mask = high ? 0x00f000f0u : 0x000f000fu;
+    const float one = high ? 0x1p20f : 0x1p24f;
+    const f16x2_t even = as_f16x2(w & mask), odd = as_f16x2(w >> 8 & mask);
+    auto value = [&](_Float16 q, uint32_t e) __attribute__((always_inline)) {
+      return static_cast<_Float16>(__builtin_fmaf(static_cast<float>(q), bf16lo(par(e)) * one, bf16hi(par(e))));
+    };
+    return u32x2_v{__builtin_bit_cast(uint32_t, (f16x2_t{value(even[0], 0u), value(odd[0], 1u)})),
+                   __builtin_bit_cast(uint32_t, (f16x2_t{value(even[1], 2u), value(odd[1], 3u)}))};
   };
   auto store_k = [&](uint32_t buf) __attribute__((always_inline)) {
     if constexpr (Q4) {
       if (has_k) {
         uint16_t* to = &s_k[buf][(kc / KC4) * KROW + 8u * (kc % KC4)];
 #pragma unroll
-        for (uint32_t j = 0; j < 2; ++j)
-          *reinterpret_cast<u32x4_v*>(to + HD / 2u * j) =
-              widen4(j == 1u, [&](uint32_t) __attribute__((always_inline)) { return xp[j * (NG - 1u)][0].x; });
+        for (uint32_t j = 0; j < 2; ++j) {
+          auto par = [&](uint32_t) __attribute__((always_inline)) { return xp[j * (NG - 1u)].x; };
+          const u32x2_v w0 = widen4(xr.x, j == 1u, par), w1 = widen4(xr.y, j == 1u, par);
+          *reinterpret_cast<u32x4_v*>(to + HD / 2u * j) = u32x4_v{w0.x, w0.y, w1.x, w1.y};
+        }
       }
       return;
     }
@@ -414,20 +415,24 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
   // them get them at the end, and no other row meets them.
   auto store_v = [&](uint32_t buf, const Blk& k) __attribute__((always_inline)) {
     if (has_v) {
-      u32x4_v w[2u / SZ];
+      u32x4_v w[2u / SZ];  // in 4 bits: four entries of both rows, of the low or the high nibbles
 #pragma unroll
       for (uint32_t j = 0; j < 2u / SZ; ++j) {
-        if constexpr (Q4)
-          w[j] = widen4(j == 1u, [&](uint32_t e) __attribute__((always_inline)) { return xp[j * (NG - 1u)][e / 4u][e % 4u]; });
-        else
+        if constexpr (Q4) {
+          auto par = [&](uint32_t e) __attribute__((always_inline)) { return xp[j * (NG - 1u)][e]; };
+          const u32x2_v r0 = widen4(xr.x, j == 1u, par), r1 = widen4(xr.y, j == 1u, par);
+          w[j] = u32x4_v{r0.x, r0.y, r1.x, r1.y};
+        } else {
           w[j] = widen(vr, j);
+        }
       }
       if (k.edge) {  // uniform
         const uint32_t bits = seen_bits(k.t, s.hi, s.lo, p.sinks) & page_bits(k);
         uint32_t bad = 0u;
 #pragma unroll
         for (uint32_t j = 0; j < 2u / SZ; ++j) {
-          w[j] &= word_masks(bits >> (v_ent + (Q4 ? 0u : 8u * j)));
+          const uint32_t own = bits >> (v_ent + (Q4 ? 0u : 8u * j));
+          w[j] &= word_masks(Q4 ? (own & 0xfu) * 0x11u : own);
 #pragma unroll
           for (uint32_t q = 0; q < 4; ++q) {
             // all ones in the exponent: adding one in its last place carries into the sign's
@@ -440,8 +445,15 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
         if (bad) s_bad = 1u;
       }
 #pragma unroll
-      for (uint32_t j = 0; j < 2u / SZ; ++j)  // in 4 bits: the other nibbles' row
-        *reinterpret_cast<u32x4_v*>(&s_v[buf][(v_dim + (Q4 ? HD / 2u * j : 0u)) * VROW + v_ent + (Q4 ? 0u : 8u * j)]) = w[j];
+      for (uint32_t j = 0; j < 2u / SZ; ++j) {
+        uint16_t* to = &s_v[buf][(v_dim + (Q4 ? HD / 2u * j : 0u)) * VROW + v_ent + (Q4 ? 0u : 8u * j)];
+        if constexpr (Q4) {
+          *reinterpret_cast<u32x2_v*>(to) = u32x2_v{w[j].x, w[j].y};
+          *reinterpret_cast<u32x2_v*>(to + VROW) = u32x2_v{w[j].z, w[j].w};
+        } else {
+          *reinterpret_cast<u32x4_v*>(to) = w[j];
+        }
+      }
     }
   };
   auto sees = [&](uint32_t e) __attribute__((always_inline)) { return e < hi && (e >= lo || e < p.sinks); };
