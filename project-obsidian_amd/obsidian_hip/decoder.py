@@ -55,6 +55,17 @@ ATTN_KEYS = ("in_norm", "q_w", "q_s", "q_b", "k_w", "k_s", "k_b", "v_w", "v_s", 
 GLOBAL_KEYS = ("embed_w", "embed_s", "embed_b", "final_norm", "lm_w", "lm_s", "lm_b")
 
 
+@dataclass
+class Scores:
+    """What T positions give to the token after each: its log probability (fp32 [T], 0
+    where there is none), the entropy of the position's distribution, and the most
+    likely ids with their log probabilities [T, top_k]."""
+    logprob: np.ndarray
+    entropy: np.ndarray
+    top_ids: np.ndarray
+    top_logprobs: np.ndarray
+
+
 class Model:
     """forward.rs:30-53. `layers` holds per-layer dicts of device pointers (or
     DeviceBuffers) with ATTN_KEYS plus a MoeLayer under "moe"; `glob` holds
@@ -88,6 +99,7 @@ class Model:
         self.moe_cfg = c.moe()
         self.graph: Optional[int] = None
         self._pf: Optional[Dict] = None      # prefill buffers, grown to the largest batch
+        self._sc: Optional[Dict] = None      # score buffers, likewise
         self.use_fused_attention = True      # one-launch attention half where the shape allows
         self.use_fused_layer = True          # ... and both halves of a layer in one launch
         self.last_seq: List[int] = []        # the tokens whose keys and values the caches hold (run_turn)
@@ -201,8 +213,10 @@ class Model:
         self.step()
         return self.read_state()[1]
 
-    def generate(self, tok: int, pos: int, n: int, graph: bool = True) -> List[int]:
-        """n greedy tokens after `tok` at `pos` (one step per token)."""
+    def generate(self, tok: int, pos: int, n: int, graph: bool = True, scores: Optional[list] = None,
+                 top_k: int = 0) -> List[int]:
+        """n greedy tokens after `tok` at `pos` (one step per token). scores: a
+        list that receives last_scores(top_k) of every token."""
         if pos + n > self.cfg.max_len:
             raise ValueError("generation runs past the cache")
         self.set_state(pos, tok)
@@ -213,7 +227,62 @@ class Model:
             else:
                 self.step()
             out.append(self.read_state()[1])
+            if scores is not None:
+                scores.append(self.last_scores(top_k))
         return out
+
+    # -- log probabilities -----------------------------------------------------
+    def _score_buffers(self, T: int, top_k: int, ws: int) -> Dict:
+        if self._sc is None or self._sc["T"] < T or self._sc["top_k"] < top_k or self._sc["ws"].nbytes < ws:
+            had = self._sc or {"T": 0, "top_k": 0}
+            ws = max(ws, had["ws"].nbytes if "ws" in had else 0)
+            T, top_k = max(T, had["T"]), max(top_k, had["top_k"])
+            self._sc = had = None  # release the smaller set first
+            e = self.exe
+            self._sc = {
+                "T": T, "top_k": top_k, "tokens": e.alloc(T, np.int32), "logprob": e.alloc(T, np.float32),
+                "entropy": e.alloc(T, np.float32), "ids": e.alloc(max(T * top_k, 1), np.int32),
+                "top": e.alloc(max(T * top_k, 1), np.float32), "ws": e.alloc(max(ws, 1), np.uint8),
+            }
+        return self._sc
+
+    @staticmethod
+    def _scores(S: Dict, T: int, top_k: int) -> Scores:
+        ids, top = (S[n].download()[:T * top_k].reshape(T, top_k) for n in ("ids", "top"))
+        return Scores(S["logprob"].download()[:T].copy(), S["entropy"].download()[:T].copy(), ids.copy(), top.copy())
+
+    def last_scores(self, top_k: int = 0) -> Scores:
+        """Of the last step (or prefill), whose logits are still there: its greedy
+        token's log probability, the entropy and the top_k alternatives (T = 1)."""
+        e, c = self.exe, self.cfg
+        S = self._score_buffers(1, top_k, e.token_logprobs_workspace(1, c.vocab, top_k))
+        e.token_logprobs(self.logits, 1, c.vocab, S["ws"], tokens=self.state.ptr + 4, logprob=S["logprob"],
+                         entropy=S["entropy"], top_k=top_k, top_ids=S["ids"] if top_k else None,
+                         top_logprobs=S["top"] if top_k else None)
+        return self._scores(S, 1, top_k)
+
+    def score(self, tokens, pos0: int = 0, top_k: int = 0) -> Scores:
+        """The tokens at positions pos0.. through every layer, as prefill takes
+        them, then for each position its distribution's entropy and alternatives
+        and the log probability of the token that follows it (0 at the last).
+        The logits [T, vocab] are never stored as a whole: a prompt of 2,000
+        over a vocabulary of 151,936 would have 1.2 GB of them. The caches hold
+        the tokens afterwards; the state is left as it is."""
+        toks = [int(t) for t in tokens]
+        T, c, e, g = len(toks), self.cfg, self.exe, self.glob
+        known = len(self.last_seq) >= pos0
+        self.last_seq = self.last_seq[:max(pos0, 0)]
+        x = self.prefill_layers(toks, pos0)
+        self.last_seq = self.last_seq + toks if known else []
+        xn = self._pf["xn"]
+        e.rmsnorm_raw(x, g["final_norm"], xn, T, c.hidden, c.rms_eps)
+        S = self._score_buffers(T, top_k, e.lm_logprobs_workspace(T, c.hidden, c.vocab, top_k))
+        S["tokens"].upload(np.array(toks[1:] + [-1] * (S["T"] - T + 1), np.int32))
+        e.lm_logprobs(xn, g["lm_w"], g["lm_s"], g["lm_b"], T, c.hidden, c.vocab, S["ws"], tokens=S["tokens"],
+                      logprob=S["logprob"], entropy=S["entropy"], top_k=top_k, top_ids=S["ids"] if top_k else None,
+                      top_logprobs=S["top"] if top_k else None, group=c.group)
+        e.device_status()
+        return self._scores(S, T, top_k)
 
     # -- prefill (forward.rs:114-261) ------------------------------------------
     def _prefill_buffers(self, T: int) -> Dict:
@@ -328,12 +397,14 @@ class Model:
         for il in range(self.cfg.n_layers):
             self.forward_layer(il)
 
-    def run_turn(self, prompt, max_new: int, eos: int, batch_min: int = 24) -> List[int]:
+    def run_turn(self, prompt, max_new: int, eos: int, batch_min: int = 24, scores: Optional[list] = None,
+                 top_k: int = 0) -> List[int]:
         """forward.rs:471-535: one turn with prefix reuse. The caches keep the
         previous turn's tokens (last_seq); the longest common prefix with this
         prompt is reused and only the rest is prefilled (batched from
         batch_min tokens, token by token below), keeping at least the last
-        prompt token; then greedy decode until max_new tokens or eos."""
+        prompt token; then greedy decode until max_new tokens or eos. scores: a
+        list that receives last_scores(top_k) of every generated token."""
         prompt = [int(t) for t in prompt]
         if not prompt:
             return []
@@ -363,12 +434,16 @@ class Model:
                 self.fill_kv(tk, lcp + i)
             nxt = self.run_one_token(suffix[-1], len(prompt) - 1)
         gen = [nxt]
+        if scores is not None:
+            scores.append(self.last_scores(top_k))
         pos = len(prompt)
         while len(gen) < max_new and nxt != eos and pos < cap:
             self.set_state(pos, nxt)  # run_one_token as a replay of the captured step
             self.replay(1)
             nxt = self.read_state()[1]
             gen.append(nxt)
+            if scores is not None:
+                scores.append(self.last_scores(top_k))
             pos += 1
         # the tokens whose keys and values the caches hold: the last generated
         # token was never fed (the reference records it too, forward.rs:521-523,
