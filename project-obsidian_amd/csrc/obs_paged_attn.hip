@@ -168,26 +168,17 @@ struct Block4 {
   u32x4_v kp[NG][PER / 4u], vp[NG][PER / 4u];  // scale and bias of the entries of its scores
 
   // at0, at1: bytes of the pages (of the kv head) of both halves; first: the block's first entry in its page (WIDE)
-  __device__ __forceinline__ void load(const Paged& a, size_t at0, size_t at1, uint32_t first, uint32_t col, uint32_t g) {
-    const uint32_t row = 8u * (col / 4u) + col % 4u, e = 8u * g, own = MODE & HALF ? col / 8u * 4u : 0u;
-    const uint8_t *kb = a.k, *kw = a.k, *vb = a.v;
-    uint32_t kr = row, ke = e;  // the lane's own
-    if constexpr (MODE & WIDE) {
-      kb += at0 + first * (HD / 2u);
-      kw += at0 + (HD / 2u << a.lp) + 4u * first;
-      vb += at0;
-    } else {
-      const size_t at = g & 2u ? at1 : at0;
-      kb += col & 8u ? at1 : at0;
-      kw += at + (HD / 2u << a.lp);
-      vb += at;
-      kr &= 15u, ke &= 15u;
-    }
-    const uint8_t* vw = vb + (HD / 2u << a.lp) + (MODE & WIDE ? 4u * first : 0u);
-    if constexpr (MODE & WIDE) vb += first;
-    const uint32_t ko = kr * (HD / 2u) + sizeof(K) * g, vo = (col << a.lp) + ke, wo = 4u * (ke + own);
+  __device__ __forceinline__ void load_keys(const Paged& a, size_t at0, size_t at1, uint32_t first, uint32_t col, uint32_t g) {
+    const uint32_t row = 8u * (col / 4u) + col % 4u;
+    const uint8_t* kb = a.k + (MODE & WIDE ? at0 + first * (HD / 2u) : col & 8u ? at1 : at0);
+    const uint32_t ko = (MODE & WIDE ? row : row & 15u) * (HD / 2u) + sizeof(K) * g;
 #pragma unroll
     for (uint32_t tt = 0; tt < 2; ++tt) k[tt] = __builtin_nontemporal_load(reinterpret_cast<const K*>(kb + 4u * tt * (HD / 2u) + ko));
+    load_params(kp, a.k, a, at0, at1, first, col, g);
+  }
+  __device__ __forceinline__ void load_values(const Paged& a, size_t at0, size_t at1, uint32_t first, uint32_t col, uint32_t g) {
+    const uint8_t* vb = a.v + (MODE & WIDE ? at0 + first : g & 2u ? at1 : at0);
+    const uint32_t vo = (col << a.lp) + (MODE & WIDE ? 8u * g : 8u * g & 15u);
 #pragma unroll
     for (uint32_t nt = 0; nt < NT / 2u; ++nt) {
       const u32x2_v* vr = reinterpret_cast<const u32x2_v*>(vb + (16u * nt << a.lp) + vo);
@@ -196,13 +187,16 @@ struct Block4 {
       else
         v[nt] = __builtin_nontemporal_load(vr);
     }
+    load_params(vp, a.v, a, at0, at1, first, col, g);
+  }
+  static __device__ __forceinline__ void load_params(u32x4_v (&to)[NG][PER / 4u], const uint8_t* side, const Paged& a, size_t at0, size_t at1,
+                                                     uint32_t first, uint32_t col, uint32_t g) {
+    const uint8_t* w = side + (HD / 2u << a.lp) + (MODE & WIDE ? at0 + 4u * first : g & 2u ? at1 : at0);
+    const uint32_t wo = 4u * ((MODE & WIDE ? 8u * g : 8u * g & 15u) + (MODE & HALF ? col / 8u * 4u : 0u));
 #pragma unroll
     for (uint32_t q = 0; q < NG; ++q)
 #pragma unroll
-      for (uint32_t i = 0; i < PER / 4u; ++i) {
-        kp[q][i] = *reinterpret_cast<const u32x4_v*>(kw + (4u * q << a.lp) + 16u * i + wo);
-        vp[q][i] = *reinterpret_cast<const u32x4_v*>(vw + (4u * q << a.lp) + 16u * i + wo);
-      }
+      for (uint32_t i = 0; i < PER / 4u; ++i) to[q][i] = *reinterpret_cast<const u32x4_v*>(w + (4u * q << a.lp) + 16u * i + wo);
   }
   // dims of query fragment ks (in q4_order): of the low nibbles, then of the high ones
   static __device__ __forceinline__ uint32_t q_dim(uint32_t ks, uint32_t g) {
@@ -228,12 +222,12 @@ __device__ __forceinline__ float column_sum(float v, uint32_t lane) {
   return v + lane_xor32_f32(v, lane);
 }
 
-// t: the lane's first entry
-template <uint32_t HD, uint32_t MODE>
+// t: the lane's first entry; then(): called when the keys were used
+template <uint32_t HD, uint32_t MODE, typename Then>
 __device__ __forceinline__ void block_step4(const Block4<HD, MODE>& blk, const bf16x8_v (&qb)[HD / 32u],
                                             const float (&qs)[HD / 64u], Column<HD>& c, Sums4<HD>& u, uint32_t t, uint32_t hi,
                                             uint32_t lo, uint32_t sinks, bool ok, bool masked, float scale_log2,
-                                            float (&sv)[Block4<HD, MODE>::PER], uint32_t lane) {
+                                            float (&sv)[Block4<HD, MODE>::PER], uint32_t lane, Then then) {
   constexpr uint32_t NG = HD / 64u, NT = HD / 16u, PER = Block4<HD, MODE>::PER;
   const f32x4_v zero = {0.0f, 0.0f, 0.0f, 0.0f};
   f32x4_v acc[2][NG];
@@ -260,6 +254,9 @@ __device__ __forceinline__ void block_step4(const Block4<HD, MODE>& blk, const b
     }
     sv[j] = s * scale_log2;
   }
+  __builtin_amdgcn_sched_barrier(0);
+  then();
+  __builtin_amdgcn_sched_barrier(0);
   uint32_t bits = 0xffu;
   if (masked) {  // uniform
     bits = ok ? seen_bits(t, hi, lo, sinks) : 0u;
@@ -414,7 +411,7 @@ __device__ __forceinline__ Found plan_find(const Paged& a, const PagedAttn& p, u
 // A part that is all of its sequence writes the output, others their maximum,
 // sum and output for paged_join_kernel.
 template <uint32_t HD, uint32_t KT, bool WEIGHT, uint32_t MODE>
-__global__ void __launch_bounds__(256, MODE& HALF ? 4 : 3) paged_decode_kernel(Paged a, PagedAttn p) {
+__global__ void __launch_bounds__(256, 3) paged_decode_kernel(Paged a, PagedAttn p) {
   constexpr uint32_t NT = HD / 16u, NG = HD / 64u;
   constexpr bool F8 = KT == KT_E4M3, Q4 = KT == KT_Q4;
   typedef typename std::conditional<Q4, Block4<HD, MODE>, Block<HD, F8, bool(MODE & KEEP)>>::type Blk;
@@ -458,45 +455,82 @@ __global__ void __launch_bounds__(256, MODE& HALF ? 4 : 3) paged_decode_kernel(P
   }
   // page ids of the wave's next 64 blocks (both halves of each), a block a lane
   uint32_t id0 = 0, id1 = 0;
-  for (uint32_t x = x0 + wave, it = 0; x < x1; x += 4u, ++it) {
-    if ((it & 63u) == 0u) {
-      const uint32_t t = s.start(min(x + 4u * lane, x1 - 1u));
-      const size_t row = static_cast<size_t>(b) * a.max_pages;
-      id0 = static_cast<uint32_t>(a.table[row + min(t >> a.lp, a.max_pages - 1u)]);
-      id1 = static_cast<uint32_t>(a.table[row + min((t + 16u) >> a.lp, a.max_pages - 1u)]);
-    }
-    const uint32_t t0 = s.start(x);
-    uint32_t p0 = __builtin_amdgcn_readlane(id0, it & 63u), p1 = __builtin_amdgcn_readlane(id1, it & 63u);
-    const bool ok0 = p0 < a.n_pages, ok1 = p1 < a.n_pages;
-    const bool whole = t0 + 32u <= s.hi && (t0 >= s.lo || t0 + 32u <= p.sinks);
-    if (!(ok0 && ok1)) {  // an id that is not there hides its half; reported where an entry of it counts
+  auto list_pages = [&](uint32_t x) __attribute__((always_inline)) {
+    const uint32_t t = s.start(min(x + 4u * lane, x1 - 1u));
+    const size_t row = static_cast<size_t>(b) * a.max_pages;
+    id0 = static_cast<uint32_t>(a.table[row + min(t >> a.lp, a.max_pages - 1u)]);
+    id1 = static_cast<uint32_t>(a.table[row + min((t + 16u) >> a.lp, a.max_pages - 1u)]);
+  };
+  struct Place {
+    uint32_t p0, p1, t0;
+    bool ok0, ok1, masked;
+  };
+  auto place = [&](uint32_t x, uint32_t i) __attribute__((always_inline)) {  // block x, the i-th listed
+    Place h;
+    h.t0 = s.start(x);
+    h.p0 = __builtin_amdgcn_readlane(id0, i & 63u), h.p1 = __builtin_amdgcn_readlane(id1, i & 63u);
+    h.ok0 = h.p0 < a.n_pages, h.ok1 = h.p1 < a.n_pages;
+    const bool whole = h.t0 + 32u <= s.hi && (h.t0 >= s.lo || h.t0 + 32u <= p.sinks);
+    h.masked = !(whole && h.ok0 && h.ok1);
+    if (!(h.ok0 && h.ok1)) {  // an id that is not there hides its half; reported where an entry of it counts
       auto counts = [&](uint32_t t) { return t < s.hi && (t + 16u > s.lo || t < p.sinks); };
-      if (lane == 0u && ((!ok0 && counts(t0)) || (!ok1 && counts(t0 + 16u)))) paged_flag(a.status);
-      p0 = ok0 ? p0 : 0u;
-      p1 = ok1 ? p1 : 0u;
+      if (lane == 0u && ((!h.ok0 && counts(h.t0)) || (!h.ok1 && counts(h.t0 + 16u)))) paged_flag(a.status);
+      h.p0 = h.ok0 ? h.p0 : 0u;
+      h.p1 = h.ok1 ? h.p1 : 0u;
     }
+    return h;
+  };
+  if constexpr (Q4) {
+    // A block's keys make room for the next one's, its values likewise: one of them is on
+    // its way at any time (one sequence of 100,003 21.1 us, with a block's loads together
+    // and four workgroups a CU 22.8; with registers for a whole second block, spilled, 27).
+    constexpr uint32_t PER = Blk::PER;
+    const uint32_t own = 8u * g + (PER == 4u ? col / 8u * 4u : 0u);
     Blk blk;
-    const bool masked = !(whole && ok0 && ok1);
-    if constexpr (Q4) {
-      constexpr uint32_t PER = Blk::PER;
-      const uint32_t own = 8u * g + (PER == 4u ? col / 8u * 4u : 0u);
-      blk.load(a, page_at<HD, KT_Q4>(a, p0, kv), page_at<HD, KT_Q4>(a, p1, kv), t0 & ((1u << a.lp) - 1u), col, g);
-      __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
+    auto keys = [&](const Place& h) __attribute__((always_inline)) {
+      blk.load_keys(a, page_at<HD, KT_Q4>(a, h.p0, kv), page_at<HD, KT_Q4>(a, h.p1, kv), h.t0 & ((1u << a.lp) - 1u), col, g);
+    };
+    auto values = [&](const Place& h) __attribute__((always_inline)) {
+      blk.load_values(a, page_at<HD, KT_Q4>(a, h.p0, kv), page_at<HD, KT_Q4>(a, h.p1, kv), h.t0 & ((1u << a.lp) - 1u), col, g);
+    };
+    auto take = [&](const Place& h, uint32_t x, auto then) __attribute__((always_inline)) {
       float sv[PER];
-      block_step4<HD, MODE>(blk, qb, qs, c, u, t0 + own, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, masked, scale, sv, lane);
+      block_step4<HD, MODE>(blk, qb, qs, c, u, h.t0 + own, s.hi, s.lo, p.sinks, g & 2u ? h.ok1 : h.ok0, h.masked, scale, sv, lane, then);
       if constexpr (WEIGHT) {
-        const uint32_t h = MODE & HALF ? col % 8u : col;
-        if (h < p.G) {
-          float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + h) * p.vis + 32u * x + own);
+        const uint32_t hh = MODE & HALF ? col % 8u : col;
+        if (hh < p.G) {
+          float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + hh) * p.vis + 32u * x + own);
 #pragma unroll
           for (uint32_t i = 0; i < PER / 4u; ++i) to[i] = make_float4(sv[4 * i], sv[4 * i + 1], sv[4 * i + 2], sv[4 * i + 3]);
         }
       }
-    } else {
-      blk.load(a, kv, col & 8u ? p1 : p0, g & 2u ? p1 : p0, t0, col, g);
+    };
+    for (uint32_t xl = x0 + wave; xl < x1; xl += 256u) {
+      list_pages(xl);
+      const uint32_t end = umin(x1, xl + 256u);
+      uint32_t x = xl, i = 0;
+      Place h = place(x, 0u);
+      keys(h);
+      values(h);
+      for (; x + 4u < end; x += 4u) {
+        const Place n = place(x + 4u, ++i);
+        take(h, x, [&]() __attribute__((always_inline)) { keys(n); });
+        __builtin_amdgcn_sched_barrier(0);
+        values(n);
+        __builtin_amdgcn_sched_barrier(0);
+        h = n;
+      }
+      take(h, x, [] {});
+    }
+  } else {
+    for (uint32_t x = x0 + wave, it = 0; x < x1; x += 4u, ++it) {
+      if ((it & 63u) == 0u) list_pages(x);
+      const Place h = place(x, it);
+      Blk blk;
+      blk.load(a, kv, col & 8u ? h.p1 : h.p0, g & 2u ? h.p1 : h.p0, h.t0, col, g);
       __builtin_amdgcn_sched_barrier(0);  // every load of the block before the first wait
       float sv[8];
-      block_step<HD, F8, bool(MODE & KEEP)>(blk, qb, c, t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? ok1 : ok0, masked, scale, sv, lane);
+      block_step<HD, F8, bool(MODE & KEEP)>(blk, qb, c, h.t0 + 8u * g, s.hi, s.lo, p.sinks, g & 2u ? h.ok1 : h.ok0, h.masked, scale, sv, lane);
       if constexpr (WEIGHT) {
         if (col < p.G) {
           float4* to = reinterpret_cast<float4*>(p.scores + (static_cast<size_t>(b) * p.nh + kv * p.G + col) * p.vis + 32u * x + 8u * g);
@@ -707,10 +741,14 @@ uint32_t decode_whole(uint64_t rows, bool f8) { return rows >= 512u && f8 ? 64u 
 // Parts of a call: three workgroups a CU are resident (DECODE_ONCE). Few rows give
 // nearly equal parts, which fill the chip once (one sequence of 100,003 entries
 // 46.6 us against 52.8 with 1,152); the parts of many sequences differ, and
-// finer ones even out (48 sequences of up to 16,000: 72.3 us against 74.6), those of 4 bits
-// yet finer (16 under a window of 8,192 30.5 us against 32.9).
+// finer ones even out (48 sequences of up to 16,000: 72.3 us against 74.6). In 4 bits yet
+// finer ones (16 under a window of 8,192 28.5 us against 31.4 with 1,152), and of few
+// sequences so few that with what rounding up adds they are resident at once (6 of up to
+// 16,000 16.7 us against 20.2).
 uint32_t decode_target(const obs_paged_kv* kv, const obs_paged_seqs* s) {
-  return s->n_seqs * kv->n_kv <= 32u ? DECODE_ONCE : kv->dtype == OBS_KV_Q4 ? 1536u : 1152u;
+  const uint32_t rows = s->n_seqs * kv->n_kv;
+  if (rows > 32u) return kv->dtype == OBS_KV_Q4 ? 1536u : 1152u;
+  return kv->dtype == OBS_KV_Q4 && s->n_seqs > 1u ? DECODE_ONCE - rows : DECODE_ONCE;
 }
 
 struct DecodePlan {
