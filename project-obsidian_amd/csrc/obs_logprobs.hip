@@ -890,7 +890,8 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   }
   barrier_but<0>();
   load_x(1u, s_x1);
-  constexpr uint32_t FR = 4u * MT, RING = 4u;  // fragments of x a group; held at once
+  constexpr uint32_t FR = 4u * MT, RING = MT == 1u ? 2u : 4u;  // fragments of x a group; held at once, fewer than those (the barrier stands between)
+  static_assert(RING < FR, "the barrier is before the first of the next group's");
   f16x8_v xa[RING];
   u32x4_v wb[2][4], raw[2];
   uint32_t rs[2], last[2];  // scales; the last word of a group's weights
@@ -939,7 +940,7 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
 #pragma unroll
   for (uint32_t j = 0; j < RING; ++j) load_a(s_x0, j);
   // A group is one stream of products without a pause, none of which waits for the one
-  // before. Beside them stand the reads of the rows four fragments ahead and the weights to
+  // before. Beside them stand the reads of the rows RING fragments ahead and the weights to
   // come: step s makes those of step s - 1 of the next group (step 0 the last ones of its own).
   // The one barrier is where the last of a group's rows and the next one's weights are read,
   // and the next one's rows have come; behind it their places are filled: with the rows of the
@@ -1046,6 +1047,21 @@ struct LmPlan {
   size_t stat, xt, logits, xp, xf, xs;
   size_t all() const { return stat + xt + logits + xp + xf + xs; }
 };
+// 32-row blocks of a workgroup, one to four, by what a launch takes: of 2,048 columns a
+// workgroup of m blocks 12 + 8 m us where each has a CU (20, 24, 33, 42 measured), and where
+// CUs hold two a round of 512 takes 20 + 11 m (30, 40, 52, 62), by the XCD with most
+// columns. Few columns so make more, smaller workgroups: 70 rows of 3,399 27 us, with three
+// blocks 39; 2,000 of 2,000 42 and, with four, 54.
+uint32_t lm_blocks(uint32_t rows, uint32_t tiles) {
+  const uint64_t blocks = (rows + 31u) / 32u;
+  uint32_t best = 4u;
+  uint64_t least = ~uint64_t(0);
+  for (uint32_t m = 4; m; --m) {
+    const uint64_t n = (blocks + m - 1u) / m * ((tiles + 7u) / 8u), us = n <= 32u ? 12u + 8u * m : (n + 63u) / 64u * (20u + 11u * m);
+    if (us < least) best = m, least = us;
+  }
+  return best;
+}
 LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   LmPlan d{};
   const uint32_t cols = T <= LM_FEW ? LM_FEW_COLS : LM_COLS;
@@ -1053,8 +1069,7 @@ LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   d.ld = (vocab + 3u) & ~3u;
   // the logits of a pass where alternatives are wanted, and its sums, are of a bounded size
   d.rows = T <= LM_FEW ? T : std::min(T, k ? 256u : 4096u);
-  const uint32_t b32 = (d.rows + 31u) / 32u, tts = (b32 + 3u) / 4u;  // 32-row blocks, workgroups of four at most
-  d.mb = std::max(2u, (b32 + tts - 1u) / tts);
+  d.mb = lm_blocks(d.rows, d.tiles);
   const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = (d.rows + 32u * d.mb - 1u) / (32u * d.mb) * d.mb;
   d.stat = up256(static_cast<size_t>(d.rows) * d.tiles * sizeof(float4));
   d.xt = up256(static_cast<size_t>(d.rows) * sizeof(float));
@@ -1199,7 +1214,8 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
     if (T <= LM_FEW)
       rc = launch_few(ctx, a);
     else
-      rc = d.mb == 2u   ? launch_many<2>(ctx, a, xp, xf, xs)
+      rc = d.mb == 1u   ? launch_many<1>(ctx, a, xp, xf, xs)
+           : d.mb == 2u ? launch_many<2>(ctx, a, xp, xf, xs)
            : d.mb == 3u ? launch_many<3>(ctx, a, xp, xf, xs)
                         : launch_many<4>(ctx, a, xp, xf, xs);
     if (rc != OBS_OK) return rc;
