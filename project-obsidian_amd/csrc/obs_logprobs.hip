@@ -555,7 +555,7 @@ __device__ __forceinline__ void lm_sums(const LmArgs& p, float (&x)[N], uint32_t
 // = lane / 16) of a product (v_mfma_f32_16x16x32_bf16) loads 16 bytes of its row, the four
 // 64, two groups; a swap of the wave's halves gives each lane 8 bytes of either (of the
 // group's 32, those from 16 (q % 2) + 8 (q / 2) on). The sums over a group's columns are a
-// product with ones. HELD: a wave has one slice, whose rows of x stay in registers.
+// product with ones. HELD: a wave has one slice, whose rows of x and sums stay in registers.
 template <uint32_t NT, bool HELD>
 __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
   constexpr uint32_t RT = 16u * NT, OROW = LM_FEW_COLS + 4u, WAVES = 8;
@@ -580,6 +580,16 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
       for (uint32_t s = 0; s < 2; ++s)
 #pragma unroll
         for (uint32_t m = 0; m < NT; ++m) xh[g][s][m] = load_x(umin(wave, slices - 1u), g, s, m);
+  }
+  f32x4_v xsh[HELD ? 4 : 1][NT];  // sums of the groups
+  if constexpr (HELD) {
+#pragma unroll
+    for (uint32_t g = 0; g < 4; ++g)
+#pragma unroll
+      for (uint32_t m = 0; m < NT; ++m) {
+        xsh[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xh[g][0][m], ones, zero, 0, 0, 0);
+        xsh[g][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xh[g][1][m], ones, xsh[g][m], 0, 0, 0);
+      }
   }
   struct Rows {
     u32x4_v w[4][2];     // two groups each
@@ -635,7 +645,10 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
               xa[s][m] = xh[g][s][m];
             else
               xa[s][m] = load_x(slice, g, s, m);
-            xs[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[s][m], ones, s ? xs[m] : zero, 0, 0, 0);
+            if constexpr (HELD)
+              xs[m] = xsh[g][m];
+            else
+              xs[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xa[s][m], ones, s ? xs[m] : zero, 0, 0, 0);
           }
 #pragma unroll
         for (uint32_t n = 0; n < 4; ++n) {
