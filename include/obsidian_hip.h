@@ -628,8 +628,10 @@ int obs_token_logprobs(obs_ctx* ctx, const void* logits, int dtype, uint32_t T, 
 
 /* The same of the logits x . dequant(W)^T of T rows x bf16 [T, in] (after the final
  * norm) and a 4-bit [vocab, in] matrix (the lm_head); the logits are not the caller's.
- * No weight is rounded (q * scale + bias enters in fp32, as in obs_q4_gemv). group 64,
- * in a multiple of 512 up to 16,384; x, w, scales, biases and ws 16-byte aligned.
+ * No weight is rounded (q * scale + bias enters in fp32, as in obs_q4_gemv), but in calls of
+ * more than 32 rows those of groups whose scale is below 2^-8 of the largest of their
+ * vocabulary row (to within 2^-15 of that scale), and hidden values below 2^-29 of their
+ * row's largest (to within 2^-39 of it). group 64, in a multiple of 512 up to 16,384; x, w, scales, biases and ws 16-byte aligned.
  * With alternatives the rows of more than 32 tokens pass by 256 at a time, whose logits
  * are in the workspace. */
 int obs_lm_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t in, uint32_t vocab, uint32_t top_k, size_t* bytes);
