@@ -247,6 +247,26 @@ def test_decode_offsets_past_32_bits(exe):
     assert np.all(np.abs(got - ref) <= bound)
 
 
+@pytest.mark.parametrize("page", [16, 32, 64])
+def test_decode_parts_of_many_blocks(exe, page):
+    """So many entries in all that a wave takes more than 64 blocks of a part: 600 sequences over the same pages."""
+    nh, nkv, hd, n, B = 8, 1, 64, 30011, 600
+    rng = np.random.default_rng(47)
+    pool = Pool(exe, rng, [n], nkv, hd, page)
+    table = exe.upload(np.repeat(pool.table, B, 0))
+    seqs = oh.PagedSeqs(table, exe.upload(np.full(B, n, np.int32)), B, pool.max_pages)
+    q = synth.bf16_normal(rng, (B, nh, hd), 2.0)
+    dq, out = exe.upload(q), exe.upload(np.full((B, nh, hd), FILL16, np.uint16))
+    ws = exe.upload(np.full(exe.sdpa_paged_workspace(pool.kv, seqs, nh), 0xFF, np.uint8))
+    exe.sdpa_paged_decode(pool.kv, seqs, dq, out, nh, ws)
+    exe.device_status()
+    got = _f64(out.download())
+    assert np.all(np.isfinite(got))
+    for b in (0, 1, 299, B - 1):
+        ref, bound, _, _ = _attend4(_f64(q[b]), pool.parts(0, "k"), pool.parts(0, "v"), np.ones(n, bool))
+        assert np.all(np.abs(got[b] - ref) <= bound), b
+
+
 @pytest.mark.parametrize("page", [16, 64])
 def test_decode_bad_pages(exe, page):
     nh, nkv, hd = 32, 4, 128
