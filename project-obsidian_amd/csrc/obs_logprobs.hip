@@ -224,6 +224,20 @@ __device__ __forceinline__ float lanes_edge(float own, uint32_t k) {
   return e < 0x00800000u ? NEG_INF : f32_unorder(static_cast<int>(e ^ 0x80000000u));
 }
 
+// The largest upper half of a key, its lower 12 bits clear, that at least k of a wave's N x 64 reach.
+template <uint32_t N>
+__device__ __forceinline__ uint32_t keys_edge(const uint32_t (&keys)[N], uint32_t k) {
+  uint32_t e = 0u;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1) {
+    uint32_t c = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) c += static_cast<uint32_t>(__popcll(__ballot(keys[i] >= (e | bit))));
+    if (c >= k) e |= bit;  // uniform
+  }
+  return e;
+}
+
 // A workgroup a row: the parts' sums joined, then the k largest. Of the tiles: what k
 // lanes of a wave reach with their own maxima keeps out all but a few, which are listed in
 // LDS and ranked by counting; the same of the k tiles' logits. Where more are listed than
@@ -258,7 +272,10 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) v[i] = i0 + 256u * i + tid < p.tiles ? v[i] : NEG_INF;
   };
-  float first[8], own = NEG_INF;  // of the first 2,048 tiles
+  float first[8], own = NEG_INF;  // maxima of the first 2,048 tiles, the thread's largest
+  // of few lanes' edges the best of four waves is nearly what all threads' is (48 rows of 151,936 logits: k = 20
+  // 16 us either way, k = 64 48 and 22)
+  const bool wide = k > 32u;
   if (k) {
     if (tid < 2u) s_n[tid] = 0u;
     if (tid < MAX_TOP + 4u) s_tile[tid] = 0xffffffffu;
@@ -289,10 +306,14 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) own = fmaxf(own, first[i]);
     for (uint32_t i = 2048u + tid; i < p.tiles; i += 256u) own = fmaxf(own, tm[static_cast<size_t>(i) * p.tstride]);
-    const float e = lanes_edge(own, k);
-    if (lane == 0u) s_edge[wave] = e;
+    if (wide) {
+      s_list[tid] = top_key(own, 0u);
+    } else {
+      const float e = lanes_edge(own, k);
+      if (lane == 0u) s_edge[wave] = e;
+    }
   }
-  const Stat r = stat_group(a, s_st, lane, wave);  // a barrier: the waves' edges are there
+  const Stat r = stat_group(a, s_st, lane, wave);  // a barrier: the waves' edges are there, or the threads' maxima
   const float ls = logf(r.s);
   const bool none = r.m == NEG_INF && r.s == 0.0f;  // no logit above -inf
   if (tid == 0u) {
@@ -312,7 +333,16 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
       for (uint32_t j = 0; j < 4; ++j) above += s_list[i + j] > key && i + j < n;  // (read before it is known to count: in flight together)
     return above;
   };
-  const float edge = fmaxf(fmaxf(s_edge[0], s_edge[1]), fmaxf(s_edge[2], s_edge[3]));
+  // what k of the 256 threads reach with the maxima that they left in s_list
+  auto threads_edge = [&]() __attribute__((always_inline)) {
+    uint32_t keys[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) keys[i] = static_cast<uint32_t>(s_list[64u * i + lane] >> 32);
+    const uint32_t e = keys_edge<4>(keys, k);
+    __syncthreads();
+    return e <= static_cast<uint32_t>(NONE_KEY >> 32) ? NEG_INF : key_value(static_cast<uint64_t>(e) << 32);
+  };
+  const float edge = wide ? threads_edge() : fmaxf(fmaxf(s_edge[0], s_edge[1]), fmaxf(s_edge[2], s_edge[3]));
   for (uint32_t i0 = 0;;) {
     uint32_t mask = 0;
 #pragma unroll
@@ -387,7 +417,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
       for (uint32_t e = 0; e < PER; ++e) x[e] = is && v + e < p.vocab ? logit(v + e) : NEG_INF;
     }
   };
-  if (low == NEG_INF) {  // uniform: fewer than k tiles; what k lanes of a wave reach with all of its logits
+  if (low == NEG_INF || p.tiles < 2u * k) {  // uniform: few tiles, some of them short; what k threads reach with all of their logits
     float m = NEG_INF;
     for (uint32_t j = wave; j < rows; j += 4u) {
       float x[PER];
@@ -395,10 +425,9 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 #pragma unroll
       for (uint32_t e = 0; e < PER; ++e) m = fmaxf(m, x[e]);
     }
-    const float e = lanes_edge(m, k);
-    if (lane == 0u) s_edge[wave] = e;
+    s_list[tid] = top_key(fmaxf(m, NEG_INF), 0u);
     __syncthreads();
-    low = fmaxf(fmaxf(s_edge[0], s_edge[1]), fmaxf(s_edge[2], s_edge[3]));
+    low = fmaxf(low, threads_edge());
   }
   for (uint32_t j0 = wave; j0 < rows; j0 += 16u) {
     float x[4][PER];
@@ -422,18 +451,12 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
   if (n > 128u && n <= CAP) {  // uniform
     constexpr uint32_t PER_LANE = CAP / 64u;
     uint64_t mine[CAP / 256u];
-    uint32_t keys[PER_LANE], e = 0u;
+    uint32_t keys[PER_LANE];
 #pragma unroll
     for (uint32_t i = 0; i < PER_LANE; ++i) keys[i] = 64u * i + lane < n ? static_cast<uint32_t>(s_list[64u * i + lane] >> 32) : 0u;
 #pragma unroll
     for (uint32_t i = 0; i < CAP / 256u; ++i) mine[i] = 256u * i + tid < n ? s_list[256u * i + tid] : 0u;
-#pragma unroll 1
-    for (uint32_t bit = 0x80000000u; bit >= 0x1000u; bit >>= 1) {
-      uint32_t c = 0;
-#pragma unroll
-      for (uint32_t i = 0; i < PER_LANE; ++i) c += static_cast<uint32_t>(__popcll(__ballot(keys[i] >= (e | bit))));
-      if (c >= k) e |= bit;  // uniform
-    }
+    const uint32_t e = keys_edge<PER_LANE>(keys, k);
     __syncthreads();
     if (tid == 0u) s_n[1] = 0u;
     __syncthreads();

@@ -236,11 +236,6 @@ __device__ __forceinline__ u32x4_v q4_order(const u32x4_v& v) {
   return u32x4_v{__builtin_amdgcn_perm(v.y, v.x, 0x05040100u), __builtin_amdgcn_perm(v.y, v.x, 0x07060302u),
                  __builtin_amdgcn_perm(v.w, v.z, 0x05040100u), __builtin_amdgcn_perm(v.w, v.z, 0x07060302u)};
 }
-// The low or high nibble of byte I.
-template <uint32_t I, bool HIGH>
-__device__ __forceinline__ float q4_nibble(uint32_t w) {
-  return static_cast<float>(w >> (8u * I + (HIGH ? 4u : 0u)) & 15u);
-}
 __device__ __forceinline__ float q4_value(float q, uint32_t par) { return __builtin_fmaf(q, bf16lo(par), bf16hi(par)); }
 // Scale and bias of a group whose least and largest values are lo and hi; `bits`: the
 // largest magnitude's, which shows a value that is not finite (the group then reads

@@ -210,14 +210,13 @@ struct Sums4 {
   float w[HD / 64u], b[HD / 64u];
 };
 
-constexpr int ROW_ROR8 = 0x128;  // lane i <- lane i ^ 8 of its 16
 // own, but in lanes 8 to 15 of 16 what other has in lanes 0 to 7
 __device__ __forceinline__ float upper_from(float own, float other) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(own), __float_as_int(other), ROW_ROR8, 0xf, 0xc, false));
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(own), __float_as_int(other), DPP_ROW_ROR8, 0xf, 0xc, false));
 }
 template <uint32_t MODE>
 __device__ __forceinline__ float column_sum(float v, uint32_t lane) {
-  if constexpr (MODE & HALF) v += dpp_f32<ROW_ROR8>(v);
+  if constexpr (MODE & HALF) v += dpp_f32<DPP_ROW_ROR8>(v);
   v += lane_xor16_f32(v, lane);
   return v + lane_xor32_f32(v, lane);
 }
@@ -266,7 +265,7 @@ __device__ __forceinline__ void block_step4(const Block4<HD, MODE>& blk, const b
   float bm = sv[0];
 #pragma unroll
   for (uint32_t j = 1; j < PER; ++j) bm = fmaxf(bm, sv[j]);
-  if constexpr (PER == 4u) bm = fmaxf(bm, dpp_f32<ROW_ROR8>(bm));
+  if constexpr (PER == 4u) bm = fmaxf(bm, dpp_f32<DPP_ROW_ROR8>(bm));
   bm = fmaxf(bm, lane_xor16_f32(bm, lane));
   bm = fmaxf(bm, lane_xor32_f32(bm, lane));
   const float m_new = fmaxf(c.m, bm), m_use = m_new == NEG_INF ? 0.0f : m_new;
@@ -319,7 +318,7 @@ __device__ __forceinline__ void block_step4(const Block4<HD, MODE>& blk, const b
     }
     if constexpr (PER == 4u) {
 #pragma unroll
-      for (uint32_t j = 0; j < 2; ++j) pk[2u + j] = static_cast<uint32_t>(dpp_i32<ROW_ROR8>(static_cast<int>(pk[j])));
+      for (uint32_t j = 0; j < 2; ++j) pk[2u + j] = static_cast<uint32_t>(dpp_i32<DPP_ROW_ROR8>(static_cast<int>(pk[j])));
     }
     pb[q] = __builtin_bit_cast(bf16x8_v, pk);
   }
