@@ -249,7 +249,7 @@ __device__ __forceinline__ uint32_t keys_edge(const uint32_t (&keys)[N], uint32_
 // its step, the next three at most.
 template <bool BF16, uint32_t TILE>
 __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
-  constexpr uint32_t CAP = 1024, SUBS = TILE ? 1u : 4u, PER = TILE == 64u ? 1u : 4u;
+  constexpr uint32_t CAP = 1024, SUBS = TILE ? 1u : 4u, PER = TILE ? TILE / 64u : 4u;
   __shared__ float s_st[3][4];
   __shared__ uint32_t s_tile[MAX_TOP + 4u], s_n[2];
   __shared__ uint64_t s_list[CAP];
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(256) logprobs_join_kernel(JoinArgs p) {
 // vocabulary, so that a lane has one vocabulary row and the scale is one factor of its sums
 // over a group, in fp32: no weight is rounded.
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
-constexpr uint32_t LM_COLS = 256, LM_FEW_COLS = 64;  // vocabulary rows of a workgroup
+constexpr uint32_t LM_FEW_COLS = 64;  // vocabulary rows of a workgroup
 
 // Eight nibbles as 16 + q in bf16, columns 0, 4, 1, 5, 2, 6, 3, 7.
 __device__ __forceinline__ bf16x8_v lm_weights(uint32_t w) {
@@ -786,10 +786,10 @@ __global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict
   }
 }
 
-// Four waves a workgroup, 32 MT tokens x 64 vocabulary rows a wave, two workgroups a CU: the
-// sums at one's end (350 us of 1,335 for 2,000 tokens with one of eight waves) beside the other's
-// products. Rows and weights come into LDS past the registers, by whole runs of a row; read by
-// the lanes that use them, 32 bytes of 32 rows a load, the weights took 165 us, the scales, two
+// Four waves a workgroup, 32 MT tokens x 32 N vocabulary rows a wave, two or three workgroups a CU:
+// the sums at one's end (350 us of 1,335 for 2,000 tokens with one of eight waves) beside the
+// other's products. Rows and weights come into LDS past the registers, by whole runs of a row; read
+// by the lanes that use them, 32 bytes of 32 rows a load, the weights took 165 us, the scales, two
 // bytes each, 150, and the rows through registers and their stores 250. 2,000 tokens take
 // 1,220 us, 1,020 TFLOP/s (a library's bf16 product of the same sizes, without the 4 bits: 1,214 us).
 typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
@@ -814,21 +814,24 @@ __device__ __forceinline__ void barrier_but() {
   __builtin_amdgcn_sched_barrier(0);
   asm volatile("" ::: "memory");
 }
-template <uint32_t MT>
+template <uint32_t MT, uint32_t N>
 struct LmTile {
-  static constexpr uint32_t THREADS = 256, ROWS = 32u * MT, COLS = 256;
-  static constexpr uint32_t XB = MT * 4096u, WB = COLS * 64u, SB = COLS * 4u;  // bytes of a group of x, of two groups' weights and scales
-  static constexpr uint32_t OROW = COLS + 8u, XLDS = XB > 16u * OROW * 4u ? XB : 16u * OROW * 4u;  // 16 rows of logits
-  static_assert(COLS == THREADS && COLS == LM_COLS, "a thread a row");
+  static constexpr uint32_t THREADS = 256, ROWS = 32u * MT, COLS = 128u * N, GB = 4u / N;  // GB: groups of a block of weights
+  static constexpr uint32_t XB = MT * 4096u, WB = COLS * 32u * GB, SB = COLS * 2u * GB;  // bytes of a group of x, of a block's weights and scales
+  static constexpr uint32_t OROW = COLS + 8u, OB = 16u * OROW * 4u, WLDS = WB > OB ? WB : OB;  // 16 rows of logits, at the end in their place
+  static constexpr uint32_t HELD = N == 1u && MT <= 2u ? 3u : 2u;                        // workgroups a CU
+  static_assert(SB == 4u * THREADS && WB == 64u * THREADS, "five loads a thread");
 };
-template <uint32_t MT>
-__global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t* __restrict__ xp, const float* __restrict__ xf,
-                                                         const uint8_t* __restrict__ xs, uint32_t ttiles, uint32_t vtiles, uint32_t turn) {
-  typedef LmTile<MT> L;
+template <uint32_t MT, uint32_t N>
+__global__ void __launch_bounds__(256, (LmTile<MT, N>::HELD)) lm_many_kernel(LmArgs p, const uint8_t* __restrict__ xp,
+                                                                           const float* __restrict__ xf, const uint8_t* __restrict__ xs,
+                                                                           uint32_t ttiles, uint32_t vtiles, uint32_t turn) {
+  typedef LmTile<MT, N> L;
+  constexpr uint32_t GB = L::GB, RB = 32u * GB, SW = GB / 2u;  // bytes of a row's block, words of its scales
   // (arrays of their own, for the compiler to tell the ones being written from those being read)
-  __shared__ __attribute__((aligned(16))) uint8_t s_x0[L::XLDS], s_x1[L::XLDS], s_w0[L::WB], s_w1[L::WB], s_s0[L::SB], s_s1[L::SB];
+  __shared__ __attribute__((aligned(16))) uint8_t s_x0[L::XB], s_x1[L::XB], s_w0[L::WLDS], s_w1[L::WLDS], s_s0[L::SB], s_s1[L::SB];
   __shared__ float s_factor[L::ROWS];
-  __shared__ uint32_t s_token[L::ROWS], s_scale[L::COLS];
+  __shared__ uint32_t s_token[L::ROWS];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wn = uniform(tid >> 6);
   const uint32_t col = lane & 31u, half = lane >> 5;
   // An XCD (blockIdx.x % 8) takes `turn` token tiles, whose rows its L2 holds, through all its column tiles, then the next.
@@ -845,16 +848,16 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
 #pragma unroll
     for (uint32_t i = 0; i < MT; ++i) lds_from16(base + 16u * (tid + 256u * i), to + 16u * (64u * wn + 256u * i));
   };
-  // Two groups of every row: four threads for 64 bytes of weights, one for the scales. A row's chunks
-  // change places by its number, so that the reads below meet every bank once. Behind the last row it again.
+  // GB groups of every row: 2 GB threads for its weights, SW for the scales. A row's chunks change
+  // places by its number, so that the reads below meet every bank once. Behind the last row it again.
   auto load_w = [&](uint32_t block, uint8_t* to, uint8_t* sto) __attribute__((always_inline)) {
-    const uint32_t bl = umin(block, groups / 2u - 1u);
+    const uint32_t bl = umin(block, groups / GB - 1u);
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
-      const uint32_t r = 64u * i + tid / 4u;
-      lds_from16(wb0 + 64u * bl + (umin(r, most) * (p.in / 2u) + 16u * (tid % 4u ^ (r >> 1 & 3u))), to + 16u * (64u * wn + 256u * i));
+      const uint32_t r = (128u / GB) * i + tid / (2u * GB);
+      lds_from16(wb0 + RB * bl + (umin(r, most) * (p.in / 2u) + 16u * (tid % (2u * GB) ^ (r >> 1 & (2u * GB - 1u)))), to + 16u * (64u * wn + 256u * i));
     }
-    lds_from4(sb0 + 4u * bl + umin(tid, most) * (2u * groups), sto + 4u * (64u * wn));
+    lds_from4(sb0 + 2u * GB * bl + (umin(tid / SW, most) * (2u * groups) + 4u * (tid % SW)), sto + 4u * (64u * wn));
   };
   load_w(0u, s_w0, s_s0);
   load_x(0u, s_x0);
@@ -864,50 +867,49 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
     s_factor[tid] = xf[t];
     s_token[tid] = p.tokens && t < p.T ? lm_token(p, t) : 0xffffffffu;
   }
-  // the largest scale of every vocabulary row of the tile: its exponent (or of the biases 2^90
-  // of it: no sum reaches fp32's range)
-  {
-    uint32_t top = 0u, btop = 0u;
-    for (uint32_t g = 0; g < groups; g += 8u) {
-      const uint32_t at = umin(tid, most) * (2u * groups) + 2u * g;
-      const u32x4_v v = *reinterpret_cast<const u32x4_v*>(sb0 + at), u = *reinterpret_cast<const u32x4_v*>(bb0 + at);
+  // The largest scale of the lane's vocabulary rows: its exponent (or of the biases 2^90 of it: no
+  // sum reaches fp32's range); a half of the wave has every other eight groups.
+  const uint32_t steps = gpad / 16u;
+  uint32_t cex[N], most_s[N] = {}, most_b[N] = {};
+  float down[N];  // brings the scales below 2^-8
+  auto params = [&](const uint8_t* from, uint32_t n, uint32_t g) __attribute__((always_inline)) {  // of eight groups from g on
+    return *reinterpret_cast<const u32x4_v*>(from + (umin(32u * N * wn + 32u * n + col, most) * (2u * groups) + 2u * umin(g, groups - 8u)));
+  };
+  for (uint32_t s = 0; s < steps; ++s)
+#pragma unroll
+    for (uint32_t n = 0; n < N; ++n) {
+      const u32x4_v v = params(sb0, n, 16u * s + 8u * half), u = params(bb0, n, 16u * s + 8u * half);
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
-        top = max(top, max(v[i] & 0x7fffu, v[i] >> 16 & 0x7fffu));
-        btop = max(btop, max(u[i] & 0x7fffu, u[i] >> 16 & 0x7fffu));
+        most_s[n] = max(most_s[n], max(v[i] & 0x7fffu, v[i] >> 16 & 0x7fffu));
+        most_b[n] = max(most_b[n], max(u[i] & 0x7fffu, u[i] >> 16 & 0x7fffu));
       }
     }
-    s_scale[tid] = umin(max(top >> 7, max(btop >> 7, 90u) - 90u), 244u);
-  }
-  __syncthreads();
-  float down[2];  // brings the lane's vocabulary rows' scales below 2^-8
-  uint32_t cex[2];
 #pragma unroll
-  for (uint32_t n = 0; n < 2; ++n) {
-    cex[n] = s_scale[64u * wn + 32u * n + col];
+  for (uint32_t n = 0; n < N; ++n) {
+    const uint32_t e = max(most_s[n] >> 7, max(most_b[n] >> 7, 90u) - 90u);
+    cex[n] = umin(max(e, __float_as_uint(lane_xor32_f32(__uint_as_float(e), lane))), 244u);
     down[n] = __uint_as_float((245u - cex[n]) << 23);
   }
-  f32x16_v acc[MT][2];
+  f32x16_v acc[MT][N];
 #pragma unroll
   for (uint32_t m = 0; m < MT; ++m)
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) acc[m][n] = f32x16_v{};
+    for (uint32_t n = 0; n < N; ++n) acc[m][n] = f32x16_v{};
   // the groups' sums with b + 8 s
-  for (uint32_t s = 0, steps = gpad / 16u; s < steps; ++s) {
+  for (uint32_t s = 0; s < steps; ++s) {
     const uint32_t g = 16u * s + 8u * half;
-    bf16x8_v bb[2][2];
+    bf16x8_v bb[N][2];
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) {
-      const uint32_t r = umin(64u * wn + 32u * n + col, most);
+    for (uint32_t n = 0; n < N; ++n)
 #pragma unroll
       for (uint32_t k = 0; k < 2; ++k) {
-        u32x4_v v = *reinterpret_cast<const u32x4_v*>((k ? sb0 : bb0) + (r * (2u * groups) + 2u * umin(g, groups - 8u)));
+        u32x4_v v = params(k ? sb0 : bb0, n, g);
         const float f = k ? 8.0f * down[n] : down[n];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) v[i] = g < groups ? pack_bf16_pair_rne(bf16lo(v[i]) * f, bf16hi(v[i]) * f) : 0u;
         bb[n][k] = __builtin_bit_cast(bf16x8_v, v);
       }
-    }
     bf16x8_v xa[LM_SUMS][MT];
 #pragma unroll
     for (uint32_t k = 0; k < LM_SUMS; ++k)
@@ -919,7 +921,7 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
 #pragma unroll
       for (uint32_t m = 0; m < MT; ++m)
 #pragma unroll
-        for (uint32_t n = 0; n < 2; ++n) {
+        for (uint32_t n = 0; n < N; ++n) {
           acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[k][m], bb[n][0], acc[m][n], 0, 0, 0);
           acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa[k][m], bb[n][1], acc[m][n], 0, 0, 0);
         }
@@ -929,29 +931,29 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   constexpr uint32_t FR = 4u * MT, RING = MT == 1u ? 2u : 4u;  // fragments of x a group; held at once, fewer than those (the barrier stands between)
   static_assert(RING < FR, "the barrier is before the first of the next group's");
   f16x8_v xa[RING];
-  u32x4_v wb[2][4], raw[2];
-  uint32_t rs[2], last[2];  // scales; the last word of a group's weights
-  f16x2_t mul[2][2], off[2];
-  uint32_t roff[2], soff[2];
+  u32x4_v wb[N][4], raw[N];
+  uint32_t rs[N], last[N];  // scales; the last word of a group's weights
+  f16x2_t mul[N][2], off[N];
+  uint32_t roff[N], soff[N];
 #pragma unroll
-  for (uint32_t n = 0; n < 2; ++n) {
-    const uint32_t r = 64u * wn + 32u * n + col;
-    roff[n] = 64u * r + 16u * (half ^ (r >> 1 & 3u));
-    soff[n] = 4u * r;
+  for (uint32_t n = 0; n < N; ++n) {
+    const uint32_t r = 32u * N * wn + 32u * n + col;
+    roff[n] = RB * r + 16u * (half ^ (r >> 1 & (2u * GB - 1u)));
+    soff[n] = 2u * GB * r;
   }
   auto load_a = [&](const uint8_t* from, uint32_t j) __attribute__((always_inline)) {  // fragment j of a group: step j / MT, rows j % MT
     xa[j % RING] = *reinterpret_cast<const f16x8_v*>(from + 16u * ((j % MT * 4u + j / MT) * 64u + lane));
   };
-  auto load_raw = [&](const uint8_t* from, const uint8_t* sfrom, uint32_t second) __attribute__((always_inline)) {
+  auto load_raw = [&](const uint8_t* from, const uint8_t* sfrom, uint32_t place) __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) {
-      raw[n] = *reinterpret_cast<const u32x4_v*>(from + (roff[n] ^ 32u * second));
-      rs[n] = *reinterpret_cast<const uint16_t*>(sfrom + soff[n] + 2u * second);
+    for (uint32_t n = 0; n < N; ++n) {
+      raw[n] = *reinterpret_cast<const u32x4_v*>(from + (roff[n] ^ 32u * place));
+      rs[n] = *reinterpret_cast<const uint16_t*>(sfrom + soff[n] + 2u * place);
     }
   };
   auto scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) {
+    for (uint32_t n = 0; n < N; ++n) {
       const float f = __uint_as_float(rs[n] << 16) * down[n];
       mul[n][0] = f16x2_of(f * 0x1p24f, f * 0x1p24f);
       mul[n][1] = f16x2_of(f * 0x1p20f, f * 0x1p20f);
@@ -966,7 +968,7 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   load_raw(s_w0, s_s0, 0u);
   scales();
 #pragma unroll
-  for (uint32_t n = 0; n < 2; ++n) {
+  for (uint32_t n = 0; n < N; ++n) {
 #pragma unroll
     for (uint32_t s = 0; s < 3; ++s)
 #pragma unroll
@@ -980,12 +982,12 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   // come: step s makes those of step s - 1 of the next group (step 0 the last ones of its own).
   // The one barrier is where the last of a group's rows and the next one's weights are read,
   // and the next one's rows have come; behind it their places are filled: with the rows of the
-  // group after the next, and at even groups the weights of the two after that, which have
-  // until the second barrier to come.
-  auto group = [&](uint32_t g, uint32_t q) __attribute__((always_inline)) {  // q = g % 4
+  // group after the next, and once a block, when its last group is read, the weights of the
+  // block after the next, which have until the second barrier to come.
+  auto group = [&](uint32_t g, uint32_t q) __attribute__((always_inline)) {  // q = g % (2 GB)
     uint8_t *const own = q & 1u ? s_x1 : s_x0, *const next = q & 1u ? s_x0 : s_x1;
-    const uint32_t wq = (q + 1u) % 4u;
-    load_raw(wq & 2u ? s_w1 : s_w0, wq & 2u ? s_s1 : s_s0, wq & 1u);
+    const uint32_t wq = (q + 1u) % (2u * GB);
+    load_raw(wq / GB ? s_w1 : s_w0, wq / GB ? s_s1 : s_s0, wq % GB);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (uint32_t s = 0; s < 4; ++s)
@@ -993,36 +995,33 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
       for (uint32_t m = 0; m < MT; ++m) {
         const uint32_t j = s * MT + m;
 #pragma unroll
-        for (uint32_t n = 0; n < 2; ++n) {
+        for (uint32_t n = 0; n < N; ++n) {
           acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(xa[j % RING], __builtin_bit_cast(f16x8_v, wb[n][s]), acc[m][n], 0, 0, 0);
-          if (n == 1u) load_a(j + RING < FR ? own : next, (j + RING) % FR);
+          if (n == N - 1u) load_a(j + RING < FR ? own : next, (j + RING) % FR);
 #pragma unroll
           for (uint32_t i = m * 4u / MT; i < (m + 1u) * 4u / MT; ++i) apart(n, (s + 3u) % 4u, i, s ? raw[n][s - 1u] : last[n]);
           __builtin_amdgcn_sched_barrier(0);
         }
         if (j == MT - 1u) scales();
         if (j + RING + 1u == FR) {
-          if (q & 1u)
+          if (q % GB == GB - 1u)
             barrier_but<5>();  // the five loads of weights behind the rows
           else
             barrier_but<0>();
           load_x(g + 2u, own);
           __builtin_amdgcn_sched_barrier(0);
-          if (!(q & 1u)) load_w((g + 4u) / 2u, q & 2u ? s_w1 : s_w0, q & 2u ? s_s1 : s_s0);
+          if (q % GB == GB - 2u) load_w((g + GB + 2u) / GB, q / GB ? s_w1 : s_w0, q / GB ? s_s1 : s_s0);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n) last[n] = raw[n][3];
+    for (uint32_t n = 0; n < N; ++n) last[n] = raw[n][3];
   };
-  for (uint32_t g = 0; g < groups; g += 4u) {  // groups is a multiple of 8
-    group(g, 0u);
-    group(g + 1u, 1u);
-    group(g + 2u, 2u);
-    group(g + 3u, 3u);
-  }
+  for (uint32_t g = 0; g < groups; g += 2u * GB)  // groups is a multiple of 8
 #pragma unroll
-  for (uint32_t n = 0; n < 2; ++n) {
+    for (uint32_t q = 0; q < 2u * GB; ++q) group(g + q, q);
+#pragma unroll
+  for (uint32_t n = 0; n < N; ++n) {
     const float up = __uint_as_float((cex[n] + 9u) << 23);
 #pragma unroll
     for (uint32_t m = 0; m < MT; ++m)
@@ -1033,28 +1032,28 @@ __global__ void __launch_bounds__(256, 2) lm_many_kernel(LmArgs p, const uint8_t
   // 32 rows at a time through LDS, eight threads for a row. (A wave a row, one after another,
   // waited for each row's reductions and token.)
   typedef float(*Rows)[L::OROW];
-  const Rows out0 = reinterpret_cast<Rows>(s_x0), out1 = reinterpret_cast<Rows>(s_x1);  // rows 0 to 15, 16 to 31
+  const Rows out0 = reinterpret_cast<Rows>(s_w0), out1 = reinterpret_cast<Rows>(s_w1);  // rows 0 to 15, 16 to 31
   const uint32_t part = tid % 8u, orow = tid / 8u;
   const float* mine = orow < 16u ? out0[orow] : out1[orow - 16u];
 #pragma unroll
   for (uint32_t m = 0; m < MT; ++m) {
     if (m) __syncthreads();
 #pragma unroll
-    for (uint32_t n = 0; n < 2; ++n)
+    for (uint32_t n = 0; n < N; ++n)
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) (i < 8u ? out0 : out1)[8u * (i / 4u % 2u) + 4u * half + i % 4u][64u * wn + 32u * n + col] = acc[m][n][i];
+      for (uint32_t i = 0; i < 16; ++i) (i < 8u ? out0 : out1)[8u * (i / 4u % 2u) + 4u * half + i % 4u][32u * N * wn + 32u * n + col] = acc[m][n][i];
     __syncthreads();
     const uint32_t r = 32u * m + orow, t = L::ROWS * tt + r, k = s_token[r] - v0;
     const float f = s_factor[r];
-    if (part == 0u && k < LM_COLS) p.xt[t] = mine[k] * f;
-    float x[32];
+    if (part == 0u && k < L::COLS) p.xt[t] = mine[k] * f;
+    float x[16u * N];
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
+    for (uint32_t i = 0; i < 4u * N; ++i) {
       const f32x4_v v = *reinterpret_cast<const f32x4_v*>(mine + 32u * i + 4u * part);
 #pragma unroll
       for (uint32_t e = 0; e < 4; ++e) x[4 * i + e] = v[e] * f;
     }
-    lm_sums<LM_COLS, 8>(p, x, t, v0, part, t < p.T);
+    lm_sums<L::COLS, 8>(p, x, t, v0, part, t < p.T);
   }
 }
 
@@ -1079,34 +1078,48 @@ LogitsPlan logits_plan(uint32_t T, uint32_t vocab, uint32_t k) {
 
 constexpr uint32_t LM_FEW = 32;
 struct LmPlan {
-  uint32_t rows, mb, tiles, ld;  // token rows of a pass, 32-row blocks of a workgroup
+  uint32_t rows, mb, nb, tiles, ld;  // token rows of a pass, a workgroup's blocks of 32 rows and of 128 columns
   size_t stat, xt, logits, xp, xf, xs;
   size_t all() const { return stat + xt + logits + xp + xf + xs; }
 };
-// 32-row blocks of a workgroup, one to four, by what a launch takes: of 2,048 columns a
-// workgroup of m blocks 12 + 8 m us where each has a CU (20, 24, 33, 42 measured), and where
-// CUs hold two a round of 512 takes 20 + 11 m (30, 40, 52, 62), by the XCD with most
-// columns. Few columns so make more, smaller workgroups: 70 rows of 3,399 27 us, with three
-// blocks 39; 2,000 of 2,000 42 and, with four, 54.
-uint32_t lm_blocks(uint32_t rows, uint32_t tiles) {
-  const uint64_t blocks = (rows + 31u) / 32u;
-  uint32_t best = 4u;
-  uint64_t least = ~uint64_t(0);
-  for (uint32_t m = 4; m; --m) {
-    const uint64_t n = (blocks + m - 1u) / m * ((tiles + 7u) / 8u), us = n <= 32u ? 12u + 8u * m : (n + 63u) / 64u * (20u + 11u * m);
-    if (us < least) best = m, least = us;
+// A workgroup's blocks of 32 rows and of 128 columns, by what a launch takes. `one`: us of 2,048
+// columns of x with a workgroup a CU, `all` with as many as CUs hold, both measured; more take
+// rounds of those, and a part of one at the end, by the XCD with most columns. (Few columns make
+// small workgroups: 70 rows of 3,399 23 us, in tiles of 96 x 256 39. Narrow tiles read weights
+// by whole lines: 64 rows of 151,936 78 us, 84 in tiles of 256 columns; many rows want wide ones:
+// 2,000 1,220 and 1,358.)
+struct LmShape {
+  uint32_t m, n, held;
+  float one, all;
+};
+const LmShape& lm_shape(uint32_t rows, uint32_t vocab) {
+  static constexpr LmShape shapes[] = {{4, 2, 2, 49.0f, 83.0f}, {3, 2, 2, 40.0f, 69.0f}, {4, 1, 2, 30.0f, 46.0f},
+                                       {3, 1, 2, 26.0f, 38.0f}, {2, 1, 3, 23.0f, 45.0f}, {1, 1, 3, 19.0f, 28.0f}};
+  const LmShape* best = nullptr;
+  float least = 0.0f;
+  for (const LmShape& s : shapes) {
+    const uint64_t tiles = (vocab + 128u * s.n - 1u) / (128u * s.n), n = ((rows + 31u) / 32u + s.m - 1u) / s.m * ((tiles + 7u) / 8u);
+    const float cu = static_cast<float>(n) / 32.0f, held = static_cast<float>(s.held);
+    const float us = cu <= 1.0f    ? s.one
+                     : cu <= held ? s.one + (s.all - s.one) * (cu - 1.0f) / (held - 1.0f)
+                                  : (cu + 0.25f * static_cast<float>(s.n)) / held * s.all;
+    if (!best || us < least) best = &s, least = us;
   }
-  return best;
+  return *best;
 }
 LmPlan lm_plan(uint32_t T, uint32_t in, uint32_t vocab, uint32_t k) {
   LmPlan d{};
-  const uint32_t cols = T <= LM_FEW ? LM_FEW_COLS : LM_COLS;
-  d.tiles = (vocab + cols - 1u) / cols;
-  d.ld = (vocab + 3u) & ~3u;
   // the logits of a pass where alternatives are wanted, and its sums, are of a bounded size
   d.rows = T <= LM_FEW ? T : std::min(T, k ? 256u : 4096u);
-  d.mb = lm_blocks(d.rows, d.tiles);
-  const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = (d.rows + 32u * d.mb - 1u) / (32u * d.mb) * d.mb;
+  if (T > LM_FEW) {
+    const LmShape& shape = lm_shape(d.rows, vocab);
+    d.mb = shape.m;
+    d.nb = shape.n;
+  }
+  const uint32_t cols = T <= LM_FEW ? LM_FEW_COLS : 128u * d.nb;
+  d.tiles = (vocab + cols - 1u) / cols;
+  d.ld = (vocab + 3u) & ~3u;
+  const size_t groups = in / 64u, gpad = (groups + 15u) & ~size_t(15), blocks = T > LM_FEW ? (d.rows + 32u * d.mb - 1u) / (32u * d.mb) * d.mb : 0u;
   d.stat = up256(static_cast<size_t>(d.rows) * d.tiles * sizeof(float4));
   d.xt = up256(static_cast<size_t>(d.rows) * sizeof(float));
   d.logits = k ? up256(static_cast<size_t>(d.rows) * d.ld * sizeof(float)) : 0u;
@@ -1150,13 +1163,13 @@ int launch_few(obs_ctx* ctx, const LmArgs& a) {
   if (a.T <= 16u) return a.in <= 2048u ? go(lm_few_kernel<1, true>) : go(lm_few_kernel<1, false>);
   return a.in <= 2048u ? go(lm_few_kernel<2, true>) : go(lm_few_kernel<2, false>);
 }
-template <uint32_t MT>
+template <uint32_t MT, uint32_t N>
 int launch_many(obs_ctx* ctx, const LmArgs& a, uint8_t* xp, float* xf, uint8_t* xs) {
-  typedef LmTile<MT> L;
+  typedef LmTile<MT, N> L;
   const uint32_t ttiles = (a.T + L::ROWS - 1u) / L::ROWS, vtiles = (a.vocab + L::COLS - 1u) / L::COLS;
   const uint32_t turn = std::max(1u, (5u << 19) / (a.in / 64u * L::XB));  // 2.5 MB of an XCD's 4 MB of L2
   OBS_LAUNCH(ctx, "lm_rows", lm_rows_kernel<MT><<<ttiles * MT * 4u, 512, 0, ctx->stream>>>(a.x, a.T, a.in, xp, xf, xs));
-  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT><<<(vtiles + 7u) / 8u * 8u * ttiles, L::THREADS, 0, ctx->stream>>>(
+  OBS_LAUNCH(ctx, "lm_many", lm_many_kernel<MT, N><<<(vtiles + 7u) / 8u * 8u * ttiles, L::THREADS, 0, ctx->stream>>>(
                                  a, xp, xf, xs, ttiles, vtiles, turn));
   return OBS_OK;
 }
@@ -1250,10 +1263,11 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
     if (T <= LM_FEW)
       rc = launch_few(ctx, a);
     else
-      rc = d.mb == 1u   ? launch_many<1>(ctx, a, xp, xf, xs)
-           : d.mb == 2u ? launch_many<2>(ctx, a, xp, xf, xs)
-           : d.mb == 3u ? launch_many<3>(ctx, a, xp, xf, xs)
-                        : launch_many<4>(ctx, a, xp, xf, xs);
+      rc = d.nb == 1u ? (d.mb == 1u   ? launch_many<1, 1>(ctx, a, xp, xf, xs)
+                         : d.mb == 2u ? launch_many<2, 1>(ctx, a, xp, xf, xs)
+                         : d.mb == 3u ? launch_many<3, 1>(ctx, a, xp, xf, xs)
+                                      : launch_many<4, 1>(ctx, a, xp, xf, xs))
+                      : (d.mb == 3u ? launch_many<3, 2>(ctx, a, xp, xf, xs) : launch_many<4, 2>(ctx, a, xp, xf, xs));
     if (rc != OBS_OK) return rc;
     const JoinArgs j{stat, reinterpret_cast<const float*>(stat), reinterpret_cast<const uint8_t*>(logits), xt, a.tokens,
                      logprob ? logprob + t0 : nullptr, entropy ? entropy + t0 : nullptr,
@@ -1262,8 +1276,10 @@ int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const ui
                      d.tiles, d.tiles, 4u, vocab, top_k};
     if (T <= LM_FEW)
       OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, LM_FEW_COLS><<<n, 256, 0, ctx->stream>>>(j));
+    else if (d.nb == 1u)
+      OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, 128><<<n, 256, 0, ctx->stream>>>(j));
     else
-      OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, LM_COLS><<<n, 256, 0, ctx->stream>>>(j));
+      OBS_LAUNCH(ctx, "logprobs_join", logprobs_join_kernel<false, 256><<<n, 256, 0, ctx->stream>>>(j));
   }
   return OBS_OK;
 }
