@@ -256,7 +256,8 @@ def test_lm_rows(exe, T):
 
 @pytest.mark.parametrize("T,H,V,k", [(1, 512, 1, 1), (3, 512, 255, 3), (40, 512, 256, 64), (5, 2048, 257, 0), (70, 4096, 777, 20), (20, 4096, 3001, 9),
                                      (600, 512, 5003, 2), (260, 1536, 513, 0), (1, 2048, 40000, 5), (24, 2048, 40001, 20), (200, 2048, 20000, 3),
-                                     (1000, 512, 5003, 0), (1500, 512, 20000, 0), (4100, 512, 300, 0), (33, 16384, 600, 2), (2, 16384, 600, 2)])
+                                     (1000, 512, 5003, 0), (1500, 512, 20000, 0), (4100, 512, 300, 0), (33, 16384, 600, 2), (2, 16384, 600, 2),
+                                     (160, 512, 30000, 3), (64, 512, 40000, 2), (150, 512, 60000, 0), (600, 4096, 3000, 0)])
 def test_lm_shapes(exe, T, H, V, k):
     _lm_case(exe, T, H, V, k, T + H + V)
 
