@@ -703,7 +703,9 @@ __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
       __syncthreads();
       // sixteen threads a row, four columns each
       const uint32_t t = tid / 16u, part = tid % 16u;
-      if (t / 4u < (p.T + 3u) / 4u) {  // whole waves
+      // whole waves; of two tiles all eight, which else get out of step (24 tokens 64 us, so 60.5), of one those
+      // with tokens (one token 47, else 52)
+      if (t < RT && (NT == 2u || t / 4u < (p.T + 3u) / 4u)) {
         float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (uint32_t w = 0; w < WAVES; ++w) {
