@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(256, (LmTile<MT, N>::HELD)) lm_many_kernel(LmA
   constexpr uint32_t GB = L::GB, RB = 32u * GB, SW = GB / 2u;  // bytes of a row's block, words of its scales
   // (arrays of their own, for the compiler to tell the ones being written from those being read)
   __shared__ __attribute__((aligned(16))) uint8_t s_x0[L::XB], s_x1[L::XB], s_w0[L::WLDS], s_w1[L::WLDS], s_s0[L::SB], s_s1[L::SB];
-  __shared__ float s_factor[L::ROWS];
+  __shared__ __attribute__((aligned(16))) int s_back[L::ROWS];  // of a row's factor the exponent, and 118 less
   __shared__ uint32_t s_token[L::ROWS];
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wn = uniform(tid >> 6);
   const uint32_t col = lane & 31u, half = lane >> 5;
@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(256, (LmTile<MT, N>::HELD)) lm_many_kernel(LmA
   load_w(1u, s_w1, s_s1);
   if (tid < L::ROWS) {
     const uint32_t t = L::ROWS * tt + tid;
-    s_factor[tid] = xf[t];
+    s_back[tid] = static_cast<int>(__float_as_uint(xf[t]) >> 23) - 245;
     s_token[tid] = p.tokens && t < p.T ? lm_token(p, t) : 0xffffffffu;
   }
   // The largest scale of the lane's vocabulary rows: its exponent (or of the biases 2^90 of it: no
@@ -1022,14 +1022,6 @@ __global__ void __launch_bounds__(256, (LmTile<MT, N>::HELD)) lm_many_kernel(LmA
   for (uint32_t g = 0; g < groups; g += 2u * GB)  // groups is a multiple of 8
 #pragma unroll
     for (uint32_t q = 0; q < 2u * GB; ++q) group(g + q, q);
-#pragma unroll
-  for (uint32_t n = 0; n < N; ++n) {
-    const float up = __uint_as_float((cex[n] + 9u) << 23);
-#pragma unroll
-    for (uint32_t m = 0; m < MT; ++m)
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) acc[m][n][i] *= up;
-  }
   barrier_but<0>();
   // 32 rows at a time through LDS, eight threads for a row. (A wave a row, one after another,
   // waited for each row's reductions and token.)
@@ -1040,20 +1032,22 @@ __global__ void __launch_bounds__(256, (LmTile<MT, N>::HELD)) lm_many_kernel(LmA
 #pragma unroll
   for (uint32_t m = 0; m < MT; ++m) {
     if (m) __syncthreads();
+    int back[16];  // rows and columns of one exponent: neither alone takes a logit out of fp32's range
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) back[i] = s_back[32u * m + 8u * (i / 4u) + 4u * half + i % 4u];
 #pragma unroll
     for (uint32_t n = 0; n < N; ++n)
 #pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) (i < 8u ? out0 : out1)[8u * (i / 4u % 2u) + 4u * half + i % 4u][32u * N * wn + 32u * n + col] = acc[m][n][i];
+      for (uint32_t i = 0; i < 16; ++i) (i < 8u ? out0 : out1)[8u * (i / 4u % 2u) + 4u * half + i % 4u][32u * N * wn + 32u * n + col] = __builtin_amdgcn_ldexpf(acc[m][n][i], back[i] + static_cast<int>(cex[n]));
     __syncthreads();
     const uint32_t r = 32u * m + orow, t = L::ROWS * tt + r, k = s_token[r] - v0;
-    const float f = s_factor[r];
-    if (part == 0u && k < L::COLS) p.xt[t] = mine[k] * f;
+    if (part == 0u && k < L::COLS) p.xt[t] = mine[k];
     float x[16u * N];
 #pragma unroll
     for (uint32_t i = 0; i < 4u * N; ++i) {
       const f32x4_v v = *reinterpret_cast<const f32x4_v*>(mine + 32u * i + 4u * part);
 #pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) x[4 * i + e] = v[e] * f;
+      for (uint32_t e = 0; e < 4; ++e) x[4 * i + e] = v[e];
     }
     lm_sums<L::COLS, 8>(p, x, t, v0, part, t < p.T);
   }

@@ -316,6 +316,25 @@ def test_lm_scales_of_all_sizes(exe, T):
     assert np.all(logits[t, got[2][:, 0]] >= logits[t, ids[:, 0]] - 2 * off.max(1))
 
 
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("e", [-110, -60, 60, 110])
+def test_lm_scales_and_rows_of_opposite_sizes(exe, T, e):
+    """Scales and biases 2^e of the usual, hidden rows 2^-e."""
+    rng = np.random.default_rng(17)
+    H, V = 512, 300
+    w, s, b = _matrix(rng, V, H)
+    s, b = (synth.f32_to_bf16_bits((_f64(y) * 2.0 ** e).astype(np.float32)) for y in (s, b))
+    x = synth.f32_to_bf16_bits((rng.standard_normal((T, H)) * 2.0 ** -e).astype(np.float32))
+    args = [exe.upload(a) for a in (x, w, s, b)]
+    tokens = rng.integers(0, V, T)
+    got = _run(exe, T, 1, tokens, lambda **kw: exe.lm_logprobs(*args, T, H, V, **kw), exe.lm_logprobs_workspace(T, H, V, 1))
+    logits, off = _logits64(_f64(x), w, s, b)
+    lp, ent, ids, tlp, bs, be = _reference(logits, tokens, 1)
+    assert _near(got[0], lp, bs + 4 * U * np.abs(lp) + 2 * off.max(1))
+    t = np.arange(T)
+    assert np.all(logits[t, got[2][:, 0]] >= logits[t, ids[:, 0]] - 2 * off.max(1))
+
+
 def test_lm_large_rows(exe):
     """Hidden rows of large magnitude: one token takes all."""
     _lm_case(exe, 7, 1024, 2000, 4, 1, scale=200.0)
