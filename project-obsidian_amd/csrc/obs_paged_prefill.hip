@@ -550,9 +550,10 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
           for (uint32_t d = 0; d < DT; ++d)
 #pragma unroll
             for (uint32_t j = 0; j < 16; ++j) {
-              const uint32_t dim = 32u * d + 8u * (j / 4u) + 4u * half + j % 4u;
-              const size_t at = ((base + dim) << a.lp) + (e & pmask);
+              // (the sum from base on: with the dim by itself first, 128 dims in bf16 and e4m3 spill two registers)
+              const size_t at = ((base + 32u * d + 8u * (j / 4u) + 4u * half + j % 4u) << a.lp) + (e & pmask);
               if constexpr (Q4) {
+                const uint32_t dim = 32u * d + 8u * (j / 4u) + 4u * half + j % 4u;
                 const uint8_t* page = a.v + page_at<HD, KT>(a, i < 16u ? p0 : p1, kv);
                 const uint32_t byte = page[((dim % (HD / 2u)) << a.lp) + (e & pmask)];
                 const uint32_t par = reinterpret_cast<const uint32_t*>(page + (HD / 2u << a.lp))[(dim / 64u << a.lp) + (e & pmask)];
