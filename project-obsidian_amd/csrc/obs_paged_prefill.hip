@@ -509,15 +509,29 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
       }
-      const float mu = m == NEG_INF ? 0.0f : m;
+      float mu = m == NEG_INF ? 0.0f : m, by = scale;
+      if constexpr (Q4) {
+        // Scores so large that the product's rounding counts, which m has and the exact product below
+        // has not: rounded as m was, they pass it by the slack at most, and P stays finite.
+        const bool large = fabsf(mu) >= 0x1p20f;
+        if (__any(large)) {  // uniform, rare
+#pragma unroll
+          for (uint32_t i = 0; i < 16; ++i) {
+            const float d = sc[i] * scale - mu;
+            sc[i] = !large ? sc[i] : d > PF_SLACK ? PF_SLACK : d;  // (NaN stays)
+          }
+          mu = large ? 0.0f : mu;
+          by = large ? 1.0f : scale;
+        }
+      }
       OpV pb[2];
 #pragma unroll
       for (uint32_t k2 = 0; k2 < 2; ++k2) {
         uint32_t pk[4];
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-          pk[i] = O::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i], scale, -mu)),
-                          __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i + 1], scale, -mu)));
+          pk[i] = O::pack(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i], by, -mu)),
+                          __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * k2 + 2 * i + 1], by, -mu)));
           l = O::add_pair(pk[i], l);
         }
         pb[k2] = __builtin_bit_cast(OpV, u32x4_v{pk[0], pk[1], pk[2], pk[3]});
