@@ -579,7 +579,8 @@ int obs_sdpa_paged_decode(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_
  * j < sinks; a row whose i is negative (len shorter than its tokens) gets zeros.
  * A row is not touched by what other rows see, NaN and infinities included.
  * The rows' own keys and values are in the pages already (obs_attn_prep_paged).
- * Entries of 4 bits enter the products rounded to fp16.
+ * Entries of 4 bits enter the products rounded to fp16 (2^-11, below 2^-14 in magnitude
+ * 2^-25), and so do the softmax weights over them (2^-11, or 2^-32 of the row's largest).
  * out bf16 [n_rows, n_heads, head_dim]; workspace as above. */
 int obs_sdpa_paged_prefill(obs_ctx* ctx, const obs_paged_kv* kv, const obs_paged_seqs* seqs, const uint16_t* q,
                            uint16_t* out, uint32_t n_heads, uint32_t window, uint32_t sinks, uint32_t q_ld, void* ws,

@@ -35,12 +35,17 @@ using obs::up256;
 // machine schedulers gained nothing.
 // The running maximum follows the scores only when they pass it by 2^8 (the sums
 // and O are in fp32 and P in bf16, which has fp32's range), so O is hardly ever
-// rescaled.
+// rescaled. Over entries of 4 bits P is fp16: weights are taken 2^7 higher there, below
+// 2^15 with the slack, and sum and O alike, so that the factor cancels where they meet, in
+// a tile's end and in the join. What lies 2^-21 below a row's largest and more is subnormal
+// then, off by 2^-32 of the largest (2^-25 without the factor, at which a sink of value
+// zero over thousands of weak entries gave them up).
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16_v;
 
 constexpr uint32_t PF_COLS = 384, PF_THREADS = 2u * PF_COLS, PF_TARGET = 256, PF_MIN_CHUNK = 4, PF_WHOLE = 12;
 constexpr uint32_t PF_TILES = 1024;  // tiles a kv head at most where they are cut into parts
-constexpr float PF_SLACK = 8.0f;
+constexpr float PF_SLACK = 8.0f, PF_LIFT = 7.0f;
+static_assert(PF_SLACK + PF_LIFT < 16.0f, "P is finite in fp16");
 
 __device__ __forceinline__ Span tile_span(const PagedAttn& p, const RowSpan& r, uint32_t n, uint32_t t0, uint32_t t1) {
   // entry of row t is n - (r1 - t); negative: nothing to see
@@ -509,7 +514,7 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) o[d][i] *= f;
       }
-      float mu = m == NEG_INF ? 0.0f : m, by = scale;
+      float mu = (m == NEG_INF ? 0.0f : m) - (Q4 ? PF_LIFT : 0.0f), by = scale;
       if constexpr (Q4) {
         // Scores so large that the product's rounding counts, which m has and the exact product below
         // has not: rounded as m was, they pass it by the slack at most, and P stays finite.
@@ -517,10 +522,10 @@ __global__ void __launch_bounds__(PF_THREADS, 3) paged_prefill_kernel(Paged a, P
         if (__any(large)) {  // uniform, rare
 #pragma unroll
           for (uint32_t i = 0; i < 16; ++i) {
-            const float d = sc[i] * scale - mu;
+            const float d = sc[i] * scale - (m == NEG_INF ? 0.0f : m);
             sc[i] = !large ? sc[i] : d > PF_SLACK ? PF_SLACK : d;  // (NaN stays)
           }
-          mu = large ? 0.0f : mu;
+          mu = large ? -PF_LIFT : mu;
           by = large ? 1.0f : scale;
         }
       }
