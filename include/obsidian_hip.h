@@ -484,7 +484,9 @@ int obs_sdpa_prefill(obs_ctx* ctx, const uint16_t* q, const uint16_t* k_cache, c
  * in e4m3 (OCP, magnitudes up to 448) with one positive fp32 scale per kv head: an
  * entry is the stored value times the scale. Or in 4 bits (OBS_KV_Q4), affine in
  * groups of 64 dims as the weights are: a dim is q * scale + bias, q in 0 .. 15,
- * scale and bias bf16, values up to 65,504 in magnitude. A (page, kv head) of keys is then
+ * scale and bias bf16. Prompts take that in fp16, where it is infinite from 65,520 in
+ * magnitude on: appended values may reach 64,900, as scale and bias are rounded too;
+ * decode takes what its fp32 sums hold. A (page, kv head) of keys is then
  * [page][head_dim / 2] bytes, byte i of an entry holding dim i in its low and dim
  * i + head_dim / 2 in its high nibble, followed by uint32 [head_dim / 64][page], the
  * scale in the low and the bias in the high half; one of values [head_dim / 2][page]
