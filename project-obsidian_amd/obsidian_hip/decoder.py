@@ -233,18 +233,31 @@ class Model:
 
     # -- log probabilities -----------------------------------------------------
     def _score_buffers(self, T: int, top_k: int, ws: int) -> Dict:
-        if self._sc is None or self._sc["T"] < T or self._sc["top_k"] < top_k or self._sc["ws"].nbytes < ws:
-            had = self._sc or {"T": 0, "top_k": 0}
-            ws = max(ws, had["ws"].nbytes if "ws" in had else 0)
-            T, top_k = max(T, had["T"]), max(top_k, had["top_k"])
-            self._sc = had = None  # release the smaller set first
-            e = self.exe
-            self._sc = {
-                "T": T, "top_k": top_k, "tokens": e.alloc(T, np.int32), "logprob": e.alloc(T, np.float32),
-                "entropy": e.alloc(T, np.float32), "ids": e.alloc(max(T * top_k, 1), np.int32),
-                "top": e.alloc(max(T * top_k, 1), np.float32), "ws": e.alloc(max(ws, 1), np.uint8),
-            }
-        return self._sc
+        """The score calls' buffers, grown to the largest call. An outgrown set is freed
+        first: the executor holds what it allocated, so dropping it here would not."""
+        S = self._sc
+        if S is None or S["T"] < T or S["top_k"] < top_k or S["ws"].nbytes < ws:
+            if S is not None:
+                T, top_k, ws = max(T, S["T"]), max(top_k, S["top_k"]), max(ws, S["ws"].nbytes)
+                self._free_scores(S)
+            self._sc, S, e = None, {}, self.exe
+            try:
+                for name, n, dtype in (("tokens", T, np.int32), ("logprob", T, np.float32), ("entropy", T, np.float32),
+                                       ("ids", max(T * top_k, 1), np.int32), ("top", max(T * top_k, 1), np.float32),
+                                       ("ws", max(ws, 1), np.uint8)):
+                    S[name] = e.alloc(n, dtype)
+            except ObsError:
+                self._free_scores(S)
+                raise
+            S["T"], S["top_k"] = T, top_k
+            self._sc = S
+        return S
+
+    @staticmethod
+    def _free_scores(S: Dict) -> None:
+        for name in ("tokens", "logprob", "entropy", "ids", "top", "ws"):
+            if name in S:
+                S[name].free()
 
     @staticmethod
     def _scores(S: Dict, T: int, top_k: int) -> Scores:
