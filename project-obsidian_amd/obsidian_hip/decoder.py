@@ -259,10 +259,12 @@ class Model:
             if name in S:
                 S[name].free()
 
-    @staticmethod
-    def _scores(S: Dict, T: int, top_k: int) -> Scores:
-        ids, top = (S[n].download()[:T * top_k].reshape(T, top_k) for n in ("ids", "top"))
-        return Scores(S["logprob"].download()[:T].copy(), S["entropy"].download()[:T].copy(), ids.copy(), top.copy())
+    def _scores(self, S: Dict, T: int, top_k: int) -> Scores:
+        """The call's own rows: the buffers may be those of a longer one."""
+        def rows(name, shape, dtype):
+            return self.exe.download_raw(S[name].ptr, shape, dtype)
+        return Scores(rows("logprob", T, np.float32), rows("entropy", T, np.float32),
+                      rows("ids", (T, top_k), np.int32), rows("top", (T, top_k), np.float32))
 
     def last_scores(self, top_k: int = 0) -> Scores:
         """Of the last step (or prefill), whose logits are still there: its greedy

@@ -97,3 +97,17 @@ def test_a_set_that_cannot_be_had(at):
     held, m = _held(m), Model()
     m.score([1] * 50, top_k=3)
     assert held == _held(m)
+
+
+@pytest.mark.parametrize("top_k", [0, 3])
+def test_a_token_brings_back_one_row(top_k):
+    """After a long scored prompt the scores of a generated token cost no more than before it."""
+    m = Model()
+    m.score([1] * 500, top_k=20)
+    for call, rows in ((lambda: m.last_scores(top_k), 1), (lambda: m.score([1] * 7, top_k=top_k), 7)):
+        m.exe.brought = 0
+        got = call()
+        assert m.exe.brought == 8 * rows * (1 + top_k)
+        assert got.logprob.shape == got.entropy.shape == (rows,)
+        assert got.top_ids.shape == got.top_logprobs.shape == (rows, top_k)
+        assert got.top_ids.dtype == np.int32 and got.top_logprobs.dtype == np.float32
