@@ -636,7 +636,8 @@ int obs_token_logprobs(obs_ctx* ctx, const void* logits, int dtype, uint32_t T, 
  * vocabulary row (to within 2^-15 of that scale), and hidden values below 2^-29 of their
  * row's largest (to within 2^-39 of it). group 64, in a multiple of 512 up to 16,384; x, w, scales, biases and ws 16-byte aligned.
  * With alternatives the rows of more than 32 tokens pass by 256 at a time, whose logits
- * are in the workspace. */
+ * are in the workspace. Either workspace is for its call's own T and top_k: fewer rows
+ * may need more bytes. */
 int obs_lm_logprobs_workspace(obs_ctx* ctx, uint32_t T, uint32_t in, uint32_t vocab, uint32_t top_k, size_t* bytes);
 int obs_lm_logprobs(obs_ctx* ctx, const uint16_t* x, const uint32_t* w, const uint16_t* scales, const uint16_t* biases,
                     uint32_t T, uint32_t in, uint32_t vocab, uint32_t group, const int32_t* tokens, float* logprob,

@@ -119,7 +119,9 @@ struct Top {
 // ---------------------------------------------------------------------------
 // A workgroup takes one part of a row, a wave a step of 1,024 logits at once: their sums,
 // and the maxima of its four tiles, of 16 lanes each (a wave's whole maximum of every
-// load cost 7 of 57 us for 777 rows in bf16). One pass; bound by the reading.
+// load cost 7 of 57 us for 777 rows in bf16). One pass; bound by the reading where rows start at 16
+// bytes (777 rows of 151,669 in bf16 52 us, 4.5 TB/s). Other rows are read by single logits (dense, seven of
+// eight of them: 167 us).
 template <bool BF16>
 struct Logits {
   static constexpr uint32_t LOAD = BF16 ? 512u : 256u, PER = LOAD / 64u, STEP = 1024u, N = STEP / LOAD;
@@ -578,7 +580,9 @@ __device__ __forceinline__ void lm_sums(const LmArgs& p, float (&x)[N], uint32_t
 // = lane / 16) of a product (v_mfma_f32_16x16x32_bf16) loads 16 bytes of its row, the four
 // 64, two groups; a swap of the wave's halves gives each lane 8 bytes of either (of the
 // group's 32, those from 16 (q % 2) + 8 (q / 2) on). The sums over a group's columns are a
-// product with ones. HELD: a wave has one slice, whose rows of x and sums stay in registers.
+// product with ones. HELD: a wave has one slice, whose rows of x and sums stay in registers. Made for
+// 2,048 columns (one token 46 us at 151,936 rows): with 512 or 1,024 six or four of the waves idle (38 and
+// 39 us), with 2,560 the second turn has two slices (90).
 template <uint32_t NT, bool HELD>
 __global__ void __launch_bounds__(512, 2) lm_few_kernel(LmArgs p) {
   constexpr uint32_t RT = 16u * NT, OROW = LM_FEW_COLS + 4u, WAVES = 8;
@@ -792,8 +796,9 @@ __global__ void __launch_bounds__(512) lm_rows_kernel(const uint16_t* __restrict
 // the sums at one's end (350 us of 1,335 for 2,000 tokens with one of eight waves) beside the
 // other's products. Rows and weights come into LDS past the registers, by whole runs of a row; read
 // by the lanes that use them, 32 bytes of 32 rows a load, the weights took 165 us, the scales, two
-// bytes each, 150, and the rows through registers and their stores 250. 2,000 tokens take
-// 1,220 us, 1,020 TFLOP/s (a library's bf16 product of the same sizes, without the 4 bits: 1,214 us).
+// bytes each, 150, and the rows through registers and their stores 250. 2,000 tokens take 1,220 to
+// 1,300 us by the card, 957 to 1,020 TFLOP/s (a library's bf16 product of 2,048, without the 4 bits:
+// 1,214 to 1,220 us, 1,045 to 1,050).
 typedef _Float16 f16x8_v __attribute__((ext_vector_type(8)));
 // Global memory to LDS: 16 (4) bytes of every lane from its address to `to` (of the wave) and on.
 typedef const __attribute__((address_space(1))) uint32_t* GlobalWords;
